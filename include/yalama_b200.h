@@ -262,6 +262,81 @@ int ylm_k_sample(const void *logits, int64_t vocab, int32_t greedy, int32_t top_
                  const uint32_t *mask_bits_dev, float u, int64_t *out_id, int64_t *topk_ids, float *topk_probs,
                  void *stream);
 
+/* ---- 8-bit K/V cache ------------------------------------------------------------
+ * A cache of half the bytes for long requests (the reference's cache is in the
+ * model's type, src/models/ModelBase.cpp:340-370). Keys and values are 8-bit codes
+ * with one scale per block of tokens and KV head: value = code * scale. Scales
+ * are powers of two, the smallest with max |x| <= 448 (E4M3) or 127 (INT8) times
+ * the scale; 0 for a block of zeros. A cache starts at slot 0; nothing has to be
+ * zeroed before the first store. Head dimension 128; keys come rotated. */
+typedef enum ylm_kv8_format {
+    YLM_KV8_E4M3 = 0, /* relative step 2^-3: for keys and values with outliers */
+    YLM_KV8_INT8 = 1  /* absolute step, the finer one for values of one magnitude */
+} ylm_kv8_format;
+typedef struct ylm_kv8_cache {
+    void *k, *v;              /* codes [hkv][cap][128], 16-byte aligned */
+    float *k_scale, *v_scale; /* [hkv][ceil(cap / block)] */
+    int32_t format;           /* ylm_kv8_format */
+    int32_t block;            /* tokens per scale: 16, 32, 64 or 128 */
+    int32_t cap;              /* slots per KV head */
+    int32_t hkv;              /* KV heads */
+} ylm_kv8_cache;
+/* Store t tokens in slots [slot, slot + t): k and v FP16, token i's KV head g at
+ * k + i * k_stride + g * 128 (strides in halves, so that both may be columns of a
+ * fused QKV projection; multiples of 8, pointers 16-byte aligned). Slots below
+ * `slot` in the first block are taken as filled: where a new token needs a larger
+ * scale they are rescaled (one more rounding; E4M3: none above 2^-6 of a unit).
+ * The other slots are left as they are. Infinities count as +-65504; NaN is kept
+ * in E4M3 and stored as 0 in INT8. t = 0 does nothing. */
+int ylm_k_kv8_store(const ylm_kv8_cache *cache, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                    int32_t t, int32_t slot, void *stream);
+/* Attention of the last t of n cached tokens (already stored): q [t][hq * 128],
+ * RoPE applied, out likewise (token strides in halves, multiples of 8; pointers
+ * 16-byte aligned); token i sees slots [0, n - t + i], scores scaled by
+ * 1 / sqrt(128), softmax in FP32. t = 1 is a decode step; a draft or a prompt's
+ * last tokens take more. At most 128 query heads per KV head.
+ * mask_bits: (n + 31) / 32 words, bit i & 31 of word i / 32 = 1 hides slot i from
+ * every head (null: none); a token that sees no slot gets zeros.
+ * acc: [hkv][cap] FP32 or null: acc[g][j] += the attention weight that slot j got
+ * from the t tokens, summed over the query heads of KV head g (zero it when
+ * the cache starts).
+ * workspace: device memory of at least ylm_k_kv8_attention_workspace bytes,
+ * 16-byte aligned, for this call alone until it has run: calls that may overlap on the GPU,
+ * and graphs that may, need one each. null: allocated and freed in stream order. */
+int ylm_k_kv8_attention(const ylm_kv8_cache *cache, const void *q, int64_t q_stride, int32_t hq, int32_t t, int32_t n,
+                        const uint32_t *mask_bits, float *acc, void *out, int64_t out_stride, void *workspace,
+                        size_t workspace_bytes, void *stream);
+/* Bytes of workspace that ylm_k_kv8_attention needs for these arguments on the
+ * current device; enough for every smaller n with the same t, too. */
+int ylm_k_kv8_attention_workspace(const ylm_kv8_cache *cache, int32_t hq, int32_t t, int32_t n, int32_t with_acc,
+                                  size_t *bytes);
+/* Evict by accumulated attention weight: of slots [0, n) of src, every KV head
+ * keeps n_keep in dst's slots [0, n_keep), in their order: the first n_sink, the
+ * last n_recent, and of the others those of the largest acc_src (ties: the lower
+ * slot; NaN counts as the smallest). kept [hkv][n_keep]: the slot each came from.
+ * acc_dst [hkv][dst cap]: the kept weights, then zeros. A dst block's scale is the largest
+ * its tokens had in src; tokens of a smaller one are rescaled to it. The caches
+ * have the same format, block and hkv; dst, acc_dst and kept do not overlap src,
+ * acc_src or one another (one spare layer serves a whole model: a layer's old
+ * buffers are the next one's dst). dst's codes behind n_keep are left as they are. */
+int ylm_k_kv8_evict(const ylm_kv8_cache *src, const ylm_kv8_cache *dst, const float *acc_src, float *acc_dst,
+                    int32_t n, int32_t n_keep, int32_t n_sink, int32_t n_recent, int32_t *kept, void *stream);
+
+/* ---- log probabilities ------------------------------------------------------------
+ * Of `rows` rows of FP16 logits [rows][ld], vocab of them used, over the softmax of
+ * the unmasked ids (natural logarithms, FP32; all buffers on the device):
+ *   logprob[r]  of ids[r]; -inf for a masked id or one outside [0, vocab) (null: not wanted)
+ *   entropy[r]  (null: not wanted)
+ *   top_ids, top_logprobs [rows][n_top]: the most likely ids, best first, ties to
+ *     the lower id; -1 and -inf where fewer ids have a logit above -inf (n_top 0..64)
+ * mask_bits: (vocab + 31) / 32 words as for ylm_k_sample, one mask for all rows, or
+ * null. Logits of masked ids are not looked at. A row whose unmasked logits hold a NaN or +inf
+ * has NaN log probabilities and entropy (its top ids: NaN first); a row that is
+ * masked or -inf throughout has logprob -inf and entropy 0. */
+int ylm_k_logprobs(const void *logits, int64_t ld, int32_t rows, int64_t vocab, const int64_t *ids,
+                   const uint32_t *mask_bits, int32_t n_top, float *logprob, float *entropy, int64_t *top_ids,
+                   float *top_logprobs, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,217 @@
+"""Log probabilities of rows of FP16 logits on the GPU, through the C ABI, against their definitions in 64 bits."""
+import numpy as np
+import pytest
+
+import kv8_reference as R
+from yalama_b200 import engine as E
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def bits(masked):
+    w = np.zeros((masked.size + 31) // 32, np.uint32)
+    for i in np.nonzero(masked)[0]:
+        w[i >> 5] |= np.uint32(1) << np.uint32(i & 31)
+    return torch.from_numpy(w.view(np.int32)).cuda()
+
+
+def run(x, ids, n_top, masked=None, ld=None, shift=0, want=("logprob", "entropy"), s=None):
+    """x [rows][vocab] float16; shift: the first logit's offset in halves from an aligned address."""
+    rows, vocab = x.shape
+    ld = vocab if ld is None else ld
+    # what lies around the rows must not count
+    buf = torch.full((shift + rows * ld + 64,), float("nan"), dtype=torch.float16, device="cuda")
+    view = buf[shift:shift + rows * ld].reshape(rows, ld)
+    view[:, :vocab] = torch.from_numpy(x).cuda()
+    o = {"logprob": torch.full((rows + 1,), 7.0, device="cuda"), "entropy": torch.full((rows + 1,), 7.0, device="cuda"),
+         "top_ids": torch.full((rows + 1, max(n_top, 1)), 7, dtype=torch.int64, device="cuda"),
+         "top": torch.full((rows + 1, max(n_top, 1)), 7.0, device="cuda")}
+    d_ids = torch.from_numpy(np.asarray(ids, np.int64)).cuda() if "logprob" in want else None
+    E.check(E.lib().ylm_k_logprobs(ptr(view), ld, rows, vocab, ptr(d_ids), None if masked is None else ptr(bits(masked)),
+                                   n_top, ptr(o["logprob"]) if "logprob" in want else None,
+                                   ptr(o["entropy"]) if "entropy" in want else None, ptr(o["top_ids"]), ptr(o["top"]),
+                                   torch.cuda.current_stream().cuda_stream if s is None else s), "logprobs")
+    torch.cuda.synchronize()
+    for name, t in o.items():  # nothing behind the last row
+        assert bool((t[rows:] == 7).all()), name
+        if name in ("logprob", "entropy") and name not in want or name.startswith("top") and not n_top:
+            assert bool((t == 7).all()), name
+    return {k: t[:rows].cpu().numpy() for k, t in o.items()}
+
+
+def check(x, ids, n_top, masked=None, **kw):
+    """z and the entropy's sum are sums of positive terms: a term takes an exponential (within 2^-21 of it), a thread
+    adds at most vocab / 128 + 8 terms one after another and 64 partial sums follow, each addition off by at most
+    2^-24 of the sum: rel = (vocab / 128 + 72) 2^-24 + 2^-21 of z. log1p and the subtractions add a few steps."""
+    rows, vocab = x.shape
+    seen = np.ones(vocab, bool) if masked is None else ~masked
+    got = run(x, ids, n_top, masked, **kw)
+    lp, ent, m, z = R.logprobs(x.astype(np.float64), seen)
+    rel = (vocab / 128 + 72) * 2.0 ** -24 + 2.0 ** -21
+    lz = np.log1p(z)
+
+    def tol(v, r):
+        return rel * z[r] / (1 + z[r]) + 2.0 ** -22 * (np.abs(v) + 2 * lz[r]) + 1e-37
+
+    for r in range(rows):
+        w = lp[r, ids[r]] if 0 <= ids[r] < vocab else -np.inf
+        if np.isfinite(w):
+            assert abs(got["logprob"][r] - w) <= tol(w, r), (r, got["logprob"][r], w)
+        else:
+            assert got["logprob"][r] == w
+        assert abs(got["entropy"][r] - ent[r]) <= rel * (z[r] / (1 + z[r]) + 2 * ent[r]) + 2.0 ** -21 * ent[r] + 1e-37
+        if n_top:
+            want = R.top(x[r].astype(np.float64), seen, n_top)
+            np.testing.assert_array_equal(got["top_ids"][r], want)
+            for i, v in zip(want, got["top"][r]):
+                assert v == -np.inf if i < 0 else abs(v - lp[r, i]) <= tol(lp[r, i], r)
+
+
+@pytest.mark.parametrize("rows,vocab,n_top", [
+    (1, 1, 0), (1, 1, 1), (1, 1, 64), (3, 2, 2), (2, 7, 7), (1, 8, 20), (5, 31, 5), (2, 63, 64), (2, 64, 64),
+    (2, 65, 64), (4, 1000, 20), (1, 4095, 20), (1, 4096, 1), (3, 8191, 64), (2, 32768, 5), (1, 128256, 20),
+    (1, 151936, 64), (3, 50257, 0), (17, 2049, 3), (40, 8200, 20), (160, 1024, 10), (300, 513, 33)])
+def test_logprobs(rows, vocab, n_top):
+    rng = np.random.default_rng(rows * 1000 + vocab)
+    x = (rng.standard_normal((rows, vocab)) * rng.uniform(0.1, 6, (rows, 1))).astype(np.float16)
+    check(x, rng.integers(0, vocab, rows), n_top)
+    masked = rng.random(vocab) < 0.3
+    check(x, rng.integers(0, vocab, rows), n_top, masked)
+    # rows that start anywhere, with room behind each
+    check(x, x.astype(np.float32).argmax(1), n_top, masked, ld=vocab + 3, shift=int(rng.integers(1, 8)))
+
+
+@pytest.mark.parametrize("vocab", [100, 3000, 40000])
+@pytest.mark.parametrize("order", ["up", "down", "same", "two", "zeros", "steps"])
+def test_orders_and_ties(vocab, order):
+    x = {"up": np.linspace(-20, 20, vocab), "down": np.linspace(20, -20, vocab), "same": np.full(vocab, 1.5),
+         "two": np.where(np.arange(vocab) % 3 == 1, 2.0, -1.0), "zeros": np.where(np.arange(vocab) % 2 == 1, 0.0, -0.0),
+         "steps": np.floor(np.arange(vocab) / 50) % 7}[order].astype(np.float16)[None]
+    for n_top in (1, 20, 64):
+        check(x, [vocab // 2], n_top)
+        check(x, [vocab - 1], n_top, np.arange(vocab) % 5 == 0)
+
+
+@pytest.mark.parametrize("vocab", [9, 1000, 128256])
+def test_certain_rows_keep_small_log_probabilities(vocab):
+    # the likeliest id's log probability is -(vocab - 1) e^-gap, far below the step of 1
+    for gap in (10, 18, 30, 60):
+        x = np.full((2, vocab), -gap / 2, np.float16)
+        x[0, vocab // 3] = gap / 2
+        x[1, vocab - 1] = gap / 2
+        check(x, [vocab // 3, 0], 3)
+        got = run(x, [vocab // 3, vocab - 1], 1)
+        assert np.all(got["logprob"] < 0) and np.all(got["entropy"] > 0)
+
+
+def test_extreme_logits():
+    x = np.full((4, 5000), -65504, np.float16)
+    x[1, 7] = 65504
+    x[2, ::2] = 65504
+    x[3] = 65504
+    check(x, [0, 7, 1, 4999], 9)
+
+
+def test_rows_without_any_id():
+    x = np.full((3, 700), -np.inf, np.float16)
+    x[1] = 1.0
+    for masked in (None, np.ones(700, bool)):
+        got = run(x, [0, 5, -1], 4, masked)
+        for r in range(3):
+            if masked is None and r == 1:
+                continue
+            assert got["logprob"][r] == -np.inf and got["entropy"][r] == 0
+            assert np.all(got["top_ids"][r] == -1) and np.all(got["top"][r] == -np.inf)
+    # masked ids and ids outside the vocabulary have no probability
+    masked = np.zeros(700, bool)
+    masked[5] = True
+    for i in (5, -1, 700, 2 ** 40, -2 ** 40):
+        assert run(x[1:2], [i], 0, masked)["logprob"][0] == -np.inf
+
+
+def test_minus_infinity_among_the_logits():
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((3, 2000)).astype(np.float16)
+    x[0, :1990] = -np.inf
+    x[1, 100:] = -np.inf
+    x[2, 5] = -np.inf
+    check(x, [1995, 3, 5], 20)
+
+
+def test_nan_and_infinity():
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((4, 3000)).astype(np.float16)
+    x[0, 1234] = np.nan
+    x[1, 17] = np.inf
+    x[2, 99] = -np.nan
+    got = run(x, [5, 17, 99, 5], 3)
+    for r in range(3):
+        assert np.isnan(got["logprob"][r]) and np.isnan(got["entropy"][r]) and np.isnan(got["top"][r]).all()
+    assert [got["top_ids"][r][0] for r in range(3)] == [1234, 17, 99]
+    assert np.isfinite(got["logprob"][3])
+    # masked, they do not count
+    masked = np.zeros(3000, bool)
+    masked[[1234, 17, 99]] = True
+    check(x, [5, 6, 7, 8], 20, masked)
+
+
+def test_outputs_that_are_not_wanted():
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((2, 500)).astype(np.float16)
+    both = run(x, [1, 2], 3)
+    for want in ((), ("logprob",), ("entropy",)):
+        got = run(x, [1, 2], 3, want=want)
+        np.testing.assert_array_equal(got["top"], both["top"])
+        for name in want:
+            np.testing.assert_array_equal(got[name], both[name])
+
+
+def test_rows_beyond_32_bits():
+    # the last row lies 4.3 G logits behind the first
+    vocab, ld, rows = 1000, 1 << 27, 33
+    rng = np.random.default_rng(4)
+    buf = torch.empty(ld * (rows - 1) + vocab, dtype=torch.float16, device="cuda")
+    x = rng.standard_normal((rows, vocab)).astype(np.float16)
+    for r in range(rows):
+        buf[r * ld:r * ld + vocab] = torch.from_numpy(x[r]).cuda()
+    ids = torch.arange(rows, device="cuda")
+    lp, ent = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    E.check(E.lib().ylm_k_logprobs(ptr(buf), ld, rows, vocab, ptr(ids), None, 0, ptr(lp), ptr(ent), None, None,
+                                   torch.cuda.current_stream().cuda_stream), "logprobs")
+    want, went, _, _ = R.logprobs(x.astype(np.float64), np.ones(vocab, bool))
+    np.testing.assert_allclose(lp.cpu().numpy(), want[np.arange(rows), np.arange(rows)], rtol=1e-5)
+    np.testing.assert_allclose(ent.cpu().numpy(), went, rtol=1e-5)
+
+
+def test_side_stream_and_captured_graph():
+    rng = np.random.default_rng(5)
+    x = torch.from_numpy(rng.standard_normal((3, 40000)).astype(np.float16)).cuda()
+    ids = torch.tensor([1, 2, 3], device="cuda")
+
+    def call(o, s):
+        E.check(E.lib().ylm_k_logprobs(ptr(x), 40000, 3, 40000, ptr(ids), None, 20, ptr(o[0]), ptr(o[1]), ptr(o[2]),
+                                       ptr(o[3]), s), "logprobs")
+
+    def outs():
+        return [torch.zeros(3, device="cuda"), torch.zeros(3, device="cuda"),
+                torch.zeros(3, 20, dtype=torch.int64, device="cuda"), torch.zeros(3, 20, device="cuda")]
+
+    want, got, cap = outs(), outs(), outs()
+    torch.cuda.synchronize()
+    call(want, torch.cuda.current_stream().cuda_stream)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    call(got, side.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(cap, torch.cuda.current_stream().cuda_stream)
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, got, cap):
+        assert torch.equal(a, b) and torch.equal(a, c)

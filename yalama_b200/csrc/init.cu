@@ -106,6 +106,10 @@ cudaError_t kernels_prepare()
         e = sample_prepare();
     if (e == cudaSuccess)
         e = gemm_tc_prepare();
+    if (e == cudaSuccess)
+        e = kv8_prepare();
+    if (e == cudaSuccess)
+        e = logprobs_prepare();
     return e;
 }
 

@@ -258,6 +258,60 @@ cudaError_t attn_prefill_tc_launch(const __half *q, const __half *k_cache, const
 cudaError_t attn_prefill_launch(const __half *q, const __half *k_cache, const __half *v_cache, int cap, int hq,
                                 int hkv, int T, __half *out, cudaStream_t s);
 
+// ------------------------------------------------------------------ 8-bit K/V cache
+struct Kv8Cache
+{
+    uint8_t *k, *v;           // [hkv][cap][128] codes
+    float *k_scale, *v_scale; // [hkv][ceil(cap / block)]
+    int format;               // 0 E4M3, 1 INT8
+    int block;                // tokens per scale: 16, 32, 64 or 128
+    int cap, hkv;
+};
+// rows [t] of k and v (token strides in halves) -> slots [slot, slot + t)
+cudaError_t kv8_store_launch(const Kv8Cache &c, const __half *k, const __half *v, int64_t k_stride, int64_t v_stride,
+                             int t, int slot, cudaStream_t s);
+struct Kv8AttnArgs
+{
+    Kv8Cache c;
+    const __half *q; // [t][hq * 128], token stride q_stride halves
+    int64_t q_stride;
+    int hq, t, n;
+    const uint32_t *mask; // bit per slot, 1 = hidden; or null
+    float *acc;           // [hkv][cap] or null
+    __half *out;
+    int64_t out_stride;
+};
+size_t kv8_attn_workspace(int hkv, int hq, int t, int n, bool acc, int num_sms);
+cudaError_t kv8_attn_launch(const Kv8AttnArgs &a, void *ws, int num_sms, cudaStream_t s);
+struct Kv8EvictArgs
+{
+    Kv8Cache src, dst;
+    const float *acc_src;
+    float *acc_dst;
+    int n, n_keep, n_sink, n_recent;
+    int32_t *kept;
+};
+cudaError_t kv8_evict_launch(const Kv8EvictArgs &a, cudaStream_t s);
+cudaError_t kv8_prepare();
+
+// ------------------------------------------------------------------ log probabilities
+struct LogprobArgs
+{
+    const __half *logits; // [rows][ld]
+    int64_t ld;
+    int rows;
+    int64_t vocab;
+    const int64_t *ids;        // [rows] or null
+    const uint32_t *mask_bits; // vocab bits, 1 = masked; or null
+    int n_top;                 // 0..64
+    float *logprob;            // [rows] or null
+    float *entropy;            // [rows] or null
+    int64_t *top_ids;          // [rows][n_top]
+    float *top_logprobs;
+};
+cudaError_t logprobs_launch(const LogprobArgs &a, int num_sms, cudaStream_t s);
+cudaError_t logprobs_prepare();
+
 // ------------------------------------------------------------------ init
 // dst[r * ld + c] = N(0, std) element ((row0 + r) * full_cols + col0 + c) of stream `key`
 cudaError_t fill_normal_launch(__half *dst, int64_t rows, int64_t cols, int64_t ld, uint64_t key, int64_t row0,

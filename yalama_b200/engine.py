@@ -104,6 +104,22 @@ class Sampling(ctypes.Structure):
     ]
 
 
+KV8_FORMATS = {"e4m3": 0, "int8": 1}
+
+
+class KV8Cache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("format", ctypes.c_int32),
+        ("block", ctypes.c_int32),
+        ("cap", ctypes.c_int32),
+        ("hkv", ctypes.c_int32),
+    ]
+
+
 class YlmError(RuntimeError):
     def __init__(self, status: int, where: str, message: str):
         self.status = Status(status) if status in Status._value2member_map_ else status
@@ -160,6 +176,18 @@ SIGNATURES = {
                                                       ctypes.c_int32, _P, _P]),
     "ylm_k_sample": (ctypes.c_int, [_P, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _P,
                                     ctypes.c_float, _I64P, _I64P, _F32P, _P]),
+    "ylm_k_kv8_store": (ctypes.c_int, [ctypes.POINTER(KV8Cache), _P, ctypes.c_int64, _P, ctypes.c_int64,
+                                       ctypes.c_int32, ctypes.c_int32, _P]),
+    "ylm_k_kv8_attention": (ctypes.c_int, [ctypes.POINTER(KV8Cache), _P, ctypes.c_int64, ctypes.c_int32,
+                                           ctypes.c_int32, ctypes.c_int32, _P, _P, _P, ctypes.c_int64, _P,
+                                           ctypes.c_size_t, _P]),
+    "ylm_k_kv8_attention_workspace": (ctypes.c_int, [ctypes.POINTER(KV8Cache), ctypes.c_int32, ctypes.c_int32,
+                                                     ctypes.c_int32, ctypes.c_int32,
+                                                     ctypes.POINTER(ctypes.c_size_t)]),
+    "ylm_k_kv8_evict": (ctypes.c_int, [ctypes.POINTER(KV8Cache), ctypes.POINTER(KV8Cache), _P, _P, ctypes.c_int32,
+                                       ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P, _P]),
+    "ylm_k_logprobs": (ctypes.c_int, [_P, ctypes.c_int64, ctypes.c_int32, ctypes.c_int64, _P, _P, ctypes.c_int32,
+                                      _P, _P, _P, _P, _P]),
 }
 
 
@@ -202,6 +230,20 @@ def _i64(a) -> np.ndarray:
 
 def _ptr(a: np.ndarray, t):
     return a.ctypes.data_as(ctypes.POINTER(t))
+
+
+def kv8_cache(k: int, v: int, k_scale: int, v_scale: int, fmt: str, block: int, cap: int, hkv: int) -> KV8Cache:
+    """Descriptor of an 8-bit K/V cache from device pointers (``fmt``: "e4m3" or "int8"); the buffers stay the
+    caller's and must outlive the calls that use it."""
+    return KV8Cache(k, v, k_scale, v_scale, KV8_FORMATS[fmt], block, cap, hkv)
+
+
+def kv8_attention_workspace(cache: KV8Cache, hq: int, t: int, n: int, with_acc: bool) -> int:
+    """Bytes of device workspace for ``ylm_k_kv8_attention`` with these arguments (and for every smaller ``n``)."""
+    b = ctypes.c_size_t()
+    check(lib().ylm_k_kv8_attention_workspace(ctypes.byref(cache), hq, t, n, int(with_acc), ctypes.byref(b)),
+          "ylm_k_kv8_attention_workspace")
+    return b.value
 
 
 def config_from_spec(spec) -> ModelConfig:
