@@ -26,11 +26,13 @@ namespace ylm {
 
 namespace cg = cooperative_groups;
 
-constexpr int LGP_THREADS = 512;
+constexpr int LGP_THREADS = 256;
 constexpr int LGP_WARPS = LGP_THREADS / 32;
 constexpr int LGP_U = 4;      // 16-byte loads in flight per thread
 constexpr int LGP_CAP = 512;  // collected candidates per CTA
 constexpr int LGP_TOP = 64;   // largest n_top
+constexpr int LGP_MAXC = 8;   // largest cluster (the portable size)
+constexpr int LGP_FILL = 3;   // rows are split until there are so many CTAs per SM
 constexpr uint32_t LGP_LOWEST = 0x0400u; // ord16 of the lowest finite value: what lies below is -inf
 
 // Running (max, z, w): z = sum e^(x - m) without one maximal element, w = sum e^(x - m) (m - x).
@@ -64,6 +66,32 @@ __device__ __forceinline__ float lgp_ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float x, float y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 
 // Key of an alternative: NaN above everything, then the value (-0 as +0), then the lower id.
@@ -121,30 +149,87 @@ struct LgpRow
 struct LgpShared
 {
     LseState st[LGP_WARPS];
-    LseState part;            // this CTA's
-    int n_top;                // candidates in top
-    int count;                // collected
+    LseState parts[LGP_MAXC]; // rank 0: every CTA's
+    int n_top;                // keys in top
+    int counts[LGP_MAXC];     // rank 0: keys in every CTA's top
+    int count;                // keys in cand
     int scan[LGP_WARPS];
     int hist[256];
     int sel[2];
-    uint64_t top[LGP_TOP];    // this CTA's best, best first
-    uint64_t cand[LGP_CAP];   // collected; in rank 0 of a cluster, later every CTA's best
+    uint32_t T;
+    bool nan, low;
+    uint16_t most[LGP_THREADS];         // each thread's largest value (ord16)
+    uint64_t top[LGP_TOP];              // the best, best first
+    alignas(16) uint64_t cand[LGP_CAP]; // collected keys
+    uint64_t lists[LGP_MAXC * LGP_TOP + LGP_TOP]; // rank 0: every CTA's best, 0 behind its last (and room to read past)
+    uint16_t owners[LGP_THREADS];       // threads with candidates
+    int n_owners;
 };
 
-// sh.cand[0, m) ranked into sh.top[0, min(m, n)): a key's place is the number of larger ones (keys are distinct)
+// sh.cand[0, m) ranked into sh.top[0, min(n, m)): a key's place is the number of
+// larger ones (the keys are distinct).
 __device__ __forceinline__ void lgp_rank(LgpShared &sh, int m, int n)
 {
+    const int pairs = (m + 1) / 2;
+    if (threadIdx.x == 0)
+    {
+        sh.n_top = min(m, n);
+        if (m & 1)
+            sh.cand[m] = 0;
+    }
+    __syncthreads();
+    const ulonglong2 *two = reinterpret_cast<const ulonglong2 *>(sh.cand);
     for (int i = threadIdx.x; i < m; i += LGP_THREADS)
     {
         const uint64_t k = sh.cand[i];
         int r = 0;
-        for (int j = 0; j < m; j++)
-            r += sh.cand[j] > k;
+#pragma unroll 8
+        for (int j = 0; j < pairs; j++)
+        {
+            const ulonglong2 t = two[j];
+            r += (t.x > k) + (t.y > k);
+        }
         if (r < n)
             sh.top[r] = k;
     }
-    if (threadIdx.x == 0)
-        sh.n_top = min(m, n);
+}
+
+// The C lists of n keys in sh.lists, each best first with 0 behind its last,
+// merged into sh.top: a key's place is the number of larger keys in every list (its
+// own index in its own), found by bisection, one step of all lists at a time.
+__device__ __forceinline__ void lgp_merge(LgpShared &sh, int C, int n)
+{
+    const int steps = 32 - __clz(n);
+    for (int i = threadIdx.x; i < C * n; i += LGP_THREADS)
+    {
+        const uint64_t k = sh.lists[i];
+        if (!k)
+            continue;
+        int lo[LGP_MAXC], hi[LGP_MAXC]; // keys [0, lo) of a list are larger than k, [hi, n) are not
+#pragma unroll
+        for (int c = 0; c < LGP_MAXC; c++)
+        {
+            lo[c] = 0;
+            hi[c] = c < C ? n : 0;
+        }
+        for (int step = 0; step < steps; step++)
+        {
+#pragma unroll
+            for (int c = 0; c < LGP_MAXC; c++)
+            {
+                const int mid = (lo[c] + hi[c]) >> 1;
+                const bool open = lo[c] < hi[c], more = open && sh.lists[c * n + mid] > k;
+                hi[c] = open && !more ? mid : hi[c];
+                lo[c] = more ? mid + 1 : lo[c];
+            }
+        }
+        int r = 0;
+#pragma unroll
+        for (int c = 0; c < LGP_MAXC; c++)
+            r += lo[c];
+        if (r < n)
+            sh.top[r] = k;
+    }
 }
 
 // The n best of vectors [v0, v1) by two 8-bit radix steps, whatever their
@@ -228,7 +313,31 @@ __device__ void lgp_select(const LgpRow &row, int v0, int v1, int n, LgpShared &
     }
 }
 
-__global__ void __launch_bounds__(LGP_THREADS, 2) logprobs_kernel(LogprobArgs a)
+// The warps' states joined (in warp 0, which sh.nan and sh.low describe to all).
+__device__ __forceinline__ LseState lgp_block(LseState s, LgpShared &sh)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncthreads();
+    if (lane == 0)
+        sh.st[warp] = s;
+    __syncthreads();
+    if (warp == 0)
+    {
+        s = lane < LGP_WARPS ? sh.st[lane] : LseState{-INFINITY, 0.f, 0.f};
+        for (int o = LGP_WARPS / 2; o > 0; o >>= 1)
+            s = lse_merge(s, LseState{__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.z, o),
+                                      __shfl_xor_sync(0xffffffffu, s.w, o)});
+        if (lane == 0)
+        {
+            sh.nan = s.z != s.z;
+            sh.low = s.m < -65000.f;
+        }
+    }
+    __syncthreads();
+    return s;
+}
+
+__global__ void __launch_bounds__(LGP_THREADS, 4) logprobs_kernel(LogprobArgs a)
 {
     __shared__ LgpShared sh;
     const int C = (int)gridDim.x, rank = (int)blockIdx.x;
@@ -236,6 +345,10 @@ __global__ void __launch_bounds__(LGP_THREADS, 2) logprobs_kernel(LogprobArgs a)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (ri >= a.rows) // the whole cluster: blockIdx.x is the rank in it
         return;
+    // the other CTAs write into rank 0's shared memory once all have started:
+    // arrive now, wait before the first such write
+    if (C > 1)
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     LgpRow row;
     row.x = a.logits + ri * a.ld;
     row.bits = a.mask_bits;
@@ -244,10 +357,27 @@ __global__ void __launch_bounds__(LGP_THREADS, 2) logprobs_kernel(LogprobArgs a)
     const int nv = (int)((a.vocab + row.off + 7) / 8), per = (nv + C - 1) / C;
     const int v0 = min(nv, rank * per), v1 = min(nv, v0 + per);
 
-    // ---- one pass: the warp's reference m, this thread's z, w and largest value
-    LseState s = {-INFINITY, 0.f, 0.f};
-    float ref = 0.f; // m, or 0 while there is none
-    __half2 tmax2 = __half2half2(__ushort_as_half(0xFC00u));
+    // the given id's logit, early: two dependent loads
+    bool has_given = false;
+    float given = 0.f;
+    if (rank == 0 && tid == 0 && a.logprob)
+    {
+        const int64_t id = a.ids[ri];
+        has_given = id >= 0 && id < a.vocab && !(a.mask_bits && (a.mask_bits[id >> 5] >> (id & 31) & 1u));
+        given = has_given ? h2f(row.x[id]) : 0.f;
+    }
+
+    // ---- one pass. Terms are 2^t, t = x L - c with L = log2 e and c = m L rounded
+    // (one multiply-add an element, whatever the size of m); c's rounding error
+    // d = m L - c, the t of the maximum itself, is taken out at the end. Per
+    // thread z' = sum 2^t and w' = sum 2^t t, per warp m. Logits below the lowest
+    // finite one count as that here: their terms vanish unless m is as low.
+    constexpr float L = 1.4426950408889634f;
+    const __half2 lowest = __half2half2(__ushort_as_half(0xFBFFu));
+    const uint64_t L2 = pack2(L, L);
+    float m = -INFINITY, c = 0.f, delta = 0.f;
+    uint64_t z2 = pack2(0.f, 0.f), w2 = z2, c2 = z2;
+    __half2 tmax2 = lowest;
     for (int v = v0 + tid; v - lane < v1; v += LGP_THREADS * LGP_U)
     {
         uint4 r[LGP_U];
@@ -255,114 +385,166 @@ __global__ void __launch_bounds__(LGP_THREADS, 2) logprobs_kernel(LogprobArgs a)
         for (int u = 0; u < LGP_U; u++)
             r[u] = v + u * LGP_THREADS < v1 ? row.load(v + u * LGP_THREADS)
                                             : make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
-        const __half2 *h = reinterpret_cast<const __half2 *>(r);
-        __half2 um = h[0];
+        __half2 *h = reinterpret_cast<__half2 *>(r);
+        __half2 um = lowest;
 #pragma unroll
-        for (int i = 1; i < 4 * LGP_U; i++)
+        for (int i = 0; i < 4 * LGP_U; i++)
+        {
+            h[i] = __hmax2_nan(h[i], lowest);
             um = __hmax2(um, h[i]);
-        um = __hmax2(um, __half2half2(__ushort_as_half(0xFC00u))); // NaN only: -inf
+        }
         tmax2 = __hmax2(tmax2, um);
         const uint32_t mine = ord16(__half_as_ushort(__hmax(__low2half(um), __high2half(um))));
-        const float top = h2f(__ushort_as_half((unsigned short)unord16(__reduce_max_sync(0xffffffffu, mine))));
+        const uint32_t most = __reduce_max_sync(0xffffffffu, mine);
+        const float top = h2f(__ushort_as_half((unsigned short)unord16(most)));
         bool skip = false; // this lane leaves out one element equal to the new maximum
-        if (top > s.m)
+        if (top > m)
         {
-            const uint32_t has = __ballot_sync(0xffffffffu, unord16(mine) == __half_as_ushort(__float2half_rn(top)));
-            skip = lane == __ffs(has) - 1;
-            // what was summed so far, with the former maximum, which lane `owner` alone counts
-            const bool counted = s.m != -INFINITY && lane == 0;
-            const float d = top - (s.m == -INFINITY ? top : s.m), f = lgp_ex2(-d * 1.4426950408889634f);
-            const float zo = s.z + (counted ? 1.f : 0.f);
-            s.w = (s.w + zo * d) * f;
-            s.z = zo * f;
-            s.m = ref = top;
+            skip = lane == __ffs(__ballot_sync(0xffffffffu, mine == most)) - 1;
+            const float2 zz = unpack2(z2), ww = unpack2(w2);
+            const float cn = top * L, dn = fmaf(top, L, -cn);
+            if (m > -INFINITY)
+            {
+                // the sums so far, with the former maximum that lane 0 counts, in the new unit
+                const float own = lane == 0 ? lgp_ex2(delta) : 0.f, shift = c - cn, f = lgp_ex2(shift);
+                const float z = zz.x + zz.y + own;
+                z2 = pack2(z * f, 0.f);
+                w2 = pack2((ww.x + ww.y + own * delta + z * shift) * f, 0.f);
+            }
+            m = top;
+            c = cn;
+            delta = dn;
+            c2 = pack2(-c, -c);
         }
         if (skip)
         {
+            float z = 0.f, w = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4 * LGP_U; i++)
+            for (int i = 0; i < 8 * LGP_U; i++)
             {
-                const float2 f = __half22float2(h[i]);
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-                {
-                    const float x = j ? f.y : f.x;
-                    if (skip && x == top)
-                    {
-                        skip = false;
-                        continue;
-                    }
-                    const float d = x - ref, e = lgp_ex2(d * 1.4426950408889634f);
-                    s.z += e;
-                    s.w -= e * fmaxf(d, -200.f);
-                }
+                const float x = h2f(i & 1 ? __high2half(h[i >> 1]) : __low2half(h[i >> 1]));
+                const float t = fmaf(x, L, -c), e = skip && x == m ? 0.f : lgp_ex2(t);
+                skip = skip && x != m;
+                z += e;
+                w += e * t;
             }
+            z2 = add2(z2, pack2(z, 0.f));
+            w2 = add2(w2, pack2(w, 0.f));
         }
         else
         {
 #pragma unroll
             for (int i = 0; i < 4 * LGP_U; i++)
             {
-                const float2 f = __half22float2(h[i]);
-                // d: -inf, far below any e > 0, would make 0 * -inf of the entropy's term
-                const float d0 = f.x - ref, d1 = f.y - ref;
-                const float e0 = lgp_ex2(d0 * 1.4426950408889634f), e1 = lgp_ex2(d1 * 1.4426950408889634f);
-                s.z += e0 + e1;
-                s.w -= e0 * fmaxf(d0, -200.f) + e1 * fmaxf(d1, -200.f);
+                const float2 x = __half22float2(h[i]);
+                const uint64_t t = fma2(pack2(x.x, x.y), L2, c2);
+                const float2 tf = unpack2(t);
+                const uint64_t e = pack2(lgp_ex2(tf.x), lgp_ex2(tf.y));
+                z2 = add2(z2, e);
+                w2 = fma2(e, t, w2);
             }
         }
     }
-    // the warp's sum (its one left-out maximum stays out), then the CTA's
-    for (int o = 16; o > 0; o >>= 1)
+    LseState s;
     {
-        s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
-        s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+        const float2 zz = unpack2(z2), ww = unpack2(w2);
+        float z = zz.x + zz.y, w = ww.x + ww.y;
+        for (int o = 16; o > 0; o >>= 1)
+        {
+            z += __shfl_xor_sync(0xffffffffu, z, o);
+            w += __shfl_xor_sync(0xffffffffu, w, o);
+        }
+        const float f = lgp_ex2(-delta);
+        s = LseState{m, z * f, -0.69314718055994531f * (w - delta * z) * f};
     }
-    if (lane == 0)
-        sh.st[warp] = s;
+    s = lgp_block(s, sh);
     if (tid == 0)
         sh.count = 0;
-    const bool nan = __syncthreads_or(s.z != s.z);
-    if (warp == 0)
+    const bool nan = sh.nan;
+    if (sh.low) // uniform: an empty part, or one whose logits are as low as what stood in for -inf
     {
-        LseState t = lane < LGP_WARPS ? sh.st[lane] : LseState{-INFINITY, 0.f, 0.f};
-        for (int o = LGP_WARPS / 2; o > 0; o >>= 1)
+        LseState t = {-INFINITY, 0.f, 0.f};
+        for (int v = v0 + tid; v < v1; v += LGP_THREADS)
+        {
+            const uint4 r = row.load(v);
+            const __half2 *h = reinterpret_cast<const __half2 *>(&r);
+#pragma unroll 1
+            for (int i = 0; i < 8; i++)
+            {
+                const float x = h2f(i & 1 ? __high2half(h[i >> 1]) : __low2half(h[i >> 1]));
+                t = x != x ? LseState{t.m, x, x} : x > -INFINITY ? lse_merge(t, LseState{x, 0.f, 0.f}) : t;
+            }
+        }
+        for (int o = 16; o > 0; o >>= 1)
             t = lse_merge(t, LseState{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.z, o),
                                       __shfl_xor_sync(0xffffffffu, t.w, o)});
-        if (lane == 0)
-            sh.part = t;
+        s = lgp_block(t, sh);
     }
 
     // ---- this CTA's best ids
     if (a.n_top)
     {
         const uint32_t mine = lgp_ord(__half_as_ushort(__hmax(__low2half(tmax2), __high2half(tmax2))));
-        uint32_t T = 0;
         bool whole = nan;
         if (!whole)
         {
-#pragma unroll 1
-            for (int b = 15; b >= 0; b--) // the largest T that n_top threads reach
-                if (__syncthreads_count(mine >= (T | 1u << b)) >= a.n_top)
-                    T |= 1u << b;
-            T = max(T, LGP_LOWEST);
-            for (uint32_t left = __ballot_sync(0xffffffffu, mine >= T); left; left &= left - 1)
+            // the largest T that n_top threads reach, bit by bit, by one warp
+            sh.most[tid] = (uint16_t)mine;
+            __syncthreads();
+            if (warp == 0)
             {
-                const int owner = warp * 32 + __ffs(left) - 1;
-                for (int v = v0 + owner + lane * LGP_THREADS; v < v1; v += 32 * LGP_THREADS)
-                {
-                    const uint4 r = row.load(v);
-                    const uint32_t *p = reinterpret_cast<const uint32_t *>(&r);
+                uint32_t v[LGP_WARPS];
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
+                for (int i = 0; i < LGP_WARPS; i++)
+                    v[i] = sh.most[i * 32 + lane];
+                uint32_t T = 0;
+                // to 12 bits: a lower T only lets a few more candidates in
+#pragma unroll 1
+                for (int b = 15; b >= 4; b--)
+                {
+                    int n = 0;
+#pragma unroll
+                    for (int i = 0; i < LGP_WARPS; i++)
+                        n += v[i] >= (T | 1u << b);
+                    if (__reduce_add_sync(0xffffffffu, n) >= a.n_top)
+                        T |= 1u << b;
+                }
+                T = max(T, LGP_LOWEST);
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < LGP_WARPS; i++)
+                {
+                    const uint32_t has = __ballot_sync(0xffffffffu, v[i] >= T);
+                    if (v[i] >= T)
+                        sh.owners[n + __popc(has & ((1u << lane) - 1u))] = (uint16_t)(i * 32 + lane);
+                    n += __popc(has);
+                }
+                if (lane == 0)
+                {
+                    sh.T = T;
+                    sh.n_owners = n;
+                }
+            }
+            __syncthreads();
+            // the owners' vectors again, dealt out over the CTA: consecutive threads take consecutive owners
+            const uint32_t T = sh.T;
+            const int n_owners = sh.n_owners, total = n_owners * ((v1 - v0 + LGP_THREADS - 1) / LGP_THREADS);
+            for (int i = tid; i < total; i += LGP_THREADS)
+            {
+                const int k = i / n_owners, v = v0 + k * LGP_THREADS + sh.owners[i - k * n_owners];
+                if (v >= v1)
+                    continue;
+                const uint4 r = row.load(v);
+                const uint32_t *p = reinterpret_cast<const uint32_t *>(&r);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                {
+                    const uint32_t o = lgp_ord(p[j >> 1] >> (16 * (j & 1)) & 0xFFFFu);
+                    if (o >= T)
                     {
-                        const uint32_t o = lgp_ord(p[i >> 1] >> (16 * (i & 1)) & 0xFFFFu);
-                        if (o >= T)
-                        {
-                            const int at = atomicAdd(&sh.count, 1);
-                            if (at < LGP_CAP)
-                                sh.cand[at] = make_key(o, (uint32_t)(8 * v - row.off + i));
-                        }
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < LGP_CAP)
+                            sh.cand[at] = make_key(o, (uint32_t)(8 * v - row.off + j));
                     }
                 }
             }
@@ -374,71 +556,80 @@ __global__ void __launch_bounds__(LGP_THREADS, 2) logprobs_kernel(LogprobArgs a)
         __syncthreads();
         lgp_rank(sh, sh.count, a.n_top);
     }
-    __syncthreads();
 
     // ---- rank 0 joins the parts and writes the row
     cg::cluster_group cl = cg::this_cluster();
+    __syncthreads();
     if (C > 1)
-        cl.sync();
-    if (rank == 0)
     {
-        LseState t = sh.part;
-        for (int c = 1; c < C; c++)
-            t = lse_merge(t, *cl.map_shared_rank(&sh.part, c));
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (tid == 0)
+        {
+            *cl.map_shared_rank(&sh.parts[rank], 0) = s;
+            *cl.map_shared_rank(&sh.counts[rank], 0) = a.n_top ? sh.n_top : 0;
+        }
+        if (tid < a.n_top)
+            *cl.map_shared_rank(&sh.lists[rank * a.n_top + tid], 0) = tid < sh.n_top ? sh.top[tid] : 0ull;
+        cl.sync();
+        if (rank != 0)
+            return;
+        if (a.n_top)
+        {
+            lgp_merge(sh, C, a.n_top);
+            __syncthreads();
+        }
+    }
+    else
+    {
+        if (tid == 0)
+        {
+            sh.parts[0] = s;
+            sh.counts[0] = sh.n_top;
+        }
+        __syncthreads();
+    }
+    if (warp < 2) // the row's state, and a lane for each alternative
+    {
+        LseState t = lane < C ? sh.parts[lane] : LseState{-INFINITY, 0.f, 0.f};
+        int found = lane < C ? sh.counts[lane] : 0;
+#pragma unroll
+        for (int o = LGP_MAXC / 2; o > 0; o >>= 1)
+        {
+            t = lse_merge(t, LseState{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.z, o),
+                                      __shfl_xor_sync(0xffffffffu, t.w, o)});
+            found += __shfl_xor_sync(0xffffffffu, found, o);
+        }
+        // lanes 0..7 hold the join, which every lane takes from lane 0
+        t.m = __shfl_sync(0xffffffffu, t.m, 0);
+        t.z = __shfl_sync(0xffffffffu, t.z, 0);
+        t.w = __shfl_sync(0xffffffffu, t.w, 0);
+        found = __shfl_sync(0xffffffffu, found, 0);
         const bool bad = t.z != t.z || t.m == INFINITY;
-        const bool none = t.m == -INFINITY && !bad;
         const float lz = bad ? NAN : log1pf(t.z);
         if (tid == 0 && a.logprob)
         {
-            const int64_t id = a.ids[ri];
-            float lp = -INFINITY;
-            if (id >= 0 && id < a.vocab && !(a.mask_bits && (a.mask_bits[id >> 5] >> (id & 31) & 1u)))
-            {
-                const float x = h2f(row.x[id]);
-                lp = bad ? NAN : x == -INFINITY ? -INFINITY : (x - t.m) - lz;
-            }
-            a.logprob[ri] = lp;
+            const float x = given;
+            a.logprob[ri] = !has_given ? -INFINITY : bad ? NAN : x == -INFINITY ? -INFINITY : (x - t.m) - lz;
         }
         if (tid == 0 && a.entropy)
-            a.entropy[ri] = bad ? NAN : none ? 0.f : lz + t.w / (1.f + t.z);
-        if (a.n_top)
+            a.entropy[ri] = bad ? NAN : lz + t.w / (1.f + t.z); // no id at all: 0
+        if (tid < a.n_top)
         {
-            if (C > 1)
-            {
-                // the parts' lists side by side (at most 8 x 64), ranked again
-                int m = 0;
-                for (int c = 0; c < C; c++)
-                {
-                    const int k = *cl.map_shared_rank(&sh.n_top, c);
-                    const uint64_t *from = cl.map_shared_rank(&sh.top[0], c);
-                    for (int i = tid; i < k; i += LGP_THREADS)
-                        sh.cand[m + i] = from[i];
-                    m += k;
-                }
-                __syncthreads();
-                lgp_rank(sh, m, a.n_top);
-                __syncthreads();
-            }
-            if (tid < a.n_top)
-            {
-                const bool is = tid < sh.n_top;
-                const uint64_t key = is ? sh.top[tid] : 0;
-                const float x = h2f(__ushort_as_half((unsigned short)unord16((uint32_t)(key >> 32))));
-                a.top_ids[ri * a.n_top + tid] = is ? (int64_t)key_idx(key) : -1;
-                a.top_logprobs[ri * a.n_top + tid] = !is ? -INFINITY : bad ? NAN : (x - t.m) - lz;
-            }
+            const bool is = tid < found;
+            const uint64_t key = is ? sh.top[tid] : 0;
+            const float x = h2f(__ushort_as_half((unsigned short)unord16((uint32_t)(key >> 32))));
+            a.top_ids[ri * a.n_top + tid] = is ? (int64_t)key_idx(key) : -1;
+            a.top_logprobs[ri * a.n_top + tid] = !is ? -INFINITY : bad ? NAN : (x - t.m) - lz;
         }
     }
-    if (C > 1)
-        cl.sync(); // the parts stay until rank 0 has read them
 }
 
 cudaError_t logprobs_launch(const LogprobArgs &a, int num_sms, cudaStream_t s)
 {
     if (a.rows <= 0)
         return cudaSuccess;
-    int C = 8;
-    while (C > 1 && (int64_t)a.rows * (C / 2) >= 4 * num_sms)
+    int C = LGP_MAXC;
+    while (C > 1 && (int64_t)a.rows * (C / 2) >= LGP_FILL * num_sms)
         C /= 2;
     cudaLaunchConfig_t cfg = {};
     const unsigned y = (unsigned)std::min(a.rows, 32768);
