@@ -68,32 +68,6 @@ __device__ __forceinline__ float lgp_ex2(float x)
     return y;
 }
 
-// Two FP32 operations in one instruction.
-__device__ __forceinline__ uint64_t pack2(float x, float y)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 // Key of an alternative: NaN above everything, then the value (-0 as +0), then the lower id.
 __device__ __forceinline__ uint32_t lgp_ord(uint32_t u)
 {
@@ -337,7 +311,7 @@ __device__ __forceinline__ LseState lgp_block(LseState s, LgpShared &sh)
     return s;
 }
 
-__global__ void __launch_bounds__(LGP_THREADS, 4) logprobs_kernel(LogprobArgs a)
+__global__ void __launch_bounds__(LGP_THREADS, 5) logprobs_kernel(LogprobArgs a)
 {
     __shared__ LgpShared sh;
     const int C = (int)gridDim.x, rank = (int)blockIdx.x;
@@ -374,17 +348,27 @@ __global__ void __launch_bounds__(LGP_THREADS, 4) logprobs_kernel(LogprobArgs a)
     // finite one count as that here: their terms vanish unless m is as low.
     constexpr float L = 1.4426950408889634f;
     const __half2 lowest = __half2half2(__ushort_as_half(0xFBFFu));
-    const uint64_t L2 = pack2(L, L);
     float m = -INFINITY, c = 0.f, delta = 0.f;
-    uint64_t z2 = pack2(0.f, 0.f), w2 = z2, c2 = z2;
+    float2 z = make_float2(0.f, 0.f), w = z; // two of each, for the two halves of a pair
     __half2 tmax2 = lowest;
+    const int inner = min(v1, nv - 1); // vectors (0, inner) lie in the row whole
     for (int v = v0 + tid; v - lane < v1; v += LGP_THREADS * LGP_U)
     {
         uint4 r[LGP_U];
+        const int first = v - lane, last = first + 31 + (LGP_U - 1) * LGP_THREADS; // the warp's vectors
+        if (!row.bits && first > 0 && last < inner)
+        {
 #pragma unroll
-        for (int u = 0; u < LGP_U; u++)
-            r[u] = v + u * LGP_THREADS < v1 ? row.load(v + u * LGP_THREADS)
-                                            : make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
+            for (int u = 0; u < LGP_U; u++)
+                r[u] = __ldg(reinterpret_cast<const uint4 *>(row.x + (8 * v - row.off)) + u * LGP_THREADS);
+        }
+        else
+        {
+#pragma unroll
+            for (int u = 0; u < LGP_U; u++)
+                r[u] = v + u * LGP_THREADS < v1 ? row.load(v + u * LGP_THREADS)
+                                                : make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
+        }
         __half2 *h = reinterpret_cast<__half2 *>(r);
         __half2 um = lowest;
 #pragma unroll
@@ -397,65 +381,51 @@ __global__ void __launch_bounds__(LGP_THREADS, 4) logprobs_kernel(LogprobArgs a)
         const uint32_t mine = ord16(__half_as_ushort(__hmax(__low2half(um), __high2half(um))));
         const uint32_t most = __reduce_max_sync(0xffffffffu, mine);
         const float top = h2f(__ushort_as_half((unsigned short)unord16(most)));
-        bool skip = false; // this lane leaves out one element equal to the new maximum
         if (top > m)
         {
-            skip = lane == __ffs(__ballot_sync(0xffffffffu, mine == most)) - 1;
-            const float2 zz = unpack2(z2), ww = unpack2(w2);
+            // the former maximum, which lane 0 counts, joins the sums, in the new unit
             const float cn = top * L, dn = fmaf(top, L, -cn);
             if (m > -INFINITY)
             {
-                // the sums so far, with the former maximum that lane 0 counts, in the new unit
                 const float own = lane == 0 ? lgp_ex2(delta) : 0.f, shift = c - cn, f = lgp_ex2(shift);
-                const float z = zz.x + zz.y + own;
-                z2 = pack2(z * f, 0.f);
-                w2 = pack2((ww.x + ww.y + own * delta + z * shift) * f, 0.f);
+                z.x += own;
+                w.x = (w.x + own * delta + z.x * shift) * f;
+                w.y = (w.y + z.y * shift) * f;
+                z.x *= f;
+                z.y *= f;
             }
             m = top;
             c = cn;
             delta = dn;
-            c2 = pack2(-c, -c);
-        }
-        if (skip)
-        {
-            float z = 0.f, w = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8 * LGP_U; i++)
+            // one element equal to the new one is left out: it becomes the lowest value
+            if (lane == __ffs(__ballot_sync(0xffffffffu, mine == most)) - 1)
             {
-                const float x = h2f(i & 1 ? __high2half(h[i >> 1]) : __low2half(h[i >> 1]));
-                const float t = fmaf(x, L, -c), e = skip && x == m ? 0.f : lgp_ex2(t);
-                skip = skip && x != m;
-                z += e;
-                w += e * t;
-            }
-            z2 = add2(z2, pack2(z, 0.f));
-            w2 = add2(w2, pack2(w, 0.f));
-        }
-        else
-        {
+                const __half th = __float2half_rn(top), low = __ushort_as_half(0xFBFFu);
+                bool open = true;
 #pragma unroll
-            for (int i = 0; i < 4 * LGP_U; i++)
-            {
-                const float2 x = __half22float2(h[i]);
-                const uint64_t t = fma2(pack2(x.x, x.y), L2, c2);
-                const float2 tf = unpack2(t);
-                const uint64_t e = pack2(lgp_ex2(tf.x), lgp_ex2(tf.y));
-                z2 = add2(z2, e);
-                w2 = fma2(e, t, w2);
+                for (int i = 0; i < 4 * LGP_U; i++)
+                {
+                    const bool x = open && __heq(__low2half(h[i]), th), y = open && !x && __heq(__high2half(h[i]), th);
+                    h[i] = __halves2half2(x ? low : __low2half(h[i]), y ? low : __high2half(h[i]));
+                    open = open && !x && !y;
+                }
             }
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * LGP_U; i++)
+        {
+            const float2 x = __half22float2(h[i]);
+            const float t0 = fmaf(x.x, L, -c), t1 = fmaf(x.y, L, -c), e0 = lgp_ex2(t0), e1 = lgp_ex2(t1);
+            z.x += e0;
+            z.y += e1;
+            w.x = fmaf(e0, t0, w.x);
+            w.y = fmaf(e1, t1, w.y);
         }
     }
     LseState s;
     {
-        const float2 zz = unpack2(z2), ww = unpack2(w2);
-        float z = zz.x + zz.y, w = ww.x + ww.y;
-        for (int o = 16; o > 0; o >>= 1)
-        {
-            z += __shfl_xor_sync(0xffffffffu, z, o);
-            w += __shfl_xor_sync(0xffffffffu, w, o);
-        }
-        const float f = lgp_ex2(-delta);
-        s = LseState{m, z * f, -0.69314718055994531f * (w - delta * z) * f};
+        const float zs = warp_sum(z.x + z.y), ws = warp_sum(w.x + w.y), f = lgp_ex2(-delta);
+        s = LseState{m, zs * f, -0.69314718055994531f * (ws - delta * zs) * f};
     }
     s = lgp_block(s, sh);
     if (tid == 0)
