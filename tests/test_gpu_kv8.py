@@ -271,6 +271,31 @@ def test_attention_rows_that_see_nothing_are_zero(t, n):
     np.testing.assert_allclose(got[-1].float().cpu().numpy(), want, rtol=2.0 ** -10, atol=1e-7)
 
 
+@pytest.mark.parametrize("hq,t,n", [(2, 5, 100), (8, 3, 64), (8, 9, 33), (4, 40, 130)])
+def test_attention_nan_of_a_later_token_stays_out_of_the_earlier_ones(hq, t, n):
+    # NaN in a key makes every output of the tokens that see it NaN, NaN in a value that dimension of theirs
+    rng = np.random.default_rng(n)
+    hkv = 2
+    k, v = rows(rng, n, hkv, 0.4), rows(rng, n, hkv, 0.4)
+    v[n - 3, 0, 17] = v[n - 1, 1, 100] = v[n - 2, 1, 3] = np.nan
+    k[n - 1, 0, 50] = np.nan
+    c = DeviceCache("e4m3", 16, n + 20, hkv)
+    c.store(half(k), half(v), 0)
+    ref = R.Cache("e4m3", 16, n + 20, hkv)
+    ref.store(k.astype(np.float64), v.astype(np.float64), 0)
+    q = rng.standard_normal((t, hq, D)).astype(np.float16)
+    kv, vv = ref.values("k", n), ref.values("v", n)
+    out, _, pv, mag = R.attention(q.astype(np.float64), np.nan_to_num(kv), np.nan_to_num(vv), t, np.zeros(n, bool))
+    bad = np.zeros((t, hq, D), bool)
+    G = hq // hkv
+    bad[t - 3:, :G, 17] = bad[t - 1:, G:, 100] = bad[t - 2:, G:, 3] = True
+    bad[t - 1, :G] = True
+    got = attend(c, half(q), t, n).float().cpu().numpy().reshape(out.shape)
+    np.testing.assert_array_equal(np.isnan(got), bad)
+    tol, _ = bounds(out, pv, mag, None)
+    assert np.all((np.abs(got - out) <= tol)[~bad])
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("sharp", [1.0, 30.0])
 def test_attention_values_of_very_different_scales(fmt, sharp):

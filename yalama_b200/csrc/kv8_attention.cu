@@ -5,23 +5,34 @@
 //   acc[head][j] += sum of softmax(x_r)_j over the rows r of the KV head
 // Row r = i * G + h of a KV head is query head h of its group, token i; token i
 // sees slots [0, n - t + i]. Scores are kept in base 2 (x * log2 e).
+//
+// Two launches: kv8_attn_kernel splits the slots over CTAs (a decode step has too
+// few rows to fill the GPU otherwise) and leaves per split and row the sums
+// (M, l, O); kv8_join_kernel joins the splits and, where asked, turns the scores
+// that the first launch kept into weights.
 #include "kv8.cuh"
 #include <algorithm>
 
 namespace ylm {
 
 constexpr int KVA_THREADS = 128;
-constexpr int KVA_ACC_TILE = 256; // slots per CTA of the accumulation
+constexpr int KVA_WARPS = KVA_THREADS / 32;
+constexpr int KVA_CHUNK = 32;     // slots a warp takes at a time
+constexpr int KVA_JOIN = 128;     // threads of the joining CTAs
+constexpr int KVA_ACC_TILE = 128; // slots per CTA of the accumulation
 
 struct Kv8Plan
 {
-    int G, rows;     // query heads per KV head, rows per KV head of a pass (G * tokens)
-    int splits, len; // splits of the slots and slots per split (a multiple of 64)
-    size_t part_off, ml_off, score_off, bytes;
+    int G, rows;      // query heads per KV head, rows per KV head of a pass (G * tokens)
+    int nt, rg;       // 8-row tiles per warp, warps of a CTA that take different rows
+    int zblocks;      // CTAs over the rows of a KV head
+    int splits, len;  // splits of the slots and slots per split
+    int pad;          // rows per slot in the kept scores (a multiple of 4)
+    size_t ml_off, score_off, bytes;
 };
 
 // Tokens of one pass. The accumulated weight keeps a pass's scores in the
-// workspace ([rows][n] FP32 per KV head), so a pass takes at most 128 rows;
+// workspace ([n][rows] FP32 per KV head), so a pass takes at most 128 rows;
 // without it 4096, which bounds the workspace and the grid.
 static int pass_tokens(int G, int t, bool acc) { return std::min(t, std::max(1, (acc ? 128 : 4096) / G)); }
 
@@ -30,17 +41,21 @@ static Kv8Plan kv8_plan(int hkv, int hq, int t, int n, bool acc, int num_sms)
     Kv8Plan p;
     p.G = hq / hkv;
     p.rows = p.G * t;
-    const int64_t groups = (int64_t)hkv * p.rows;
-    const int want = (int)std::max<int64_t>(1, (num_sms * 8 + groups - 1) / groups);
-    p.len = std::max(64, ((n + want - 1) / want + 63) / 64 * 64);
+    p.nt = p.rows <= 8 ? 1 : 2;
+    p.rg = p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
+    p.zblocks = (p.rows + 8 * p.nt * p.rg - 1) / (8 * p.nt * p.rg);
+    const int unit = KVA_CHUNK * (KVA_WARPS / p.rg); // slots of one round of a CTA's warps
+    const int64_t groups = (int64_t)hkv * p.zblocks;
+    const int want = (int)std::max<int64_t>(1, (int64_t)num_sms * (p.nt == 1 ? 3 : 2) / groups);
+    p.len = std::max(1, ((n + want - 1) / want + unit - 1) / unit) * unit;
     p.splits = (n + p.len - 1) / p.len;
     // room for the most splits that any length up to n takes, so that a
     // workspace for n serves every smaller length
-    const size_t heads_rows = (size_t)hkv * p.rows, most = heads_rows * std::min(want, (n + 63) / 64);
-    p.part_off = 0;
-    p.ml_off = p.part_off + most * YLM_HEAD_DIM * sizeof(float);
+    const size_t most = (size_t)hkv * p.rows * std::min(want, (n + unit - 1) / unit);
+    p.pad = (p.rows + 3) / 4 * 4;
+    p.ml_off = most * YLM_HEAD_DIM * sizeof(float);
     p.score_off = p.ml_off + (most * 2 * sizeof(float) + 255) / 256 * 256;
-    p.bytes = p.score_off + (acc ? heads_rows * n * sizeof(float) : 0);
+    p.bytes = p.score_off + (acc ? (size_t)hkv * n * p.pad * sizeof(float) : 0);
     return p;
 }
 
@@ -60,102 +75,415 @@ struct Kv8Pass
 {
     Kv8AttnArgs a;
     Kv8Plan p;
-    float *part, *ml, *scores;
+    float *part, *ml, *scores; // [row][split][128], [row][split][2], [hkv][n][pad]
 };
 
-// One warp per slot in turn, lane l holding dimensions [4l, 4l + 4).
-template <int FMT> __global__ void __launch_bounds__(KVA_THREADS) kv8_attn_kernel(Kv8Pass w)
+__device__ __forceinline__ float kva_ex2(float x)
 {
-    __shared__ float om[KVA_THREADS / 32][YLM_HEAD_DIM], mm[KVA_THREADS / 32], lm[KVA_THREADS / 32];
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// D += A B, m16n8k16, FP16 operands, FP32 accumulation
+__device__ __forceinline__ void kva_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// the 8 x 8 matrix of 16-bit values held two to a lane, transposed
+__device__ __forceinline__ uint32_t kva_transpose(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t kva_word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// 2^lv is a value block's scale (a block of zeros: the clamp's 2^-64 does as well)
+__device__ __forceinline__ float kva_log_scale(float s)
+{
+    return (float)max(-64, min(64, (int)(__float_as_uint(s) >> 23 & 255u) - 127));
+}
+
+// Both products run on the tensor cores with the slots as rows of the A operand,
+// so that 8 query rows fill the N dimension: S^T = K Q^T and O^T = V^T P^T
+// (m16n8k16; NT tiles of 8 query rows share each decoded fragment). Lane
+// (g, c) = (lane / 4, lane % 4).
+//  S^T: the head dimension is summed in a permuted order in which every A
+//    fragment comes from 16-byte loads of code rows: lane (g, c) loads
+//    dimensions [16c, 16c + 16) and 64 + [16c, 16c + 16) of slots g and g + 8, and k-step
+//    j takes word j % 4 of piece j / 4; Q's fragments are in the same order.
+//  O^T: lane (g, c) loads dimensions [16g, 16g + 16) of slots 2c, 2c + 1, 2c + 8
+//    and 2c + 9; one byte permute pairs the codes of two slots of a dimension into a
+//    fragment's halves, and M-tile i holds dimension 16g + 2i in row g, 16g + 2i + 1 in row
+//    g + 8. P^T is S^T's accumulator packed to FP16 and transposed 8 x 8 at a time.
+// No shared memory on the way: a warp keeps the codes of its next 32 slots in
+// flight in registers while it works on the current ones.
+//
+// Scales: ks multiplies the scores. vs enters the exponent: with y = x + log2 vs,
+// the PV weight is w = 2^(y - M) and the softmax sum takes w / vs (exact: vs is a power of two),
+// M >= max y - 8 moving only when y outgrows it, so that w <= 2^14 and the values' scales
+// never cost FP16 range. M is kept less 6 to the true reference.
+template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8Pass w)
+{
+    __shared__ __align__(16) float om[KVA_WARPS][8 * NT][YLM_HEAD_DIM + 8];
+    __shared__ float mm[KVA_WARPS][8 * NT], lm[KVA_WARPS][8 * NT];
     const Kv8AttnArgs &a = w.a;
-    const int G = w.p.G, sp = blockIdx.x, r = blockIdx.y, g = blockIdx.z;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int token = r / G, h = r % G;
-    const int see = a.n - a.t + token + 1;
-    const int j1 = min(see, (sp + 1) * w.p.len);
-    const int nb = (a.c.cap + a.c.block - 1) / a.c.block;
-    const float *ks = a.c.k_scale + (size_t)g * nb, *vs = a.c.v_scale + (size_t)g * nb;
-    const __half *q = a.q + token * a.q_stride + (size_t)(g * G + h) * YLM_HEAD_DIM + lane * 4;
-    float qf[4];
-    for (int i = 0; i < 4; i++)
-        qf[i] = h2f(q[i]);
-    float M = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    float *score = w.scores + ((size_t)g * w.p.rows + r) * a.n;
-    for (int j = sp * w.p.len + warp; j < min(a.n, (sp + 1) * w.p.len); j += KVA_THREADS / 32)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int sp = blockIdx.x, kvh = blockIdx.y;
+    const int RG = w.p.rg, subs = KVA_WARPS / RG, sub = warp / RG;
+    const int R = w.p.rows, G = w.p.G;
+    const int row0 = ((int)blockIdx.z * RG + warp % RG) * 8 * NT; // first of this warp's rows
+    const int n = a.n, first = n - a.t;                           // slots >= first are hidden from some row
+    const int j_end = min(n, (sp + 1) * w.p.len);
+    const int nb = (a.c.cap + a.c.block - 1) / a.c.block, bshift = 31 - __clz(a.c.block);
+    const uint8_t *kc = a.c.k + (size_t)kvh * a.c.cap * YLM_HEAD_DIM + c * 16;
+    const uint8_t *vc = a.c.v + (size_t)kvh * a.c.cap * YLM_HEAD_DIM + g * 16;
+    const float *ksp = a.c.k_scale + (size_t)kvh * nb, *vsp = a.c.v_scale + (size_t)kvh * nb;
+
+    // Q fragments and, for the accumulator's columns 2c and 2c + 1 of each tile, the last slot their token sees
+    uint32_t q[NT][8][2];
+    int see[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
     {
-        float x = -INFINITY;
-        const bool hidden = j >= j1 || (a.mask && (a.mask[j >> 5] >> (j & 31) & 1u));
-        const size_t at = ((size_t)g * a.c.cap + j) * YLM_HEAD_DIM + lane * 4;
-        if (!hidden)
+        const int r = row0 + 8 * t + g;
+        const bool is = r < R;
+        const __half *src = a.q + (is ? r / G : 0) * a.q_stride + (size_t)(kvh * G + (is ? r % G : 0)) * YLM_HEAD_DIM + c * 16;
+#pragma unroll
+        for (int p = 0; p < 2; p++)
         {
-            const uint32_t kc = *reinterpret_cast<const uint32_t *>(a.c.k + at);
-            const uint32_t d0 = kv8_decode2<FMT>(kc), d1 = kv8_decode2<FMT>(kc >> 16);
-            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&d0));
-            const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&d1));
-            x = warp_sum(qf[0] * f0.x + qf[1] * f0.y + qf[2] * f1.x + qf[3] * f1.y) * ks[j / a.c.block] *
-                (float)(1.4426950408889634 / 11.313708498984760);
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
+            if (is)
+            {
+                x = *reinterpret_cast<const uint4 *>(src + p * 64);
+                y = *reinterpret_cast<const uint4 *>(src + p * 64 + 8);
+            }
+            q[t][4 * p][0] = x.x, q[t][4 * p][1] = x.y, q[t][4 * p + 1][0] = x.z, q[t][4 * p + 1][1] = x.w;
+            q[t][4 * p + 2][0] = y.x, q[t][4 * p + 2][1] = y.y, q[t][4 * p + 3][0] = y.z, q[t][4 * p + 3][1] = y.w;
         }
-        if (w.a.acc && lane == 0)
-            score[j] = x;
-        if (x == -INFINITY)
-            continue;
-        const float Mn = fmaxf(M, x), f = exp2f(M - Mn), p = exp2f(x - Mn);
-        const uint32_t vc = *reinterpret_cast<const uint32_t *>(a.c.v + at);
-        const uint32_t d0 = kv8_decode2<FMT>(vc), d1 = kv8_decode2<FMT>(vc >> 16);
-        const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&d0));
-        const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&d1));
-        const float pv = p * vs[j / a.c.block];
-        M = Mn;
-        L = L * f + p;
-        o[0] = o[0] * f + pv * f0.x;
-        o[1] = o[1] * f + pv * f0.y;
-        o[2] = o[2] * f + pv * f1.x;
-        o[3] = o[3] * f + pv * f1.y;
+        for (int i = 0; i < 2; i++)
+            see[t][i] = first + (row0 + 8 * t + 2 * c + i) / G;
     }
-    for (int i = 0; i < 4; i++)
-        om[warp][lane * 4 + i] = o[i];
-    if (lane == 0)
+
+    uint4 K[2][4], V[2][4];
+    float ks[2], vs[2], ks_next[2], vs_next[2];
+    auto load_k = [&](int j0) {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+        {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+            {
+                const uint8_t *p = kc + (size_t)min(j0 + 16 * s + g + 8 * i, n - 1) * YLM_HEAD_DIM;
+                K[s][2 * i] = *reinterpret_cast<const uint4 *>(p);
+                K[s][2 * i + 1] = *reinterpret_cast<const uint4 *>(p + 64);
+            }
+            ks_next[s] = ksp[min(j0 + 16 * s, n - 1) >> bshift];
+        }
+    };
+    auto load_v = [&](int j0) {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+        {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                V[s][i] = *reinterpret_cast<const uint4 *>(
+                    vc + (size_t)min(j0 + 16 * s + 2 * c + (i & 1) + 8 * (i >> 1), n - 1) * YLM_HEAD_DIM);
+            vs_next[s] = vsp[min(j0 + 16 * s, n - 1) >> bshift];
+        }
+    };
+
+    float O[NT][8][4], M[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
     {
-        mm[warp] = M;
-        lm[warp] = L;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                O[t][i][e] = 0.f;
+        M[t][0] = M[t][1] = -INFINITY;
+        l[t][0] = l[t][1] = 0.f;
     }
+    const int step = KVA_CHUNK * subs;
+    int j0 = sp * w.p.len + sub * KVA_CHUNK;
+    if (row0 < R && j0 < j_end)
+    {
+        load_k(j0);
+        load_v(j0);
+    }
+    for (; row0 < R && j0 < j_end; j0 += step)
+    {
+        const int jn = j0 + step;
+        // ---- S^T
+        float S[2][NT][4];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+        {
+            ks[s] = ks_next[s];
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+                S[s][t][0] = S[s][t][1] = S[s][t][2] = S[s][t][3] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+            {
+                const uint32_t lo = kva_word(K[s][j >> 2], j & 3), hi = kva_word(K[s][2 + (j >> 2)], j & 3);
+                const uint32_t a0 = kv8_decode2<FMT>(lo), a2 = kv8_decode2<FMT>(lo >> 16);
+                const uint32_t a1 = kv8_decode2<FMT>(hi), a3 = kv8_decode2<FMT>(hi >> 16);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                    kva_mma(S[s][t], a0, a1, a2, a3, q[t][j][0], q[t][j][1]);
+            }
+        }
+        if (jn < j_end)
+            load_k(jn);
+        // ---- scores in base 2, hidden slots -inf
+        bool edge[2]; // some row does not see some slot of the half
+        uint32_t off[2];
+        float grow = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+        {
+            const int js = j0 + 16 * s;
+            const float f = ks[s] * (float)(1.4426950408889634 / 11.313708498984760);
+            vs[s] = kva_log_scale(vs_next[s]);
+            off[s] = js + 16 <= n ? 0u : js >= n ? 0xFFFFu : 0xFFFFu << (n - js) & 0xFFFFu;
+            if (a.mask && js < n)
+                off[s] |= a.mask[js >> 5] >> (js & 16) & 0xFFFFu;
+            edge[s] = js + 15 > first;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    S[s][t][e] *= f;
+            if (off[s] || edge[s])
+            {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                    {
+                        const int k = g + 8 * (e >> 1);
+                        if (off[s] >> k & 1u || js + k > see[t][e & 1])
+                            S[s][t][e] = -INFINITY;
+                    }
+            }
+            if (a.acc)
+            {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        if (js + g + 8 * i < n && row0 + 8 * t + 2 * c < w.p.pad)
+                            *reinterpret_cast<float2 *>(w.scores + ((size_t)kvh * n + js + g + 8 * i) * w.p.pad + row0 +
+                                                        8 * t + 2 * c) = make_float2(S[s][t][2 * i], S[s][t][2 * i + 1]);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    grow = fmaxf(grow, S[s][t][e] + vs[s] - M[t][e & 1]);
+        }
+        // ---- the reference follows where a score outgrew it by more than 2^8 (M is the reference less 6).
+        // M = -inf makes grow +inf, or NaN (kept out by fmaxf) where the score is -inf, too
+        if (__any_sync(0xffffffffu, grow > 14.f))
+        {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                {
+                    float m = fmaxf(fmaxf(S[0][t][i], S[0][t][i + 2]) + vs[0], fmaxf(S[1][t][i], S[1][t][i + 2]) + vs[1]);
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16)) - 6.f;
+                    if (m > M[t][i])
+                    {
+                        const float f = kva_ex2(M[t][i] - m);
+                        M[t][i] = m;
+                        l[t][i] *= f;
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                        {
+                            O[t][k][i] *= f;
+                            O[t][k][i + 2] *= f;
+                        }
+                    }
+                }
+        }
+        // ---- O^T
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+        {
+            uint32_t P[NT][2];
+            const float unscale = __uint_as_float((uint32_t)(127 - (int)vs[s]) << 23);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+            {
+                float e4[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                {
+                    // nothing seen so far: M = -inf, and every weight 0
+                    const float m = M[t][e & 1];
+                    e4[e] = kva_ex2(S[s][t][e] + (vs[s] - (m == -INFINITY ? 0.f : m)));
+                }
+                l[t][0] += (e4[0] + e4[2]) * unscale;
+                l[t][1] += (e4[1] + e4[3]) * unscale;
+                const __half2 lo = __floats2half2_rn(e4[0], e4[1]), hi = __floats2half2_rn(e4[2], e4[3]);
+                P[t][0] = kva_transpose(*reinterpret_cast<const uint32_t *>(&lo));
+                P[t][1] = kva_transpose(*reinterpret_cast<const uint32_t *>(&hi));
+            }
+            // hidden slots may hold anything, NaN codes too: 0 x NaN must not arise
+            if (off[s])
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (off[s] >> (2 * c + (i & 1) + 8 * (i >> 1)) & 1u)
+                        V[s][i] = make_uint4(0, 0, 0, 0);
+            if (FMT == KV8_E4M3 && edge[s] && a.t > 1)
+            {
+                // a slot that some rows do not see: its NaN codes are taken out and put
+                // back as NaN into the rows that do see it
+                uint32_t nan = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        nan |= (kva_word(V[s][i], k) & 0x7F7F7F7Fu) + 0x01010101u;
+                if (__any_sync(0xffffffffu, nan & 0x80808080u))
+                {
+                    uint32_t seen[NT][2];
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+                            seen[t][i] = kva_transpose((S[s][t][2 * i] == -INFINITY ? 0u : 0x3C00u) |
+                                                       (S[s][t][2 * i + 1] == -INFINITY ? 0u : 0x3C000000u));
+                    uint32_t *v = reinterpret_cast<uint32_t *>(&V[s][0]);
+                    uint32_t flag[16]; // 1 (0x38 in E4M3) where a code is NaN
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                    {
+                        const uint32_t hit = ((v[k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                        flag[k] = (hit >> 7) * 0x38u;
+                        v[k] &= ~((hit >> 7) * 0xFFu);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                    {
+                        const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+                        const uint32_t x = __byte_perm(flag[i >> 1], flag[4 + (i >> 1)], sel);
+                        const uint32_t y = __byte_perm(flag[8 + (i >> 1)], flag[12 + (i >> 1)], sel);
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+                        {
+                            float d[4] = {0.f, 0.f, 0.f, 0.f};
+                            kva_mma(d, kv8_decode2<FMT>(x), kv8_decode2<FMT>(x >> 16), kv8_decode2<FMT>(y),
+                                    kv8_decode2<FMT>(y >> 16), seen[t][0], seen[t][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (d[e] > 0.f)
+                                    O[t][i][e] = NAN;
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+            {
+                const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+                const uint32_t x = __byte_perm(kva_word(V[s][0], i >> 1), kva_word(V[s][1], i >> 1), sel);
+                const uint32_t y = __byte_perm(kva_word(V[s][2], i >> 1), kva_word(V[s][3], i >> 1), sel);
+                const uint32_t a0 = kv8_decode2<FMT>(x), a1 = kv8_decode2<FMT>(x >> 16);
+                const uint32_t a2 = kv8_decode2<FMT>(y), a3 = kv8_decode2<FMT>(y >> 16);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                    kva_mma(O[t][i], a0, a1, a2, a3, P[t][0], P[t][1]);
+            }
+        }
+        if (jn < j_end)
+            load_v(jn);
+    }
+
+    // ---- join the warps that share rows, and leave the split's sums
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+        {
+            float s = l[t][i];
+            s += __shfl_xor_sync(0xffffffffu, s, 4);
+            s += __shfl_xor_sync(0xffffffffu, s, 8);
+            s += __shfl_xor_sync(0xffffffffu, s, 16);
+            if (g == 0)
+            {
+                mm[warp][8 * t + 2 * c + i] = M[t][i];
+                lm[warp][8 * t + 2 * c + i] = s;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                *reinterpret_cast<float2 *>(&om[warp][8 * t + 2 * c + i][16 * g + 2 * k]) =
+                    make_float2(O[t][k][i], O[t][k][i + 2]);
+        }
     __syncthreads();
-    M = mm[0];
-    for (int i = 1; i < KVA_THREADS / 32; i++)
-        M = fmaxf(M, mm[i]);
-    L = 0.f;
-    float O = 0.f;
-    for (int i = 0; i < KVA_THREADS / 32; i++)
+    // a warp per row in turn, lane = 4 dimensions
+    for (int r = warp; r < RG * 8 * NT; r += KVA_WARPS)
     {
-        const float f = mm[i] == -INFINITY ? 0.f : exp2f(mm[i] - M);
-        L += lm[i] * f;
-        O += om[i][tid] * f;
-    }
-    const size_t row = ((size_t)g * w.p.rows + r) * w.p.splits + sp;
-    w.part[row * YLM_HEAD_DIM + tid] = O;
-    if (tid == 0)
-    {
-        w.ml[2 * row] = M;
-        w.ml[2 * row + 1] = L;
+        const int rg = r / (8 * NT), lr = r % (8 * NT), row = (int)blockIdx.z * RG * 8 * NT + r;
+        if (row >= R)
+            break;
+        float m = -INFINITY;
+        for (int s = 0; s < subs; s++)
+            m = fmaxf(m, mm[s * RG + rg][lr]);
+        float L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < subs; s++)
+        {
+            const float ms = mm[s * RG + rg][lr], f = ms == -INFINITY ? 0.f : kva_ex2(ms - m);
+            const float4 x = *reinterpret_cast<const float4 *>(&om[s * RG + rg][lr][lane * 4]);
+            // NaN that a slot with NaN codes put into O where no finite score was seen must stay
+            L += lm[s * RG + rg][lr] * f;
+            o.x += x.x * f;
+            o.y += x.y * f;
+            o.z += x.z * f;
+            o.w += x.w * f;
+        }
+        const size_t at = ((size_t)kvh * R + row) * w.p.splits + sp;
+        *reinterpret_cast<float4 *>(w.part + at * YLM_HEAD_DIM + lane * 4) = o;
+        if (lane == 0)
+            *reinterpret_cast<float2 *>(w.ml + 2 * at) = make_float2(m, L);
     }
 }
 
-// M and 1 / L of one row over its splits (0 and 0 where every slot is hidden)
+// M and 1 / l of one row over its splits, by one warp (0 and 0 where every slot is hidden)
 __device__ __forceinline__ float2 kv8_row_state(const float *ml, int splits)
 {
+    const int lane = threadIdx.x & 31;
     float M = -INFINITY, L = 0.f;
-    for (int s = 0; s < splits; s++)
-        M = fmaxf(M, ml[2 * s]);
-    if (M == -INFINITY)
+    for (int s = lane; s < splits; s += 32)
+    {
+        const float2 x = *reinterpret_cast<const float2 *>(ml + 2 * s);
+        const float m = fmaxf(M, x.x);
+        if (m > -INFINITY)
+            L = L * kva_ex2(M - m) + x.y * kva_ex2(x.x - m);
+        M = m;
+    }
+    const float m = warp_max(M);
+    if (m == -INFINITY)
         return make_float2(0.f, 0.f);
-    for (int s = 0; s < splits; s++)
-        L += ml[2 * s + 1] * exp2f(ml[2 * s] - M);
-    return make_float2(M, 1.f / L);
+    L = warp_sum(L * kva_ex2(M - m));
+    return make_float2(m, 1.f / L);
 }
 
 // Joins the splits: CTAs [0, hkv * rows) write one output row each, the others
 // add the weights of KVA_ACC_TILE slots of one KV head to acc.
-__global__ void __launch_bounds__(KVA_THREADS) kv8_join_kernel(Kv8Pass w)
+__global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(const Kv8Pass w)
 {
     const Kv8AttnArgs &a = w.a;
     const int G = w.p.G, R = w.p.rows, S = w.p.splits, tid = threadIdx.x;
@@ -166,27 +494,51 @@ __global__ void __launch_bounds__(KVA_THREADS) kv8_join_kernel(Kv8Pass w)
         const int g = b / R, r = b % R;
         const float *ml = w.ml + (size_t)b * S * 2;
         const float2 st = kv8_row_state(ml, S);
+        const float *part = w.part + (size_t)b * S * YLM_HEAD_DIM + tid;
         float O = 0.f;
+#pragma unroll 8
         for (int s = 0; s < S; s++)
-            if (ml[2 * s] != -INFINITY)
-                O += w.part[((size_t)b * S + s) * YLM_HEAD_DIM + tid] * exp2f(ml[2 * s] - st.x);
+        {
+            const float m = ml[2 * s];
+            O += part[(size_t)s * YLM_HEAD_DIM] * (m == -INFINITY ? 0.f : kva_ex2(m - st.x));
+        }
         a.out[(r / G) * a.out_stride + (size_t)(g * G + r % G) * YLM_HEAD_DIM + tid] = f2h(O * st.y);
         return;
     }
     __shared__ float2 state[128];
     b -= rows;
     const int tiles = (a.n + KVA_ACC_TILE - 1) / KVA_ACC_TILE;
-    const int g = b / tiles, j0 = b % tiles * KVA_ACC_TILE;
-    if (tid < R)
-        state[tid] = kv8_row_state(w.ml + ((size_t)g * R + tid) * S * 2, S);
-    __syncthreads();
-    for (int j = j0 + tid; j < min(a.n, j0 + KVA_ACC_TILE); j += KVA_THREADS)
+    const int g = b / tiles, j = b % tiles * KVA_ACC_TILE + tid;
+    for (int r = tid >> 5; r < w.p.pad; r += KVA_JOIN / 32)
     {
-        float sum = 0.f;
-        for (int r = 0; r < R; r++)
-            sum += exp2f(w.scores[((size_t)g * R + r) * a.n + j] - state[r].x) * state[r].y;
-        a.acc[(size_t)g * a.c.cap + j] += sum;
+        const float2 st = r < R ? kv8_row_state(w.ml + ((size_t)g * R + r) * S * 2, S) : make_float2(0.f, 0.f);
+        if ((tid & 31) == 0)
+            state[r] = st;
     }
+    __syncthreads();
+    if (j >= a.n)
+        return;
+    const float4 *x = reinterpret_cast<const float4 *>(w.scores + ((size_t)g * a.n + j) * w.p.pad);
+    float sum = 0.f;
+    for (int r = 0; r < w.p.pad; r += 4)
+    {
+        const float4 v = x[r >> 2];
+        const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (r + i < R)
+                sum += kva_ex2(f[i] - state[r + i].x) * state[r + i].y;
+    }
+    a.acc[(size_t)g * a.c.cap + j] += sum;
+}
+
+template <int FMT> static void attn_launch(const Kv8Pass &w, cudaStream_t s)
+{
+    const dim3 grid((unsigned)w.p.splits, (unsigned)w.a.c.hkv, (unsigned)w.p.zblocks);
+    if (w.p.nt == 1)
+        kv8_attn_kernel<FMT, 1><<<grid, KVA_THREADS, 0, s>>>(w);
+    else
+        kv8_attn_kernel<FMT, 2><<<grid, KVA_THREADS, 0, s>>>(w);
 }
 
 cudaError_t kv8_attn_launch(const Kv8AttnArgs &args, void *ws, int num_sms, cudaStream_t s)
@@ -201,19 +553,18 @@ cudaError_t kv8_attn_launch(const Kv8AttnArgs &args, void *ws, int num_sms, cuda
         w.a.q = args.q + i0 * args.q_stride;
         w.a.out = args.out + i0 * args.out_stride;
         w.p = kv8_plan(args.c.hkv, args.hq, w.a.t, w.a.n, args.acc != nullptr, num_sms);
-        w.part = reinterpret_cast<float *>(static_cast<char *>(ws) + w.p.part_off);
+        w.part = static_cast<float *>(ws);
         w.ml = reinterpret_cast<float *>(static_cast<char *>(ws) + w.p.ml_off);
         w.scores = reinterpret_cast<float *>(static_cast<char *>(ws) + w.p.score_off);
-        const dim3 grid((unsigned)w.p.splits, (unsigned)w.p.rows, (unsigned)args.c.hkv);
         if (args.c.format == KV8_E4M3)
-            kv8_attn_kernel<KV8_E4M3><<<grid, KVA_THREADS, 0, s>>>(w);
+            attn_launch<KV8_E4M3>(w, s);
         else
-            kv8_attn_kernel<KV8_INT8><<<grid, KVA_THREADS, 0, s>>>(w);
+            attn_launch<KV8_INT8>(w, s);
         cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess)
             return e;
         const int tiles = args.acc ? (w.a.n + KVA_ACC_TILE - 1) / KVA_ACC_TILE : 0;
-        kv8_join_kernel<<<(unsigned)(args.c.hkv * (w.p.rows + tiles)), KVA_THREADS, 0, s>>>(w);
+        kv8_join_kernel<<<(unsigned)(args.c.hkv * (w.p.rows + tiles)), KVA_JOIN, 0, s>>>(w);
         e = cudaGetLastError();
         if (e != cudaSuccess)
             return e;
