@@ -18,8 +18,10 @@ namespace ylm {
 constexpr int KVA_THREADS = 128;
 constexpr int KVA_WARPS = KVA_THREADS / 32;
 constexpr int KVA_CHUNK = 32;     // slots a warp takes at a time
+constexpr int KVA_BUF = KVA_CHUNK * YLM_HEAD_DIM; // bytes of a chunk's K or V
+constexpr int KVA_RING = 4 * KVA_BUF;             // a warp's two K and two V chunks
+constexpr int KVA_SMEM = KVA_WARPS * KVA_RING;
 constexpr int KVA_JOIN = 128;     // threads of the joining CTAs
-constexpr int KVA_ACC_TILE = 128; // slots per CTA of the accumulation
 
 struct Kv8Plan
 {
@@ -27,7 +29,8 @@ struct Kv8Plan
     int nt, rg;       // 8-row tiles per warp, warps of a CTA that take different rows
     int zblocks;      // CTAs over the rows of a KV head
     int splits, len;  // splits of the slots and slots per split
-    int pad;          // rows per slot in the kept scores (a multiple of 4)
+    int pad;          // rows, rounded up to a multiple of 4: stride of the kept scores and of (M, l)
+    int tile;         // slots per CTA of the accumulation
     size_t ml_off, score_off, bytes;
 };
 
@@ -51,10 +54,12 @@ static Kv8Plan kv8_plan(int hkv, int hq, int t, int n, bool acc, int num_sms)
     p.splits = (n + p.len - 1) / p.len;
     // room for the most splits that any length up to n takes, so that a
     // workspace for n serves every smaller length
-    const size_t most = (size_t)hkv * p.rows * std::min(want, (n + unit - 1) / unit);
+    const size_t most = (size_t)hkv * std::min(want, (n + unit - 1) / unit);
     p.pad = (p.rows + 3) / 4 * 4;
-    p.ml_off = most * YLM_HEAD_DIM * sizeof(float);
-    p.score_off = p.ml_off + (most * 2 * sizeof(float) + 255) / 256 * 256;
+    p.ml_off = most * p.rows * YLM_HEAD_DIM * sizeof(float);
+    p.score_off = p.ml_off + (most * p.pad * 2 * sizeof(float) + 255) / 256 * 256;
+    // slots per accumulating CTA: about four CTAs per SM, each of which finds every row's state first
+    p.tile = std::max(KVA_JOIN, (int)(((int64_t)hkv * n / (num_sms * 4) + KVA_JOIN - 1) / KVA_JOIN) * KVA_JOIN);
     p.bytes = p.score_off + (acc ? (size_t)hkv * n * p.pad * sizeof(float) : 0);
     return p;
 }
@@ -75,7 +80,7 @@ struct Kv8Pass
 {
     Kv8AttnArgs a;
     Kv8Plan p;
-    float *part, *ml, *scores; // [row][split][128], [row][split][2], [hkv][n][pad]
+    float *part, *ml, *scores; // [hkv][rows][split][128], [hkv][split][pad][2], [hkv][n][pad]
 };
 
 __device__ __forceinline__ float kva_ex2(float x)
@@ -122,8 +127,9 @@ __device__ __forceinline__ float kva_log_scale(float s)
 //    and 2c + 9; one byte permute pairs the codes of two slots of a dimension into a
 //    fragment's halves, and M-tile i holds dimension 16g + 2i in row g, 16g + 2i + 1 in row
 //    g + 8. P^T is S^T's accumulator packed to FP16 and transposed 8 x 8 at a time.
-// No shared memory on the way: a warp keeps the codes of its next 32 slots in
-// flight in registers while it works on the current ones.
+// Each warp streams its own chunks of 32 slots through a ring of two K and two V
+// buffers (cp.async, no barrier between warps): while it works on one chunk the next
+// one's K and V are in flight.
 //
 // Scales: ks multiplies the scores. vs enters the exponent: with y = x + log2 vs,
 // the PV weight is w = 2^(y - M) and the softmax sum takes w / vs (exact: vs is a power of two),
@@ -131,8 +137,11 @@ __device__ __forceinline__ float kva_log_scale(float s)
 // never cost FP16 range. M is kept less 6 to the true reference.
 template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8Pass w)
 {
-    __shared__ __align__(16) float om[KVA_WARPS][8 * NT][YLM_HEAD_DIM + 8];
+    extern __shared__ __align__(128) uint8_t ring[]; // a warp's two K and two V chunks; at the end the sums O
+    float(*om)[8 * NT][YLM_HEAD_DIM + 8] = reinterpret_cast<float(*)[8 * NT][YLM_HEAD_DIM + 8]>(ring);
+    static_assert(sizeof(float) * 8 * NT * (YLM_HEAD_DIM + 8) <= KVA_RING, "a warp's O fits its ring");
     __shared__ float mm[KVA_WARPS][8 * NT], lm[KVA_WARPS][8 * NT];
+    pdl_launch_dependents(); // the joining CTAs may start; they wait for this grid's end
     const Kv8AttnArgs &a = w.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int sp = blockIdx.x, kvh = blockIdx.y;
@@ -142,8 +151,8 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
     const int n = a.n, first = n - a.t;                           // slots >= first are hidden from some row
     const int j_end = min(n, (sp + 1) * w.p.len);
     const int nb = (a.c.cap + a.c.block - 1) / a.c.block, bshift = 31 - __clz(a.c.block);
-    const uint8_t *kc = a.c.k + (size_t)kvh * a.c.cap * YLM_HEAD_DIM + c * 16;
-    const uint8_t *vc = a.c.v + (size_t)kvh * a.c.cap * YLM_HEAD_DIM + g * 16;
+    const uint8_t *kc = a.c.k + (size_t)kvh * a.c.cap * YLM_HEAD_DIM;
+    const uint8_t *vc = a.c.v + (size_t)kvh * a.c.cap * YLM_HEAD_DIM;
     const float *ksp = a.c.k_scale + (size_t)kvh * nb, *vsp = a.c.v_scale + (size_t)kvh * nb;
 
     // Q fragments and, for the accumulator's columns 2c and 2c + 1 of each tile, the last slot their token sees
@@ -171,31 +180,52 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
             see[t][i] = first + (row0 + 8 * t + 2 * c + i) / G;
     }
 
-    uint4 K[2][4], V[2][4];
-    float ks[2], vs[2], ks_next[2], vs_next[2];
-    auto load_k = [&](int j0) {
-#pragma unroll
-        for (int s = 0; s < 2; s++)
+    // ---- the warp's ring: chunk (row r, 16-byte piece q) at r * 128 + (q ^ f(r)) * 16 with
+    // f(r) = 2 ((r / 2) % 4) ^ 4 (r % 2), which spreads the pieces that eight lanes read
+    // together (K: four pieces of two rows; V: two pieces of four even or four odd rows) over all banks
+    uint8_t *mine = ring + warp * KVA_RING;
+    const uint32_t ring_at = smem_u32(mine);
+    // this lane copies piece lane % 8 of rows 4 i + lane / 8: f there for even i, and for odd i
+    const uint32_t dst_even = (lane >> 3) * 128 + (((lane & 7) ^ (((lane >> 4) & 1) << 1) ^ ((lane >> 3 & 1) << 2)) << 4);
+    const uint32_t dst_odd = (lane >> 3) * 128 + (((lane & 7) ^ ((2 + ((lane >> 4) & 1)) << 1) ^ ((lane >> 3 & 1) << 2)) << 4);
+    auto copy = [&](const uint8_t *src, int j0, uint32_t at) {
+        const int r0 = j0 + (lane >> 3);
+        const uint8_t *p = src + (size_t)r0 * YLM_HEAD_DIM + (lane & 7) * 16;
+        if (j0 + KVA_CHUNK <= n)
         {
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 8; i++)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i * 512 + (i & 1 ? dst_odd : dst_even)),
+                             "l"(p + i * 512)
+                             : "memory");
+        }
+        else
+        {
+            // rows behind the last slot are not read and arrive as zeros
+#pragma unroll
+            for (int i = 0; i < 8; i++)
             {
-                const uint8_t *p = kc + (size_t)min(j0 + 16 * s + g + 8 * i, n - 1) * YLM_HEAD_DIM;
-                K[s][2 * i] = *reinterpret_cast<const uint4 *>(p);
-                K[s][2 * i + 1] = *reinterpret_cast<const uint4 *>(p + 64);
+                const bool in = r0 + 4 * i < n;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                 at + i * 512 + (i & 1 ? dst_odd : dst_even)),
+                             "l"(in ? p + i * 512 : src), "r"(in ? 16 : 0)
+                             : "memory");
             }
-            ks_next[s] = ksp[min(j0 + 16 * s, n - 1) >> bshift];
         }
     };
-    auto load_v = [&](int j0) {
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    // the lane's reads: K pieces c and 4 + c of row g (+ 8 k, same f), V piece g of rows 2c (+ 8) and 2c + 1 (+ 8)
+    const uint32_t fg = ((g >> 1 & 3) << 1) ^ ((g & 1) << 2), fc = c << 1;
+    const uint32_t k_lo = g * 128 + ((c ^ fg) << 4), k_hi = g * 128 + (((4 + c) ^ fg) << 4);
+    const uint32_t v_even = c * 256 + ((g ^ fc) << 4), v_odd = c * 256 + 128 + ((g ^ fc ^ 4) << 4);
+    float ks[2], vs[2], ks_next[2], vs_next[2];
+    auto load_scales = [&](int j0) {
 #pragma unroll
         for (int s = 0; s < 2; s++)
         {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                V[s][i] = *reinterpret_cast<const uint4 *>(
-                    vc + (size_t)min(j0 + 16 * s + 2 * c + (i & 1) + 8 * (i >> 1), n - 1) * YLM_HEAD_DIM);
-            vs_next[s] = vsp[min(j0 + 16 * s, n - 1) >> bshift];
+            const int b = min(j0 + 16 * s, n - 1) >> bshift;
+            ks_next[s] = ksp[b];
+            vs_next[s] = vsp[b];
         }
     };
 
@@ -213,27 +243,46 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
     }
     const int step = KVA_CHUNK * subs;
     int j0 = sp * w.p.len + sub * KVA_CHUNK;
+    int phase = 0; // the buffers of this round: 0 or 1
     if (row0 < R && j0 < j_end)
     {
-        load_k(j0);
-        load_v(j0);
+        load_scales(j0);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+        {
+            if (j0 + i * step < j_end)
+                copy(kc, j0 + i * step, ring_at + i * KVA_BUF);
+            commit();
+            if (j0 + i * step < j_end)
+                copy(vc, j0 + i * step, ring_at + (2 + i) * KVA_BUF);
+            commit();
+        }
     }
-    for (; row0 < R && j0 < j_end; j0 += step)
+    for (; row0 < R && j0 < j_end; j0 += step, phase ^= 1)
     {
-        const int jn = j0 + step;
+        // in flight: this round's K and V, the next one's K and V
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+        __syncwarp();
+        const uint8_t *kb = mine + phase * KVA_BUF, *vb = mine + (2 + phase) * KVA_BUF;
         // ---- S^T
         float S[2][NT][4];
 #pragma unroll
         for (int s = 0; s < 2; s++)
         {
             ks[s] = ks_next[s];
+            vs[s] = kva_log_scale(vs_next[s]);
+            uint4 K[4];
+            K[0] = *reinterpret_cast<const uint4 *>(kb + s * 2048 + k_lo);
+            K[1] = *reinterpret_cast<const uint4 *>(kb + s * 2048 + k_hi);
+            K[2] = *reinterpret_cast<const uint4 *>(kb + s * 2048 + 1024 + k_lo);
+            K[3] = *reinterpret_cast<const uint4 *>(kb + s * 2048 + 1024 + k_hi);
 #pragma unroll
             for (int t = 0; t < NT; t++)
                 S[s][t][0] = S[s][t][1] = S[s][t][2] = S[s][t][3] = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j++)
             {
-                const uint32_t lo = kva_word(K[s][j >> 2], j & 3), hi = kva_word(K[s][2 + (j >> 2)], j & 3);
+                const uint32_t lo = kva_word(K[j >> 2], j & 3), hi = kva_word(K[2 + (j >> 2)], j & 3);
                 const uint32_t a0 = kv8_decode2<FMT>(lo), a2 = kv8_decode2<FMT>(lo >> 16);
                 const uint32_t a1 = kv8_decode2<FMT>(hi), a3 = kv8_decode2<FMT>(hi >> 16);
 #pragma unroll
@@ -241,8 +290,12 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                     kva_mma(S[s][t], a0, a1, a2, a3, q[t][j][0], q[t][j][1]);
             }
         }
-        if (jn < j_end)
-            load_k(jn);
+        __syncwarp(); // every lane has read this K
+        if (j0 + 2 * step < j_end)
+            copy(kc, j0 + 2 * step, ring_at + phase * KVA_BUF);
+        commit();
+        if (j0 + step < j_end)
+            load_scales(j0 + step);
         // ---- scores in base 2, hidden slots -inf
         bool edge[2]; // some row does not see some slot of the half
         uint32_t off[2];
@@ -252,7 +305,6 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
         {
             const int js = j0 + 16 * s;
             const float f = ks[s] * (float)(1.4426950408889634 / 11.313708498984760);
-            vs[s] = kva_log_scale(vs_next[s]);
             off[s] = js + 16 <= n ? 0u : js >= n ? 0xFFFFu : 0xFFFFu << (n - js) & 0xFFFFu;
             if (a.mask && js < n)
                 off[s] |= a.mask[js >> 5] >> (js & 16) & 0xFFFFu;
@@ -318,9 +370,16 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                 }
         }
         // ---- O^T
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+        __syncwarp();
 #pragma unroll
         for (int s = 0; s < 2; s++)
         {
+            uint4 V[4];
+            V[0] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + v_even);
+            V[1] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + v_odd);
+            V[2] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + 1024 + v_even);
+            V[3] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + 1024 + v_odd);
             uint32_t P[NT][2];
             const float unscale = __uint_as_float((uint32_t)(127 - (int)vs[s]) << 23);
 #pragma unroll
@@ -345,7 +404,7 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (off[s] >> (2 * c + (i & 1) + 8 * (i >> 1)) & 1u)
-                        V[s][i] = make_uint4(0, 0, 0, 0);
+                        V[i] = make_uint4(0, 0, 0, 0);
             if (FMT == KV8_E4M3 && edge[s] && a.t > 1)
             {
                 // a slot that some rows do not see: its NaN codes are taken out and put
@@ -355,7 +414,7 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        nan |= (kva_word(V[s][i], k) & 0x7F7F7F7Fu) + 0x01010101u;
+                        nan |= (kva_word(V[i], k) & 0x7F7F7F7Fu) + 0x01010101u;
                 if (__any_sync(0xffffffffu, nan & 0x80808080u))
                 {
                     uint32_t seen[NT][2];
@@ -365,7 +424,7 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                         for (int i = 0; i < 2; i++)
                             seen[t][i] = kva_transpose((S[s][t][2 * i] == -INFINITY ? 0u : 0x3C00u) |
                                                        (S[s][t][2 * i + 1] == -INFINITY ? 0u : 0x3C000000u));
-                    uint32_t *v = reinterpret_cast<uint32_t *>(&V[s][0]);
+                    uint32_t *v = reinterpret_cast<uint32_t *>(&V[0]);
                     uint32_t flag[16]; // 1 (0x38 in E4M3) where a code is NaN
 #pragma unroll
                     for (int k = 0; k < 16; k++)
@@ -398,8 +457,8 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
             for (int i = 0; i < 8; i++)
             {
                 const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
-                const uint32_t x = __byte_perm(kva_word(V[s][0], i >> 1), kva_word(V[s][1], i >> 1), sel);
-                const uint32_t y = __byte_perm(kva_word(V[s][2], i >> 1), kva_word(V[s][3], i >> 1), sel);
+                const uint32_t x = __byte_perm(kva_word(V[0], i >> 1), kva_word(V[1], i >> 1), sel);
+                const uint32_t y = __byte_perm(kva_word(V[2], i >> 1), kva_word(V[3], i >> 1), sel);
                 const uint32_t a0 = kv8_decode2<FMT>(x), a1 = kv8_decode2<FMT>(x >> 16);
                 const uint32_t a2 = kv8_decode2<FMT>(y), a3 = kv8_decode2<FMT>(y >> 16);
 #pragma unroll
@@ -407,9 +466,12 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                     kva_mma(O[t][i], a0, a1, a2, a3, P[t][0], P[t][1]);
             }
         }
-        if (jn < j_end)
-            load_v(jn);
+        __syncwarp(); // every lane has read this V
+        if (j0 + 2 * step < j_end)
+            copy(vc, j0 + 2 * step, ring_at + (2 + phase) * KVA_BUF);
+        commit();
     }
+    __syncthreads(); // the rings become the warps' sums
 
     // ---- join the warps that share rows, and leave the split's sums
 #pragma unroll
@@ -454,91 +516,142 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
             o.z += x.z * f;
             o.w += x.w * f;
         }
-        const size_t at = ((size_t)kvh * R + row) * w.p.splits + sp;
-        *reinterpret_cast<float4 *>(w.part + at * YLM_HEAD_DIM + lane * 4) = o;
+        *reinterpret_cast<float4 *>(w.part + (((size_t)kvh * R + row) * w.p.splits + sp) * YLM_HEAD_DIM + lane * 4) = o;
         if (lane == 0)
-            *reinterpret_cast<float2 *>(w.ml + 2 * at) = make_float2(m, L);
+            *reinterpret_cast<float2 *>(w.ml + 2 * (((size_t)kvh * w.p.splits + sp) * w.p.pad + row)) = make_float2(m, L);
     }
 }
 
-// M and 1 / l of one row over its splits, by one warp (0 and 0 where every slot is hidden)
-__device__ __forceinline__ float2 kv8_row_state(const float *ml, int splits)
-{
-    const int lane = threadIdx.x & 31;
-    float M = -INFINITY, L = 0.f;
-    for (int s = lane; s < splits; s += 32)
-    {
-        const float2 x = *reinterpret_cast<const float2 *>(ml + 2 * s);
-        const float m = fmaxf(M, x.x);
-        if (m > -INFINITY)
-            L = L * kva_ex2(M - m) + x.y * kva_ex2(x.x - m);
-        M = m;
-    }
-    const float m = warp_max(M);
-    if (m == -INFINITY)
-        return make_float2(0.f, 0.f);
-    L = warp_sum(L * kva_ex2(M - m));
-    return make_float2(m, 1.f / L);
-}
-
-// Joins the splits: CTAs [0, hkv * rows) write one output row each, the others
-// add the weights of KVA_ACC_TILE slots of one KV head to acc.
+// Joins the splits. CTAs [0, hkv * rows) write one output row each: every warp
+// finds the row's M and l from the splits' (a lane each), then takes every fourth
+// split's O, four dimensions a lane. The others add the weights of p.tile
+// slots of one KV head to acc: first the M and 1 / l of every row, by all threads.
 __global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(const Kv8Pass w)
 {
     const Kv8AttnArgs &a = w.a;
-    const int G = w.p.G, R = w.p.rows, S = w.p.splits, tid = threadIdx.x;
+    const int G = w.p.G, R = w.p.rows, S = w.p.splits, pad = w.p.pad;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rows = a.c.hkv * R;
     int b = blockIdx.x;
+    pdl_wait();
     if (b < rows)
     {
+        __shared__ float4 om[KVA_JOIN / 32][32];
         const int g = b / R, r = b % R;
-        const float *ml = w.ml + (size_t)b * S * 2;
-        const float2 st = kv8_row_state(ml, S);
-        const float *part = w.part + (size_t)b * S * YLM_HEAD_DIM + tid;
-        float O = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < S; s++)
+        const float2 *ml = reinterpret_cast<const float2 *>(w.ml) + (size_t)g * S * pad + r;
+        const float4 *part = reinterpret_cast<const float4 *>(w.part) + (size_t)b * S * (YLM_HEAD_DIM / 4) + lane;
+        float M = -INFINITY, L = 0.f;
+        for (int s = lane; s < S; s += 32)
+            M = fmaxf(M, ml[(size_t)s * pad].x);
+        M = warp_max(M);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < S; s0 += 32)
         {
-            const float m = ml[2 * s];
-            O += part[(size_t)s * YLM_HEAD_DIM] * (m == -INFINITY ? 0.f : kva_ex2(m - st.x));
+            const float2 x = s0 + lane < S ? ml[(size_t)(s0 + lane) * pad] : make_float2(-INFINITY, 0.f);
+            const float f = x.x == -INFINITY ? 0.f : kva_ex2(x.x - M);
+            L += x.y * f;
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+            {
+                const int s = s0 + 4 * k + warp;
+                const float fs = __shfl_sync(0xffffffffu, f, 4 * k + warp);
+                if (s < S)
+                {
+                    const float4 v = part[(size_t)s * (YLM_HEAD_DIM / 4)];
+                    o.x += v.x * fs;
+                    o.y += v.y * fs;
+                    o.z += v.z * fs;
+                    o.w += v.w * fs;
+                }
+            }
         }
-        a.out[(r / G) * a.out_stride + (size_t)(g * G + r % G) * YLM_HEAD_DIM + tid] = f2h(O * st.y);
+        L = warp_sum(L);
+        om[warp][lane] = o;
+        __syncthreads();
+        const float *of = reinterpret_cast<const float *>(om);
+        const float sum = (of[tid] + of[128 + tid]) + (of[256 + tid] + of[384 + tid]);
+        a.out[(r / G) * a.out_stride + (size_t)(g * G + r % G) * YLM_HEAD_DIM + tid] =
+            f2h(M == -INFINITY ? sum : sum / L); // no slot seen: 0
         return;
     }
-    __shared__ float2 state[128];
+    __shared__ float2 state[128], join[KVA_JOIN];
     b -= rows;
-    const int tiles = (a.n + KVA_ACC_TILE - 1) / KVA_ACC_TILE;
-    const int g = b / tiles, j = b % tiles * KVA_ACC_TILE + tid;
-    for (int r = tid >> 5; r < w.p.pad; r += KVA_JOIN / 32)
+    const int tiles = (a.n + w.p.tile - 1) / w.p.tile;
+    const int g = b / tiles, j0 = b % tiles * w.p.tile, j1 = min(a.n, j0 + w.p.tile);
+    const int parts = KVA_JOIN / pad, part = tid / pad, r = tid % pad;
+    if (part < parts)
     {
-        const float2 st = r < R ? kv8_row_state(w.ml + ((size_t)g * R + r) * S * 2, S) : make_float2(0.f, 0.f);
-        if ((tid & 31) == 0)
-            state[r] = st;
+        const float2 *ml = reinterpret_cast<const float2 *>(w.ml) + (size_t)g * S * pad + r;
+        float M = -INFINITY, L = 0.f;
+        if (r < R)
+#pragma unroll 4
+            for (int s = part; s < S; s += parts)
+            {
+                const float2 x = ml[(size_t)s * pad];
+                const float m = fmaxf(M, x.x), ref = m == -INFINITY ? 0.f : m;
+                L = L * kva_ex2(M - ref) + x.y * kva_ex2(x.x - ref);
+                M = m;
+            }
+        join[tid] = make_float2(M, L);
     }
     __syncthreads();
-    if (j >= a.n)
-        return;
-    const float4 *x = reinterpret_cast<const float4 *>(w.scores + ((size_t)g * a.n + j) * w.p.pad);
-    float sum = 0.f;
-    for (int r = 0; r < w.p.pad; r += 4)
+    if (tid < pad)
     {
-        const float4 v = x[r >> 2];
-        const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (r + i < R)
-                sum += kva_ex2(f[i] - state[r + i].x) * state[r + i].y;
+        float M = -INFINITY, L = 0.f;
+        for (int p = 0; p < parts; p++)
+            M = fmaxf(M, join[p * pad + tid].x);
+        const float ref = M == -INFINITY ? 0.f : M;
+        for (int p = 0; p < parts; p++)
+            L += join[p * pad + tid].y * kva_ex2(join[p * pad + tid].x - ref);
+        // a row that sees nothing, and one that is not there, weigh nothing
+        state[tid] = M == -INFINITY ? make_float2(0.f, 0.f) : make_float2(M, 1.f / L);
     }
-    a.acc[(size_t)g * a.c.cap + j] += sum;
+    __syncthreads();
+    float *acc = a.acc + (size_t)g * a.c.cap;
+    const float4 *x = reinterpret_cast<const float4 *>(w.scores) + (size_t)g * a.n * (pad / 4);
+    constexpr int U = 4; // slots of a thread whose loads are in flight together
+    for (int j = j0 + tid; j < j1; j += KVA_JOIN * U)
+    {
+        float sum[U], old[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+        {
+            sum[u] = 0.f;
+            old[u] = j + u * KVA_JOIN < j1 ? acc[j + u * KVA_JOIN] : 0.f;
+        }
+        for (int i = 0; i < pad; i += 4)
+        {
+            float4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                v[u] = x[(size_t)min(j + u * KVA_JOIN, j1 - 1) * (pad / 4) + (i >> 2)];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+            {
+                sum[u] += kva_ex2(v[u].x - state[i].x) * state[i].y;
+                // rows that are not there: whatever their scores hold must not count
+                if (i + 1 < R)
+                    sum[u] += kva_ex2(v[u].y - state[i + 1].x) * state[i + 1].y;
+                if (i + 2 < R)
+                    sum[u] += kva_ex2(v[u].z - state[i + 2].x) * state[i + 2].y;
+                if (i + 3 < R)
+                    sum[u] += kva_ex2(v[u].w - state[i + 3].x) * state[i + 3].y;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (j + u * KVA_JOIN < j1)
+                acc[j + u * KVA_JOIN] = old[u] + sum[u];
+    }
 }
 
 template <int FMT> static void attn_launch(const Kv8Pass &w, cudaStream_t s)
 {
     const dim3 grid((unsigned)w.p.splits, (unsigned)w.a.c.hkv, (unsigned)w.p.zblocks);
     if (w.p.nt == 1)
-        kv8_attn_kernel<FMT, 1><<<grid, KVA_THREADS, 0, s>>>(w);
+        kv8_attn_kernel<FMT, 1><<<grid, KVA_THREADS, KVA_SMEM, s>>>(w);
     else
-        kv8_attn_kernel<FMT, 2><<<grid, KVA_THREADS, 0, s>>>(w);
+        kv8_attn_kernel<FMT, 2><<<grid, KVA_THREADS, KVA_SMEM, s>>>(w);
 }
 
 cudaError_t kv8_attn_launch(const Kv8AttnArgs &args, void *ws, int num_sms, cudaStream_t s)
@@ -563,15 +676,38 @@ cudaError_t kv8_attn_launch(const Kv8AttnArgs &args, void *ws, int num_sms, cuda
         cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess)
             return e;
-        const int tiles = args.acc ? (w.a.n + KVA_ACC_TILE - 1) / KVA_ACC_TILE : 0;
-        kv8_join_kernel<<<(unsigned)(args.c.hkv * (w.p.rows + tiles)), KVA_JOIN, 0, s>>>(w);
-        e = cudaGetLastError();
+        const int tiles = args.acc ? (w.a.n + w.p.tile - 1) / w.p.tile : 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(args.c.hkv * (w.p.rows + tiles)));
+        cfg.blockDim = dim3(KVA_JOIN);
+        cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, kv8_join_kernel, w);
         if (e != cudaSuccess)
             return e;
     }
     return cudaSuccess;
 }
 
-cudaError_t kv8_prepare() { return cudaSuccess; }
+template <typename F> static cudaError_t kva_smem(F *f)
+{
+    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, KVA_SMEM);
+}
+
+cudaError_t kv8_prepare()
+{
+    cudaError_t e = kva_smem(kv8_attn_kernel<KV8_E4M3, 1>);
+    if (e == cudaSuccess)
+        e = kva_smem(kv8_attn_kernel<KV8_E4M3, 2>);
+    if (e == cudaSuccess)
+        e = kva_smem(kv8_attn_kernel<KV8_INT8, 1>);
+    if (e == cudaSuccess)
+        e = kva_smem(kv8_attn_kernel<KV8_INT8, 2>);
+    return e;
+}
 
 } // namespace ylm
