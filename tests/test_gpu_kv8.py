@@ -392,7 +392,9 @@ def test_attention_is_reproducible():
 @pytest.mark.parametrize("hkv,n,keep,sink,recent,block", [
     (1, 1, 1, 0, 0, 16), (2, 2, 1, 1, 0, 16), (2, 2, 1, 0, 1, 16), (3, 100, 37, 4, 8, 16), (8, 515, 200, 0, 0, 32),
     (2, 1000, 999, 3, 100, 64), (2, 1000, 1000, 0, 0, 128), (4, 700, 64, 32, 32, 128), (1, 5000, 2047, 4, 1024, 64),
-    (2, 1025, 1, 0, 0, 16), (2, 300, 0, 0, 0, 16), (1, 0, 0, 0, 0, 16), (1, 2048, 129, 129, 0, 32)])
+    (2, 1025, 1, 0, 0, 16), (2, 300, 0, 0, 0, 16), (1, 0, 0, 0, 0, 16), (1, 2048, 129, 129, 0, 32),
+    (2, 4097, 2000, 4, 100, 64), (1, 9000, 9000, 0, 9000, 16), (2, 12289, 5000, 300, 4500, 32),
+    (1, 40000, 15001, 4, 9000, 128), (3, 33333, 100, 0, 0, 64)])
 def test_evict(hkv, n, keep, sink, recent, block, fmt):
     rng = np.random.default_rng(n + keep)
     cap, cap_d = n + 9, keep + 50
@@ -416,9 +418,10 @@ def run_evict(c, ref, w, n, keep, sink, recent, cap_d):
 
 
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few", "special", "negative", "near"])
-def test_evict_ties_and_special_weights(kind):
+@pytest.mark.parametrize("size", [3001, 17000])
+def test_evict_ties_and_special_weights(kind, size):
     rng = np.random.default_rng(4)
-    n, hkv = 3001, 2
+    n, hkv = size, 2
     c, ref = filled(rng, "e4m3", 16, n, hkv, n)
     w = np.zeros((hkv, n), np.float32)
     if kind == "equal":
@@ -432,7 +435,7 @@ def test_evict_ties_and_special_weights(kind):
         w[:] = rng.standard_normal((hkv, n))
     elif kind == "near":  # differ in the last bits only
         w[:] = (np.float32(1.0).view(np.uint32) + rng.integers(0, 500, (hkv, n)).astype(np.uint32)).view(np.float32)
-    for keep, sink, recent in ((1500, 4, 64), (10, 0, 0), (2900, 0, 1)):
+    for keep, sink, recent in ((n // 2, 4, 64), (10, 0, 0), (n - 101, 0, 1), (70, 6, 64), (n - 1, 2, 2)):
         run_evict(c, ref, w, n, keep, sink, recent, keep + 3)
 
 

@@ -1,6 +1,7 @@
 // The 8-bit K/V cache: storing rows and evicting slots (attention over it:
 // kv8_attention.cu; formats and the power-of-two scales: kv8.cuh).
 #include "kv8.cuh"
+#include <cooperative_groups.h>
 
 namespace ylm {
 
@@ -120,15 +121,12 @@ cudaError_t kv8_store_launch(const Kv8Cache &c, const __half *k, const __half *v
 }
 
 // ------------------------------------------------------------------ eviction
-// The kept slots of one KV head: the first n_sink, the last n_recent, and of the
-// others those of the largest accumulated weight, ties to the lower slot.
-// A slot's key is 0xFFFFFFFF where it is protected, else the weight's bits in
-// an order-preserving form (NaN, as the smallest, and -0 as +0).
-__device__ __forceinline__ uint32_t evict_key(const float *acc, int i, int n_sink, int first_recent)
+// The kept slots of one KV head: the first n_sink, the last n_recent (both
+// protected: their weights are not looked at), and of the others those of the largest
+// accumulated weight, ties to the lower slot. A weight's key is its bits in an
+// order-preserving form (NaN, as the smallest, and -0 as +0).
+__device__ __forceinline__ uint32_t evict_key(float a)
 {
-    if (i < n_sink || i >= first_recent)
-        return 0xFFFFFFFFu;
-    const float a = acc[i];
     if (a != a)
         return 0u;
     const uint32_t u = __float_as_uint(a + 0.f);
@@ -136,99 +134,188 @@ __device__ __forceinline__ uint32_t evict_key(const float *acc, int i, int n_sin
 }
 
 constexpr int KEV_THREADS = 1024;
+constexpr int KEV_WARPS = KEV_THREADS / 32;
+constexpr int KEV_BINS = 2048;  // a radix step finds 11 bits of the key (the last one 10)
+constexpr int KEV_MAXC = 8;     // largest cluster (the portable size)
+constexpr int KEV_SLICE = 4096; // slots per CTA below which a KV head takes fewer CTAs
 
-// One CTA per KV head: the key of the n_keep-th slot by four 8-bit radix steps
-// (the histogram of a digit over the keys that share the digits found so
-// far), then the kept slots in ascending order by block scans.
+// Exclusive scan over the CTA in thread order; *total gets the sum. The sums fit 32 bits.
+__device__ __forceinline__ int kev_scan(int v, int *warp_sums, int *total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        x += lane >= o ? y : 0;
+    }
+    __syncthreads();
+    if (lane == 31)
+        warp_sums[warp] = x;
+    __syncthreads();
+    int s = warp_sums[lane]; // KEV_WARPS == 32: every warp scans the warps' sums
+    const int own = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const int y = __shfl_up_sync(0xffffffffu, s, o);
+        s += lane >= o ? y : 0;
+    }
+    *total = __shfl_sync(0xffffffffu, s, 31);
+    return x - v + __shfl_sync(0xffffffffu, s - own, warp);
+}
+
+// One cluster per KV head, a contiguous slice of the slots per CTA. The key of the
+// n_keep-th slot is found in three radix steps of 11, 11 and 10 bits: each CTA counts a
+// digit over its keys that share the digits found so far and adds the counts that are
+// not 0 (few: weights share few exponents) to every CTA's sums, in which each
+// CTA then finds the digit. One cluster barrier a step, as each step has sums of its
+// own. The kept slots are then placed in order, a warp taking consecutive slots (the
+// slice stays in L1 between the passes).
 __global__ void __launch_bounds__(KEV_THREADS) kv8_select_kernel(Kv8EvictArgs a)
 {
-    __shared__ int hist[256];
-    __shared__ uint32_t sel_prefix;
-    __shared__ int sel_need, wsum[2][KEV_THREADS / 32];
-    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ int hist[KEV_BINS], sums[3][KEV_BINS];
+    __shared__ int warp_sums[KEV_WARPS];
+    __shared__ int found[2];              // digit, and how many keys of it are kept
+    __shared__ int counts[2][KEV_MAXC];   // keys above and equal to the n_keep-th, of every CTA
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)gridDim.x, rank = (int)blockIdx.x, g = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
     const float *acc = a.acc_src + (size_t)g * a.src.cap;
     float *acc_dst = a.acc_dst + (size_t)g * a.dst.cap;
-    const int recent = a.n - a.n_recent;
-    uint32_t prefix = 0;
-    int need = a.n_keep; // of the keys equal to the prefix (so far), how many are kept
-    for (int shift = 24; shift >= 0 && a.n_keep > 0; shift -= 8)
-    {
-        if (tid < 256)
-            hist[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < a.n; i += KEV_THREADS)
-        {
-            const uint32_t key = evict_key(acc, i, a.n_sink, recent);
-            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-                atomicAdd(&hist[(key >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (tid == 0)
-        {
-            int b = 255;
-            while (b > 0 && need > hist[b])
-                need -= hist[b--];
-            sel_prefix = prefix | ((uint32_t)b << shift);
-            sel_need = need;
-        }
-        __syncthreads();
-        prefix = sel_prefix;
-        need = sel_need;
-    }
-    // kept: key > prefix, and the first `need` of key == prefix
-    int base_gt = 0, base_eq = 0;
-    for (int i0 = 0; i0 < a.n && a.n_keep > 0; i0 += KEV_THREADS)
-    {
-        const int i = i0 + tid;
-        uint32_t key = 0;
-        bool gt = false, eq = false;
-        if (i < a.n)
-        {
-            key = evict_key(acc, i, a.n_sink, recent);
-            gt = key > prefix;
-            eq = key == prefix;
-        }
-        const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0)
-        {
-            wsum[0][warp] = __popc(mg);
-            wsum[1][warp] = __popc(me);
-        }
-        __syncthreads();
-        int pg = base_gt, pe = base_eq;
-        for (int w = 0; w < KEV_THREADS / 32; w++)
-        {
-            if (w < warp)
-            {
-                pg += wsum[0][w];
-                pe += wsum[1][w];
-            }
-            base_gt += wsum[0][w];
-            base_eq += wsum[1][w];
-        }
-        __syncthreads();
-        const uint32_t below = (1u << lane) - 1u;
-        pg += __popc(mg & below);
-        pe += __popc(me & below);
-        if (gt || (eq && pe < need))
-        {
-            const int at = pg + min(pe, need);
-            a.kept[(size_t)g * a.n_keep + at] = i;
-            acc_dst[at] = acc[i];
-        }
-    }
-    for (int i = a.n_keep + tid; i < a.dst.cap; i += KEV_THREADS)
+    const int recent = a.n - a.n_recent, per = (a.n + C - 1) / C;
+    const int i0 = min(a.n, rank * per), i1 = min(a.n, i0 + per);
+    for (int i = a.n_keep + rank * KEV_THREADS + tid; i < a.dst.cap; i += C * KEV_THREADS)
         acc_dst[i] = 0.f;
+    if (a.n_keep == 0)
+        return; // every CTA of every cluster
+    for (int i = tid; i < KEV_BINS; i += KEV_THREADS)
+        hist[i] = sums[0][i] = sums[1][i] = sums[2][i] = 0;
+    if (C > 1) // the sums are 0 before another CTA adds to them: waited for before the first addition
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    uint32_t prefix = 0, known = 0;              // digits found, and the bits that they cover
+    int need = a.n_keep - a.n_sink - a.n_recent; // of the keys equal to the prefix (so far), how many are kept
+    if (need == 0)
+        prefix = 0xFFFFFFFFu; // above every key
+    if (need == 0 && C > 1)
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int lo = max(i0, a.n_sink), hi_end = min(i1, recent);
+#pragma unroll 1
+    for (int step = 0; step < 3 && need > 0; step++)
+    {
+        const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bins = step < 2 ? 2048 : 1024;
+        int *mine = C > 1 ? hist : sums[step];
+        __syncthreads();
+#pragma unroll 4
+        for (int i = lo + tid; i < hi_end; i += KEV_THREADS)
+        {
+            const uint32_t key = evict_key(acc[i]);
+            if ((key & known) == prefix)
+                atomicAdd(&mine[(key >> shift) & (bins - 1)], 1);
+        }
+        __syncthreads();
+        if (C > 1)
+        {
+            if (step == 0)
+                asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            for (int i = tid; i < bins; i += KEV_THREADS)
+            {
+                const int v = hist[i];
+                hist[i] = 0;
+                if (v)
+                    for (int c = 0; c < C; c++)
+                        atomicAdd(cl.map_shared_rank(&sums[step][i], c), v);
+            }
+            cl.sync();
+        }
+        // thread t looks at the bins from the top: bins - 1 - 2t and the next one below
+        const int hi = bins - 1 - 2 * tid;
+        const int n1 = hi > 0 ? sums[step][hi] : 0, n0 = hi > 0 ? sums[step][hi - 1] : 0;
+        int all;
+        const int above = kev_scan(n0 + n1, warp_sums, &all);
+        if (hi > 0 && above < need && above + n1 + n0 >= need)
+        {
+            const bool upper = above + n1 >= need;
+            found[0] = upper ? hi : hi - 1;
+            found[1] = need - above - (upper ? 0 : n1);
+        }
+        __syncthreads();
+        prefix |= (uint32_t)found[0] << shift;
+        known |= (uint32_t)(bins - 1) << shift;
+        need = found[1];
+    }
+
+    // kept: key > prefix, and the first `need` of key == prefix. A warp takes consecutive slots.
+    const int each = ((i1 - i0 + KEV_WARPS - 1) / KEV_WARPS + 31) / 32 * 32;
+    const int w0 = min(i1, i0 + warp * each), w1 = min(i1, w0 + each);
+    auto look = [&](int i, float &x, bool &more, bool &same) {
+        x = i < w1 ? acc[i] : 0.f;
+        const bool held = i < a.n_sink || i >= recent;
+        const uint32_t key = evict_key(x);
+        more = i < w1 && (held || key > prefix);
+        same = i < w1 && !held && key == prefix;
+    };
+    int gt = 0, eq = 0;
+#pragma unroll 4
+    for (int i = w0 + lane; i - lane < w1; i += 32)
+    {
+        float x;
+        bool more, same;
+        look(i, x, more, same);
+        gt += more;
+        eq += same;
+    }
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    int gt_all, eq_all;
+    gt = __shfl_sync(0xffffffffu, kev_scan(lane == 0 ? gt : 0, warp_sums, &gt_all), 0);
+    eq = __shfl_sync(0xffffffffu, kev_scan(lane == 0 ? eq : 0, warp_sums, &eq_all), 0);
+    if (C > 1)
+    {
+        if (tid < C)
+        {
+            *cl.map_shared_rank(&counts[0][rank], tid) = gt_all;
+            *cl.map_shared_rank(&counts[1][rank], tid) = eq_all;
+        }
+        cl.sync();
+        for (int c = 0; c < rank; c++)
+        {
+            gt += counts[0][c];
+            eq += counts[1][c];
+        }
+    }
+    const uint32_t below = (1u << lane) - 1u;
+#pragma unroll 4
+    for (int i = w0 + lane; i - lane < w1; i += 32)
+    {
+        float x;
+        bool more, same;
+        look(i, x, more, same);
+        const uint32_t mg = __ballot_sync(0xffffffffu, more), me = __ballot_sync(0xffffffffu, same);
+        const int eq_at = eq + __popc(me & below);
+        if (more || (same && eq_at < need))
+        {
+            const int at = gt + __popc(mg & below) + min(eq_at, need);
+            a.kept[(size_t)g * a.n_keep + at] = i;
+            acc_dst[at] = x;
+        }
+        gt += __popc(mg);
+        eq += __popc(me);
+    }
 }
 
 // One CTA per (destination block, KV head, K or V): the block's scale is the
 // largest of its tokens' old scales, and a token whose old block had a smaller
-// one is rescaled to it. Eight threads move a token's 128 codes.
+// one is rescaled to it. Eight threads move a token's 128 codes, which are on
+// their way before the scales are known.
 template <int FMT> __global__ void __launch_bounds__(256) kv8_move_kernel(Kv8EvictArgs a)
 {
     __shared__ int from[128];
     __shared__ float old[128];
-    __shared__ float top;
+    __shared__ float tops[4];
     const bool is_v = blockIdx.z != 0;
     const int g = blockIdx.y, b = blockIdx.x, tid = threadIdx.x;
     const int block = a.src.block, lo = b * block, m = min(block, a.n_keep - lo);
@@ -236,54 +323,73 @@ template <int FMT> __global__ void __launch_bounds__(256) kv8_move_kernel(Kv8Evi
     const float *src_scale = (is_v ? a.src.v_scale : a.src.k_scale) + (size_t)g * src_blocks;
     const uint8_t *src = (is_v ? a.src.v : a.src.k) + (size_t)g * a.src.cap * YLM_HEAD_DIM;
     uint8_t *dst = (is_v ? a.dst.v : a.dst.k) + ((size_t)g * a.dst.cap + lo) * YLM_HEAD_DIM;
+    pdl_wait();
+    int f = 0;
     if (tid < m)
+        from[tid] = f = a.kept[(size_t)g * a.n_keep + lo + tid];
+    __syncthreads();
+    uint4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
     {
-        from[tid] = a.kept[(size_t)g * a.n_keep + lo + tid];
-        old[tid] = src_scale[from[tid] / block];
+        const int i = (tid >> 3) + 32 * k;
+        if (i < m)
+            x[k] = *reinterpret_cast<const uint4 *>(src + (size_t)from[i] * YLM_HEAD_DIM + (tid & 7) * 16);
+    }
+    if (tid < 128)
+    {
+        const float s = tid < m ? src_scale[f / block] : 0.f;
+        old[tid] = s;
+        const float t = warp_max(s);
+        if ((tid & 31) == 0)
+            tops[tid >> 5] = t;
     }
     __syncthreads();
-    if (tid < 32)
+    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), inv = top > 0.f ? 1.f / top : 1.f;
+    if (tid == 0)
+        ((is_v ? a.dst.v_scale : a.dst.k_scale) + (size_t)g * dst_blocks)[b] = top;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
     {
-        float s = 0.f;
-        for (int i = tid; i < m; i += 32)
-            s = fmaxf(s, old[i]);
-        s = warp_max(s);
-        if (tid == 0)
-        {
-            top = s;
-            ((is_v ? a.dst.v_scale : a.dst.k_scale) + (size_t)g * dst_blocks)[b] = s;
-        }
-    }
-    __syncthreads();
-    const float inv = top > 0.f ? 1.f / top : 1.f;
-    for (int e = tid; e < m * 8; e += 256)
-    {
-        const int i = e >> 3, c = e & 7;
-        uint4 x = *reinterpret_cast<const uint4 *>(src + (size_t)from[i] * YLM_HEAD_DIM + c * 16);
+        const int i = (tid >> 3) + 32 * k;
+        if (i >= m)
+            continue;
         if (old[i] != top)
         {
             const float ratio = old[i] * inv;
-            x.x = kv8_rescale4<FMT>(x.x, ratio);
-            x.y = kv8_rescale4<FMT>(x.y, ratio);
-            x.z = kv8_rescale4<FMT>(x.z, ratio);
-            x.w = kv8_rescale4<FMT>(x.w, ratio);
+            x[k].x = kv8_rescale4<FMT>(x[k].x, ratio);
+            x[k].y = kv8_rescale4<FMT>(x[k].y, ratio);
+            x[k].z = kv8_rescale4<FMT>(x[k].z, ratio);
+            x[k].w = kv8_rescale4<FMT>(x[k].w, ratio);
         }
-        *reinterpret_cast<uint4 *>(dst + (size_t)i * YLM_HEAD_DIM + c * 16) = x;
+        *reinterpret_cast<uint4 *>(dst + (size_t)i * YLM_HEAD_DIM + (tid & 7) * 16) = x[k];
     }
 }
 
 cudaError_t kv8_evict_launch(const Kv8EvictArgs &a, cudaStream_t s)
 {
-    kv8_select_kernel<<<(unsigned)a.src.hkv, KEV_THREADS, 0, s>>>(a);
-    cudaError_t e = cudaGetLastError();
+    int C = 1;
+    while (C < KEV_MAXC && a.n > C * KEV_SLICE)
+        C *= 2;
+    cudaLaunchAttribute at[1];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)C, (unsigned)a.src.hkv);
+    cfg.blockDim = dim3(KEV_THREADS);
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_select_kernel, a);
     if (e != cudaSuccess || a.n_keep == 0)
         return e;
-    const dim3 grid((unsigned)((a.n_keep + a.src.block - 1) / a.src.block), (unsigned)a.src.hkv, 2);
-    if (a.src.format == KV8_E4M3)
-        kv8_move_kernel<KV8_E4M3><<<grid, 256, 0, s>>>(a);
-    else
-        kv8_move_kernel<KV8_INT8><<<grid, 256, 0, s>>>(a);
-    return cudaGetLastError();
+    cfg.gridDim = dim3((unsigned)((a.n_keep + a.src.block - 1) / a.src.block), (unsigned)a.src.hkv, 2);
+    cfg.blockDim = dim3(256);
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    return a.src.format == KV8_E4M3 ? cudaLaunchKernelEx(&cfg, kv8_move_kernel<KV8_E4M3>, a)
+                                    : cudaLaunchKernelEx(&cfg, kv8_move_kernel<KV8_INT8>, a);
 }
 
 } // namespace ylm
