@@ -43,34 +43,33 @@ template <int FMT> __device__ __forceinline__ uint32_t kv8_encode2(float lo, flo
         return (uint32_t)(__float2int_rn(lo) & 0xFF) | ((uint32_t)(__float2int_rn(hi) & 0xFF) << 8);
 }
 
-// Two codes (low half of c) to two FP16 numbers, exactly.
-template <int FMT> __device__ __forceinline__ uint32_t kv8_decode2(uint32_t c)
+// Four codes to four FP16 numbers, exactly: codes 0 and 1 in lo, 2 and 3 in hi.
+template <int FMT> __device__ __forceinline__ void kv8_decode4(uint32_t c, uint32_t &lo, uint32_t &hi)
 {
-    uint32_t r;
     if constexpr (FMT == KV8_E4M3)
-        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(c));
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(c));
     else
     {
         // biased byte u = code + 128 under the exponent of 1024: the half 1024 + u, less 1152
-        const uint32_t h = __byte_perm(c ^ 0x8080u, 0x64646464u, 0x4140);
-        const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&h), __floats2half2_rn(1152.f, 1152.f));
-        r = *reinterpret_cast<const uint32_t *>(&d);
+        const uint32_t u = c ^ 0x80808080u, h0 = __byte_perm(u, 0x64646464u, 0x4140), h1 = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
+        const __half2 d0 = __hsub2(*reinterpret_cast<const __half2 *>(&h0), bias);
+        const __half2 d1 = __hsub2(*reinterpret_cast<const __half2 *>(&h1), bias);
+        lo = *reinterpret_cast<const uint32_t *>(&d0);
+        hi = *reinterpret_cast<const uint32_t *>(&d1);
     }
-    return r;
 }
 
 // Four codes to the codes of code * ratio (ratio <= 1 where the scale grew).
 template <int FMT> __device__ __forceinline__ uint32_t kv8_rescale4(uint32_t c, float ratio)
 {
-    uint32_t out = 0;
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-    {
-        const uint32_t d = kv8_decode2<FMT>(i ? c >> 16 : c);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&d));
-        out |= kv8_encode2<FMT>(f.x * ratio, f.y * ratio) << (16 * i);
-    }
-    return out;
+    uint32_t lo, hi;
+    kv8_decode4<FMT>(c, lo, hi);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&lo));
+    const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    return kv8_encode2<FMT>(f.x * ratio, f.y * ratio) | kv8_encode2<FMT>(g.x * ratio, g.y * ratio) << 16;
 }
 
 } // namespace ylm

@@ -21,7 +21,7 @@ constexpr int KVA_CHUNK = 32;     // slots a warp takes at a time
 constexpr int KVA_BUF = KVA_CHUNK * YLM_HEAD_DIM; // bytes of a chunk's K or V
 constexpr int KVA_RING = 4 * KVA_BUF;             // a warp's two K and two V chunks
 constexpr int KVA_SMEM = KVA_WARPS * KVA_RING;
-constexpr int KVA_JOIN = 128;     // threads of the joining CTAs
+constexpr int KVA_JOIN = 256;     // threads of the joining CTAs
 
 struct Kv8Plan
 {
@@ -30,6 +30,7 @@ struct Kv8Plan
     int zblocks;      // CTAs over the rows of a KV head
     int splits, len;  // splits of the slots and slots per split
     int pad;          // rows, rounded up to a multiple of 4: stride of the kept scores and of (M, l)
+    int lps;          // lanes that share a slot's rows in the accumulation, four rows a load
     int tile;         // slots per CTA of the accumulation
     size_t ml_off, score_off, bytes;
 };
@@ -59,7 +60,9 @@ static Kv8Plan kv8_plan(int hkv, int hq, int t, int n, bool acc, int num_sms)
     p.ml_off = most * p.rows * YLM_HEAD_DIM * sizeof(float);
     p.score_off = p.ml_off + (most * p.pad * 2 * sizeof(float) + 255) / 256 * 256;
     // slots per accumulating CTA: about four CTAs per SM, each of which finds every row's state first
-    p.tile = std::max(KVA_JOIN, (int)(((int64_t)hkv * n / (num_sms * 4) + KVA_JOIN - 1) / KVA_JOIN) * KVA_JOIN);
+    p.lps = !acc || p.pad < 8 ? 1 : p.pad < 32 ? 2 : p.pad < 64 ? 8 : 16;
+    const int round = 4 * KVA_JOIN / p.lps;
+    p.tile = std::max(1, (int)(((int64_t)hkv * n / (num_sms * 4) + round - 1) / round)) * round;
     p.bytes = p.score_off + (acc ? (size_t)hkv * n * p.pad * sizeof(float) : 0);
     return p;
 }
@@ -188,6 +191,8 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
     // this lane copies piece lane % 8 of rows 4 i + lane / 8: f there for even i, and for odd i
     const uint32_t dst_even = (lane >> 3) * 128 + (((lane & 7) ^ (((lane >> 4) & 1) << 1) ^ ((lane >> 3 & 1) << 2)) << 4);
     const uint32_t dst_odd = (lane >> 3) * 128 + (((lane & 7) ^ ((2 + ((lane >> 4) & 1)) << 1) ^ ((lane >> 3 & 1) << 2)) << 4);
+    // a step reads the codes once; what it writes for the join should stay in L2
+    const uint64_t policy = l2_policy_evict_first();
     auto copy = [&](const uint8_t *src, int j0, uint32_t at) {
         const int r0 = j0 + (lane >> 3);
         const uint8_t *p = src + (size_t)r0 * YLM_HEAD_DIM + (lane & 7) * 16;
@@ -195,8 +200,9 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
         {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i * 512 + (i & 1 ? dst_odd : dst_even)),
-                             "l"(p + i * 512)
+                asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(
+                                 at + i * 512 + (i & 1 ? dst_odd : dst_even)),
+                             "l"(p + i * 512), "l"(policy)
                              : "memory");
         }
         else
@@ -282,9 +288,9 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
 #pragma unroll
             for (int j = 0; j < 8; j++)
             {
-                const uint32_t lo = kva_word(K[j >> 2], j & 3), hi = kva_word(K[2 + (j >> 2)], j & 3);
-                const uint32_t a0 = kv8_decode2<FMT>(lo), a2 = kv8_decode2<FMT>(lo >> 16);
-                const uint32_t a1 = kv8_decode2<FMT>(hi), a3 = kv8_decode2<FMT>(hi >> 16);
+                uint32_t a0, a1, a2, a3;
+                kv8_decode4<FMT>(kva_word(K[j >> 2], j & 3), a0, a2);
+                kv8_decode4<FMT>(kva_word(K[2 + (j >> 2)], j & 3), a1, a3);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
                     kva_mma(S[s][t], a0, a1, a2, a3, q[t][j][0], q[t][j][1]);
@@ -385,13 +391,14 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
 #pragma unroll
             for (int t = 0; t < NT; t++)
             {
+                // nothing seen so far: M = -inf, and every weight 0
+                const float shift[2] = {vs[s] - (M[t][0] == -INFINITY ? 0.f : M[t][0]),
+                                        vs[s] - (M[t][1] == -INFINITY ? 0.f : M[t][1])};
                 float e4[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                 {
-                    // nothing seen so far: M = -inf, and every weight 0
-                    const float m = M[t][e & 1];
-                    e4[e] = kva_ex2(S[s][t][e] + (vs[s] - (m == -INFINITY ? 0.f : m)));
+                    e4[e] = kva_ex2(S[s][t][e] + shift[e & 1]);
                 }
                 l[t][0] += (e4[0] + e4[2]) * unscale;
                 l[t][1] += (e4[1] + e4[3]) * unscale;
@@ -439,12 +446,14 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                         const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
                         const uint32_t x = __byte_perm(flag[i >> 1], flag[4 + (i >> 1)], sel);
                         const uint32_t y = __byte_perm(flag[8 + (i >> 1)], flag[12 + (i >> 1)], sel);
+                        uint32_t a0, a1, a2, a3;
+                        kv8_decode4<FMT>(x, a0, a1);
+                        kv8_decode4<FMT>(y, a2, a3);
 #pragma unroll
                         for (int t = 0; t < NT; t++)
                         {
                             float d[4] = {0.f, 0.f, 0.f, 0.f};
-                            kva_mma(d, kv8_decode2<FMT>(x), kv8_decode2<FMT>(x >> 16), kv8_decode2<FMT>(y),
-                                    kv8_decode2<FMT>(y >> 16), seen[t][0], seen[t][1]);
+                            kva_mma(d, a0, a1, a2, a3, seen[t][0], seen[t][1]);
 #pragma unroll
                             for (int e = 0; e < 4; e++)
                                 if (d[e] > 0.f)
@@ -459,8 +468,9 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                 const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
                 const uint32_t x = __byte_perm(kva_word(V[0], i >> 1), kva_word(V[1], i >> 1), sel);
                 const uint32_t y = __byte_perm(kva_word(V[2], i >> 1), kva_word(V[3], i >> 1), sel);
-                const uint32_t a0 = kv8_decode2<FMT>(x), a1 = kv8_decode2<FMT>(x >> 16);
-                const uint32_t a2 = kv8_decode2<FMT>(y), a3 = kv8_decode2<FMT>(y >> 16);
+                uint32_t a0, a1, a2, a3;
+                kv8_decode4<FMT>(x, a0, a1);
+                kv8_decode4<FMT>(y, a2, a3);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
                     kva_mma(O[t][i], a0, a1, a2, a3, P[t][0], P[t][1]);
@@ -523,11 +533,13 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
 }
 
 // Joins the splits. CTAs [0, hkv * rows) write one output row each: every warp
-// finds the row's M and l from the splits' (a lane each), then takes every fourth
+// finds the row's M and l from the splits' (a lane each), then takes every eighth
 // split's O, four dimensions a lane. The others add the weights of p.tile
-// slots of one KV head to acc: first the M and 1 / l of every row, by all threads.
-__global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(const Kv8Pass w)
+// slots of one KV head to acc: first the M and 1 / l of every row, by all threads,
+// then the slots, each by the LPS lanes (a power of two) that share its rows.
+template <int LPS> __global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(const Kv8Pass w)
 {
+    constexpr int WARPS = KVA_JOIN / 32;
     const Kv8AttnArgs &a = w.a;
     const int G = w.p.G, R = w.p.rows, S = w.p.splits, pad = w.p.pad;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -536,7 +548,7 @@ __global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(const Kv8Pass w)
     pdl_wait();
     if (b < rows)
     {
-        __shared__ float4 om[KVA_JOIN / 32][32];
+        __shared__ float4 om[WARPS][32];
         const int g = b / R, r = b % R;
         const float2 *ml = reinterpret_cast<const float2 *>(w.ml) + (size_t)g * S * pad + r;
         const float4 *part = reinterpret_cast<const float4 *>(w.part) + (size_t)b * S * (YLM_HEAD_DIM / 4) + lane;
@@ -551,10 +563,10 @@ __global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(const Kv8Pass w)
             const float f = x.x == -INFINITY ? 0.f : kva_ex2(x.x - M);
             L += x.y * f;
 #pragma unroll
-            for (int k = 0; k < 8; k++)
+            for (int k = 0; k < 32 / WARPS; k++)
             {
-                const int s = s0 + 4 * k + warp;
-                const float fs = __shfl_sync(0xffffffffu, f, 4 * k + warp);
+                const int s = s0 + WARPS * k + warp;
+                const float fs = __shfl_sync(0xffffffffu, f, WARPS * k + warp);
                 if (s < S)
                 {
                     const float4 v = part[(size_t)s * (YLM_HEAD_DIM / 4)];
@@ -568,17 +580,36 @@ __global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(const Kv8Pass w)
         L = warp_sum(L);
         om[warp][lane] = o;
         __syncthreads();
-        const float *of = reinterpret_cast<const float *>(om);
-        const float sum = (of[tid] + of[128 + tid]) + (of[256 + tid] + of[384 + tid]);
-        a.out[(r / G) * a.out_stride + (size_t)(g * G + r % G) * YLM_HEAD_DIM + tid] =
-            f2h(M == -INFINITY ? sum : sum / L); // no slot seen: 0
+        if (tid < YLM_HEAD_DIM)
+        {
+            const float *of = reinterpret_cast<const float *>(om);
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < WARPS; k++)
+                sum += of[k * YLM_HEAD_DIM + tid];
+            a.out[(r / G) * a.out_stride + (size_t)(g * G + r % G) * YLM_HEAD_DIM + tid] =
+                f2h(M == -INFINITY ? sum : sum / L); // no slot seen: 0
+        }
         return;
     }
-    __shared__ float2 state[128], join[KVA_JOIN];
+    __shared__ __align__(16) float2 state[128];
+    __shared__ float2 join[KVA_JOIN];
     b -= rows;
     const int tiles = (a.n + w.p.tile - 1) / w.p.tile;
     const int g = b / tiles, j0 = b % tiles * w.p.tile, j1 = min(a.n, j0 + w.p.tile);
-    const int parts = KVA_JOIN / pad, part = tid / pad, r = tid % pad;
+    float *acc = a.acc + (size_t)g * a.c.cap;
+    const float4 *x = reinterpret_cast<const float4 *>(w.scores) + (size_t)g * a.n * (pad / 4);
+    constexpr int U = 4, PER = KVA_JOIN / LPS; // slots in flight per thread, slots per round of the CTA
+    const int l = tid % LPS;
+    // the first scores are on their way while the state is found
+    float4 v[U];
+    auto load = [&](int j, int i) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            v[u] = x[(size_t)min(j + u * PER, j1 - 1) * (pad / 4) + i];
+    };
+    load(j0 + tid / LPS, l);
+    const int parts = min(16, KVA_JOIN / pad), part = tid / pad, r = tid % pad;
     if (part < parts)
     {
         const float2 *ml = reinterpret_cast<const float2 *>(w.ml) + (size_t)g * S * pad + r;
@@ -603,45 +634,42 @@ __global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(const Kv8Pass w)
         const float ref = M == -INFINITY ? 0.f : M;
         for (int p = 0; p < parts; p++)
             L += join[p * pad + tid].y * kva_ex2(join[p * pad + tid].x - ref);
-        // a row that sees nothing, and one that is not there, weigh nothing
+        // a row that sees nothing weighs nothing
         state[tid] = M == -INFINITY ? make_float2(0.f, 0.f) : make_float2(M, 1.f / L);
     }
     __syncthreads();
-    float *acc = a.acc + (size_t)g * a.c.cap;
-    const float4 *x = reinterpret_cast<const float4 *>(w.scores) + (size_t)g * a.n * (pad / 4);
-    constexpr int U = 4; // slots of a thread whose loads are in flight together
-    for (int j = j0 + tid; j < j1; j += KVA_JOIN * U)
+    const float4 *st = reinterpret_cast<const float4 *>(state); // two rows each
+    for (int jb = j0; jb < j1; jb += PER * U)
     {
-        float sum[U], old[U];
-#pragma unroll
-        for (int u = 0; u < U; u++)
+        const int j = jb + tid / LPS;
+        float sum[U] = {};
+        for (int i = l; i < pad / 4; i += LPS)
         {
-            sum[u] = 0.f;
-            old[u] = j + u * KVA_JOIN < j1 ? acc[j + u * KVA_JOIN] : 0.f;
-        }
-        for (int i = 0; i < pad; i += 4)
-        {
-            float4 v[U];
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                v[u] = x[(size_t)min(j + u * KVA_JOIN, j1 - 1) * (pad / 4) + (i >> 2)];
+            if (jb > j0 || i > l)
+                load(j, i);
+            const float4 s0 = st[2 * i], s1 = st[2 * i + 1];
 #pragma unroll
             for (int u = 0; u < U; u++)
             {
-                sum[u] += kva_ex2(v[u].x - state[i].x) * state[i].y;
+                sum[u] += kva_ex2(v[u].x - s0.x) * s0.y;
                 // rows that are not there: whatever their scores hold must not count
-                if (i + 1 < R)
-                    sum[u] += kva_ex2(v[u].y - state[i + 1].x) * state[i + 1].y;
-                if (i + 2 < R)
-                    sum[u] += kva_ex2(v[u].z - state[i + 2].x) * state[i + 2].y;
-                if (i + 3 < R)
-                    sum[u] += kva_ex2(v[u].w - state[i + 3].x) * state[i + 3].y;
+                if (4 * i + 1 < R)
+                    sum[u] += kva_ex2(v[u].y - s0.z) * s0.w;
+                if (4 * i + 2 < R)
+                    sum[u] += kva_ex2(v[u].z - s1.x) * s1.y;
+                if (4 * i + 3 < R)
+                    sum[u] += kva_ex2(v[u].w - s1.z) * s1.w;
             }
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (j + u * KVA_JOIN < j1)
-                acc[j + u * KVA_JOIN] = old[u] + sum[u];
+        {
+#pragma unroll
+            for (int o = 1; o < LPS; o <<= 1)
+                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+            if (l == 0 && j + u * PER < j1)
+                acc[j + u * PER] += sum[u];
+        }
     }
 }
 
@@ -686,7 +714,10 @@ cudaError_t kv8_attn_launch(const Kv8AttnArgs &args, void *ws, int num_sms, cuda
         at[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = at;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, kv8_join_kernel, w);
+        e = w.p.lps == 1   ? cudaLaunchKernelEx(&cfg, kv8_join_kernel<1>, w)
+            : w.p.lps == 2 ? cudaLaunchKernelEx(&cfg, kv8_join_kernel<2>, w)
+            : w.p.lps == 8 ? cudaLaunchKernelEx(&cfg, kv8_join_kernel<8>, w)
+                           : cudaLaunchKernelEx(&cfg, kv8_join_kernel<16>, w);
         if (e != cudaSuccess)
             return e;
     }
