@@ -26,7 +26,7 @@ constexpr int KVA_JOIN = 256;     // threads of the joining CTAs
 struct Kv8Plan
 {
     int G, rows;      // query heads per KV head, rows per KV head of a pass (G * tokens)
-    int nt, rg;       // 8-row tiles per warp, warps of a CTA that take different rows
+    int nt;           // 8-row tiles per CTA, 1 or 2
     int zblocks;      // CTAs over the rows of a KV head
     int splits, len;  // splits of the slots and slots per split
     int pad;          // rows, rounded up to a multiple of 4: stride of the kept scores and of (M, l)
@@ -46,9 +46,9 @@ static Kv8Plan kv8_plan(int hkv, int hq, int t, int n, bool acc, int num_sms)
     p.G = hq / hkv;
     p.rows = p.G * t;
     p.nt = p.rows <= 8 ? 1 : 2;
-    p.rg = p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
-    p.zblocks = (p.rows + 8 * p.nt * p.rg - 1) / (8 * p.nt * p.rg);
-    const int unit = KVA_CHUNK * (KVA_WARPS / p.rg); // slots of one round of a CTA's warps
+    p.zblocks = (p.rows + 8 * p.nt - 1) / (8 * p.nt);
+    const int unit = KVA_CHUNK * KVA_WARPS; // slots of one round of a CTA's warps
+    // one wave of CTAs: as many as the SMs hold
     const int64_t groups = (int64_t)hkv * p.zblocks;
     const int want = (int)std::max<int64_t>(1, (int64_t)num_sms * (p.nt == 1 ? 3 : 2) / groups);
     p.len = std::max(1, ((n + want - 1) / want + unit - 1) / unit) * unit;
@@ -120,7 +120,8 @@ __device__ __forceinline__ float kva_log_scale(float s)
 
 // Both products run on the tensor cores with the slots as rows of the A operand,
 // so that 8 query rows fill the N dimension: S^T = K Q^T and O^T = V^T P^T
-// (m16n8k16; NT tiles of 8 query rows share each decoded fragment). Lane
+// (m16n8k16; NT tiles of 8 query rows share each decoded fragment; more rows
+// than 16 go to CTAs of their own, which read the codes from L2 again). Lane
 // (g, c) = (lane / 4, lane % 4).
 //  S^T: the head dimension is summed in a permuted order in which every A
 //    fragment comes from 16-byte loads of code rows: lane (g, c) loads
@@ -148,9 +149,8 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
     const Kv8AttnArgs &a = w.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int sp = blockIdx.x, kvh = blockIdx.y;
-    const int RG = w.p.rg, subs = KVA_WARPS / RG, sub = warp / RG;
     const int R = w.p.rows, G = w.p.G;
-    const int row0 = ((int)blockIdx.z * RG + warp % RG) * 8 * NT; // first of this warp's rows
+    const int row0 = (int)blockIdx.z * 8 * NT; // first of this CTA's rows
     const int n = a.n, first = n - a.t;                           // slots >= first are hidden from some row
     const int j_end = min(n, (sp + 1) * w.p.len);
     const int nb = (a.c.cap + a.c.block - 1) / a.c.block, bshift = 31 - __clz(a.c.block);
@@ -247,10 +247,10 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
         M[t][0] = M[t][1] = -INFINITY;
         l[t][0] = l[t][1] = 0.f;
     }
-    const int step = KVA_CHUNK * subs;
-    int j0 = sp * w.p.len + sub * KVA_CHUNK;
+    constexpr int step = KVA_CHUNK * KVA_WARPS;
+    int j0 = sp * w.p.len + warp * KVA_CHUNK;
     int phase = 0; // the buffers of this round: 0 or 1
-    if (row0 < R && j0 < j_end)
+    if (j0 < j_end)
     {
         load_scales(j0);
 #pragma unroll
@@ -264,7 +264,7 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
             commit();
         }
     }
-    for (; row0 < R && j0 < j_end; j0 += step, phase ^= 1)
+    for (; j0 < j_end; j0 += step, phase ^= 1)
     {
         // in flight: this round's K and V, the next one's K and V
         asm volatile("cp.async.wait_group 3;" ::: "memory");
@@ -504,31 +504,28 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                     make_float2(O[t][k][i], O[t][k][i + 2]);
         }
     __syncthreads();
-    // a warp per row in turn, lane = 4 dimensions
-    for (int r = warp; r < RG * 8 * NT; r += KVA_WARPS)
+    // the warps' sums, joined: a warp per row in turn, lane = 4 dimensions
+    for (int r = warp; r < 8 * NT && row0 + r < R; r += KVA_WARPS)
     {
-        const int rg = r / (8 * NT), lr = r % (8 * NT), row = (int)blockIdx.z * RG * 8 * NT + r;
-        if (row >= R)
-            break;
-        float m = -INFINITY;
-        for (int s = 0; s < subs; s++)
-            m = fmaxf(m, mm[s * RG + rg][lr]);
-        float L = 0.f;
+        float m = mm[0][r], L = 0.f;
+#pragma unroll
+        for (int s = 1; s < KVA_WARPS; s++)
+            m = fmaxf(m, mm[s][r]);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < subs; s++)
+#pragma unroll
+        for (int s = 0; s < KVA_WARPS; s++)
         {
-            const float ms = mm[s * RG + rg][lr], f = ms == -INFINITY ? 0.f : kva_ex2(ms - m);
-            const float4 x = *reinterpret_cast<const float4 *>(&om[s * RG + rg][lr][lane * 4]);
-            // NaN that a slot with NaN codes put into O where no finite score was seen must stay
-            L += lm[s * RG + rg][lr] * f;
+            const float ms = mm[s][r], f = ms == -INFINITY ? 0.f : kva_ex2(ms - m);
+            const float4 x = *reinterpret_cast<const float4 *>(&om[s][r][lane * 4]);
+            L += lm[s][r] * f;
             o.x += x.x * f;
             o.y += x.y * f;
             o.z += x.z * f;
             o.w += x.w * f;
         }
-        *reinterpret_cast<float4 *>(w.part + (((size_t)kvh * R + row) * w.p.splits + sp) * YLM_HEAD_DIM + lane * 4) = o;
+        *reinterpret_cast<float4 *>(w.part + (((size_t)kvh * R + row0 + r) * w.p.splits + sp) * YLM_HEAD_DIM + lane * 4) = o;
         if (lane == 0)
-            *reinterpret_cast<float2 *>(w.ml + 2 * (((size_t)kvh * w.p.splits + sp) * w.p.pad + row)) = make_float2(m, L);
+            *reinterpret_cast<float2 *>(w.ml + 2 * (((size_t)kvh * w.p.splits + sp) * w.p.pad + row0 + r)) = make_float2(m, L);
     }
 }
 
