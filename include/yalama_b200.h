@@ -157,6 +157,15 @@ int ylm_set_sampling(ylm_engine *e, const ylm_sampling *s);
 /* ChatSession::Sample (ChatSession.cpp:560-593) on the current logits;
  * greedy = IsGreedy || first generated token (ChatSession.cpp:140). */
 int ylm_sample(ylm_engine *e, int32_t greedy, int64_t *next_id);
+/* Log probability of `id` on the current logits, the entropy of their softmax and the
+ * n_top (0..64) most likely ids, best first (ylm_k_logprobs; natural logarithms, host
+ * memory): what a service returns as a token's `logprobs` after ylm_sample,
+ * ylm_decode or ylm_infer. masked != 0: over the ids that ylm_set_sampling left
+ * unmasked; -inf for an id that is masked or outside the vocabulary. The state of
+ * the token loop does not change. Tensor parallel: gathers the logits first, as
+ * ylm_logits does. YLM_NOT_READY before the first logits. No counterpart in the reference. */
+int ylm_logprobs(ylm_engine *e, int64_t id, int32_t n_top, int32_t masked, float *logprob, float *entropy,
+                 int64_t *top_ids, float *top_logprobs);
 /* One decode step and its sample in one graph launch: Infer({id}) + Sample. */
 int ylm_decode(ylm_engine *e, int64_t id, int32_t greedy, int64_t *next_id);
 /* The token loop of ChatSession::Generate (ChatSession.cpp:113-230) on token

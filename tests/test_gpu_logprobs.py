@@ -215,3 +215,49 @@ def test_side_stream_and_captured_graph():
     torch.cuda.synchronize()
     for a, b, c in zip(want, got, cap):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_engine_logprobs_of_a_generated_token():
+    """ylm_logprobs after a prefill and after decode steps: the engine's own logits in 64 bits; masked ids left
+    out on request; neither the logits nor the tokens that follow change."""
+    from yalama_b200 import synth
+    spec = synth.tiny_spec("qwen3")
+    eng = E.Engine(None, E.config_from_spec(spec), init_seed=0)
+    with pytest.raises(E.YlmError) as ei:
+        eng.logprobs(0)
+    assert ei.value.status == E.Status.NOT_READY
+    prompt = synth.prompt_ids(0, 16, spec.vocab)
+    plain = eng.generate(prompt, 8)["ids"]
+    eng.set_sampling(greedy=True, masked_ids=[int(plain[1]), 3])
+    eng.begin_infer()
+    assert eng.infer(prompt)[0] == E.Status.OK
+    token, ids = eng.sample(True), []
+    rel = (spec.vocab / 128 + 72) * 2.0 ** -24 + 2.0 ** -21  # as in check()
+    for step in range(8):
+        x = eng.logits().astype(np.float64)[None]
+        for masked in (False, True):
+            seen = np.ones(spec.vocab, bool)
+            if masked:
+                seen[[int(plain[1]), 3]] = False
+            lp, ent, _, z = R.logprobs(x, seen)
+            got = eng.logprobs(token, 5, masked)
+            tol = rel + 2.0 ** -21 * (20 + ent[0])
+            if np.isfinite(lp[0, token]):
+                assert abs(got["logprob"] - lp[0, token]) <= tol
+            else:
+                assert got["logprob"] == -np.inf
+            assert abs(got["entropy"] - ent[0]) <= rel * (1 + 2 * ent[0]) + 2.0 ** -21 * ent[0]
+            want = R.top(x[0], seen, 5)
+            np.testing.assert_array_equal(got["top_ids"], want)
+            assert np.all(np.abs(got["top_logprobs"] - lp[0, want]) <= tol)
+        np.testing.assert_array_equal(eng.logits(), x[0].astype(np.float32))
+        assert eng.logprobs(-1)["logprob"] == -np.inf and eng.logprobs(spec.vocab)["logprob"] == -np.inf
+        ids.append(token)
+        st, token = eng.decode(token, True)
+        assert st == E.Status.OK
+    assert ids == [int(i) for i in plain]
+    for bad in (dict(n_top=65), dict(n_top=-1)):
+        with pytest.raises(E.YlmError):
+            eng.logprobs(0, **bad) if bad["n_top"] > 0 else E.check(
+                E.lib().ylm_logprobs(eng._h, 0, -1, 0, None, None, None, None), "x")
+    eng.close()

@@ -120,6 +120,10 @@ def test_logprobs_of_no_rows_is_fine():
     assert logprobs(rows=0, x=None) == OK
 
 
+def test_engine_logprobs_refuses_a_null_engine():
+    assert E.lib().ylm_logprobs(None, 0, 0, 0, None, None, None, None) == INV
+
+
 def test_kv8_struct_layout_matches_c(tmp_path):
     import os
     import subprocess

@@ -289,6 +289,7 @@ struct ylm_engine
     int *cand_count = nullptr, *smp_counter = nullptr;
     int parts = 1;
     int64_t *dbg_ids = nullptr;
+    char *lgp_out = nullptr; // ylm_logprobs: the given id and its results
     float *dbg_probs = nullptr;
     uint32_t *mask_bits = nullptr;
 
@@ -383,7 +384,7 @@ struct ylm_engine
         for (void *p : {(void *)wblob, (void *)kc, (void *)vc, (void *)rcos, (void *)rsin, (void *)x, (void *)x2,
                         (void *)qkv, (void *)att, (void *)act, (void *)logits, (void *)logits_local, (void *)ar,
                         (void *)partial, (void *)counters, (void *)dstate, (void *)cand, (void *)cand_count,
-                        (void *)smp_counter, (void *)dbg_ids, (void *)dbg_probs, (void *)mask_bits, (void *)pX,
+                        (void *)smp_counter, (void *)lgp_out, (void *)dbg_ids, (void *)dbg_probs, (void *)mask_bits, (void *)pX,
                         (void *)pXn, (void *)pQKV, (void *)pQ, (void *)pO, (void *)pA, (void *)pIds, (void *)ds_xt, (void *)ds_actt, (void *)ds_gen, (void *)ds_xstat,
                         (void *)ds_sink, (void *)pick_cand, (void *)pick_counter, (void *)ds_pick_mb})
             // logits_local is logits itself without tensor parallelism: free once
@@ -1521,6 +1522,46 @@ struct ylm_engine
         last_k = do_greedy ? 0 : std::max(1, std::min(top_k, 64));
     }
 
+    // log probabilities on the current logits; the buffers come with the first call
+    void logprobs(int64_t id, int n_top, bool masked, float *lp, float *ent, int64_t *ids, float *tops)
+    {
+        struct Out
+        {
+            int64_t id, top_ids[64];
+            float logprob, entropy, top[64];
+        } h;
+        if (!has_logits)
+            fail(YLM_NOT_READY, "no logits yet");
+        gather_logits();
+        if (!lgp_out)
+            lgp_out = dalloc<char>(sizeof(Out));
+        Out *d = reinterpret_cast<Out *>(lgp_out);
+        h.id = id;
+        CK(cudaMemcpyAsync(&d->id, &h.id, sizeof(h.id), cudaMemcpyHostToDevice, st));
+        LogprobArgs a;
+        a.logits = logits;
+        a.ld = V;
+        a.rows = 1;
+        a.vocab = V;
+        a.ids = &d->id;
+        a.mask_bits = masked ? mask_bits : nullptr;
+        a.n_top = n_top;
+        a.logprob = &d->logprob;
+        a.entropy = &d->entropy;
+        a.top_ids = d->top_ids;
+        a.top_logprobs = d->top;
+        CK(logprobs_launch(a, sms, st));
+        CK(cudaMemcpyAsync(&h, d, sizeof(h), cudaMemcpyDeviceToHost, st));
+        CK(cudaStreamSynchronize(st));
+        *lp = h.logprob;
+        *ent = h.entropy;
+        for (int i = 0; i < n_top; i++)
+        {
+            ids[i] = h.top_ids[i];
+            tops[i] = h.top[i];
+        }
+    }
+
     // one decode step + sample (one graph launch)
     int decode(int64_t id, bool do_greedy, int64_t *next)
     {
@@ -1855,6 +1896,18 @@ int ylm_sample(ylm_engine *e, int32_t greedy, int64_t *next_id)
             fail(YLM_INVALID_ARG, "null argument");
         CK(cudaSetDevice(e->dev));
         *next_id = e->sample(greedy != 0);
+        return YLM_OK;
+    });
+}
+
+int ylm_logprobs(ylm_engine *e, int64_t id, int32_t n_top, int32_t masked, float *logprob, float *entropy,
+                 int64_t *top_ids, float *top_logprobs)
+{
+    return guarded([&]() -> int {
+        if (!e || !logprob || !entropy || n_top < 0 || n_top > 64 || (n_top && (!top_ids || !top_logprobs)))
+            fail(YLM_INVALID_ARG, "bad argument");
+        CK(cudaSetDevice(e->dev));
+        e->logprobs(id, n_top, masked != 0, logprob, entropy, top_ids, top_logprobs);
         return YLM_OK;
     });
 }

@@ -150,6 +150,7 @@ SIGNATURES = {
     "ylm_logits_device": (ctypes.c_int, [_P, ctypes.POINTER(_P), _I64P]),
     "ylm_set_sampling": (ctypes.c_int, [_P, ctypes.POINTER(Sampling)]),
     "ylm_sample": (ctypes.c_int, [_P, ctypes.c_int32, _I64P]),
+    "ylm_logprobs": (ctypes.c_int, [_P, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _F32P, _F32P, _I64P, _F32P]),
     "ylm_decode": (ctypes.c_int, [_P, ctypes.c_int64, ctypes.c_int32, _I64P]),
     "ylm_generate": (ctypes.c_int, [_P, _I64P, ctypes.c_int32, ctypes.c_int32, _I64P, ctypes.c_int32, _I64P, _I32P,
                                     _F64P, _F64P]),
@@ -382,6 +383,15 @@ class Engine:
         out = ctypes.c_int64()
         check(lib().ylm_sample(self._h, int(greedy), ctypes.byref(out)), "ylm_sample")
         return out.value
+
+    def logprobs(self, token: int, n_top: int = 0, masked: bool = False) -> dict:
+        """Log probability of ``token`` on the current logits, their entropy, and the ``n_top`` most likely
+        (id, log probability) pairs; ``masked``: over the ids that ``set_sampling`` left unmasked."""
+        lp, ent = ctypes.c_float(), ctypes.c_float()
+        ids, top = np.zeros(max(1, n_top), np.int64), np.zeros(max(1, n_top), np.float32)
+        check(lib().ylm_logprobs(self._h, int(token), n_top, int(masked), ctypes.byref(lp), ctypes.byref(ent),
+                                 _ptr(ids, ctypes.c_int64), _ptr(top, ctypes.c_float)), "ylm_logprobs")
+        return {"logprob": lp.value, "entropy": ent.value, "top_ids": ids[:n_top], "top_logprobs": top[:n_top]}
 
     def decode(self, token: int, greedy: bool):
         out = ctypes.c_int64()
