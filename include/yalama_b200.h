@@ -308,7 +308,7 @@ int ylm_k_kv8_store(const ylm_kv8_cache *cache, const void *k, int64_t k_stride,
  * every head (null: none); a token that sees no slot gets zeros.
  * acc: [hkv][cap] FP32 or null: acc[g][j] += the attention weight that slot j got
  * from the t tokens, summed over the query heads of KV head g (zero it when
- * the cache starts).
+ * the cache starts; calls that add to the same acc must not overlap).
  * workspace: device memory of at least ylm_k_kv8_attention_workspace bytes,
  * 16-byte aligned, for this call alone until it has run: calls that may overlap on the GPU,
  * and graphs that may, need one each. null: allocated and freed in stream order. */
@@ -332,7 +332,7 @@ int ylm_k_kv8_evict(const ylm_kv8_cache *src, const ylm_kv8_cache *dst, const fl
                     int32_t n, int32_t n_keep, int32_t n_sink, int32_t n_recent, int32_t *kept, void *stream);
 
 /* ---- log probabilities ------------------------------------------------------------
- * Of `rows` rows of FP16 logits [rows][ld], vocab of them used, over the softmax of
+ * Of `rows` rows of FP16 logits [rows][ld], vocab (at most 2^30) of them used, over the softmax of
  * the unmasked ids (natural logarithms, FP32; all buffers on the device):
  *   logprob[r]  of ids[r]; -inf for a masked id or one outside [0, vocab) (null: not wanted)
  *   entropy[r]  (null: not wanted)

@@ -342,6 +342,36 @@ def test_attention_strided_rows_and_untouched_neighbours():
     assert bool((out[:, 12 * D:] == 7).all())
 
 
+def torch_attention(c, q, n, t):
+    """The definition in 64 bits on the GPU, for shapes that numpy takes long for."""
+    hq, hkv = q.shape[1], c.hkv
+    table = torch.from_numpy(R.numbers(np.arange(256, dtype=np.uint8), c.fmt)).cuda()
+    k, v = (table[c.code[x][:, :n].long()] * c.scale[x].double().repeat_interleave(c.block, 1)[:, :n, None] for x in "kv")
+    out = torch.empty(t, hq, D, dtype=torch.float64, device="cuda")
+    see = torch.arange(n, device="cuda")[None] <= torch.arange(n - t, n, device="cuda")[:, None]
+    for h in range(hq):
+        x = (q[:, h].double() @ k[h // (hq // hkv)].T / np.sqrt(D)).masked_fill(~see, -float("inf"))
+        out[:, h] = torch.softmax(x, 1) @ v[h // (hq // hkv)]
+    return out
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hq,hkv,t,n,block", [(2, 2, 4150, 4200, 64), (32, 1, 300, 700, 16), (8, 1, 1, 70001, 128),
+                                              (24, 8, 1, 40000, 32)])
+def test_attention_of_many_rows_and_long_contexts(hq, hkv, t, n, block, fmt):
+    g = torch.Generator(device="cuda").manual_seed(n)
+    c = DeviceCache(fmt, block, n + 5, hkv)
+    k, v = (torch.randn(n, hkv, D, generator=g, device="cuda").half() for _ in "kv")
+    c.store(k, v, 0)
+    q = torch.randn(t, hq, D, generator=g, device="cuda").half()
+    got = attend(c, q, t, n).double().reshape(t, hq, D)
+    want = torch_attention(c, q, n, t)
+    # rounding of the result and of P: at most 2^-11 of the result and of sum p |v|, and |v| < 6
+    assert float((got - want).abs().max()) <= 2.0 ** -11 * (6 + 6) + 2.0 ** -14
+    rel = float((got - want).norm() / want.norm())
+    assert rel <= 2.0 ** -11
+
+
 @pytest.mark.parametrize("n", [1, 64, 1000, 20000])
 def test_attention_workspace(n):
     """The size asked for is enough (and what lies behind it is not written), one byte less is refused, a workspace

@@ -171,6 +171,19 @@ def test_outputs_that_are_not_wanted():
             np.testing.assert_array_equal(got[name], both[name])
 
 
+def test_more_rows_than_a_grid_dimension():
+    rng = np.random.default_rng(6)
+    rows, vocab = 70001, 37
+    x = rng.standard_normal((rows, vocab)).astype(np.float16)
+    ids = rng.integers(0, vocab, rows)
+    got = run(x, ids, 2)
+    lp, ent, _, _ = R.logprobs(x.astype(np.float64), np.ones(vocab, bool))
+    np.testing.assert_allclose(got["logprob"], lp[np.arange(rows), ids], rtol=1e-5, atol=1e-6)
+    np.testing.assert_allclose(got["entropy"], ent, rtol=1e-5)
+    best = np.argsort(-x.astype(np.float64), 1, kind="stable")[:, :2]
+    np.testing.assert_array_equal(got["top_ids"], best)
+
+
 def test_rows_beyond_32_bits():
     # the last row lies 4.3 G logits behind the first
     vocab, ld, rows = 1000, 1 << 27, 33

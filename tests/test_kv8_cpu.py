@@ -108,7 +108,7 @@ def test_evict_refuses(bad):
 
 
 @pytest.mark.parametrize("bad", [dict(x=None), dict(ld=99), dict(rows=-1), dict(vocab=0), dict(vocab=-5),
-                                 dict(vocab=2 ** 31, ld=2 ** 31), dict(n_top=-1), dict(n_top=65), dict(ids=None),
+                                 dict(vocab=2 ** 31, ld=2 ** 31), dict(vocab=2 ** 30 + 1, ld=2 ** 31), dict(n_top=-1), dict(n_top=65), dict(ids=None),
                                  dict(ti=None), dict(tl=None), dict(lp=None, ent=None, n_top=0), dict(x=A + 1),
                                  dict(ids=2 * A + 4), dict(mask=A + 2), dict(lp=A + 2), dict(ent=A + 1),
                                  dict(ti=A + 4), dict(tl=A + 2)], ids=str)

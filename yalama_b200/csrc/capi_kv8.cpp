@@ -244,8 +244,8 @@ int ylm_k_logprobs(const void *logits, int64_t ld, int32_t rows, int64_t vocab, 
                    const uint32_t *mask_bits, int32_t n_top, float *logprob, float *entropy, int64_t *top_ids,
                    float *top_logprobs, void *stream)
 {
-    if (rows < 0 || vocab <= 0 || vocab > 0x7FFFFFFF || ld < vocab)
-        return refuse(YLM_INVALID_ARG, "needs rows >= 0, 1 <= vocab < 2^31 and ld >= vocab");
+    if (rows < 0 || vocab <= 0 || vocab > 1 << 30 || ld < vocab)
+        return refuse(YLM_INVALID_ARG, "needs rows >= 0, 1 <= vocab <= 2^30 and ld >= vocab");
     if (n_top < 0 || n_top > 64)
         return refuse(YLM_INVALID_ARG, "n_top must be 0..64");
     if ((logprob && !ids) || (n_top && (!top_ids || !top_logprobs)))
