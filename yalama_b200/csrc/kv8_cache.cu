@@ -136,8 +136,11 @@ __device__ __forceinline__ uint32_t evict_key(float a)
 constexpr int KEV_THREADS = 1024;
 constexpr int KEV_WARPS = KEV_THREADS / 32;
 constexpr int KEV_BINS = 2048;  // a radix step finds 11 bits of the key (the last one 10)
-constexpr int KEV_MAXC = 8;     // largest cluster (the portable size)
-constexpr int KEV_SLICE = 4096; // slots per CTA below which a KV head takes fewer CTAs
+constexpr int KEV_MAXC = 8;     // CTAs of a cluster (the portable size)
+// Slots up to which one CTA selects alone: the cluster's barriers cost more than they divide.
+// One against eight CTAs a head, us for the eviction of half the slots (8 heads): 2100 slots 9.2 / 11.5,
+// 6000 slots 12.4 / 12.7, 8000 slots 15.0 / 13.9, 20000 slots 31.7 / 23.8.
+constexpr int KEV_ALONE = 6144;
 
 // Exclusive scan over the CTA in thread order; *total gets the sum. The sums fit 32 bits.
 __device__ __forceinline__ int kev_scan(int v, int *warp_sums, int *total)
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(KEV_THREADS) kv8_select_kernel(Kv8EvictArgs a)
 #pragma unroll 4
         for (int i = lo + tid; i < hi_end; i += KEV_THREADS)
         {
-            const uint32_t key = evict_key(acc[i]);
+            const uint32_t key = evict_key(__ldg(acc + i));
             if ((key & known) == prefix)
                 atomicAdd(&mine[(key >> shift) & (bins - 1)], 1);
         }
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(KEV_THREADS) kv8_select_kernel(Kv8EvictArgs a)
     const int each = ((i1 - i0 + KEV_WARPS - 1) / KEV_WARPS + 31) / 32 * 32;
     const int w0 = min(i1, i0 + warp * each), w1 = min(i1, w0 + each);
     auto look = [&](int i, float &x, bool &more, bool &same) {
-        x = i < w1 ? acc[i] : 0.f;
+        x = i < w1 ? __ldg(acc + i) : 0.f;
         const bool held = i < a.n_sink || i >= recent;
         const uint32_t key = evict_key(x);
         more = i < w1 && (held || key > prefix);
@@ -368,9 +371,7 @@ template <int FMT> __global__ void __launch_bounds__(256) kv8_move_kernel(Kv8Evi
 
 cudaError_t kv8_evict_launch(const Kv8EvictArgs &a, cudaStream_t s)
 {
-    int C = 1;
-    while (C < KEV_MAXC && a.n > C * KEV_SLICE)
-        C *= 2;
+    const int C = a.n <= KEV_ALONE ? 1 : KEV_MAXC;
     cudaLaunchAttribute at[1];
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)C, (unsigned)a.src.hkv);

@@ -32,7 +32,12 @@ constexpr int LGP_U = 4;      // 16-byte loads in flight per thread
 constexpr int LGP_CAP = 512;  // collected candidates per CTA
 constexpr int LGP_TOP = 64;   // largest n_top
 constexpr int LGP_MAXC = 8;   // largest cluster (the portable size)
-constexpr int LGP_FILL = 3;   // rows are split until there are so many CTAs per SM
+// CTAs per row: halved from LGP_MAXC while that leaves LGP_FILL CTAs per SM or parts
+// are shorter than LGP_PART ids. Measured, us for 1 / 2 / 4 / 8 CTAs a row (8 alternatives): 151936 ids, 16 rows
+// 22.5 / 17.8 / 13.7 / 12.7, 74 rows 23.2 / 18.7 / 16.7 / 18.7, 200 rows 34.1 / 27.3 / 33.9 / 41.2,
+// 450 rows 43.6 / 50.2 / 57.0 / 79.9; 32768 ids, 16 rows 10.5 / 9.9 / 9.1 / 9.8, 200 rows 12.1 / 12.0 / 16.8 / 26.0.
+constexpr int LGP_FILL = 2;
+constexpr int LGP_PART = 8192;
 constexpr uint32_t LGP_LOWEST = 0x0400u; // ord16 of the lowest finite value: what lies below is -inf
 
 // Running (max, z, w): z = sum e^(x - m) without one maximal element, w = sum e^(x - m) (m - x).
@@ -599,7 +604,7 @@ cudaError_t logprobs_launch(const LogprobArgs &a, int num_sms, cudaStream_t s)
     if (a.rows <= 0)
         return cudaSuccess;
     int C = LGP_MAXC;
-    while (C > 1 && (int64_t)a.rows * (C / 2) >= LGP_FILL * num_sms)
+    while (C > 1 && ((int64_t)a.rows * (C / 2) >= LGP_FILL * num_sms || a.vocab < C * LGP_PART))
         C /= 2;
     cudaLaunchConfig_t cfg = {};
     const unsigned y = (unsigned)std::min(a.rows, 32768);
