@@ -13,6 +13,8 @@ constexpr int KST_THREADS = 256;
 // block-wide maximum gives the scale, and leave as 8-byte codes.
 //   s_new = max(scale_of(max |x| of the new rows), s_old if older tokens share the block)
 // Infinities count as +-65504; NaN takes no part in the maximum.
+// Measured (B200, 8 KV heads): one token 1.5 us, the launch; 2048 tokens 3.3 us = 3.9 TB/s of rows in and codes
+// out, launch and one round of loads; the rows are read once and no other pass exists.
 template <int FMT, int P>
 __global__ void __launch_bounds__(KST_THREADS)
     kv8_store_kernel(Kv8Cache cache, const __half *k, const __half *v, int64_t k_stride, int64_t v_stride, int t,
@@ -175,7 +177,10 @@ __device__ __forceinline__ int kev_scan(int v, int *warp_sums, int *total)
 // not 0 (few: weights share few exponents) to every CTA's sums, in which each
 // CTA then finds the digit. One cluster barrier a step, as each step has sums of its
 // own. The kept slots are then placed in order, a warp taking consecutive slots (the
-// slice stays in L1 between the passes).
+// slice stays in L1 between the passes). Protected slots are counted, not sorted: they would
+// all meet in one bin.
+// Measured (B200, 8 heads): 65536 slots 19 us, of which the barriers and remote additions take a
+// third; 2100 slots 6.6 us (one CTA a head). One CTA a head with 8-bit digits took 192 us for 65536.
 __global__ void __launch_bounds__(KEV_THREADS) kv8_select_kernel(Kv8EvictArgs a)
 {
     __shared__ int hist[KEV_BINS], sums[3][KEV_BINS];
@@ -313,7 +318,8 @@ __global__ void __launch_bounds__(KEV_THREADS) kv8_select_kernel(Kv8EvictArgs a)
 // One CTA per (destination block, KV head, K or V): the block's scale is the
 // largest of its tokens' old scales, and a token whose old block had a smaller
 // one is rescaled to it. Eight threads move a token's 128 codes, which are on
-// their way before the scales are known.
+// their way before the scales are known. Launched as a programmatic dependent of the
+// selection. Measured (B200): 40000 of 65536 slots, 8 heads, 164 MB in and out, 29 us = 5.6 TB/s: HBM.
 template <int FMT> __global__ void __launch_bounds__(256) kv8_move_kernel(Kv8EvictArgs a)
 {
     __shared__ int from[128];
