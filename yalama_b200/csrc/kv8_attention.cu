@@ -6,12 +6,15 @@
 // Row r = i * G + h of a KV head is query head h of its group, token i; token i
 // sees slots [0, n - t + i]. Scores are kept in base 2 (x * log2 e).
 //
-// Two launches: kv8_attn_kernel splits the slots over CTAs (a decode step has too
-// few rows to fill the GPU otherwise) and leaves per split and row the sums
-// (M, l, O); kv8_join_kernel joins the splits and, where asked, turns the scores
-// that the first launch kept into weights.
+// kv8_attn_kernel splits the slots over CTAs (a decode step has too few rows to
+// fill the GPU otherwise), which leaves sums (M, l, O) per split and row. Up to
+// KVA_ALONE slots the splits of a KV head are one cluster, which joins them through
+// distributed shared memory and adds the weights from scores kept there: one launch, no
+// workspace. Beyond, sums and scores go through the workspace, and kv8_join_kernel
+// joins the splits and turns the scores into weights.
 #include "kv8.cuh"
 #include <algorithm>
+#include <cooperative_groups.h>
 
 namespace ylm {
 
@@ -22,12 +25,20 @@ constexpr int KVA_BUF = KVA_CHUNK * YLM_HEAD_DIM; // bytes of a chunk's K or V
 constexpr int KVA_RING = 4 * KVA_BUF;             // a warp's two K and two V chunks
 constexpr int KVA_SMEM = KVA_WARPS * KVA_RING;
 constexpr int KVA_JOIN = 256;     // threads of the joining CTAs
+constexpr int KVA_CLUSTER = 8;    // most splits of a cluster (the portable size)
+// Slots up to which the splits of a KV head are one cluster. One launch against two, us of device time (8 heads of
+// 4 query heads; with kept weights): 100 slots 4.3 / 5.2 (5.5 / 6.2), 611 slots 5.0 / 5.3 (6.2 / 7.0), 1000 slots
+// 5.7 / 5.5 (6.9 / 7.4), 2000 slots 6.5 / 5.5 (8.2 / 7.7); a caller that launches each step also saves the second launch.
+constexpr int KVA_ALONE = 1024;
+constexpr int KVA_ALONE_LEN = KVA_ALONE / KVA_CLUSTER;
+static_assert(KVA_ALONE_LEN % (KVA_CHUNK * KVA_WARPS) == 0, "a split is whole rounds of its warps");
 
 struct Kv8Plan
 {
     int G, rows;      // query heads per KV head, rows per KV head of a pass (G * tokens)
     int nt;           // 8-row tiles per CTA, 1 or 2
     int zblocks;      // CTAs over the rows of a KV head
+    int cluster;      // 1: the splits are one cluster
     int splits, len;  // splits of the slots and slots per split
     int pad;          // rows, rounded up to a multiple of 4: stride of the kept scores and of (M, l)
     int lps;          // lanes that share a slot's rows in the accumulation, four rows a load
@@ -50,7 +61,10 @@ static Kv8Plan kv8_plan(int hkv, int hq, int t, int n, bool acc, int num_sms)
     const int unit = KVA_CHUNK * KVA_WARPS; // slots of one round of a CTA's warps
     // one wave of CTAs: as many as the SMs hold
     const int64_t groups = (int64_t)hkv * p.zblocks;
-    const int want = (int)std::max<int64_t>(1, (int64_t)num_sms * (p.nt == 1 ? 3 : 2) / groups);
+    // (rows of several CTAs would meet in acc: they go the other way)
+    p.cluster = n <= KVA_ALONE && (!acc || p.zblocks == 1);
+    const int want = p.cluster ? KVA_CLUSTER
+                               : (int)std::max<int64_t>(1, (int64_t)num_sms * (p.nt == 1 ? 3 : 2) / groups);
     p.len = std::max(1, ((n + want - 1) / want + unit - 1) / unit) * unit;
     p.splits = (n + p.len - 1) / p.len;
     // room for the most splits that any length up to n takes, so that a
@@ -63,7 +77,7 @@ static Kv8Plan kv8_plan(int hkv, int hq, int t, int n, bool acc, int num_sms)
     p.lps = !acc || p.pad < 8 ? 1 : p.pad < 32 ? 2 : p.pad < 64 ? 8 : 16; // at most pad / 4
     const int round = 4 * KVA_JOIN / p.lps;
     p.tile = std::max(1, (int)(((int64_t)hkv * n / (num_sms * 4) + round - 1) / round)) * round;
-    p.bytes = p.score_off + (acc ? (size_t)hkv * n * p.pad * sizeof(float) : 0);
+    p.bytes = p.cluster ? 0 : p.score_off + (acc ? (size_t)hkv * n * p.pad * sizeof(float) : 0);
     return p;
 }
 
@@ -148,13 +162,16 @@ __device__ __forceinline__ float kva_log_scale(float s)
 // 64 / 8 heads over 4099 slots 13.6 us: bound by the instructions that decode every code once per 16 rows.
 // Registers as the buffers instead of the ring: 131071 slots 52 us, 611 slots 7.2 us (with the join of that
 // time); three CTAs an SM (NT = 1) at 168 registers; without the decode (wrong values) 131071 slots take 1 us less.
-template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8Pass w)
+template <int FMT, int NT, bool CLUSTER>
+__global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8Pass w)
 {
     extern __shared__ __align__(128) uint8_t ring[]; // a warp's two K and two V chunks; at the end the sums O
     float(*om)[8 * NT][YLM_HEAD_DIM + 8] = reinterpret_cast<float(*)[8 * NT][YLM_HEAD_DIM + 8]>(ring);
     static_assert(sizeof(float) * 8 * NT * (YLM_HEAD_DIM + 8) <= KVA_RING, "a warp's O fits its ring");
     __shared__ float mm[KVA_WARPS][8 * NT], lm[KVA_WARPS][8 * NT];
-    pdl_launch_dependents(); // the joining CTAs may start; they wait for this grid's end
+    float *kept = reinterpret_cast<float *>(ring + KVA_SMEM); // CLUSTER: scores [slot of the split][8 * NT]
+    if (!CLUSTER)
+        pdl_launch_dependents(); // the joining CTAs may start; they wait for this grid's end
     const Kv8AttnArgs &a = w.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int sp = blockIdx.x, kvh = blockIdx.y;
@@ -347,7 +364,10 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int i = 0; i < 2; i++)
-                        if (js + g + 8 * i < n && row0 + 8 * t + 2 * c < w.p.pad)
+                        if (CLUSTER)
+                            *reinterpret_cast<float2 *>(kept + (js - sp * w.p.len + g + 8 * i) * 8 * NT + 8 * t + 2 * c) =
+                                make_float2(S[s][t][2 * i], S[s][t][2 * i + 1]);
+                        else if (js + g + 8 * i < n && row0 + 8 * t + 2 * c < w.p.pad)
                             *reinterpret_cast<float2 *>(w.scores + ((size_t)kvh * n + js + g + 8 * i) * w.p.pad + row0 +
                                                         8 * t + 2 * c) = make_float2(S[s][t][2 * i], S[s][t][2 * i + 1]);
             }
@@ -532,9 +552,100 @@ template <int FMT, int NT> __global__ void __launch_bounds__(KVA_THREADS, NT == 
             o.z += x.z * f;
             o.w += x.w * f;
         }
+        if (CLUSTER)
+        {
+            // in place: a lane's own four dimensions, and the row's M and l by the lane that read them last
+            *reinterpret_cast<float4 *>(&om[0][r][lane * 4]) = o;
+            __syncwarp();
+            if (lane == 0)
+            {
+                mm[0][r] = m;
+                lm[0][r] = L;
+            }
+            continue;
+        }
         *reinterpret_cast<float4 *>(w.part + (((size_t)kvh * R + row0 + r) * w.p.splits + sp) * YLM_HEAD_DIM + lane * 4) = o;
         if (lane == 0)
             *reinterpret_cast<float2 *>(w.ml + 2 * (((size_t)kvh * w.p.splits + sp) * w.p.pad + row0 + r)) = make_float2(m, L);
+    }
+    if constexpr (CLUSTER)
+    {
+        // ---- the splits, joined: row r by warp r % 4 of rank r / 4 % C
+        namespace cg = cooperative_groups;
+        cg::cluster_group cl = cg::this_cluster();
+        __shared__ float2 state[8 * NT];
+        const int C = (int)gridDim.x;
+        cl.sync();
+        for (int r = sp * KVA_WARPS + warp; r < 8 * NT && row0 + r < R; r += C * KVA_WARPS)
+        {
+            float m[KVA_CLUSTER], M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int s = 0; s < KVA_CLUSTER; s++)
+            {
+                m[s] = s < C ? *cl.map_shared_rank(&mm[0][r], s) : -INFINITY;
+                M = fmaxf(M, m[s]);
+            }
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int s = 0; s < KVA_CLUSTER; s++)
+            {
+                if (s >= C)
+                    break;
+                const float f = m[s] == -INFINITY ? 0.f : kva_ex2(m[s] - M);
+                const float4 x = *reinterpret_cast<const float4 *>(cl.map_shared_rank(&om[0][r][lane * 4], s));
+                L += *cl.map_shared_rank(&lm[0][r], s) * f;
+                o.x += x.x * f;
+                o.y += x.y * f;
+                o.z += x.z * f;
+                o.w += x.w * f;
+            }
+            const float inv = M == -INFINITY ? 1.f : 1.f / L; // no slot seen: 0
+            const int row = row0 + r;
+            const __half2 lo = __floats2half2_rn(o.x * inv, o.y * inv), hi = __floats2half2_rn(o.z * inv, o.w * inv);
+            *reinterpret_cast<uint2 *>(a.out + (row / G) * a.out_stride + (size_t)(kvh * G + row % G) * YLM_HEAD_DIM + lane * 4) =
+                make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+        }
+        if (a.acc) // all rows are this CTA's: the plan sees to it
+        {
+            if (tid < 8 * NT)
+            {
+                float m[KVA_CLUSTER], M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int s = 0; s < KVA_CLUSTER; s++)
+                {
+                    m[s] = s < C ? *cl.map_shared_rank(&mm[0][tid], s) : -INFINITY;
+                    M = fmaxf(M, m[s]);
+                }
+#pragma unroll
+                for (int s = 0; s < KVA_CLUSTER; s++)
+                    if (s < C && m[s] != -INFINITY)
+                        L += *cl.map_shared_rank(&lm[0][tid], s) * kva_ex2(m[s] - M);
+                // a row that sees nothing weighs nothing
+                state[tid] = M == -INFINITY ? make_float2(0.f, 0.f) : make_float2(M, 1.f / L);
+            }
+            __syncthreads();
+            float *acc = a.acc + (size_t)kvh * a.c.cap;
+            for (int j = sp * w.p.len + tid; j < j_end; j += KVA_THREADS)
+            {
+                const float4 *x = reinterpret_cast<const float4 *>(kept + (j - sp * w.p.len) * 8 * NT);
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * NT; i++)
+                {
+                    const float4 v = x[i];
+                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                    {
+                        const float2 st = state[4 * i + k];
+                        if (4 * i + k < R) // rows that are not there must not count
+                            sum += kva_ex2(e[k] - st.x) * st.y;
+                    }
+                }
+                acc[j] += sum;
+            }
+        }
+        cl.sync(); // the sums stay until every CTA has read them
     }
 }
 
@@ -681,13 +792,33 @@ template <int LPS> __global__ void __launch_bounds__(KVA_JOIN) kv8_join_kernel(c
     }
 }
 
-template <int FMT> static void attn_launch(const Kv8Pass &w, cudaStream_t s)
+// Dynamic shared memory: the rings, and for a cluster the scores of a split
+static constexpr int kva_smem(int nt, bool cluster)
 {
-    const dim3 grid((unsigned)w.p.splits, (unsigned)w.a.c.hkv, (unsigned)w.p.zblocks);
+    return KVA_SMEM + (cluster ? KVA_ALONE_LEN * 8 * nt * (int)sizeof(float) : 0);
+}
+
+template <int FMT, int NT, bool CLUSTER> static cudaError_t attn_launch(const Kv8Pass &w, cudaStream_t s)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)w.p.splits, (unsigned)w.a.c.hkv, (unsigned)w.p.zblocks);
+    cfg.blockDim = dim3(KVA_THREADS);
+    cfg.dynamicSmemBytes = kva_smem(NT, CLUSTER);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CLUSTER ? (unsigned)w.p.splits : 1;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = CLUSTER ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kv8_attn_kernel<FMT, NT, CLUSTER>, w);
+}
+
+template <int FMT> static cudaError_t attn_launch_fmt(const Kv8Pass &w, cudaStream_t s)
+{
     if (w.p.nt == 1)
-        kv8_attn_kernel<FMT, 1><<<grid, KVA_THREADS, KVA_SMEM, s>>>(w);
-    else
-        kv8_attn_kernel<FMT, 2><<<grid, KVA_THREADS, KVA_SMEM, s>>>(w);
+        return w.p.cluster ? attn_launch<FMT, 1, true>(w, s) : attn_launch<FMT, 1, false>(w, s);
+    return w.p.cluster ? attn_launch<FMT, 2, true>(w, s) : attn_launch<FMT, 2, false>(w, s);
 }
 
 cudaError_t kv8_attn_launch(const Kv8AttnArgs &args, void *ws, int num_sms, cudaStream_t s)
@@ -705,13 +836,11 @@ cudaError_t kv8_attn_launch(const Kv8AttnArgs &args, void *ws, int num_sms, cuda
         w.part = static_cast<float *>(ws);
         w.ml = reinterpret_cast<float *>(static_cast<char *>(ws) + w.p.ml_off);
         w.scores = reinterpret_cast<float *>(static_cast<char *>(ws) + w.p.score_off);
-        if (args.c.format == KV8_E4M3)
-            attn_launch<KV8_E4M3>(w, s);
-        else
-            attn_launch<KV8_INT8>(w, s);
-        cudaError_t e = cudaGetLastError();
+        cudaError_t e = args.c.format == KV8_E4M3 ? attn_launch_fmt<KV8_E4M3>(w, s) : attn_launch_fmt<KV8_INT8>(w, s);
         if (e != cudaSuccess)
             return e;
+        if (w.p.cluster)
+            continue;
         const int tiles = args.acc ? (w.a.n + w.p.tile - 1) / w.p.tile : 0;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(args.c.hkv * (w.p.rows + tiles)));
@@ -732,21 +861,25 @@ cudaError_t kv8_attn_launch(const Kv8AttnArgs &args, void *ws, int num_sms, cuda
     return cudaSuccess;
 }
 
-template <typename F> static cudaError_t kva_smem(F *f)
+template <int FMT> static cudaError_t prepare_fmt()
 {
-    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, KVA_SMEM);
+    const auto opt_in = [](const void *f, int bytes) {
+        return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    cudaError_t e = opt_in((const void *)kv8_attn_kernel<FMT, 1, false>, kva_smem(1, false));
+    if (e == cudaSuccess)
+        e = opt_in((const void *)kv8_attn_kernel<FMT, 2, false>, kva_smem(2, false));
+    if (e == cudaSuccess)
+        e = opt_in((const void *)kv8_attn_kernel<FMT, 1, true>, kva_smem(1, true));
+    if (e == cudaSuccess)
+        e = opt_in((const void *)kv8_attn_kernel<FMT, 2, true>, kva_smem(2, true));
+    return e;
 }
 
 cudaError_t kv8_prepare()
 {
-    cudaError_t e = kva_smem(kv8_attn_kernel<KV8_E4M3, 1>);
-    if (e == cudaSuccess)
-        e = kva_smem(kv8_attn_kernel<KV8_E4M3, 2>);
-    if (e == cudaSuccess)
-        e = kva_smem(kv8_attn_kernel<KV8_INT8, 1>);
-    if (e == cudaSuccess)
-        e = kva_smem(kv8_attn_kernel<KV8_INT8, 2>);
-    return e;
+    const cudaError_t e = prepare_fmt<KV8_E4M3>();
+    return e == cudaSuccess ? prepare_fmt<KV8_INT8>() : e;
 }
 
 } // namespace ylm
