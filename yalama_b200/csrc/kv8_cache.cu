@@ -315,21 +315,22 @@ __global__ void __launch_bounds__(KEV_THREADS) kv8_select_kernel(Kv8EvictArgs a)
     }
 }
 
-// One CTA per (destination block, KV head, K or V): the block's scale is the
+// One CTA per (128 destination slots, KV head, K or V), whole blocks: a block's scale is the
 // largest of its tokens' old scales, and a token whose old block had a smaller
 // one is rescaled to it. Eight threads move a token's 128 codes, which are on
 // their way before the scales are known. Launched as a programmatic dependent of the
-// selection. Measured (B200): 40000 of 65536 slots, 8 heads, 164 MB in and out, 29 us = 5.6 TB/s: HBM.
+// selection. Measured (B200): 40000 of 65536 slots, 8 heads, 164 MB in and out, 24 us at every
+// block size: HBM. A CTA per block took 30 us with blocks of 64 and 80 us with blocks of 16.
+constexpr int KEV_MOVE = 128; // the largest block
 template <int FMT> __global__ void __launch_bounds__(256) kv8_move_kernel(Kv8EvictArgs a)
 {
-    __shared__ int from[128];
-    __shared__ float old[128];
-    __shared__ float tops[4];
+    __shared__ int from[KEV_MOVE];
+    __shared__ float old[KEV_MOVE], seg[KEV_MOVE / 16], top[KEV_MOVE / 16]; // per 16 tokens: the largest; of their block
     const bool is_v = blockIdx.z != 0;
-    const int g = blockIdx.y, b = blockIdx.x, tid = threadIdx.x;
-    const int block = a.src.block, lo = b * block, m = min(block, a.n_keep - lo);
-    const int src_blocks = (a.src.cap + block - 1) / block, dst_blocks = (a.dst.cap + block - 1) / block;
-    const float *src_scale = (is_v ? a.src.v_scale : a.src.k_scale) + (size_t)g * src_blocks;
+    const int g = blockIdx.y, lo = (int)blockIdx.x * KEV_MOVE, tid = threadIdx.x;
+    const int block = a.src.block, shift = 31 - __clz(block), m = min(KEV_MOVE, a.n_keep - lo);
+    const size_t src_blocks = (a.src.cap + block - 1) >> shift, dst_blocks = (a.dst.cap + block - 1) >> shift;
+    const float *src_scale = (is_v ? a.src.v_scale : a.src.k_scale) + g * src_blocks;
     const uint8_t *src = (is_v ? a.src.v : a.src.k) + (size_t)g * a.src.cap * YLM_HEAD_DIM;
     uint8_t *dst = (is_v ? a.dst.v : a.dst.k) + ((size_t)g * a.dst.cap + lo) * YLM_HEAD_DIM;
     pdl_wait();
@@ -345,27 +346,38 @@ template <int FMT> __global__ void __launch_bounds__(256) kv8_move_kernel(Kv8Evi
         if (i < m)
             x[k] = *reinterpret_cast<const uint4 *>(src + (size_t)from[i] * YLM_HEAD_DIM + (tid & 7) * 16);
     }
-    if (tid < 128)
+    if (tid < KEV_MOVE)
     {
-        const float s = tid < m ? src_scale[f / block] : 0.f;
+        float s = tid < m ? src_scale[f >> shift] : 0.f;
         old[tid] = s;
-        const float t = warp_max(s);
-        if ((tid & 31) == 0)
-            tops[tid >> 5] = t;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+            s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+        if ((tid & 15) == 0)
+            seg[tid >> 4] = s;
     }
     __syncthreads();
-    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), inv = top > 0.f ? 1.f / top : 1.f;
-    if (tid == 0)
-        ((is_v ? a.dst.v_scale : a.dst.k_scale) + (size_t)g * dst_blocks)[b] = top;
+    if (tid < KEV_MOVE / 16)
+    {
+        const int s0 = tid >> (shift - 4) << (shift - 4); // the block's first 16 tokens
+        float t = seg[s0];
+        for (int k = 1; k < block / 16; k++)
+            t = fmaxf(t, seg[s0 + k]);
+        top[tid] = t;
+        if (s0 == tid && tid * 16 < m)
+            ((is_v ? a.dst.v_scale : a.dst.k_scale) + g * dst_blocks)[(lo + tid * 16) >> shift] = t;
+    }
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < 4; k++)
     {
         const int i = (tid >> 3) + 32 * k;
         if (i >= m)
             continue;
-        if (old[i] != top)
+        const float now = top[i >> 4];
+        if (old[i] != now)
         {
-            const float ratio = old[i] * inv;
+            const float ratio = now > 0.f ? old[i] / now : 1.f;
             x[k].x = kv8_rescale4<FMT>(x[k].x, ratio);
             x[k].y = kv8_rescale4<FMT>(x[k].y, ratio);
             x[k].z = kv8_rescale4<FMT>(x[k].z, ratio);
@@ -391,7 +403,7 @@ cudaError_t kv8_evict_launch(const Kv8EvictArgs &a, cudaStream_t s)
     cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_select_kernel, a);
     if (e != cudaSuccess || a.n_keep == 0)
         return e;
-    cfg.gridDim = dim3((unsigned)((a.n_keep + a.src.block - 1) / a.src.block), (unsigned)a.src.hkv, 2);
+    cfg.gridDim = dim3((unsigned)((a.n_keep + KEV_MOVE - 1) / KEV_MOVE), (unsigned)a.src.hkv, 2);
     cfg.blockDim = dim3(256);
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
