@@ -238,7 +238,7 @@ def test_attention(hq, hkv, t, n, block, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("t,n", [(1, 70), (5, 130), (20, 20)])
+@pytest.mark.parametrize("t,n", [(1, 70), (5, 130), (20, 20), (1, 1400), (3, 1100), (9, 1301)])
 def test_attention_hidden_slots_may_hold_anything(fmt, t, n):
     rng = np.random.default_rng(n)
     c, ref = filled(rng, fmt, 16, n + 50, 2, n)
@@ -253,7 +253,7 @@ def test_attention_hidden_slots_may_hold_anything(fmt, t, n):
     assert bool((acc[:, :n][:, torch.from_numpy(hidden).cuda()] == 0).all())
 
 
-@pytest.mark.parametrize("t,n", [(1, 40), (6, 300), (40, 64)])
+@pytest.mark.parametrize("t,n", [(1, 40), (6, 300), (40, 64), (1, 1200), (3, 1500), (12, 1100)])
 def test_attention_rows_that_see_nothing_are_zero(t, n):
     rng = np.random.default_rng(n)
     c, ref = filled(rng, "e4m3", 32, n, 2, n)
@@ -272,7 +272,7 @@ def test_attention_rows_that_see_nothing_are_zero(t, n):
     np.testing.assert_allclose(got[-1].float().cpu().numpy(), want, rtol=2.0 ** -10, atol=1e-7)
 
 
-@pytest.mark.parametrize("hq,t,n", [(2, 5, 100), (8, 3, 64), (8, 9, 33), (4, 40, 130)])
+@pytest.mark.parametrize("hq,t,n", [(2, 5, 100), (8, 3, 64), (8, 9, 33), (4, 40, 130), (2, 5, 1200), (8, 4, 1153)])
 def test_attention_nan_of_a_later_token_stays_out_of_the_earlier_ones(hq, t, n):
     # NaN in a key makes every output of the tokens that see it NaN, NaN in a value that dimension of theirs
     rng = np.random.default_rng(n)
@@ -298,11 +298,12 @@ def test_attention_nan_of_a_later_token_stays_out_of_the_earlier_ones(hq, t, n):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n", [400, 1300])
 @pytest.mark.parametrize("sharp", [1.0, 30.0])
-def test_attention_values_of_very_different_scales(fmt, sharp):
+def test_attention_values_of_very_different_scales(fmt, sharp, n):
     # first tokens that take most of the weight with values near zero, and blocks of values 2^20 apart
     rng = np.random.default_rng(int(sharp))
-    n, hkv, hq = 400, 2, 8
+    hkv, hq = 2, 8
     k = rng.standard_normal((n, hkv, D)).astype(np.float16)
     v = rng.standard_normal((n, hkv, D))
     v[:16] *= 2.0 ** -14
@@ -313,7 +314,7 @@ def test_attention_values_of_very_different_scales(fmt, sharp):
     q = (rng.standard_normal((1, hq, D)) * 0.3).astype(np.float16)
     for h in range(hq):
         q[0, h] = q[0, h] + np.float16(0.02 * sharp) * k[3, h // 4]
-    for lo, hi in ((0, 400), (0, 48), (0, 90)):
+    for lo, hi in ((0, n), (0, 48), (0, 90)):
         c, ref = DeviceCache(fmt, 16, n, hkv), R.Cache(fmt, 16, n, hkv)
         c.store(half(k[lo:hi]), half(v[lo:hi]), 0)
         ref.store(k[lo:hi].astype(np.float64), v[lo:hi].astype(np.float64), 0)
@@ -321,23 +322,25 @@ def test_attention_values_of_very_different_scales(fmt, sharp):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-def test_attention_of_large_scores(fmt):
+@pytest.mark.parametrize("n", [190, 1190])
+def test_attention_of_large_scores(fmt, n):
     # scores in the thousands: one slot takes everything
     rng = np.random.default_rng(7)
-    c, ref = filled(rng, fmt, 64, 200, 1, 190)
+    c, ref = filled(rng, fmt, 64, n + 10, 1, n)
     q = (rng.standard_normal((3, 4, D)) * 60).astype(np.float16)
-    check_attention(c, ref, q, 3, 190, None, torch.zeros(1, 200, device="cuda"))
+    check_attention(c, ref, q, 3, n, None, torch.zeros(1, n + 10, device="cuda"))
 
 
-def test_attention_strided_rows_and_untouched_neighbours():
+@pytest.mark.parametrize("n", [280, 1280])
+def test_attention_strided_rows_and_untouched_neighbours(n):
     rng = np.random.default_rng(11)
-    c, ref = filled(rng, "int8", 32, 300, 4, 280)
+    c, ref = filled(rng, "int8", 32, n + 20, 4, n)
     qkv = rng.standard_normal((6, 20, D)).astype(np.float16)  # 12 query heads, then keys and values
     d = half(qkv)
     out = torch.full((6, 14 * D), 7.0, dtype=torch.float16, device="cuda")
-    attend(c, d[:, :12], 6, 280, out=out[:, :12 * D])
-    want, _, pv, mag = R.attention(qkv[:, :12].astype(np.float64), ref.values("k", 280), ref.values("v", 280), 6,
-                                   np.zeros(280, bool))
+    attend(c, d[:, :12], 6, n, out=out[:, :12 * D])
+    want, _, pv, mag = R.attention(qkv[:, :12].astype(np.float64), ref.values("k", n), ref.values("v", n), 6,
+                                   np.zeros(n, bool))
     tol, _ = bounds(want, pv, mag, None)
     assert np.all(np.abs(out[:, :12 * D].float().cpu().numpy().reshape(want.shape) - want) <= tol)
     assert bool((out[:, 12 * D:] == 7).all())
@@ -535,12 +538,13 @@ def step(c, d, q, k, v, slot, acc, acc_d, out, kept, ws, s):
     evict(c, d, acc, acc_d, slot + k.shape[0], kept.shape[1], 2, 4, kept, s)
 
 
+@pytest.mark.parametrize("n", [700, 2500])
 @pytest.mark.parametrize("own_ws", [True, False])
-def test_side_stream_and_captured_graphs(own_ws):
+def test_side_stream_and_captured_graphs(own_ws, n):
     """The three calls on a side stream, and captured in two graphs that are replayed together, each with its own
     buffers, give what the same calls give one after another."""
     rng = np.random.default_rng(9)
-    n, hkv, hq, t = 700, 2, 8, 3
+    hkv, hq, t = 2, 8, 3
     sides = []
     for _ in range(2):
         k0, v0 = half(rows(rng, n, hkv)), half(rows(rng, n, hkv))
@@ -552,6 +556,7 @@ def test_side_stream_and_captured_graphs(own_ws):
         c, d = DeviceCache("e4m3", 32, n + t, hkv), DeviceCache("e4m3", 32, 400, hkv)
         c.store(k0, v0, 0)
         need = E.kv8_attention_workspace(c.h, hq, t, n + t, True)
+        assert (need > 0) == (n > 1024)
         return [c, d, q, k, v, n, torch.zeros(hkv, n + t, device="cuda"), torch.zeros(hkv, 400, device="cuda"),
                 torch.zeros(t, hq * D, dtype=torch.float16, device="cuda"),
                 torch.zeros(hkv, 300, dtype=torch.int32, device="cuda"),
@@ -599,12 +604,13 @@ def test_side_stream_and_captured_graphs(own_ws):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-def test_a_long_request_on_a_fixed_budget(fmt):
+@pytest.mark.parametrize("prompt,budget,cap", [(517, 256, 640), (1500, 1100, 1536)])
+def test_a_long_request_on_a_fixed_budget(fmt, prompt, budget, cap):
     """A prompt is stored, its last tokens' attention weighs the slots, the cache is evicted to its budget, decode
     steps follow behind the kept slots, it is evicted again into the first cache's buffers, and the request's
     logits are scored. Every step is held to the definitions in 64 bits."""
     rng = np.random.default_rng(12)
-    hq, hkv, block, prompt, budget, cap = 8, 2, 32, 517, 256, 640
+    hq, hkv, block = 8, 2, 32
     c, d = DeviceCache(fmt, block, cap, hkv), DeviceCache(fmt, block, cap, hkv)
     ref = R.Cache(fmt, block, cap, hkv)
     k, v = rows(rng, prompt, hkv, 0.4), rows(rng, prompt, hkv, 0.4)
