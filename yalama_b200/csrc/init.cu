@@ -108,8 +108,6 @@ cudaError_t kernels_prepare()
         e = gemm_tc_prepare();
     if (e == cudaSuccess)
         e = kv8_prepare();
-    if (e == cudaSuccess)
-        e = logprobs_prepare();
     return e;
 }
 

@@ -310,7 +310,6 @@ struct LogprobArgs
     float *top_logprobs;
 };
 cudaError_t logprobs_launch(const LogprobArgs &a, int num_sms, cudaStream_t s);
-cudaError_t logprobs_prepare();
 
 // ------------------------------------------------------------------ init
 // dst[r * ld + c] = N(0, std) element ((row0 + r) * full_cols + col0 + c) of stream `key`
