@@ -23,7 +23,7 @@
 // Measured (B200): 600 rows of 151936 ids 45.9 us, with 8 alternatives 51.8 us = 3.5 TB/s. Without any arithmetic
 // the same loads take 36 us (all CTAs start and end together, and 8 SMs have five rows where the others
 // have four); the exponentials and sums add the rest (about nine instructions an id, one of them ex2). One row of
-// 128256 ids with 20 alternatives 9.8 us: a chain of latencies (2.5 us the pass, about 1 us each the sums, the threshold,
+// 128256 ids with 20 alternatives 9.1 us, with 64 11.3 us: a chain of latencies (2.5 us the pass, about 1 us each the sums, the threshold,
 // the candidates, the cluster barrier and the join). Packed FP32 pairs, two loads in flight instead of four,
 // and the next loads issued before the current sums gave the same or longer times; a pass per alternative (the
 // first version) 1301 us and 543 us.
@@ -154,17 +154,17 @@ struct LgpShared
     int n_owners;
 };
 
-// keys[0, m) ranked into sh.top[0, n): a key's place is the number of larger ones. The
-// keys are distinct but for zeros, which stand for none and come last; keys[m] is 0 or
-// not there. One copy of the code for both calls: the second one finds it in the instruction
-// cache, worth 1.3 us of one row's 11.1 (a merge by bisection, fewer steps, took that longer).
-__device__ __noinline__ void lgp_rank(LgpShared &sh, const uint64_t *keys, int m, int n)
+// sh.cand[0, m) ranked into sh.top[0, n): a key's place is the number of larger ones (the
+// keys are distinct; where m is odd, sh.cand[m] is 0). One copy of the code for both
+// calls: the second one finds it in the instruction cache, worth 1.3 us of one row's 11.1
+// (a merge by bisection, fewer steps, took that longer).
+__device__ __noinline__ void lgp_rank(LgpShared &sh, int m, int n)
 {
     const int pairs = (m + 1) / 2;
-    const ulonglong2 *two = reinterpret_cast<const ulonglong2 *>(keys);
+    const ulonglong2 *two = reinterpret_cast<const ulonglong2 *>(sh.cand);
     for (int i = threadIdx.x; i < m; i += LGP_THREADS)
     {
-        const uint64_t k = keys[i];
+        const uint64_t k = sh.cand[i];
         int r = 0;
 #pragma unroll 4
         for (int j = 0; j < pairs; j++)
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(LGP_THREADS, 5) logprobs_kernel(LogprobArgs a)
                 sh.cand[sh.count] = 0;
         }
         __syncthreads();
-        lgp_rank(sh, sh.cand, sh.count, a.n_top);
+        lgp_rank(sh, sh.count, a.n_top);
     }
 
     // ---- rank 0 joins the parts and writes the row
@@ -513,6 +513,7 @@ __global__ void __launch_bounds__(LGP_THREADS, 5) logprobs_kernel(LogprobArgs a)
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         if (tid == 0)
         {
+            sh.count = 0;
             *cl.map_shared_rank(&sh.parts[rank], 0) = s;
             *cl.map_shared_rank(&sh.counts[rank], 0) = a.n_top ? sh.n_top : 0;
         }
@@ -523,7 +524,23 @@ __global__ void __launch_bounds__(LGP_THREADS, 5) logprobs_kernel(LogprobArgs a)
             return;
         if (a.n_top)
         {
-            lgp_rank(sh, sh.lists, C * a.n_top, a.n_top);
+            // every list has ceil(n / C) keys that reach its own ceil(n / C)-th: the smallest of these is reached by
+            // n keys, and what lies below it is not among the n best
+            const int part = (a.n_top + C - 1) / C - 1;
+            uint64_t least = ~0ull;
+            for (int c = 0; c < C; c++)
+                least = min(least, sh.lists[c * a.n_top + part]);
+            for (int i = tid; i < C * a.n_top; i += LGP_THREADS)
+            {
+                const uint64_t k = sh.lists[i];
+                if (k && k >= least)
+                    sh.cand[atomicAdd(&sh.count, 1)] = k;
+            }
+            __syncthreads();
+            if (tid == 0 && (sh.count & 1))
+                sh.cand[sh.count] = 0;
+            __syncthreads();
+            lgp_rank(sh, sh.count, a.n_top);
             __syncthreads();
         }
     }
