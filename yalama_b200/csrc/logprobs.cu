@@ -12,18 +12,19 @@
 // terms refer to is shared by a warp, so that it moves seldom.
 //
 // The alternatives need no second pass over the row: each thread also keeps the
-// largest value it saw. With T the n_top-th largest of these, at least n_top ids have
-// a value >= T, so every alternative does, and only the threads whose largest is >= T
-// (n_top and a few) have any: the CTA reads those threads' vectors again (L1 or
-// L2), dealt out over all its threads, collects the ids >= T, and ranks them by
+// largest value it saw in each half of its vectors. With T the n_top-th largest of the threads'
+// values, at least n_top ids have a value >= T, so every alternative does, and only the halves
+// whose largest is >= T (n_top and a few) have any: the CTA reads those again,
+// dealt out over all its threads, collects the ids >= T, and ranks them by
 // counting. Where that collects more than LGP_CAP (many equal values, or the largest
 // ones all in one thread's part) or the row has a NaN, a radix select over the part
 // takes its place. Rank 0 of the cluster joins the CTAs' sums and lists.
 //
-// Measured (B200): 600 rows of 151936 ids 45.9 us, with 8 alternatives 51.8 us = 3.5 TB/s. Without any arithmetic
+// Measured (B200): 600 rows of 151936 ids 45.9 us, with 8 alternatives 51.2 us = 3.6 TB/s (of DRAM also the halves
+// read again, a tenth of the row). Without any arithmetic
 // the same loads take 36 us (all CTAs start and end together, and 8 SMs have five rows where the others
 // have four); the exponentials and sums add the rest (about nine instructions an id, one of them ex2). One row of
-// 128256 ids with 20 alternatives 9.1 us, with 64 11.3 us: a chain of latencies (2.5 us the pass, about 1 us each the sums, the threshold,
+// 128256 ids with 20 alternatives 9.5 us, with 64 11.4 us: a chain of latencies (2.5 us the pass, about 1 us each the sums, the threshold,
 // the candidates, the cluster barrier and the join). Packed FP32 pairs, two loads in flight instead of four,
 // and the next loads issued before the current sums gave the same or longer times; a pass per alternative (the
 // first version) 1301 us and 543 us.
@@ -37,7 +38,8 @@ namespace cg = cooperative_groups;
 
 constexpr int LGP_THREADS = 256;
 constexpr int LGP_WARPS = LGP_THREADS / 32;
-constexpr int LGP_U = 4;      // 16-byte loads in flight per thread
+constexpr int LGP_U = 4;      // 16-byte loads in flight per thread: a unit, of two halves
+static_assert(LGP_U == 4, "a half is two vectors");
 constexpr int LGP_CAP = 512;  // collected candidates per CTA
 constexpr int LGP_TOP = 64;   // largest n_top
 constexpr int LGP_MAXC = 8;   // largest cluster (the portable size)
@@ -150,7 +152,7 @@ struct LgpShared
     uint64_t top[LGP_TOP];              // the best, best first
     alignas(16) uint64_t cand[LGP_CAP]; // collected keys
     alignas(16) uint64_t lists[LGP_MAXC * LGP_TOP]; // rank 0: every CTA's best, 0 behind its last
-    uint16_t owners[LGP_THREADS];       // threads with candidates
+    uint16_t owners[LGP_THREADS * 2]; // halves of threads' vectors with candidates
     int n_owners;
 };
 
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(LGP_THREADS, 5) logprobs_kernel(LogprobArgs a)
     const __half2 lowest = __half2half2(__ushort_as_half(0xFBFFu));
     float m = -INFINITY, c = 0.f, delta = 0.f;
     float2 z = make_float2(0.f, 0.f), w = z; // two of each, for the two halves of a pair
-    __half2 tmax2 = lowest;
+    __half2 tmax2[2] = {lowest, lowest}; // the largest values seen in the first and second half of this thread's units
     const int inner = min(v1, nv - 1); // vectors (0, inner) lie in the row whole
     for (int v = v0 + tid; v - lane < v1; v += LGP_THREADS * LGP_U)
     {
@@ -341,14 +343,18 @@ __global__ void __launch_bounds__(LGP_THREADS, 5) logprobs_kernel(LogprobArgs a)
                                                 : make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
         }
         __half2 *h = reinterpret_cast<__half2 *>(r);
-        __half2 um = lowest;
+        __half2 um;
 #pragma unroll
-        for (int i = 0; i < 4 * LGP_U; i++)
+        for (int u = 0; u < LGP_U; u++)
         {
-            h[i] = __hmax2_nan(h[i], lowest);
-            um = __hmax2(um, h[i]);
+#pragma unroll
+            for (int i = 4 * u; i < 4 * u + 4; i++)
+            {
+                h[i] = __hmax2_nan(h[i], lowest);
+                tmax2[u >> 1] = __hmax2(tmax2[u >> 1], h[i]);
+            }
         }
-        tmax2 = __hmax2(tmax2, um);
+        um = __hmax2(tmax2[0], tmax2[1]);
         const uint32_t mine = ord16(__half_as_ushort(__hmax(__low2half(um), __high2half(um))));
         const uint32_t most = __reduce_max_sync(0xffffffffu, mine);
         const float top = h2f(__ushort_as_half((unsigned short)unord16(most)));
@@ -425,12 +431,18 @@ __global__ void __launch_bounds__(LGP_THREADS, 5) logprobs_kernel(LogprobArgs a)
     // ---- this CTA's best ids
     if (a.n_top)
     {
-        const uint32_t mine = lgp_ord(__half_as_ushort(__hmax(__low2half(tmax2), __high2half(tmax2))));
         bool whole = nan;
         if (!whole)
         {
+            uint32_t mine[2], most = 0;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+            {
+                mine[u] = lgp_ord(__half_as_ushort(__hmax(__low2half(tmax2[u]), __high2half(tmax2[u]))));
+                most = max(most, mine[u]);
+            }
             // the largest T that n_top threads reach, bit by bit, by one warp
-            sh.most[tid] = (uint16_t)mine;
+            sh.most[tid] = (uint16_t)most;
             __syncthreads();
             if (warp == 0)
             {
@@ -450,29 +462,26 @@ __global__ void __launch_bounds__(LGP_THREADS, 5) logprobs_kernel(LogprobArgs a)
                     if (__reduce_add_sync(0xffffffffu, n) >= a.n_top)
                         T |= 1u << b;
                 }
-                T = max(T, LGP_LOWEST);
-                int n = 0;
-#pragma unroll
-                for (int i = 0; i < LGP_WARPS; i++)
-                {
-                    const uint32_t has = __ballot_sync(0xffffffffu, v[i] >= T);
-                    if (v[i] >= T)
-                        sh.owners[n + __popc(has & ((1u << lane) - 1u))] = (uint16_t)(i * 32 + lane);
-                    n += __popc(has);
-                }
                 if (lane == 0)
                 {
-                    sh.T = T;
-                    sh.n_owners = n;
+                    sh.T = max(T, LGP_LOWEST);
+                    sh.n_owners = 0;
                 }
             }
             __syncthreads();
-            // the owners' vectors again, dealt out over the CTA: consecutive threads take consecutive owners
             const uint32_t T = sh.T;
-            const int n_owners = sh.n_owners, total = n_owners * ((v1 - v0 + LGP_THREADS - 1) / LGP_THREADS);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (mine[u] >= T)
+                    sh.owners[atomicAdd(&sh.n_owners, 1)] = (uint16_t)(u * (LGP_U / 2) * LGP_THREADS + tid);
+            __syncthreads();
+            // the owners' vectors again, dealt out over the CTA: consecutive threads take consecutive owners
+            constexpr int STEP = LGP_THREADS * LGP_U;
+            const int n_owners = sh.n_owners, total = n_owners * (LGP_U / 2) * ((v1 - v0 + STEP - 1) / STEP);
             for (int i = tid; i < total; i += LGP_THREADS)
             {
-                const int k = i / n_owners, v = v0 + k * LGP_THREADS + sh.owners[i - k * n_owners];
+                const int k = i / n_owners; // unit k / 2, vector k % 2 of the owner's half
+                const int v = v0 + (k >> 1) * STEP + (k & 1) * LGP_THREADS + sh.owners[i - k * n_owners];
                 if (v >= v1)
                     continue;
                 const uint4 r = row.load(v);
