@@ -29,7 +29,6 @@
 // and the next loads issued before the current sums gave the same or longer times; a pass per alternative (the
 // first version) 1301 us and 543 us.
 #include "ylm_common.cuh"
-#include <algorithm>
 #include <cooperative_groups.h>
 
 namespace ylm {
@@ -606,8 +605,8 @@ cudaError_t logprobs_launch(const LogprobArgs &a, int num_sms, cudaStream_t s)
     while (C > 1 && ((int64_t)a.rows * (C / 2) >= LGP_FILL * num_sms || a.vocab < C * LGP_PART))
         C /= 2;
     cudaLaunchConfig_t cfg = {};
-    const unsigned y = (unsigned)std::min(a.rows, 32768);
-    cfg.gridDim = dim3((unsigned)C, y, (unsigned)((a.rows + (int64_t)y - 1) / y));
+    const int64_t z = ((int64_t)a.rows + 65534) / 65535; // a grid's y and z end at 65535
+    cfg.gridDim = dim3((unsigned)C, (unsigned)((a.rows + z - 1) / z), (unsigned)z);
     cfg.blockDim = dim3(LGP_THREADS);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
