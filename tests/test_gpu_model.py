@@ -1,6 +1,7 @@
 """Model-level parity on the GPU: the engine's token loop (prefill, decode,
 sampling, KV-cache state machine) against the oracle's FP16-storage forward on
 the same seeded weights, through the C ABI."""
+import ctypes
 import json
 import os
 import time
@@ -423,3 +424,20 @@ def test_fused_greedy_pick_is_the_argmax(fam):
         lg = eng.logits(as_float32=False)
         assert nxt == int(np.argmax(lg))
         tok = nxt
+
+
+@pytest.mark.parametrize("count", [1, 2, 3])
+def test_generate_writes_no_more_than_max_new_ids(count):
+    spec, eng = make(FAMILIES["llama"])
+    prompt = synth.prompt_ids(12, 32, spec.vocab)
+    want = [int(t) for t in eng.generate(prompt, 4, eos_ids=[])["ids"]]
+    p = np.asarray(prompt, np.int64)
+    out = np.full(16, -77, np.int64)
+    n, a, b = ctypes.c_int32(), ctypes.c_double(), ctypes.c_double()
+    i64 = ctypes.POINTER(ctypes.c_int64)
+    E.check(E.lib().ylm_generate(eng._h, p.ctypes.data_as(i64), p.size, count, None, 0, out.ctypes.data_as(i64),
+                                 ctypes.byref(n), ctypes.byref(a), ctypes.byref(b)), "ylm_generate")
+    assert n.value == count and out[:count].tolist() == want[:count]
+    assert (out[count:] == -77).all()
+    # the last slot written belongs to the last step that ran
+    assert eng.info()["last_kv_index"] == len(prompt) - 1 + count - 1

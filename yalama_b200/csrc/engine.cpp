@@ -1971,6 +1971,8 @@ int ylm_generate(ylm_engine *e, const int64_t *prompt, int32_t n_prompt, int32_t
         out_ids[(*n_out)++] = next;
         if (!kv)
             ids.push_back(next);
+        if (generated >= max_new)
+            return finish();
 
         if (!kv || e->last == 0 || e->u_next >= 0.f || !e->opt.use_cuda_graph)
         {
