@@ -163,7 +163,11 @@ int ylm_sample(ylm_engine *e, int32_t greedy, int64_t *next_id);
  * ylm_decode or ylm_infer. masked != 0: over the ids that ylm_set_sampling left
  * unmasked; -inf for an id that is masked or outside the vocabulary. The state of
  * the token loop does not change. Tensor parallel: gathers the logits first, as
- * ylm_logits does. YLM_NOT_READY before the first logits. No counterpart in the reference. */
+ * ylm_logits does. After ylm_generate the logits are those that the last token it read
+ * was chosen by, except where it stopped at an EOS id with the next step already
+ * on its way: that step's logits have taken their place. YLM_NOT_READY then (until the
+ * next step), after a step that failed, and before the first logits. To score every
+ * token of an answer, step with ylm_decode. No counterpart in the reference. */
 int ylm_logprobs(ylm_engine *e, int64_t id, int32_t n_top, int32_t masked, float *logprob, float *entropy,
                  int64_t *top_ids, float *top_logprobs);
 /* One decode step and its sample in one graph launch: Infer({id}) + Sample. */

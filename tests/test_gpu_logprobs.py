@@ -274,3 +274,78 @@ def test_engine_logprobs_of_a_generated_token():
             eng.logprobs(0, **bad) if bad["n_top"] > 0 else E.check(
                 E.lib().ylm_logprobs(eng._h, 0, -1, 0, None, None, None, None), "x")
     eng.close()
+
+
+def test_engine_logprobs_after_a_token_loop():
+    """After ylm_generate the log probabilities are those of the last token it read, or refused where the loop had
+    run a step past an EOS, whose logits belong to no token of the request."""
+    from yalama_b200 import synth
+    spec = synth.tiny_spec("llama", tied=False, rope_theta=5e5, heads=8, kv_heads=2)
+    eng, ref = (E.Engine(None, E.config_from_spec(spec), init_seed=0) for _ in range(2))
+    for e in (eng, ref):
+        e.set_sampling(greedy=True)
+    prompt = synth.prompt_ids(12, 32, spec.vocab)
+    ids = [int(t) for t in eng.generate(prompt, 20)["ids"]]
+    stop = next(i for i in range(3, len(ids) - 1) if ids[i] not in ids[:i])
+
+    def want(count):
+        """The log probabilities that token `count` was chosen by."""
+        ref.begin_infer()
+        ref.infer(prompt)
+        for t in ids[:count]:
+            ref.infer([t])
+        return ref.logprobs(ids[count], 5)
+
+    def same(a, b):
+        assert a["logprob"] == b["logprob"] and a["entropy"] == b["entropy"]
+        np.testing.assert_array_equal(a["top_ids"], b["top_ids"])
+        np.testing.assert_array_equal(a["top_logprobs"], b["top_logprobs"])
+
+    # the loop ends at max_new
+    for count in (1, 2, 7):
+        eng.generate(prompt, count)
+        same(eng.logprobs(ids[count - 1], 5), want(count - 1))
+    # at an EOS that is also the last token allowed: no step ran past it
+    r = eng.generate(prompt, stop + 1, eos_ids=[ids[stop]])
+    assert [int(t) for t in r["ids"]] == ids[:stop]
+    same(eng.logprobs(ids[stop], 5), want(stop))
+    # at an EOS with another step on its way
+    r = eng.generate(prompt, 20, eos_ids=[ids[stop]])
+    assert [int(t) for t in r["ids"]] == ids[:stop]
+    with pytest.raises(E.YlmError) as ei:
+        eng.logprobs(ids[stop], 5)
+    assert ei.value.status == E.Status.NOT_READY
+    # the next step has logits of its own
+    eng.infer([ids[stop]])
+    same(eng.logprobs(ids[stop + 1], 5), want(stop + 1))
+    eng.generate(prompt, 20, eos_ids=[ids[stop]])
+    eng.decode(ids[stop], True)
+    same(eng.logprobs(ids[stop + 1], 5), want(stop + 1))
+    eng.generate(prompt, 4)
+    same(eng.logprobs(ids[3], 5), want(3))
+    eng.close()
+    ref.close()
+
+
+def test_engine_logprobs_after_a_failed_step():
+    """A step whose bounded wait ran out leaves logits of no token; the next request has its own."""
+    from yalama_b200 import synth
+    spec = synth.tiny_spec("llama", tied=False, rope_theta=5e5, heads=8, kv_heads=2)
+    eng = E.Engine(None, E.config_from_spec(spec), init_seed=0, wait_limit_us=2000)
+    prompt = synth.prompt_ids(13, 24, spec.vocab)
+    eng.begin_infer()
+    eng.infer(prompt)
+    want = eng.logprobs(5, 3)
+    eng.debug_drop_output(0)
+    with pytest.raises(E.YlmError) as ei:
+        eng.infer([5])
+    assert ei.value.status == E.Status.DEVICE_TIMEOUT
+    eng.debug_drop_output(-1)
+    with pytest.raises(E.YlmError) as ei:
+        eng.logprobs(5, 3)
+    assert ei.value.status == E.Status.NOT_READY
+    eng.begin_infer()
+    eng.infer(prompt)
+    got = eng.logprobs(5, 3)
+    assert got["logprob"] == want["logprob"] and got["entropy"] == want["entropy"]
+    eng.close()

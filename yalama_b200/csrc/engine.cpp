@@ -328,6 +328,9 @@ struct ylm_engine
     int last = 0;
     int max_seq = 0;
     bool has_logits = false;
+    // the logits buffer holds, or may hold, a step that is not part of the request: one that ylm_generate had on its
+    // way past an EOS, or one that failed. ylm_logprobs refuses until the next step
+    bool logits_foreign = false;
 
     int greedy = 1, top_k = 40;
     float temp = 0.6f;
@@ -1461,6 +1464,7 @@ struct ylm_engine
                 CK(cudaEventCreate(&ev_b));
             }
             CK(cudaEventRecord(ev_a, st));
+            logits_foreign = true;
             run_prefill(n);
             CK(cudaEventRecord(ev_b, st));
             pull_state_sync();
@@ -1483,11 +1487,13 @@ struct ylm_engine
                 fail(YLM_SEQUENCE_LENGTH_EXCEEDED, "position beyond the RoPE table");
             fill_state(ids[0], slot, pos, true, 0);
             push_state();
+            logits_foreign = true;
             launch_forward(false);
             pull_state_sync();
             last++;
         }
         has_logits = true;
+        logits_foreign = false;
         return YLM_OK;
     }
 
@@ -1532,6 +1538,8 @@ struct ylm_engine
         } h;
         if (!has_logits)
             fail(YLM_NOT_READY, "no logits yet");
+        if (logits_foreign)
+            fail(YLM_NOT_READY, "the logits are not of a step of this request");
         gather_logits();
         if (!lgp_out)
             lgp_out = dalloc<char>(sizeof(Out));
@@ -1586,10 +1594,12 @@ struct ylm_engine
             fail(YLM_SEQUENCE_LENGTH_EXCEEDED, "position beyond the RoPE table");
         fill_state(id, slot, pos, do_greedy, 0);
         push_state();
+        logits_foreign = true;
         launch_forward(true, do_greedy);
         pull_state_sync();
         last++;
         has_logits = true;
+        logits_foreign = false;
         note_sample(do_greedy);
         *next = hout->next_token;
         return YLM_OK;
@@ -2052,6 +2062,7 @@ int ylm_generate(ylm_engine *e, const int64_t *prompt, int32_t n_prompt, int32_t
         e->fill_state(next, e->last + 1, e->opt.rope_compat ? e->last : e->last + 1, greedy, 1);
         e->push_state();
         auto t_prev = clk::now();
+        e->logits_foreign = true; // until the loop ends with the step that it read last
         launch(0);
         for (int k = 0;; k++)
         {
@@ -2075,16 +2086,18 @@ int ylm_generate(ylm_engine *e, const int64_t *prompt, int32_t n_prompt, int32_t
             {
                 if (more)
                 {
-                    // discard the step launched past the end
+                    // discard the step launched past the end (its logits stay in the buffer)
                     CK(cudaStreamSynchronize(e->st));
                     e->last--;
                     e->calls--;
                 }
+                e->logits_foreign = more;
                 break;
             }
             out_ids[(*n_out)++] = next;
             if (!more)
             {
+                e->logits_foreign = false;
                 if (why != YLM_OK && generated < max_new)
                 {
                     status = why;
