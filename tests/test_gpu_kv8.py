@@ -649,3 +649,26 @@ def test_a_long_request_on_a_fixed_budget(fmt, prompt, budget, cap):
     np.testing.assert_array_equal(top_ids.cpu().numpy()[0], R.top(x[0], np.ones(vocab, bool), 3))
     np.testing.assert_allclose(top.cpu().numpy()[0], ref_lp[0][top_ids.cpu().numpy()[0]], rtol=1e-5, atol=1e-5)
     assert float(lp[0]) == float(top[0, 0])
+
+
+def test_a_failed_call_does_not_fail_the_next_one():
+    # a workspace that no device has is refused by the allocator, before any launch
+    c, ref = DeviceCache("e4m3", 16, 32, 1), R.Cache("e4m3", 16, 32, 1)
+    q = torch.zeros(1, 8 * 128 * D, dtype=torch.float16, device="cuda")
+    big = E.kv8_cache(ptr(c.code["k"]), ptr(c.code["v"]), ptr(c.scale["k"]), ptr(c.scale["v"]), "e4m3", 16, 1 << 30, 8)
+    assert E.kv8_attention_workspace(big, 8 * 128, 1, 1 << 30, True) > 1 << 42
+    acc = torch.zeros(32, device="cuda")
+    for _ in range(2):
+        assert E.lib().ylm_k_kv8_attention(big, ptr(q), q.stride(0), 8 * 128, 1, 1 << 30, None, ptr(acc), ptr(q),
+                                           q.stride(0), None, 0, stream()) == E.Status.CUDA_ERROR
+    k = rows(np.random.default_rng(0), 20, 1)
+    c.store(half(k), half(k), 0)
+    ref.store(k.astype(np.float64), k.astype(np.float64), 0)
+    c.same_as(ref, 20)
+    # nor a launch elsewhere in the library
+    assert E.lib().ylm_k_kv8_attention(big, ptr(q), q.stride(0), 8 * 128, 1, 1 << 30, None, ptr(acc), ptr(q),
+                                       q.stride(0), None, 0, stream()) == E.Status.CUDA_ERROR
+    a = torch.ones(130, 128, dtype=torch.float16, device="cuda")
+    o = torch.zeros(130, 130, dtype=torch.float16, device="cuda")
+    E.check(E.lib().ylm_k_gemm(ptr(a), ptr(a), 130, 130, 128, ptr(o), 1, stream()), "gemm")
+    assert bool((o == 128).all())

@@ -25,8 +25,17 @@ int done(cudaError_t e)
         set_last_error("");
         return YLM_OK;
     }
+    // the runtime keeps a failed call's error until it is asked for, and a later launch of this library would
+    // take it for its own
+    cudaGetLastError();
     set_last_error(cudaGetErrorString(e));
     return YLM_CUDA_ERROR;
+}
+
+int no_device()
+{
+    cudaGetLastError();
+    return refuse(YLM_CUDA_ERROR, "device set-up failed");
 }
 
 bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -112,7 +121,7 @@ int ylm_k_kv8_store(const ylm_kv8_cache *cache, const void *k, int64_t k_stride,
     if (k_stride < row || v_stride < row || k_stride % 8 || v_stride % 8)
         return refuse(YLM_INVALID_ARG, "token strides must be multiples of 8 halves and hold hkv x 128");
     if (prepare_device() != cudaSuccess)
-        return refuse(YLM_CUDA_ERROR, "device set-up failed");
+        return no_device();
     return done(kv8_store_launch(to_kernel(*cache), static_cast<const __half *>(k), static_cast<const __half *>(v),
                                  k_stride, v_stride, t, slot, static_cast<cudaStream_t>(stream)));
 }
@@ -126,7 +135,7 @@ int ylm_k_kv8_attention_workspace(const ylm_kv8_cache *cache, int32_t hq, int32_
         return refuse(YLM_INVALID_ARG, f);
     const int sms = sm_count();
     if (!sms)
-        return refuse(YLM_CUDA_ERROR, "no device");
+        return no_device();
     *bytes = kv8_attn_workspace(cache->hkv, hq, t, n, with_acc != 0, sms);
     return done(cudaSuccess);
 }
@@ -150,7 +159,7 @@ int ylm_k_kv8_attention(const ylm_kv8_cache *cache, const void *q, int64_t q_str
         return refuse(YLM_INVALID_ARG, "workspace must be 16-byte aligned");
     const int sms = sm_count();
     if (!sms || prepare_device() != cudaSuccess)
-        return refuse(YLM_CUDA_ERROR, "device set-up failed");
+        return no_device();
     const size_t need = kv8_attn_workspace(cache->hkv, hq, t, n, acc != nullptr, sms);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     void *ws = workspace;
@@ -226,7 +235,7 @@ int ylm_k_kv8_evict(const ylm_kv8_cache *src, const ylm_kv8_cache *dst, const fl
             if (overlap(to[i].p, to[i].n, to[j].p, to[j].n))
                 return refuse(YLM_INVALID_ARG, "the destination's buffers must not overlap");
     if (prepare_device() != cudaSuccess)
-        return refuse(YLM_CUDA_ERROR, "device set-up failed");
+        return no_device();
     Kv8EvictArgs a;
     a.src = to_kernel(*src);
     a.dst = to_kernel(*dst);
@@ -261,7 +270,7 @@ int ylm_k_logprobs(const void *logits, int64_t ld, int32_t rows, int64_t vocab, 
         return refuse(YLM_INVALID_ARG, "null logits");
     const int sms = sm_count();
     if (!sms || prepare_device() != cudaSuccess)
-        return refuse(YLM_CUDA_ERROR, "device set-up failed");
+        return no_device();
     LogprobArgs a;
     a.logits = static_cast<const __half *>(logits);
     a.ld = ld;

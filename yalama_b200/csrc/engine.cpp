@@ -67,7 +67,10 @@ struct YlmError : std::runtime_error
     {                                                                                                                 \
         cudaError_t e_ = (call);                                                                                      \
         if (e_ != cudaSuccess)                                                                                        \
+        {                                                                                                             \
+            cudaGetLastError(); /* reported here, not by the next launch */                                           \
             fail(YLM_CUDA_ERROR, "%s:%d %s: %s", __FILE__, __LINE__, #call, cudaGetErrorString(e_));                  \
+        }                                                                                                             \
     } while (0)
 
 #define NK(call)                                                                                                      \

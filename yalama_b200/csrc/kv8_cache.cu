@@ -87,30 +87,34 @@ __global__ void __launch_bounds__(KST_THREADS)
     }
 }
 
+template <int FMT, int P>
+static cudaError_t store_launch(const Kv8Cache &c, const __half *k, const __half *v, int64_t ks, int64_t vs, int t,
+                                int slot, cudaStream_t s)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(((int64_t)slot + t - 1) / c.block - slot / c.block + 1), (unsigned)c.hkv, 2);
+    cfg.blockDim = dim3(KST_THREADS);
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, kv8_store_kernel<FMT, P>, c, k, v, ks, vs, t, slot);
+}
+
 template <int FMT>
 static cudaError_t store_fmt(const Kv8Cache &c, const __half *k, const __half *v, int64_t ks, int64_t vs, int t,
                              int slot, cudaStream_t s)
 {
-    const int blocks = (int)(((int64_t)slot + t - 1) / c.block) - slot / c.block + 1;
-    const dim3 grid((unsigned)blocks, (unsigned)c.hkv, 2);
     switch (c.block)
     {
     case 16:
-        kv8_store_kernel<FMT, 1><<<grid, KST_THREADS, 0, s>>>(c, k, v, ks, vs, t, slot);
-        break;
+        return store_launch<FMT, 1>(c, k, v, ks, vs, t, slot, s);
     case 32:
-        kv8_store_kernel<FMT, 2><<<grid, KST_THREADS, 0, s>>>(c, k, v, ks, vs, t, slot);
-        break;
+        return store_launch<FMT, 2>(c, k, v, ks, vs, t, slot, s);
     case 64:
-        kv8_store_kernel<FMT, 4><<<grid, KST_THREADS, 0, s>>>(c, k, v, ks, vs, t, slot);
-        break;
+        return store_launch<FMT, 4>(c, k, v, ks, vs, t, slot, s);
     case 128:
-        kv8_store_kernel<FMT, 8><<<grid, KST_THREADS, 0, s>>>(c, k, v, ks, vs, t, slot);
-        break;
+        return store_launch<FMT, 8>(c, k, v, ks, vs, t, slot, s);
     default:
         return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 cudaError_t kv8_store_launch(const Kv8Cache &c, const __half *k, const __half *v, int64_t k_stride, int64_t v_stride,
