@@ -291,7 +291,7 @@ typedef struct ylm_kv8_cache {
     float *k_scale, *v_scale; /* [hkv][ceil(cap / block)] */
     int32_t format;           /* ylm_kv8_format */
     int32_t block;            /* tokens per scale: 16, 32, 64 or 128 */
-    int32_t cap;              /* slots per KV head */
+    int32_t cap;              /* slots per KV head, at most 2^30 */
     int32_t hkv;              /* KV heads */
 } ylm_kv8_cache;
 /* Store t tokens in slots [slot, slot + t): k and v FP16, token i's KV head g at

@@ -135,3 +135,21 @@ def test_kv8_struct_layout_matches_c(tmp_path):
     subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "l")], check=True)
     got = [int(v) for v in subprocess.run([str(tmp_path / "l")], capture_output=True, text=True).stdout.split()]
     assert got == [ctypes.sizeof(E.KV8Cache)] + [getattr(E.KV8Cache, f).offset for f in fields]
+
+
+@pytest.mark.parametrize("cap", [2 ** 30 + 1, 2 ** 31 - 4000, 2 ** 31 - 1])
+def test_slots_whose_arithmetic_leaves_32_bits_are_refused(cap):
+    """More slots than any device holds: block counts, splits and strides over the slots would pass 32 bits."""
+    c, size = cache(cap=cap, hkv=1), ctypes.c_size_t()
+    good = cache(k=11 * A, v=12 * A, k_scale=13 * A, v_scale=14 * A, hkv=1)
+    assert store(c, slot=cap - 1) == INV
+    assert attend(c, n=cap) == INV
+    assert E.lib().ylm_k_kv8_attention_workspace(c, 4, 1, cap, 1, ctypes.byref(size)) == INV
+    assert evict(src=c, dst=good, n=50) == INV
+    far = [1 << 52, 1 << 53, 1 << 54, 1 << 55]  # so far apart that nothing overlaps
+    big = cache(k=far[0], v=far[1], k_scale=far[2], v_scale=far[3], cap=cap, hkv=1)
+    assert evict(src=good, dst=big, acc_dst=1 << 56, kept=1 << 57) == INV
+    # the largest that is taken: refused for its slots only, so these reach the device (or its absence)
+    c = cache(cap=2 ** 30, hkv=1)
+    assert attend(c, n=2 ** 30 + 1) == INV
+    assert E.lib().ylm_k_kv8_attention_workspace(c, 4, 1, 2 ** 30, 1, ctypes.byref(size)) != INV

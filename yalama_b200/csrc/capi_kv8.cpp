@@ -49,8 +49,9 @@ const char *cache_fault(const ylm_kv8_cache *c)
         return "unknown cache format";
     if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)
         return "cache block must be 16, 32, 64 or 128 tokens";
-    if (c->cap <= 0 || c->hkv <= 0 || c->hkv > 65535)
-        return "cache needs cap > 0 and 1..65535 KV heads";
+    // 2^30 slots of one head are 256 GiB of codes: no device holds more, and slot arithmetic keeps to 32 bits
+    if (c->cap <= 0 || c->cap > 1 << 30 || c->hkv <= 0 || c->hkv > 65535)
+        return "cache needs 1..2^30 slots and 1..65535 KV heads";
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
         return "cache codes must be 16-byte aligned and scales 4-byte aligned";
     return nullptr;
