@@ -306,7 +306,9 @@ int ylm_k_kv8_store(const ylm_kv8_cache *cache, const void *k, int64_t k_stride,
 /* Attention of the last t of n cached tokens (already stored): q [t][hq * 128],
  * RoPE applied, out likewise (token strides in halves, multiples of 8; pointers
  * 16-byte aligned); token i sees slots [0, n - t + i], scores scaled by
- * 1 / sqrt(128), softmax in FP32. t = 1 is a decode step; a draft or a prompt's
+ * 1 / sqrt(128). Scores, softmax statistics, sums and acc are FP32; each slot's weight is rounded to
+ * FP16 for the product with the values (by 2^-11 of itself; of weights below
+ * 2^-25 of the row's largest, by 2^-36 of that one), the result once more. t = 1 is a decode step; a draft or a prompt's
  * last tokens take more. At most 128 query heads per KV head.
  * mask_bits: (n + 31) / 32 words, bit i & 31 of word i / 32 = 1 hides slot i from
  * every head (null: none); a token that sees no slot gets zeros.

@@ -672,3 +672,79 @@ def test_a_failed_call_does_not_fail_the_next_one():
     o = torch.zeros(130, 130, dtype=torch.float16, device="cuda")
     E.check(E.lib().ylm_k_gemm(ptr(a), ptr(a), 130, 130, 128, ptr(o), 1, stream()), "gemm")
     assert bool((o == 128).all())
+
+
+# ---------------------------------------------------------------- values and scores far apart
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("t,n", [(1, 20), (3, 22), (1, 1100), (2, 1200)])
+@pytest.mark.parametrize("hq", [2, 8, 24])
+def test_attention_of_small_values_beside_a_block_of_large_ones(fmt, t, n, hq):
+    """A block with one channel of 30000 and small values elsewhere, whose scales are 2^24 apart: the other channels
+    come from the small values alone, and keep their digits."""
+    rng = np.random.default_rng(n + hq)
+    hkv = 2
+    k = rng.standard_normal((n, hkv, D)).astype(np.float16)
+    v = (1 + rng.random((n, hkv, D))) * 2.0 ** -11
+    v[:16] = 0
+    v[:16, :, 0] = rng.choice([-30000, 30000], (16, hkv))
+    v = v.astype(np.float16)
+    c, ref = DeviceCache(fmt, 16, n, hkv), R.Cache(fmt, 16, n, hkv)
+    c.store(half(k), half(v), 0)
+    ref.store(k.astype(np.float64), v.astype(np.float64), 0)
+    scale = ref.scale["v"]
+    assert np.all(scale[:, 0] / scale[:, 1] >= 2.0 ** 23)
+    hidden = np.zeros(n, bool)
+    hidden[18:n - t] = True
+    q = (rng.standard_normal((t, hq, D)) * 0.2).astype(np.float16)
+    check_attention(c, ref, q, t, n, hidden, torch.zeros(hkv, n, device="cuda"))
+    check_attention(c, ref, q, t, n)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n", [12, 1100])
+@pytest.mark.parametrize("order", ["first", "last"])
+def test_attention_of_large_values_behind_a_slot_that_takes_the_weight(fmt, n, order):
+    """One slot of value 0 takes all but about 2^-24 of the weight; what is left meets values of 20000."""
+    rng = np.random.default_rng(n)
+    hkv, hq = 1, 4
+    at = 0 if order == "first" else 11
+    q = np.repeat(rng.standard_normal((1, 1, D)), hq, 1).astype(np.float16)
+    k = (rng.standard_normal((n, hkv, D)) * 0.05).astype(np.float16)
+    v = (rng.standard_normal((n, hkv, D)) * 8000).astype(np.float16)
+    v[at] = 0
+    length = float((q[0, 0].astype(np.float64) ** 2).sum())
+    k[at, 0] = (q[0, 0].astype(np.float64) * (15.8 * np.sqrt(D) / length)).astype(np.float16)
+    c, ref = DeviceCache(fmt, 16, n, hkv), R.Cache(fmt, 16, n, hkv)
+    c.store(half(k), half(v), 0)
+    ref.store(k.astype(np.float64), v.astype(np.float64), 0)
+    hidden = np.zeros(n, bool)
+    hidden[12:] = True
+    out, _, _, _ = R.attention(q.astype(np.float64), ref.values("k", n), ref.values("v", n), 1, hidden)
+    assert 2.0 ** -15 < np.abs(out).max() < 2.0 ** -5
+    check_attention(c, ref, q, 1, n, hidden, torch.zeros(hkv, n, device="cuda"))
+
+
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("t,n,hq", [(1, 300, 8), (1, 1300, 8), (4, 500, 16), (6, 1400, 24)])
+@pytest.mark.parametrize("seed", range(4))
+def test_attention_of_values_at_random_scales(fmt, t, n, hq, seed):
+    """Every block of values at a scale of its own, up to 2^26 apart, some blocks of zeros, some slots hidden; each
+    block uses a few dimensions only, so that small values stand alone in many."""
+    rng = np.random.default_rng(100 * n + seed)
+    hkv, nb = 2, -(-n // 16)
+    k = rng.standard_normal((n, hkv, D)).astype(np.float16)
+    size = np.exp2(rng.uniform(-14, 12, (nb, hkv)))
+    size[rng.random((nb, hkv)) < 0.1] = 0
+    v = rng.standard_normal((n, hkv, D)) * np.repeat(size, 16, 0)[:n, :, None]
+    v *= np.repeat(rng.random((nb, hkv, D)) < 0.1, 16, 0)[:n]
+    v = v.astype(np.float16)
+    c, ref = DeviceCache(fmt, 16, n, hkv), R.Cache(fmt, 16, n, hkv)
+    c.store(half(k), half(v), 0)
+    ref.store(k.astype(np.float64), v.astype(np.float64), 0)
+    q = (rng.standard_normal((t, hq, D)) * 0.5).astype(np.float16)
+    check_attention(c, ref, q, t, n, None, torch.zeros(hkv, n, device="cuda"))
+    check_attention(c, ref, q, t, n, rng.random(n) < 0.7)

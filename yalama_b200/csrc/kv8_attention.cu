@@ -15,6 +15,7 @@
 #include "kv8.cuh"
 #include <algorithm>
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace ylm {
 
@@ -25,6 +26,11 @@ constexpr int KVA_BUF = KVA_CHUNK * YLM_HEAD_DIM; // bytes of a chunk's K or V
 constexpr int KVA_RING = 4 * KVA_BUF;             // a warp's two K and two V chunks
 constexpr int KVA_SMEM = KVA_WARPS * KVA_RING;
 constexpr int KVA_JOIN = 256;     // threads of the joining CTAs
+// FP16 weights: the largest score seen weighs 2^KVA_LEAD when the reference is set, and the reference moves when one
+// passes 2^KVA_MOST (FP16 ends at 2^16). A higher lead keeps more of the small weights, and moves the reference more
+// often: 8 x 4099 (64 / 8 heads) 12.9 us at a lead of 6, 13.0 at 9, 13.1 at 11, 13.4 at 12; one row the same at all.
+constexpr float KVA_LEAD = 11.f, KVA_MOST = 15.9f;
+constexpr float KVA_LIFT = 10.f;  // octaves below the largest value scale from which weights are lifted
 constexpr int KVA_CLUSTER = 8;    // most splits of a cluster (the portable size)
 // Slots up to which the splits of a KV head are one cluster. One launch against two, us of device time (8 heads of
 // 4 query heads; with kept weights): 100 slots 4.3 / 5.2 (5.5 / 6.2), 611 slots 5.0 / 5.3 (6.2 / 7.0), 1000 slots
@@ -132,6 +138,9 @@ __device__ __forceinline__ float kva_log_scale(float s)
     return (float)max(-64, min(64, (int)(__float_as_uint(s) >> 23 & 255u) - 127));
 }
 
+// 2^e, exactly, for a whole e of at most 64 either way
+__device__ __forceinline__ float kva_pow2(float e) { return __uint_as_float((uint32_t)(127 + (int)e) << 23); }
+
 // Both products run on the tensor cores with the slots as rows of the A operand,
 // so that 8 query rows fill the N dimension: S^T = K Q^T and O^T = V^T P^T
 // (m16n8k16; NT tiles of 8 query rows share each decoded fragment; more rows
@@ -150,11 +159,15 @@ __device__ __forceinline__ float kva_log_scale(float s)
 // one's K and V are in flight.
 //
 // Scales: ks multiplies the scores. vs enters the exponent: with y = x + log2 vs,
-// the PV weight is w = 2^(y - M) and the softmax sum takes w / vs (exact: vs is a power of two),
-// M >= max y - 8 moving only when y outgrows it, so that w <= 2^14 and the values' scales
-// never cost FP16 range. M is kept less 6 to the true reference. w enters P V rounded
-// to FP16 (the matrix unit's operand, 2^-11 of each weight, 2^28 of range below the
-// largest); M, l, the scores and both accumulators are FP32.
+// the PV weight is w = 2^(y - M) and the softmax sum takes w / vs (exact: vs is a power of two).
+// M is the largest y less KVA_LEAD, moving only when some w passes 2^KVA_MOST. w enters P V
+// rounded to FP16, the matrix unit's operand: off by 2^-11 of itself at most down to 2^-25 of the
+// largest (2^-14, FP16's smallest normal number), and by 2^-36 of the largest below (2^-25, half its
+// smallest step). That is the size of the result's own rounding to FP16; what a second product with the
+// weights' next 11 bits would add took 2 to 9 % longer at one row and 13 to 26 % with more. M, l, the
+// scores and both accumulators are FP32.
+// Slots whose values have a scale far below the largest have small w however large their softmax weight, and may
+// alone reach a dimension: their weights are lifted for the product (KVA_LIFT).
 //
 // Measured (B200, E4M3, 8 KV heads of 4 query heads, decode step without kept weights, both launches):
 // 131071 slots 48.4 us = 5.55 TB/s, and 6.4 TB/s for each slot more: bound by HBM behind about 7 us of
@@ -273,6 +286,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
         M[t][0] = M[t][1] = -INFINITY;
         l[t][0] = l[t][1] = 0.f;
     }
+    float vs_top = -INFINITY; // largest value scale so far of a half with a slot that is not masked
     constexpr int step = KVA_CHUNK * KVA_WARPS;
     int j0 = sp * w.p.len + warp * KVA_CHUNK;
     int phase = 0; // the buffers of this round: 0 or 1
@@ -377,9 +391,9 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
                 for (int e = 0; e < 4; e++)
                     grow = fmaxf(grow, S[s][t][e] + vs[s] - M[t][e & 1]);
         }
-        // ---- the reference follows where a score outgrew it by more than 2^8 (M is the reference less 6).
+        // ---- the reference follows where a score outgrew it by 2^(KVA_MOST - KVA_LEAD) (M is the reference less KVA_LEAD).
         // M = -inf makes grow +inf, or NaN (kept out by fmaxf) where the score is -inf, too
-        if (__any_sync(0xffffffffu, grow > 14.f))
+        if (__any_sync(0xffffffffu, grow > KVA_MOST))
         {
 #pragma unroll
             for (int t = 0; t < NT; t++)
@@ -389,7 +403,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
                     float m = fmaxf(fmaxf(S[0][t][i], S[0][t][i + 2]) + vs[0], fmaxf(S[1][t][i], S[1][t][i + 2]) + vs[1]);
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16)) - 6.f;
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16)) - KVA_LEAD;
                     if (m > M[t][i])
                     {
                         const float f = kva_ex2(M[t][i] - m);
@@ -407,104 +421,155 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
         // ---- O^T
         asm volatile("cp.async.wait_group 3;" ::: "memory");
         __syncwarp();
+        const auto weigh = [&](auto far_values) {
+            constexpr bool FAR = decltype(far_values)::value;
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-        {
-            uint4 V[4];
-            V[0] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + v_even);
-            V[1] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + v_odd);
-            V[2] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + 1024 + v_even);
-            V[3] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + 1024 + v_odd);
-            uint32_t P[NT][2];
-            const float unscale = __uint_as_float((uint32_t)(127 - (int)vs[s]) << 23);
-#pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int s = 0; s < 2; s++)
             {
-                // nothing seen so far: M = -inf, and every weight 0
-                const float shift[2] = {vs[s] - (M[t][0] == -INFINITY ? 0.f : M[t][0]),
-                                        vs[s] - (M[t][1] == -INFINITY ? 0.f : M[t][1])};
-                float e4[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                {
-                    e4[e] = kva_ex2(S[s][t][e] + shift[e & 1]);
-                }
-                l[t][0] += (e4[0] + e4[2]) * unscale;
-                l[t][1] += (e4[1] + e4[3]) * unscale;
-                const __half2 lo = __floats2half2_rn(e4[0], e4[1]), hi = __floats2half2_rn(e4[2], e4[3]);
-                P[t][0] = kva_transpose(*reinterpret_cast<const uint32_t *>(&lo));
-                P[t][1] = kva_transpose(*reinterpret_cast<const uint32_t *>(&hi));
-            }
-            // hidden slots may hold anything, NaN codes too: 0 x NaN must not arise
-            if (off[s])
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (off[s] >> (2 * c + (i & 1) + 8 * (i >> 1)) & 1u)
-                        V[i] = make_uint4(0, 0, 0, 0);
-            if (FMT == KV8_E4M3 && edge[s] && a.t > 1)
-            {
-                // a slot that some rows do not see: its NaN codes are taken out and put
-                // back as NaN into the rows that do see it
-                uint32_t nan = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        nan |= (kva_word(V[i], k) & 0x7F7F7F7Fu) + 0x01010101u;
-                if (__any_sync(0xffffffffu, nan & 0x80808080u))
-                {
-                    uint32_t seen[NT][2];
+                uint4 V[4];
+                V[0] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + v_even);
+                V[1] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + v_odd);
+                V[2] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + 1024 + v_even);
+                V[3] = *reinterpret_cast<const uint4 *>(vb + s * 2048 + 1024 + v_odd);
+                float lift[NT][2];
+                if (FAR)
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
                         for (int i = 0; i < 2; i++)
-                            seen[t][i] = kva_transpose((S[s][t][2 * i] == -INFINITY ? 0u : 0x3C00u) |
-                                                       (S[s][t][2 * i + 1] == -INFINITY ? 0u : 0x3C000000u));
-                    uint32_t *v = reinterpret_cast<uint32_t *>(&V[0]);
-                    uint32_t flag[16]; // 1 (0x38 in E4M3) where a code is NaN
+                        {
+                            float m = fmaxf(S[s][t][i], S[s][t][i + 2]);
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                            // -inf (or NaN) where the row sees none of these slots: no weight, any lift
+                            lift[t][i] = fminf(fmaxf(floorf(KVA_LEAD - (m + vs[s] - M[t][i])), 0.f), 64.f);
 #pragma unroll
-                    for (int k = 0; k < 16; k++)
+                            for (int k = 0; k < 8; k++)
+                            {
+                                O[t][k][i] *= kva_pow2(lift[t][i]);
+                                O[t][k][i + 2] *= kva_pow2(lift[t][i]);
+                            }
+                        }
+                uint32_t P[NT][2];
+                const float unscale = kva_pow2(-vs[s]);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                {
+                    // nothing seen so far: M = -inf, and every weight 0
+                    const float shift[2] = {vs[s] - (M[t][0] == -INFINITY ? 0.f : M[t][0]),
+                                            vs[s] - (M[t][1] == -INFINITY ? 0.f : M[t][1])};
+                    float e4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
                     {
-                        const uint32_t hit = ((v[k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                        flag[k] = (hit >> 7) * 0x38u;
-                        v[k] &= ~((hit >> 7) * 0xFFu);
+                        e4[e] = kva_ex2(S[s][t][e] + shift[e & 1]);
                     }
+                    l[t][0] += (e4[0] + e4[2]) * unscale;
+                    l[t][1] += (e4[1] + e4[3]) * unscale;
+                    if (FAR)
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
+                        for (int e = 0; e < 4; e++)
+                            e4[e] = kva_ex2(S[s][t][e] + (shift[e & 1] + lift[t][e & 1]));
+                    const __half2 lo = __floats2half2_rn(e4[0], e4[1]), hi = __floats2half2_rn(e4[2], e4[3]);
+                    P[t][0] = kva_transpose(*reinterpret_cast<const uint32_t *>(&lo));
+                    P[t][1] = kva_transpose(*reinterpret_cast<const uint32_t *>(&hi));
+                }
+                // hidden slots may hold anything, NaN codes too: 0 x NaN must not arise
+                if (off[s])
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (off[s] >> (2 * c + (i & 1) + 8 * (i >> 1)) & 1u)
+                            V[i] = make_uint4(0, 0, 0, 0);
+                if (FMT == KV8_E4M3 && edge[s] && a.t > 1)
+                {
+                    // a slot that some rows do not see: its NaN codes are taken out and put
+                    // back as NaN into the rows that do see it
+                    uint32_t nan = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            nan |= (kva_word(V[i], k) & 0x7F7F7F7Fu) + 0x01010101u;
+                    if (__any_sync(0xffffffffu, nan & 0x80808080u))
                     {
-                        const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
-                        const uint32_t x = __byte_perm(flag[i >> 1], flag[4 + (i >> 1)], sel);
-                        const uint32_t y = __byte_perm(flag[8 + (i >> 1)], flag[12 + (i >> 1)], sel);
-                        uint32_t a0, a1, a2, a3;
-                        kv8_decode4<FMT>(x, a0, a1);
-                        kv8_decode4<FMT>(y, a2, a3);
+                        uint32_t seen[NT][2];
 #pragma unroll
                         for (int t = 0; t < NT; t++)
-                        {
-                            float d[4] = {0.f, 0.f, 0.f, 0.f};
-                            kva_mma(d, a0, a1, a2, a3, seen[t][0], seen[t][1]);
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (d[e] > 0.f)
-                                    O[t][i][e] = NAN;
+                            for (int i = 0; i < 2; i++)
+                                seen[t][i] = kva_transpose((S[s][t][2 * i] == -INFINITY ? 0u : 0x3C00u) |
+                                                           (S[s][t][2 * i + 1] == -INFINITY ? 0u : 0x3C000000u));
+                        uint32_t *v = reinterpret_cast<uint32_t *>(&V[0]);
+                        uint32_t flag[16]; // 1 (0x38 in E4M3) where a code is NaN
+#pragma unroll
+                        for (int k = 0; k < 16; k++)
+                        {
+                            const uint32_t hit = ((v[k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                            flag[k] = (hit >> 7) * 0x38u;
+                            v[k] &= ~((hit >> 7) * 0xFFu);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                        {
+                            const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+                            const uint32_t x = __byte_perm(flag[i >> 1], flag[4 + (i >> 1)], sel);
+                            const uint32_t y = __byte_perm(flag[8 + (i >> 1)], flag[12 + (i >> 1)], sel);
+                            uint32_t a0, a1, a2, a3;
+                            kv8_decode4<FMT>(x, a0, a1);
+                            kv8_decode4<FMT>(y, a2, a3);
+#pragma unroll
+                            for (int t = 0; t < NT; t++)
+                            {
+                                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                                kva_mma(d, a0, a1, a2, a3, seen[t][0], seen[t][1]);
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    if (d[e] > 0.f)
+                                        O[t][i][e] = NAN;
+                            }
                         }
                     }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-            {
-                const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
-                const uint32_t x = __byte_perm(kva_word(V[0], i >> 1), kva_word(V[1], i >> 1), sel);
-                const uint32_t y = __byte_perm(kva_word(V[2], i >> 1), kva_word(V[3], i >> 1), sel);
-                uint32_t a0, a1, a2, a3;
-                kv8_decode4<FMT>(x, a0, a1);
-                kv8_decode4<FMT>(y, a2, a3);
+                for (int i = 0; i < 8; i++)
+                {
+                    const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+                    const uint32_t x = __byte_perm(kva_word(V[0], i >> 1), kva_word(V[1], i >> 1), sel);
+                    const uint32_t y = __byte_perm(kva_word(V[2], i >> 1), kva_word(V[3], i >> 1), sel);
+                    uint32_t a0, a1, a2, a3;
+                    kv8_decode4<FMT>(x, a0, a1);
+                    kv8_decode4<FMT>(y, a2, a3);
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-                    kva_mma(O[t][i], a0, a1, a2, a3, P[t][0], P[t][1]);
+                    for (int t = 0; t < NT; t++)
+                    {
+                        kva_mma(O[t][i], a0, a1, a2, a3, P[t][0], P[t][1]);
+                    }
+                }
+                if (FAR)
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                            {
+                                O[t][k][i] *= kva_pow2(-lift[t][i]);
+                                O[t][k][i + 2] *= kva_pow2(-lift[t][i]);
+                            }
             }
-        }
+        };
+        // Values of a scale far below the largest so far: their weights would lose digits to FP16's range, although
+        // nothing else may reach their dimensions. Each row's are lifted by a power of two of its own while they
+        // are added, and the row's sums with them.
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+            if (off[s] != 0xFFFFu)
+                vs_top = fmaxf(vs_top, vs[s]);
+        if (fminf(vs[0], vs[1]) < vs_top - KVA_LIFT) // uniform over the warp
+            weigh(std::true_type{});
+        else
+            weigh(std::false_type{});
         __syncwarp(); // every lane has read this V
         if (j0 + 2 * step < j_end)
             copy(vc, j0 + 2 * step, ring_at + (2 + phase) * KVA_BUF);
