@@ -347,7 +347,9 @@ int ylm_k_kv8_evict(const ylm_kv8_cache *src, const ylm_kv8_cache *dst, const fl
  * mask_bits: (vocab + 31) / 32 words as for ylm_k_sample, one mask for all rows, or
  * null. Logits of masked ids are not looked at. A row whose unmasked logits hold a NaN or +inf
  * has NaN log probabilities and entropy (its top ids: NaN first); a row that is
- * masked or -inf throughout has logprob -inf and entropy 0. */
+ * masked or -inf throughout has logprob -inf and entropy 0. A log probability is off by
+ * at most (vocab / 400 + 72) 2^-24 + 2^-19 (the FP32 sum of its row: 2.5e-5 at 151936 ids, where
+ * 1e-7 is usual) and 2^-22 of itself; tested to 20 million ids. */
 int ylm_k_logprobs(const void *logits, int64_t ld, int32_t rows, int64_t vocab, const int64_t *ids,
                    const uint32_t *mask_bits, int32_t n_top, float *logprob, float *entropy, int64_t *top_ids,
                    float *top_logprobs, void *stream);

@@ -1,4 +1,6 @@
 """Log probabilities of rows of FP16 logits on the GPU, through the C ABI, against their definitions in 64 bits."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -348,4 +350,128 @@ def test_engine_logprobs_after_a_failed_step():
     eng.infer(prompt)
     got = eng.logprobs(5, 3)
     assert got["logprob"] == want["logprob"] and got["entropy"] == want["entropy"]
+    eng.close()
+
+
+# ---------------------------------------------------------------- special values in one CTA's part of a row
+
+PARTS = [(3000, 1), (20001, 2), (40000, 4), (131077, 8)]  # ids, CTAs a row (one to four rows)
+
+
+def part(vocab, parts, i):
+    """The ids well inside part i of a row."""
+    per = vocab // parts
+    return slice(i * per + 16, (i + 1) * per - 16)
+
+
+@pytest.mark.parametrize("vocab,parts", PARTS)
+def test_parts_without_ids(vocab, parts):
+    """Whole parts that are -inf or masked beside parts that are not, and fewer open ids than alternatives."""
+    rng = np.random.default_rng(vocab)
+    for i in range(parts):
+        own = part(vocab, parts, i)
+        x = rng.standard_normal((3, vocab)).astype(np.float16)
+        x[0, own] = -np.inf                       # one part has next to no id
+        x[1, :own.start], x[1, own.stop:] = -np.inf, -np.inf  # only one has
+        x[2] = -np.inf                            # seven ids, all in one
+        few = np.sort(rng.choice(np.arange(own.start, own.stop), 7, replace=False))
+        x[2, few] = rng.standard_normal(7) * 3
+        for n_top in (1, 20, 64):
+            check(x, [vocab - 1, own.start + 3, few[2]], n_top)
+        masked = np.ones(vocab, bool)             # the same by a mask
+        masked[few] = False
+        y = rng.standard_normal((2, vocab)).astype(np.float16)
+        check(y, [few[0], (few[0] + 1) % vocab], 20, masked)
+        check(y, [few[6], few[1]], 20, masked, ld=vocab + 5, shift=3)
+        check(y, [few[0], own.start], 20, ~masked)
+        masked = np.zeros(vocab, bool)
+        masked[own] = True
+        check(y, [own.start, vocab - 1], 20, masked)
+
+
+@pytest.mark.parametrize("vocab,parts", PARTS)
+def test_parts_with_nan_or_infinity(vocab, parts):
+    rng = np.random.default_rng(vocab + 1)
+    for i in range(parts):
+        own = part(vocab, parts, i)
+        x = rng.standard_normal((4, vocab)).astype(np.float16)
+        at = own.start + 7
+        x[0, at], x[1, at], x[2, at] = np.nan, np.inf, -np.nan
+        x[2, vocab - 2] = np.nan  # two: the lower id first
+        got = run(x, [5, at, 9, 5], 20)
+        for r in range(3):
+            assert np.isnan(got["logprob"][r]) and np.isnan(got["entropy"][r]) and np.isnan(got["top"][r]).all()
+        assert got["top_ids"][0][0] == at and got["top_ids"][1][0] == at
+        assert list(got["top_ids"][2][:2]) == [at, vocab - 2]
+        rest = np.where(np.isnan(x[0]), -np.inf, x[0]).astype(np.float64)
+        np.testing.assert_array_equal(got["top_ids"][0][1:], R.top(rest, np.ones(vocab, bool), 19))
+        masked = np.zeros(vocab, bool)
+        masked[[at, vocab - 2]] = True
+        check(x, [5, 6, 9, 8], 20, masked)
+
+
+@pytest.mark.parametrize("vocab,parts", PARTS)
+def test_parts_of_the_lowest_and_the_highest_values(vocab, parts):
+    rng = np.random.default_rng(vocab + 2)
+    for i in range(parts):
+        own = part(vocab, parts, i)
+        x = rng.standard_normal((4, vocab)).astype(np.float16)
+        x[0, own] = -65504
+        x[1] = -65504
+        x[1, own] = -np.inf
+        x[2] = -65504
+        x[2, own.start + 5] = -65472
+        x[3, own] = 65504
+        check(x, [own.start, 0, own.start + 5, own.start + 9], 20)
+
+
+@pytest.mark.parametrize("vocab,parts", PARTS)
+def test_rows_of_several_parts_without_any_id(vocab, parts):
+    for masked in (None, np.ones(vocab, bool)):
+        x = np.full((2, vocab), -np.inf if masked is None else 1.0, np.float16)
+        got = run(x, [0, vocab - 1], 20, masked)
+        assert np.all(got["logprob"] == -np.inf) and np.all(got["entropy"] == 0)
+        assert np.all(got["top_ids"] == -1) and np.all(got["top"] == -np.inf)
+
+
+@pytest.mark.parametrize("vocab", [3000017, 20000003])
+def test_vocabularies_beyond_any_model(vocab):
+    """One row, eight CTAs: a thread adds vocab / 4096 terms to a sum, and 72 additions join the sums."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (torch.randn(1, vocab, generator=g, device="cuda") * 2).half()
+    ids = torch.tensor([vocab - 1], device="cuda")
+    lp, ent = torch.zeros(1, device="cuda"), torch.zeros(1, device="cuda")
+    top_ids, top = torch.zeros(1, 20, dtype=torch.int64, device="cuda"), torch.zeros(1, 20, device="cuda")
+    E.check(E.lib().ylm_k_logprobs(ptr(x), vocab, 1, vocab, ptr(ids), None, 20, ptr(lp), ptr(ent), ptr(top_ids),
+                                   ptr(top), torch.cuda.current_stream().cuda_stream), "logprobs")
+    want = torch.log_softmax(x.double(), 1)
+    went = -(want.exp() * want).sum(1)
+    rel = (vocab / 4096 + 72) * 2.0 ** -24 + 2.0 ** -21
+    tol = rel + 2.0 ** -21 * 40  # log probabilities of at most 40
+    assert abs(float(lp) - float(want[0, -1])) <= tol
+    assert abs(float(ent) - float(went)) <= rel * (1 + 2 * float(went)) + 2.0 ** -21 * float(went)
+    best = torch.sort(x[0].float(), descending=True, stable=True).indices[:20]
+    assert torch.equal(top_ids[0], best)
+    assert float((top[0].double() - want[0, best]).abs().max()) <= tol
+
+
+def test_engine_logprobs_refuses_bad_counts():
+    """Refused for the count alone: every pointer is good."""
+    from yalama_b200 import synth
+    spec = synth.tiny_spec("llama")
+    eng = E.Engine(None, E.config_from_spec(spec), init_seed=0)
+    eng.begin_infer()
+    eng.infer(synth.prompt_ids(0, 8, spec.vocab))
+    lp, ent = ctypes.c_float(), ctypes.c_float()
+    ids, top = np.zeros(128, np.int64), np.zeros(128, np.float32)
+
+    def call(n_top, i=ids, t=top):
+        return E.lib().ylm_logprobs(eng._h, 0, n_top, 0, ctypes.byref(lp), ctypes.byref(ent),
+                                    None if i is None else E._ptr(i, ctypes.c_int64),
+                                    None if t is None else E._ptr(t, ctypes.c_float))
+
+    for n_top in (-1, -2 ** 31, 65, 2 ** 31 - 1):
+        assert call(n_top) == E.Status.INVALID_ARG
+    assert call(1, None) == E.Status.INVALID_ARG and call(1, ids, None) == E.Status.INVALID_ARG
+    assert call(64) == E.Status.OK and call(0, None, None) == E.Status.OK
     eng.close()
