@@ -333,7 +333,9 @@ int ylm_k_kv8_attention_workspace(const ylm_kv8_cache *cache, int32_t hq, int32_
  * its tokens had in src; tokens of a smaller one are rescaled to it. The caches
  * have the same format, block and hkv; dst, acc_dst and kept do not overlap src,
  * acc_src or one another (one spare layer serves a whole model: a layer's old
- * buffers are the next one's dst). dst's codes behind n_keep are left as they are. */
+ * buffers are the next one's dst). Afterwards dst and acc_dst are the layer's cache and
+ * weights together: acc_src is in src's slots, which dst does not have. dst's codes
+ * behind n_keep are left as they are. */
 int ylm_k_kv8_evict(const ylm_kv8_cache *src, const ylm_kv8_cache *dst, const float *acc_src, float *acc_dst,
                     int32_t n, int32_t n_keep, int32_t n_sink, int32_t n_recent, int32_t *kept, void *stream);
 
