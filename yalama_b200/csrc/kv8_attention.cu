@@ -10,7 +10,7 @@
 // fill the GPU otherwise), which leaves sums (M, l, O) per split and row. Up to
 // KVA_ALONE slots the splits of a KV head are one cluster, which joins them through
 // distributed shared memory and adds the weights from scores kept there: one launch, no
-// workspace. Beyond, sums and scores go through the workspace, and kv8_join_kernel
+// workspace. Beyond (and where weights are kept of more than 16 rows a KV head), sums and scores go through the workspace, and kv8_join_kernel
 // joins the splits and turns the scores into weights.
 #include "kv8.cuh"
 #include <algorithm>
@@ -34,7 +34,8 @@ constexpr float KVA_LIFT = 10.f;  // octaves below the largest value scale from 
 constexpr int KVA_CLUSTER = 8;    // most splits of a cluster (the portable size)
 // Slots up to which the splits of a KV head are one cluster. One launch against two, us of device time (8 heads of
 // 4 query heads; with kept weights): 100 slots 4.3 / 5.2 (5.5 / 6.2), 611 slots 5.0 / 5.3 (6.2 / 7.0), 1000 slots
-// 5.7 / 5.5 (6.9 / 7.4), 2000 slots 6.5 / 5.5 (8.2 / 7.7); a caller that launches each step also saves the second launch.
+// 5.7 / 5.5 (6.9 / 7.4), 2000 slots 6.5 / 5.5 (8.2 / 7.7). Without weights two launches are the faster already at 1000
+// slots, by 0.2 us in a captured graph; a caller that launches each step saves more than that with the second launch.
 constexpr int KVA_ALONE = 1024;
 constexpr int KVA_ALONE_LEN = KVA_ALONE / KVA_CLUSTER;
 static_assert(KVA_ALONE_LEN % (KVA_CHUNK * KVA_WARPS) == 0, "a split is whole rounds of its warps");
@@ -169,10 +170,11 @@ __device__ __forceinline__ float kva_pow2(float e) { return __uint_as_float((uin
 // Slots whose values have a scale far below the largest have small w however large their softmax weight, and may
 // alone reach a dimension: their weights are lifted for the product (KVA_LIFT).
 //
-// Measured (B200, E4M3, 8 KV heads of 4 query heads, decode step without kept weights, both launches):
-// 131071 slots 48.4 us = 5.55 TB/s, and 6.4 TB/s for each slot more: bound by HBM behind about 7 us of
-// start, tail and join; 8200 slots 8.5 us, 611 slots 5.2 us: bound by the two launches' latency. Eight tokens of
-// 64 / 8 heads over 4099 slots 13.6 us: bound by the instructions that decode every code once per 16 rows.
+// Measured (B200, E4M3, 8 KV heads of 4 query heads, decode step without kept weights): 131071 slots 48.1 us =
+// 5.58 TB/s in both launches (INT8 49.6 us), and 6.4 TB/s for each slot more: bound by HBM behind about 7 us of
+// start, tail and join; 8200 slots 8.2 us, bound by the two launches' latency; 611 slots 5.1 us in one launch, bound by
+// the latency of one chunk a warp and of the cluster's join. Eight tokens of 64 / 8 heads over 4099 slots 13.1 us:
+// bound by the instructions that decode every code once per 16 rows.
 // Registers as the buffers instead of the ring: 131071 slots 52 us, 611 slots 7.2 us (with the join of that
 // time); three CTAs an SM (NT = 1) at 168 registers; without the decode (wrong values) 131071 slots take 1 us less.
 template <int FMT, int NT, bool CLUSTER>
@@ -230,7 +232,10 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
     // this lane copies piece lane % 8 of rows 4 i + lane / 8: f there for even i, and for odd i
     const uint32_t dst_even = (lane >> 3) * 128 + (((lane & 7) ^ (((lane >> 4) & 1) << 1) ^ ((lane >> 3 & 1) << 2)) << 4);
     const uint32_t dst_odd = (lane >> 3) * 128 + (((lane & 7) ^ ((2 + ((lane >> 4) & 1)) << 1) ^ ((lane >> 3 & 1) << 2)) << 4);
-    // a step reads the codes once; what it writes for the join should stay in L2
+    // A decode step reads the codes once, and what it writes for the join should stay in L2: 131071 slots with kept
+    // weights 61.1 us against 62.4 with the normal policy, 32000 slots 17.6 against 18.2. The CTAs of more than 16 rows
+    // read the same codes at about the same time and find them in L2 under either policy: 8 tokens of 64 / 8 heads
+    // over 60000 and 131071 slots, 64 tokens over 30000, and several passes over 60000 differ by 0.5 % at most.
     const uint64_t policy = l2_policy_evict_first();
     auto copy = [&](const uint8_t *src, int j0, uint32_t at) {
         const int r0 = j0 + (lane >> 3);

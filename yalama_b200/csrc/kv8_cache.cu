@@ -323,8 +323,10 @@ __global__ void __launch_bounds__(KEV_THREADS) kv8_select_kernel(Kv8EvictArgs a)
 // largest of its tokens' old scales, and a token whose old block had a smaller
 // one is rescaled to it. Eight threads move a token's 128 codes, which are on
 // their way before the scales are known. Launched as a programmatic dependent of the
-// selection. Measured (B200): 40000 of 65536 slots, 8 heads, 164 MB in and out, 24 us at every
-// block size: HBM. A CTA per block took 30 us with blocks of 64 and 80 us with blocks of 16.
+// selection. Measured (B200): 40000 of 65536 slots, 8 heads, 82 MB in and 82 MB out, 24 us at every
+// block size (26 under the profiler, which saw 84 MB read from DRAM and 34 MB written: the other writes were
+// still in L2, so the memory is at 55 % of its rate meanwhile). It waits for loads and at its barriers.
+// A CTA per block took 30 us with blocks of 64 and 80 us with blocks of 16.
 constexpr int KEV_MOVE = 128; // the largest block
 template <int FMT> __global__ void __launch_bounds__(256) kv8_move_kernel(Kv8EvictArgs a)
 {

@@ -29,7 +29,8 @@
 // 128256 ids with 20 alternatives 9.5 us, with 64 11.4 us: a chain of latencies (2.5 us the pass, about 1 us each the sums, the threshold,
 // the candidates, the cluster barrier and the join). Packed FP32 pairs, two loads in flight instead of four,
 // and the next loads issued before the current sums gave the same or longer times; a pass per alternative (the
-// first version) 1301 us and 543 us.
+// first version) 1301 us and 543 us. Five CTAs an SM hold the kernel to 48 registers, for which it spills 12 bytes
+// a thread. A mask puts every vector on the checked path: one row of 128256 ids 7.8 us against 6.1.
 #include "ylm_common.cuh"
 #include <cooperative_groups.h>
 
