@@ -299,6 +299,8 @@ typedef struct ylm_kv8_cache {
  * fused QKV projection; multiples of 8, pointers 16-byte aligned). Slots below
  * `slot` in the first block are taken as filled: where a new token needs a larger
  * scale they are rescaled (one more rounding; E4M3: none above 2^-6 of a unit).
+ * A block keeps the scale of a token that was in it although another is stored in its place
+ * (a rejected draft), until the block is stored from its first slot again.
  * The other slots are left as they are. Infinities count as +-65504; NaN is kept
  * in E4M3 and stored as 0 in INT8. t = 0 does nothing. */
 int ylm_k_kv8_store(const ylm_kv8_cache *cache, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
