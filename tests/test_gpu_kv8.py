@@ -748,3 +748,43 @@ def test_attention_of_values_at_random_scales(fmt, t, n, hq, seed):
     q = (rng.standard_normal((t, hq, D)) * 0.5).astype(np.float16)
     check_attention(c, ref, q, t, n, None, torch.zeros(hkv, n, device="cuda"))
     check_attention(c, ref, q, t, n, rng.random(n) < 0.7)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("t,n,hq", [(1, 40, 2), (1, 300, 8), (1, 1300, 8), (3, 500, 16), (2, 1300, 24)])
+@pytest.mark.parametrize("size", [500, 1500, 2500, 4000, 6000, 10000, 20000])
+def test_attention_of_the_largest_scores(fmt, t, n, hq, size):
+    """Scores up to 10^10, where FP32 steps by octaves and more: one slot takes each row, its value is the result, and
+    the row's weight adds up to one."""
+    rng = np.random.default_rng(n + size)
+    hkv = 2
+    k = np.clip(rng.standard_normal((n, hkv, D)) * size, -65504, 65504).astype(np.float16)
+    v = (rng.standard_normal((n, hkv, D)) * np.exp2(rng.integers(-8, 8, -(-n // 16))).repeat(16)[:n, None, None])
+    v = v.astype(np.float16)
+    c, ref = DeviceCache(fmt, 16, n, hkv), R.Cache(fmt, 16, n, hkv)
+    c.store(half(k), half(v), 0)
+    ref.store(k.astype(np.float64), v.astype(np.float64), 0)
+    q = np.clip(rng.standard_normal((t, hq, D)) * size, -65504, 65504).astype(np.float16)
+    acc = torch.zeros(hkv, n, device="cuda")
+    got = attend(c, half(q), t, n, acc=acc).float().cpu().numpy().astype(np.float64).reshape(t, hq, D)
+    same = attend(c, half(q), t, n).float().cpu().numpy().astype(np.float64).reshape(t, hq, D)
+    kv, vv = ref.values("k", n), ref.values("v", n)
+    G, weight, sure = hq // hkv, np.zeros((hkv, n)), np.ones(hkv, bool)
+    for h in range(hq):
+        for i in range(t):
+            m, g = n - t + i + 1, h // G
+            x = kv[g, :m] @ q[i, h].astype(np.float64) / np.sqrt(D)
+            err = 2.0 ** -17 * (np.abs(kv[g, :m]) @ np.abs(q[i, h].astype(np.float64))).max() / np.sqrt(D)
+            best = int(x.argmax())
+            weight[g, best] += 1
+            if np.partition(x, -2)[-2] + err + 21 < x[best]:  # by more than the sums' rounding and 30 octaves
+                lo = hi = vv[g, best]
+            else:
+                lo, hi, sure[g] = vv[g, :m].min(0), vv[g, :m].max(0), False
+            for out in (got, same):
+                assert np.all(out[i, h] >= lo - EPS16 * np.abs(lo) * 2 - 2.0 ** -24)
+                assert np.all(out[i, h] <= hi + EPS16 * np.abs(hi) * 2 + 2.0 ** -24)
+    assert sure.any()
+    acc = acc.cpu().numpy()
+    np.testing.assert_allclose(acc[sure], weight[sure], rtol=2.0 ** -12, atol=2.0 ** -12)
+    np.testing.assert_allclose(acc.sum(1), weight.sum(1), rtol=2.0 ** -12)

@@ -28,7 +28,7 @@ constexpr int KVA_SMEM = KVA_WARPS * KVA_RING;
 constexpr int KVA_JOIN = 256;     // threads of the joining CTAs
 // FP16 weights: the largest score seen weighs 2^KVA_LEAD when the reference is set, and the reference moves when one
 // passes 2^KVA_MOST (FP16 ends at 2^16). A higher lead keeps more of the small weights, and moves the reference more
-// often: 8 x 4099 (64 / 8 heads) 12.9 us at a lead of 6, 13.0 at 9, 13.1 at 11, 13.4 at 12; one row the same at all.
+// often: 8 x 4099 (64 / 8 heads) 1 % longer at a lead of 11 than at 9, 3 % at 12; one row the same at all.
 constexpr float KVA_LEAD = 11.f, KVA_MOST = 15.9f;
 constexpr float KVA_LIFT = 10.f;  // octaves below the largest value scale from which weights are lifted
 constexpr int KVA_CLUSTER = 8;    // most splits of a cluster (the portable size)
@@ -139,7 +139,7 @@ __device__ __forceinline__ float kva_log_scale(float s)
     return (float)max(-64, min(64, (int)(__float_as_uint(s) >> 23 & 255u) - 127));
 }
 
-// 2^e, exactly, for a whole e of at most 64 either way
+// 2^e, exactly, for a whole e of at most 126 either way
 __device__ __forceinline__ float kva_pow2(float e) { return __uint_as_float((uint32_t)(127 + (int)e) << 23); }
 
 // Both products run on the tensor cores with the slots as rows of the A operand,
@@ -159,21 +159,24 @@ __device__ __forceinline__ float kva_pow2(float e) { return __uint_as_float((uin
 // buffers (cp.async, no barrier between warps): while it works on one chunk the next
 // one's K and V are in flight.
 //
-// Scales: ks multiplies the scores. vs enters the exponent: with y = x + log2 vs,
-// the PV weight is w = 2^(y - M) and the softmax sum takes w / vs (exact: vs is a power of two).
-// M is the largest y less KVA_LEAD, moving only when some w passes 2^KVA_MOST. w enters P V
+// Scales: ks multiplies the scores. vs enters the exponent: the PV weight of score x is
+// w = 2^((x - mx) + (log2 vs + cx)) and the softmax sum takes w / vs (exact: vs is a power of two). The
+// reference is the score mx of a slot that had the largest vs 2^x, with cx = KVA_LEAD less its own log2 vs,
+// and moves only when some w would pass 2^KVA_MOST. It is kept as a score and a small whole number
+// because x - mx is exact where it matters: scores of 2^24 and beyond step by octaves, and mx less the lead in one
+// number was off by as many. w enters P V
 // rounded to FP16, the matrix unit's operand: off by 2^-11 of itself at most down to 2^-25 of the
 // largest (2^-14, FP16's smallest normal number), and by 2^-36 of the largest below (2^-25, half its
 // smallest step). That is the size of the result's own rounding to FP16; what a second product with the
-// weights' next 11 bits would add took 2 to 9 % longer at one row and 13 to 26 % with more. M, l, the
-// scores and both accumulators are FP32.
+// weights' next 11 bits would add took 2 to 9 % longer at one row and 13 to 26 % with more. The
+// reference, l, the scores and both accumulators are FP32; a split's (M, l, O) leave in units of 2^(x - mx), M = mx.
 // Slots whose values have a scale far below the largest have small w however large their softmax weight, and may
 // alone reach a dimension: their weights are lifted for the product (KVA_LIFT).
 //
-// Measured (B200, E4M3, 8 KV heads of 4 query heads, decode step without kept weights): 131071 slots 48.1 us =
-// 5.58 TB/s in both launches (INT8 49.6 us), and 6.4 TB/s for each slot more: bound by HBM behind about 7 us of
-// start, tail and join; 8200 slots 8.2 us, bound by the two launches' latency; 611 slots 5.1 us in one launch, bound by
-// the latency of one chunk a warp and of the cluster's join. Eight tokens of 64 / 8 heads over 4099 slots 13.1 us:
+// Measured (B200, E4M3, 8 KV heads of 4 query heads, decode step without kept weights): 131071 slots 48.8 us =
+// 5.50 TB/s in both launches (INT8 49.7 us), and 6.4 TB/s for each slot more: bound by HBM behind about 7 us of
+// start, tail and join; 8200 slots 8.3 us, bound by the two launches' latency; 611 slots 5.2 us in one launch, bound by
+// the latency of one chunk a warp and of the cluster's join. Eight tokens of 64 / 8 heads over 4099 slots 13.4 us:
 // bound by the instructions that decode every code once per 16 rows.
 // Registers as the buffers instead of the ring: 131071 slots 52 us, 611 slots 7.2 us (with the join of that
 // time); three CTAs an SM (NT = 1) at 168 registers; without the decode (wrong values) 131071 slots take 1 us less.
@@ -279,7 +282,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
         }
     };
 
-    float O[NT][8][4], M[NT][2], l[NT][2];
+    float O[NT][8][4], l[NT][2];
+    float mx[NT][2], cx[NT][2]; // the reference score (-inf: nothing seen), and the lead less its value scale
 #pragma unroll
     for (int t = 0; t < NT; t++)
     {
@@ -288,8 +292,8 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 O[t][i][e] = 0.f;
-        M[t][0] = M[t][1] = -INFINITY;
-        l[t][0] = l[t][1] = 0.f;
+        mx[t][0] = mx[t][1] = -INFINITY;
+        cx[t][0] = cx[t][1] = l[t][0] = l[t][1] = 0.f;
     }
     float vs_top = -INFINITY; // largest value scale so far of a half with a slot that is not masked
     constexpr int step = KVA_CHUNK * KVA_WARPS;
@@ -394,10 +398,10 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    grow = fmaxf(grow, S[s][t][e] + vs[s] - M[t][e & 1]);
+                    grow = fmaxf(grow, (S[s][t][e] - mx[t][e & 1]) + (vs[s] + cx[t][e & 1]));
         }
-        // ---- the reference follows where a score outgrew it by 2^(KVA_MOST - KVA_LEAD) (M is the reference less KVA_LEAD).
-        // M = -inf makes grow +inf, or NaN (kept out by fmaxf) where the score is -inf, too
+        // ---- the reference follows where a weight would pass 2^KVA_MOST. mx = -inf makes grow +inf, or NaN
+        // (kept out by fmaxf) where the score is -inf, too
         if (__any_sync(0xffffffffu, grow > KVA_MOST))
         {
 #pragma unroll
@@ -405,14 +409,22 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
 #pragma unroll
                 for (int i = 0; i < 2; i++)
                 {
-                    float m = fmaxf(fmaxf(S[0][t][i], S[0][t][i + 2]) + vs[0], fmaxf(S[1][t][i], S[1][t][i + 2]) + vs[1]);
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16)) - KVA_LEAD;
-                    if (m > M[t][i])
+                    float m[2];
+#pragma unroll
+                    for (int s = 0; s < 2; s++)
                     {
-                        const float f = kva_ex2(M[t][i] - m);
-                        M[t][i] = m;
+                        m[s] = fmaxf(S[s][t][i], S[s][t][i + 2]);
+                        m[s] = fmaxf(m[s], __shfl_xor_sync(0xffffffffu, m[s], 4));
+                        m[s] = fmaxf(m[s], __shfl_xor_sync(0xffffffffu, m[s], 8));
+                        m[s] = fmaxf(m[s], __shfl_xor_sync(0xffffffffu, m[s], 16));
+                    }
+                    const bool second = (m[1] - m[0]) + (vs[1] - vs[0]) > 0.f;
+                    const float top = second ? m[1] : m[0], v = second ? vs[1] : vs[0];
+                    if ((top - mx[t][i]) + (v + cx[t][i]) > KVA_LEAD)
+                    {
+                        const float f = kva_ex2((mx[t][i] - top) + (KVA_LEAD - v - cx[t][i]));
+                        mx[t][i] = top;
+                        cx[t][i] = KVA_LEAD - v;
                         l[t][i] *= f;
 #pragma unroll
                         for (int k = 0; k < 8; k++)
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
                             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                             // -inf (or NaN) where the row sees none of these slots: no weight, any lift
-                            lift[t][i] = fminf(fmaxf(floorf(KVA_LEAD - (m + vs[s] - M[t][i])), 0.f), 64.f);
+                            lift[t][i] = fminf(fmaxf(floorf(KVA_LEAD - ((m - mx[t][i]) + (vs[s] + cx[t][i]))), 0.f), 64.f);
 #pragma unroll
                             for (int k = 0; k < 8; k++)
                             {
@@ -461,21 +473,21 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
 #pragma unroll
                 for (int t = 0; t < NT; t++)
                 {
-                    // nothing seen so far: M = -inf, and every weight 0
-                    const float shift[2] = {vs[s] - (M[t][0] == -INFINITY ? 0.f : M[t][0]),
-                                            vs[s] - (M[t][1] == -INFINITY ? 0.f : M[t][1])};
+                    // nothing seen so far: mx = -inf, and every weight 0
+                    const float ref[2] = {mx[t][0] == -INFINITY ? 0.f : mx[t][0], mx[t][1] == -INFINITY ? 0.f : mx[t][1]};
+                    const float shift[2] = {vs[s] + cx[t][0], vs[s] + cx[t][1]};
                     float e4[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                     {
-                        e4[e] = kva_ex2(S[s][t][e] + shift[e & 1]);
+                        e4[e] = kva_ex2((S[s][t][e] - ref[e & 1]) + shift[e & 1]);
                     }
                     l[t][0] += (e4[0] + e4[2]) * unscale;
                     l[t][1] += (e4[1] + e4[3]) * unscale;
                     if (FAR)
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            e4[e] = kva_ex2(S[s][t][e] + (shift[e & 1] + lift[t][e & 1]));
+                            e4[e] = kva_ex2((S[s][t][e] - ref[e & 1]) + (shift[e & 1] + lift[t][e & 1]));
                     const __half2 lo = __floats2half2_rn(e4[0], e4[1]), hi = __floats2half2_rn(e4[2], e4[3]);
                     P[t][0] = kva_transpose(*reinterpret_cast<const uint32_t *>(&lo));
                     P[t][1] = kva_transpose(*reinterpret_cast<const uint32_t *>(&hi));
@@ -592,15 +604,17 @@ __global__ void __launch_bounds__(KVA_THREADS, NT == 1 ? 3 : 2) kv8_attn_kernel(
             s += __shfl_xor_sync(0xffffffffu, s, 4);
             s += __shfl_xor_sync(0xffffffffu, s, 8);
             s += __shfl_xor_sync(0xffffffffu, s, 16);
+            // to 2^(score - mx), without the lead and the reference's value scale
+            const float own = kva_pow2(-cx[t][i]);
             if (g == 0)
             {
-                mm[warp][8 * t + 2 * c + i] = M[t][i];
-                lm[warp][8 * t + 2 * c + i] = s;
+                mm[warp][8 * t + 2 * c + i] = mx[t][i];
+                lm[warp][8 * t + 2 * c + i] = s * own;
             }
 #pragma unroll
             for (int k = 0; k < 8; k++)
                 *reinterpret_cast<float2 *>(&om[warp][8 * t + 2 * c + i][16 * g + 2 * k]) =
-                    make_float2(O[t][k][i], O[t][k][i + 2]);
+                    make_float2(O[t][k][i] * own, O[t][k][i + 2] * own);
         }
     __syncthreads();
     // the warps' sums, joined: a warp per row in turn, lane = 4 dimensions
