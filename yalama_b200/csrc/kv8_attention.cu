@@ -10,8 +10,9 @@
 // fill the GPU otherwise), which leaves sums (M, l, O) per split and row. Up to
 // KVA_ALONE slots the splits of a KV head are one cluster, which joins them through
 // distributed shared memory and adds the weights from scores kept there: one launch, no
-// workspace. Beyond (and where weights are kept of more than 16 rows a KV head), sums and scores go through the workspace, and kv8_join_kernel
-// joins the splits and turns the scores into weights.
+// workspace. Beyond (and where weights are kept of more than 16 rows a KV head), sums and
+// scores go through the workspace, and kv8_join_kernel joins the splits and turns the
+// scores into weights.
 #include "kv8.cuh"
 #include <algorithm>
 #include <cooperative_groups.h>
@@ -30,7 +31,9 @@ constexpr int KVA_JOIN = 256;     // threads of the joining CTAs
 // passes 2^KVA_MOST (FP16 ends at 2^16). A higher lead keeps more of the small weights, and moves the reference more
 // often: 8 x 4099 (64 / 8 heads) 1 % longer at a lead of 11 than at 9, 3 % at 12; one row the same at all.
 constexpr float KVA_LEAD = 11.f, KVA_MOST = 15.9f;
-constexpr float KVA_LIFT = 10.f;  // octaves below the largest value scale from which weights are lifted
+// Octaves below the largest value scale from which weights are lifted: above it, slots of equal softmax weight stay 15
+// octaves clear of FP16's smallest normal number.
+constexpr float KVA_LIFT = 10.f;
 constexpr int KVA_CLUSTER = 8;    // most splits of a cluster (the portable size)
 // Slots up to which the splits of a KV head are one cluster. One launch against two, us of device time (8 heads of
 // 4 query heads; with kept weights): 100 slots 4.3 / 5.2 (5.5 / 6.2), 611 slots 5.0 / 5.3 (6.2 / 7.0), 1000 slots
