@@ -341,6 +341,84 @@ int ylm_k_kv8_attention_workspace(const ylm_kv8_cache *cache, int32_t hq, int32_
 int ylm_k_kv8_evict(const ylm_kv8_cache *src, const ylm_kv8_cache *dst, const float *acc_src, float *acc_dst,
                     int32_t n, int32_t n_keep, int32_t n_sink, int32_t n_recent, int32_t *kept, void *stream);
 
+/* ---- a step of several requests with drafted tokens, on a paged cache ---------------
+ * The reference answers one request at a time, one token a step, and queues the others
+ * (GPU_QUEUE_TIMED_OUT); its cache is one block per layer (src/models/ModelBase.cpp:340-370). These calls are for a
+ * caller's own token loop over many requests, drafted tokens included: append, attention, and once the
+ * model's picks are known (ylm_k_logprobs with n_top = 1: top_ids) accept.
+ *
+ * The cache of a layer is a pool of pages; a request's tokens [i * page, (i + 1) * page) lie on the
+ * page that its row of the page table names. FP16, head dimension 128. Calls on one pool are
+ * ordered by the caller (one stream, or events). */
+typedef struct ylm_paged_cache {
+    void *k, *v;     /* [n_pages][hkv][page][128], 16-byte aligned */
+    int32_t n_pages;
+    int32_t page;    /* tokens a page: 16, 32, 64 or 128 */
+    int32_t hkv;     /* KV heads */
+} ylm_paged_cache;
+/* The step's rows and whom they belong to. Request s has rows [row_start[s], row_start[s + 1]) and
+ * length[s] tokens in the cache before the step; its row i goes to slot length[s] + i and to position
+ * length[s] + depth(i). With parent, the rows are trees: parent[row_start[s] + i] is the row of request s that row i
+ * follows (an earlier one), -1 for one that follows the cached tokens; without, chains (depth i).
+ * The arrays are on the device: a captured graph serves other lengths, tables and trees, and any rows within
+ * `rows` and max_rows. Rows that belong to no request are left as they were. */
+typedef struct ylm_paged_step {
+    const int32_t *row_start;  /* [n_seq + 1], not decreasing */
+    const int32_t *length;     /* [n_seq] */
+    const int32_t *page_table; /* [n_seq][table_ld]; entries behind a request's last slot are not looked at */
+    const int32_t *parent;     /* [rows], or null */
+    int32_t *fault;            /* null, or a word that gets the bits of what was met and left out (never cleared) */
+    int32_t n_seq;             /* requests, at most 65535 */
+    int32_t table_ld;          /* pages a request can have (at most 2^30 tokens) */
+    int32_t rows;              /* rows of the step's buffers */
+    int32_t max_rows;          /* most rows of one request: sizes grids and workspace; at most 128 with parent */
+} ylm_paged_step;
+#define YLM_TREE_ROWS 128
+/* A request whose rows do not lie in [0, rows), are more than max_rows, or reach behind table_ld pages is left out as
+ * a whole; a slot whose page is not in the pool is not written, and no row sees it; a parent that is no earlier row
+ * counts as -1; a row behind max_pos is not appended. */
+typedef enum ylm_step_fault {
+    YLM_STEP_BAD_REQUEST = 1,
+    YLM_STEP_BAD_PAGE = 2,
+    YLM_STEP_BAD_PARENT = 4,
+    YLM_STEP_BAD_POSITION = 8
+} ylm_step_fault;
+/* Append the step's keys and values, and turn its queries. q, k, v: [rows], token strides in halves (columns of a
+ * fused projection will do; multiples of 8, pointers 16-byte aligned); row r's head h at q + r * q_stride + h * 128.
+ * q_norm, k_norm [128] or null: per-head RMSNorm with eps; rope_cos, rope_sin [max_pos][64] FP16, or both null: no
+ * rotation. Both in FP32 and rounded once (the engine's own step rounds after every operation, as the reference does:
+ * values differ by FP16 steps). q_out [rows][hq * 128], which may be q; hq = 0: keys and values alone. */
+int ylm_k_paged_append(const ylm_paged_cache *cache, const ylm_paged_step *step, const void *q, int64_t q_stride,
+                       const void *k, int64_t k_stride, const void *v, int64_t v_stride, int32_t hq,
+                       const void *q_norm, const void *k_norm, float eps, const void *rope_cos, const void *rope_sin,
+                       int32_t max_pos, void *q_out, int64_t q_out_stride, void *stream);
+/* Attention of the step's rows, whose keys and values have been appended: row i of a request sees the request's
+ * cached tokens, its ancestors and itself, scores scaled by 1 / sqrt(128). q, out: [rows][hq * 128] (strides as
+ * above), RoPE applied; at most 128 query heads per KV head. Scores, softmax statistics and sums are FP32. A row that
+ * sees no slot (its pages are not in the pool), or only scores of -inf, gets zeros; what hidden slots hold
+ * does not matter, NaN and infinities either.
+ * workspace: device memory of at least ylm_k_paged_attention_workspace bytes, 16-byte aligned, for this call alone
+ * until it has run: calls that may overlap on the GPU, and graphs that may, need one each. null: allocated and
+ * freed in stream order. */
+int ylm_k_paged_attention(const ylm_paged_cache *cache, const ylm_paged_step *step, const void *q, int64_t q_stride,
+                          int32_t hq, void *out, int64_t out_stride, void *workspace, size_t workspace_bytes,
+                          void *stream);
+/* Bytes of workspace that ylm_k_paged_attention needs on the current device for any step of this hq, hkv and
+ * max_rows (or fewer). */
+int ylm_k_paged_attention_workspace(const ylm_paged_cache *cache, const ylm_paged_step *step, int32_t hq,
+                                    size_t *bytes);
+/* Accept drafted tokens. tokens[r] is row r's token, picks[r] the token that the model chose to follow it
+ * (greedy or sampled: a drafted token is kept where it is the one that was chosen anyway). Of each request with rows:
+ * row 0 is accepted, then the lowest child of the last accepted row whose token is that row's pick, and so on;
+ * accepted [n_seq][max_rows]: these rows, -1 behind; n_accepted; next_token: the last one's pick;
+ * new_length = length + n_accepted. The keys and values of accepted row number j move to slot length + j, in `layers`
+ * layers whose pools lie layer_stride halves apart from cache's on (0 layers: none); the slots behind new_length hold
+ * anything then. A request without rows, or left out: 0 accepted, next_token -1, its length. The results
+ * must not overlap the step, the tokens or the picks. */
+int ylm_k_paged_accept(const ylm_paged_cache *cache, const ylm_paged_step *step, const int64_t *tokens,
+                       const int64_t *picks, int32_t layers, int64_t layer_stride, int32_t *accepted,
+                       int32_t *n_accepted, int64_t *next_token, int32_t *new_length, void *stream);
+
 /* ---- log probabilities ------------------------------------------------------------
  * Of `rows` rows of FP16 logits [rows][ld], vocab (at most 2^30) of them used, over the softmax of
  * the unmasked ids (natural logarithms, FP32; all buffers on the device):

@@ -2,43 +2,13 @@
 // cache and of the log probabilities: argument checks, the attention's
 // workspace, and the launches. Every check comes before any device work; the
 // reason of a refusal is the calling thread's ylm_last_error().
-#include "../../include/yalama_b200.h"
-#include "ylm_kernels.h"
+#include "capi_common.h"
 
-#include <cuda_runtime.h>
 #include <cstdio>
 
 using namespace ylm;
 
 namespace {
-
-int refuse(int status, const char *why)
-{
-    set_last_error(why);
-    return status;
-}
-
-int done(cudaError_t e)
-{
-    if (e == cudaSuccess)
-    {
-        set_last_error("");
-        return YLM_OK;
-    }
-    // the runtime keeps a failed call's error until it is asked for, and a later launch of this library would
-    // take it for its own
-    cudaGetLastError();
-    set_last_error(cudaGetErrorString(e));
-    return YLM_CUDA_ERROR;
-}
-
-int no_device()
-{
-    cudaGetLastError();
-    return refuse(YLM_CUDA_ERROR, "device set-up failed");
-}
-
-bool aligned(const void *p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // Null when the cache can be used, else what is wrong with it.
 const char *cache_fault(const ylm_kv8_cache *c)
@@ -75,21 +45,6 @@ size_t code_bytes(const ylm_kv8_cache &c) { return (size_t)c.hkv * c.cap * YLM_H
 size_t scale_bytes(const ylm_kv8_cache &c)
 {
     return (size_t)c.hkv * (((size_t)c.cap + c.block - 1) / c.block) * sizeof(float);
-}
-
-bool overlap(const void *a, size_t na, const void *b, size_t nb)
-{
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + nb && y < x + na;
-}
-
-int sm_count()
-{
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 0;
-    return n;
 }
 
 const char *attention_fault(const ylm_kv8_cache *c, int32_t hq, int32_t t, int32_t n)
@@ -134,7 +89,7 @@ int ylm_k_kv8_attention_workspace(const ylm_kv8_cache *cache, int32_t hq, int32_
         return refuse(YLM_INVALID_ARG, "null bytes");
     if (const char *f = attention_fault(cache, hq, t, n))
         return refuse(YLM_INVALID_ARG, f);
-    const int sms = sm_count();
+    const int sms = device_sms();
     if (!sms)
         return no_device();
     *bytes = kv8_attn_workspace(cache->hkv, hq, t, n, with_acc != 0, sms);
@@ -158,7 +113,7 @@ int ylm_k_kv8_attention(const ylm_kv8_cache *cache, const void *q, int64_t q_str
         return refuse(YLM_INVALID_ARG, "mask_bits and acc must be 4-byte aligned");
     if (workspace && !aligned(workspace, 16))
         return refuse(YLM_INVALID_ARG, "workspace must be 16-byte aligned");
-    const int sms = sm_count();
+    const int sms = device_sms();
     if (!sms || prepare_device() != cudaSuccess)
         return no_device();
     const size_t need = kv8_attn_workspace(cache->hkv, hq, t, n, acc != nullptr, sms);
@@ -269,7 +224,7 @@ int ylm_k_logprobs(const void *logits, int64_t ld, int32_t rows, int64_t vocab, 
         return done(cudaSuccess);
     if (!logits)
         return refuse(YLM_INVALID_ARG, "null logits");
-    const int sms = sm_count();
+    const int sms = device_sms();
     if (!sms || prepare_device() != cudaSuccess)
         return no_device();
     LogprobArgs a;

@@ -1,0 +1,261 @@
+// Kernel-level C ABI entry points (include/yalama_b200.h) of a step of several requests on a paged K/V cache:
+// argument checks, the attention's workspace, and the launches. Every check comes before any device work; what lies
+// in the step's device arrays is checked by the kernels (paged.cuh).
+#include "capi_common.h"
+
+#include <cstdio>
+
+using namespace ylm;
+
+static_assert(YLM_STEP_BAD_REQUEST == 1 && YLM_STEP_BAD_PAGE == 2 && YLM_STEP_BAD_PARENT == 4 &&
+                  YLM_STEP_BAD_POSITION == 8,
+              "the bits of paged.cuh");
+
+namespace {
+
+// Null when the cache and the step can be used, else what is wrong with them.
+const char *step_fault(const ylm_paged_cache *c, const ylm_paged_step *st)
+{
+    if (!c || !c->k || !c->v)
+        return "null cache buffer";
+    if (!aligned(c->k, 16) || !aligned(c->v, 16))
+        return "cache pages must be 16-byte aligned";
+    if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
+        return "a page must be 16, 32, 64 or 128 tokens";
+    if (c->n_pages <= 0 || c->hkv <= 0 || c->hkv > 65535)
+        return "cache needs 1 page at least and 1..65535 KV heads";
+    if (!st)
+        return "null step";
+    if (st->n_seq < 0 || st->n_seq > 65535 || st->rows < 0 || st->max_rows < 0)
+        return "a step has 0..65535 requests, and rows and max_rows of 0 at least";
+    if (st->n_seq == 0)
+        return nullptr;
+    if (!st->row_start || !st->length || !st->page_table)
+        return "null step buffer";
+    if (!aligned(st->row_start, 4) || !aligned(st->length, 4) || !aligned(st->page_table, 4) ||
+        !aligned(st->parent, 4) || !aligned(st->fault, 4))
+        return "the step's buffers must be 4-byte aligned";
+    // 2^30 slots of one request: slot arithmetic keeps to 32 bits
+    if (st->table_ld <= 0 || (int64_t)st->table_ld * c->page > 1 << 30)
+        return "a request's table needs 1 page at least and 2^30 slots at most";
+    if (st->parent && st->max_rows > YLM_TREE_ROWS)
+        return "a tree has at most 128 rows a request";
+    return nullptr;
+}
+
+PagedCache to_kernel(const ylm_paged_cache &c)
+{
+    PagedCache k;
+    k.k = static_cast<__half *>(c.k);
+    k.v = static_cast<__half *>(c.v);
+    k.n_pages = c.n_pages;
+    k.page = c.page;
+    k.page_shift = c.page == 16 ? 4 : c.page == 32 ? 5 : c.page == 64 ? 6 : 7;
+    k.hkv = c.hkv;
+    return k;
+}
+
+PagedStep to_kernel(const ylm_paged_step &st)
+{
+    PagedStep k;
+    k.row_start = st.row_start;
+    k.length = st.length;
+    k.table = st.page_table;
+    k.parent = st.parent;
+    k.fault = st.fault;
+    k.n_seq = st.n_seq;
+    k.table_ld = st.table_ld;
+    k.rows = st.rows;
+    k.max_rows = st.max_rows < st.rows ? st.max_rows : st.rows;
+    return k;
+}
+
+bool bad_rows(const void *p, int64_t stride, int64_t heads)
+{
+    return stride < heads * YLM_HEAD_DIM || stride % 8 || !p || !aligned(p, 16);
+}
+
+const char *heads_fault(const ylm_paged_cache *c, int32_t hq)
+{
+    if (hq <= 0 || hq % c->hkv || hq / c->hkv > 128)
+        return "query heads must be a multiple of the KV heads, at most 128 to one";
+    return nullptr;
+}
+
+} // namespace
+
+extern "C" {
+
+int ylm_k_paged_append(const ylm_paged_cache *cache, const ylm_paged_step *step, const void *q, int64_t q_stride,
+                       const void *k, int64_t k_stride, const void *v, int64_t v_stride, int32_t hq,
+                       const void *q_norm, const void *k_norm, float eps, const void *rope_cos, const void *rope_sin,
+                       int32_t max_pos, void *q_out, int64_t q_out_stride, void *stream)
+{
+    if (const char *f = step_fault(cache, step))
+        return refuse(YLM_INVALID_ARG, f);
+    if (hq < 0 || hq > 65535)
+        return refuse(YLM_INVALID_ARG, "needs 0..65535 query heads");
+    if (!rope_cos != !rope_sin || (rope_cos && max_pos <= 0))
+        return refuse(YLM_INVALID_ARG, "the rotation needs both tables and max_pos > 0");
+    if (!aligned(q_norm, 16) || !aligned(k_norm, 16) || !aligned(rope_cos, 16) || !aligned(rope_sin, 16))
+        return refuse(YLM_INVALID_ARG, "norm weights and tables must be 16-byte aligned");
+    if (step->n_seq == 0 || step->rows == 0)
+        return done(cudaSuccess);
+    if (bad_rows(k, k_stride, cache->hkv) || bad_rows(v, v_stride, cache->hkv) ||
+        (hq && (bad_rows(q, q_stride, hq) || bad_rows(q_out, q_out_stride, hq))))
+        return refuse(YLM_INVALID_ARG,
+                      "rows must be 16-byte aligned, their strides multiples of 8 halves that hold the heads");
+    if (prepare_device() != cudaSuccess)
+        return no_device();
+    PagedAppendArgs a;
+    a.c = to_kernel(*cache);
+    a.st = to_kernel(*step);
+    a.q = static_cast<const __half *>(q);
+    a.k = static_cast<const __half *>(k);
+    a.v = static_cast<const __half *>(v);
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.hq = hq;
+    a.q_norm = static_cast<const __half *>(q_norm);
+    a.k_norm = static_cast<const __half *>(k_norm);
+    a.eps = eps;
+    a.rope_cos = static_cast<const __half *>(rope_cos);
+    a.rope_sin = static_cast<const __half *>(rope_sin);
+    a.max_pos = max_pos;
+    a.q_out = static_cast<__half *>(q_out);
+    a.q_out_stride = q_out_stride;
+    return done(paged_append_launch(a, static_cast<cudaStream_t>(stream)));
+}
+
+int ylm_k_paged_attention_workspace(const ylm_paged_cache *cache, const ylm_paged_step *step, int32_t hq, size_t *bytes)
+{
+    if (!bytes)
+        return refuse(YLM_INVALID_ARG, "null bytes");
+    if (const char *f = step_fault(cache, step))
+        return refuse(YLM_INVALID_ARG, f);
+    if (const char *f = heads_fault(cache, hq))
+        return refuse(YLM_INVALID_ARG, f);
+    const int sms = device_sms();
+    if (!sms)
+        return no_device();
+    PagedAttnArgs a = {};
+    a.c = to_kernel(*cache);
+    a.st = to_kernel(*step);
+    a.hq = hq;
+    *bytes = paged_attn_workspace(a, sms);
+    return done(cudaSuccess);
+}
+
+int ylm_k_paged_attention(const ylm_paged_cache *cache, const ylm_paged_step *step, const void *q, int64_t q_stride,
+                          int32_t hq, void *out, int64_t out_stride, void *workspace, size_t workspace_bytes,
+                          void *stream)
+{
+    if (const char *f = step_fault(cache, step))
+        return refuse(YLM_INVALID_ARG, f);
+    if (const char *f = heads_fault(cache, hq))
+        return refuse(YLM_INVALID_ARG, f);
+    if (step->n_seq == 0 || step->rows == 0)
+        return done(cudaSuccess);
+    if (bad_rows(q, q_stride, hq) || bad_rows(out, out_stride, hq))
+        return refuse(YLM_INVALID_ARG,
+                      "rows must be 16-byte aligned, their strides multiples of 8 halves that hold the heads");
+    if (workspace && !aligned(workspace, 16))
+        return refuse(YLM_INVALID_ARG, "workspace must be 16-byte aligned");
+    const int sms = device_sms();
+    if (!sms || prepare_device() != cudaSuccess)
+        return no_device();
+    PagedAttnArgs a;
+    a.c = to_kernel(*cache);
+    a.st = to_kernel(*step);
+    a.q = static_cast<const __half *>(q);
+    a.q_stride = q_stride;
+    a.hq = hq;
+    a.out = static_cast<__half *>(out);
+    a.out_stride = out_stride;
+    const size_t need = paged_attn_workspace(a, sms);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    void *ws = workspace;
+    if (workspace)
+    {
+        if (workspace_bytes < need)
+        {
+            char msg[96];
+            snprintf(msg, sizeof(msg), "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+            return refuse(YLM_INVALID_ARG, msg);
+        }
+    }
+    else if (need)
+    {
+        const cudaError_t e = cudaMallocAsync(&ws, need, s);
+        if (e != cudaSuccess)
+            return done(e);
+    }
+    cudaError_t e = paged_attn_launch(a, ws, sms, s);
+    if (ws && !workspace)
+    {
+        const cudaError_t f = cudaFreeAsync(ws, s);
+        e = e != cudaSuccess ? e : f;
+    }
+    return done(e);
+}
+
+int ylm_k_paged_accept(const ylm_paged_cache *cache, const ylm_paged_step *step, const int64_t *tokens,
+                       const int64_t *picks, int32_t layers, int64_t layer_stride, int32_t *accepted,
+                       int32_t *n_accepted, int64_t *next_token, int32_t *new_length, void *stream)
+{
+    if (const char *f = step_fault(cache, step))
+        return refuse(YLM_INVALID_ARG, f);
+    const int64_t layer = (int64_t)cache->n_pages * cache->hkv * cache->page * YLM_HEAD_DIM;
+    if (layers < 0 || (layers > 1 && (layer_stride < layer || layer_stride % 8)))
+        return refuse(YLM_INVALID_ARG, "layers must not overlap, and their stride be a multiple of 8 halves");
+    if (step->n_seq == 0)
+        return done(cudaSuccess);
+    if ((step->rows && (!tokens || !picks)) || !aligned(tokens, 8) || !aligned(picks, 8))
+        return refuse(YLM_INVALID_ARG, "tokens and picks must be 8-byte aligned");
+    if ((step->rows && step->max_rows && !accepted) || !n_accepted || !next_token || !new_length || !aligned(accepted, 4) ||
+        !aligned(n_accepted, 4) || !aligned(next_token, 8) || !aligned(new_length, 4))
+        return refuse(YLM_INVALID_ARG, "null or misaligned output");
+    const PagedStep st = to_kernel(*step);
+    // every block of a request reads the step while the first one writes the results
+    const size_t n = st.n_seq;
+    const struct
+    {
+        const void *p;
+        size_t n;
+    } in[] = {{st.row_start, (n + 1) * 4},
+              {st.length, n * 4},
+              {st.table, n * st.table_ld * 4},
+              {st.parent, st.parent ? (size_t)st.rows * 4 : 0},
+              {tokens, (size_t)st.rows * 8},
+              {picks, (size_t)st.rows * 8}},
+      out[] = {{accepted, n * step->max_rows * 4}, {n_accepted, n * 4}, {next_token, n * 8}, {new_length, n * 4}};
+    for (const auto &o : out)
+        for (const auto &i : in)
+            if (overlap(o.p, o.n, i.p, i.n))
+                return refuse(YLM_INVALID_ARG, "the results must not overlap the step, the tokens or the picks");
+    for (size_t i = 0; i < 4; i++)
+        for (size_t j = i + 1; j < 4; j++)
+            if (overlap(out[i].p, out[i].n, out[j].p, out[j].n))
+                return refuse(YLM_INVALID_ARG, "the results must not overlap one another");
+    if (prepare_device() != cudaSuccess)
+        return no_device();
+    const int sms = device_sms();
+    if (!sms)
+        return no_device();
+    PagedAcceptArgs a;
+    a.c = to_kernel(*cache);
+    a.st = st;
+    a.tokens = tokens;
+    a.picks = picks;
+    a.layers = layers;
+    a.layer_stride = layer_stride;
+    a.accepted = accepted;
+    a.accepted_ld = step->max_rows;
+    a.n_accepted = n_accepted;
+    a.next_token = next_token;
+    a.new_length = new_length;
+    return done(paged_accept_launch(a, sms, static_cast<cudaStream_t>(stream)));
+}
+
+} // extern "C"

@@ -108,6 +108,8 @@ cudaError_t kernels_prepare()
         e = gemm_tc_prepare();
     if (e == cudaSuccess)
         e = kv8_prepare();
+    if (e == cudaSuccess)
+        e = paged_prepare();
     return e;
 }
 

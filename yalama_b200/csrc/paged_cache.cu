@@ -1,0 +1,259 @@
+// Paged K/V cache of several requests: a step's rows appended (with q/k-norm and rotation on the way), and its
+// drafted tokens accepted (their keys and values moved to consecutive slots). Device rules: paged.cuh.
+#include "paged.cuh"
+#include <algorithm>
+
+namespace ylm {
+
+// ------------------------------------------------------------------ append
+//   x' = x * rsqrt(mean(x^2) + eps) * w   (where there is a norm)
+//   y_d = x'_d cos_d - x'_{d+64} sin_d,  y_{d+64} = x'_{d+64} cos_d + x'_d sin_d   for d < 64
+// in FP32, rounded to FP16 once.
+constexpr int PA_THREADS = 256;
+constexpr int PA_HEADS = PA_THREADS / 16; // 16 lanes a head, 8 dimensions each
+
+__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedAppendArgs a)
+{
+    const int lane = threadIdx.x & 31, l = threadIdx.x & 15;
+    const int r = blockIdx.x;
+    const PagedStep &st = a.st;
+    if (st.fault && blockIdx.y == 0)
+        for (int64_t s = (int64_t)r * PA_THREADS + threadIdx.x; s < st.n_seq; s += (int64_t)gridDim.x * PA_THREADS)
+        {
+            PagedRequest q;
+            bool bad;
+            paged_request(st, a.c.page, (int)s, q, bad);
+            if (bad)
+                paged_fault(st, PAGED_BAD_REQUEST);
+        }
+    const int s = paged_find(st, r, lane);
+    PagedRequest q;
+    bool bad = false;
+    if (s < 0 || !paged_request(st, a.c.page, s, q, bad) || r < q.row0 || r >= q.row0 + q.t)
+        return;
+    const int i = r - q.row0, slot = q.n + i;
+    int pos = slot;
+    if (st.parent)
+    {
+        PagedTree tree;
+        if (tree.load(st, q, lane))
+            paged_fault(st, PAGED_BAD_PARENT);
+        pos = q.n;
+        for (int p = tree.of(i); p >= 0; p = tree.of(p))
+            pos++;
+    }
+    if (a.rope_cos && pos >= a.max_pos)
+    {
+        paged_fault(st, PAGED_BAD_POSITION);
+        return;
+    }
+    const int page = paged_page(st, a.c, s, slot);
+    if (page < 0)
+        paged_fault(st, PAGED_BAD_PAGE);
+    const int h = blockIdx.y * PA_HEADS + (threadIdx.x >> 4); // query heads, then keys, then values
+    const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.c.hkv, is = h < a.hq + 2 * a.c.hkv;
+    const int g = is_q ? h : is_k ? h - a.hq : h - a.hq - a.c.hkv;
+    const __half *src = is_q ? a.q + (int64_t)r * a.q_stride : is_k ? a.k + (int64_t)r * a.k_stride
+                                                                     : a.v + (int64_t)r * a.v_stride;
+    __half *dst = nullptr;
+    if (is_q)
+        dst = a.q_out + (int64_t)r * a.q_out_stride + g * YLM_HEAD_DIM;
+    else if (is && page >= 0)
+        dst = (is_k ? a.c.k : a.c.v) + paged_offset(a.c, page, slot) + (size_t)g * a.c.page * YLM_HEAD_DIM;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (is)
+        w = *reinterpret_cast<const uint4 *>(src + g * YLM_HEAD_DIM + l * 8);
+    // (every lane takes part in the shuffles, whatever its head is)
+    const __half *norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+    const bool turn = a.rope_cos && (is_q || is_k);
+    if (__any_sync(0xffffffffu, norm != nullptr || turn))
+    {
+        float x[8];
+        unpack8(w, x);
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            ss += x[e] * x[e];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (norm)
+        {
+            float nw[8];
+            unpack8(*reinterpret_cast<const uint4 *>(norm + l * 8), nw);
+            const float d = rsqrtf(ss * (1.0f / YLM_HEAD_DIM) + a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                x[e] = x[e] * d * nw[e];
+        }
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            y[e] = __shfl_xor_sync(0xffffffffu, x[e], 8);
+        if (turn)
+        {
+            float c[8], sn[8];
+            const int64_t at = (int64_t)pos * 64 + (l & 7) * 8;
+            unpack8(*reinterpret_cast<const uint4 *>(a.rope_cos + at), c);
+            unpack8(*reinterpret_cast<const uint4 *>(a.rope_sin + at), sn);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                x[e] = fmaf(x[e], c[e], l < 8 ? -y[e] * sn[e] : y[e] * sn[e]);
+        }
+        if (norm || turn)
+        {
+            __half2 *o = reinterpret_cast<__half2 *>(&w);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                o[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+        }
+    }
+    if (dst)
+        *reinterpret_cast<uint4 *>(dst + l * 8) = w;
+}
+
+cudaError_t paged_append_launch(const PagedAppendArgs &a, cudaStream_t s)
+{
+    if (a.st.rows <= 0 || a.st.n_seq <= 0)
+        return cudaSuccess;
+    const int heads = a.hq + 2 * a.c.hkv;
+    paged_append_kernel<<<dim3((unsigned)a.st.rows, (unsigned)((heads + PA_HEADS - 1) / PA_HEADS)), PA_THREADS, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ accept
+// The walk: from row 0, to the lowest child whose token is the row's pick, until there is none. The rows of the
+// path only rise, so path[j] >= j: moved in order, no slot is overwritten before it has been read.
+// Each CTA of a request walks for itself (a warp, a shuffle and four ballots a step) and then moves its share of the
+// 2 * layers * hkv rows of 256 bytes that an accepted token has, 16 lanes each.
+constexpr int AC_THREADS = 128;
+constexpr int AC_HALF = AC_THREADS / 16;
+constexpr int AC_BATCH = 8; // rows in flight per 16 lanes
+
+__global__ void __launch_bounds__(AC_THREADS) paged_accept_kernel(const PagedAcceptArgs a)
+{
+    __shared__ int path[PAGED_TREE];
+    __shared__ int64_t from[PAGED_TREE], to[PAGED_TREE];
+    __shared__ int count_s;
+    const PagedStep &st = a.st;
+    const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+    const bool writes = blockIdx.x == 0;
+    PagedRequest q;
+    bool bad;
+    const bool is = paged_request(st, a.c.page, s, q, bad);
+    int count = 0, last = 0;
+    if (!is)
+    {
+        if (bad && writes && tid == 0)
+            paged_fault(st, PAGED_BAD_REQUEST);
+    }
+    else if (!st.parent)
+    {
+        // a chain: the rows up to the first whose token is not the pick before it; they are in place already
+        __shared__ int first;
+        if (tid == 0)
+            first = q.t;
+        __syncthreads();
+        for (int i = 1 + tid; i < q.t; i += AC_THREADS)
+            if (a.tokens[q.row0 + i] != a.picks[q.row0 + i - 1])
+            {
+                atomicMin(&first, i);
+                break;
+            }
+        __syncthreads();
+        count = first;
+        last = count - 1;
+    }
+    else
+    {
+        if (tid < 32)
+        {
+            PagedTree tree;
+            if (tree.load(st, q, lane) && writes)
+                paged_fault(st, PAGED_BAD_PARENT);
+            int64_t token[PAGED_TREE / 32];
+#pragma unroll
+            for (int k = 0; k < PAGED_TREE / 32; k++)
+                token[k] = lane + 32 * k < q.t ? a.tokens[q.row0 + lane + 32 * k] : 0;
+            int cur = 0, m = 0;
+            for (;;)
+            {
+                if (lane == 0)
+                    path[m] = cur;
+                m++;
+                const int64_t pick = a.picks[q.row0 + cur];
+                int next = -1;
+#pragma unroll
+                for (int k = PAGED_TREE / 32 - 1; k >= 0; k--)
+                {
+                    // (rows behind the last have no parent)
+                    const unsigned hit = __ballot_sync(0xffffffffu, tree.p[k] == cur && token[k] == pick);
+                    if (hit)
+                        next = 32 * k + __ffs(hit) - 1;
+                }
+                if (next < 0)
+                    break;
+                cur = next; // > its parent: at most t steps
+            }
+            __syncwarp();
+            for (int j = lane; j < m; j += 32)
+            {
+                const int x = q.n + path[j], y = q.n + j;
+                const int px = paged_page(st, a.c, s, x), py = paged_page(st, a.c, s, y);
+                if ((px < 0 || py < 0) && writes)
+                    paged_fault(st, PAGED_BAD_PAGE);
+                from[j] = px < 0 || py < 0 || x == y ? -1 : (int64_t)paged_offset(a.c, px, x);
+                to[j] = px < 0 || py < 0 || x == y ? -1 : (int64_t)paged_offset(a.c, py, y);
+            }
+            if (lane == 0)
+                count_s = m;
+        }
+        __syncthreads();
+        count = count_s;
+        last = path[count - 1];
+        // this half warp's heads of the layers' keys and values
+        const int l = tid & 15, rows = 2 * a.layers * a.c.hkv;
+        for (int h = blockIdx.x * AC_HALF + (tid >> 4); h < rows; h += gridDim.x * AC_HALF)
+        {
+            const int layer = h / (2 * a.c.hkv), g = h % (2 * a.c.hkv);
+            __half *pool = (g < a.c.hkv ? a.c.k : a.c.v) + (int64_t)layer * a.layer_stride +
+                           (size_t)(g < a.c.hkv ? g : g - a.c.hkv) * a.c.page * YLM_HEAD_DIM + l * 8;
+            for (int j0 = 1; j0 < count; j0 += AC_BATCH)
+            {
+                uint4 x[AC_BATCH];
+#pragma unroll
+                for (int u = 0; u < AC_BATCH; u++)
+                    if (j0 + u < count && from[j0 + u] >= 0)
+                        x[u] = *reinterpret_cast<const uint4 *>(pool + from[j0 + u]);
+#pragma unroll
+                for (int u = 0; u < AC_BATCH; u++)
+                    if (j0 + u < count && from[j0 + u] >= 0)
+                        *reinterpret_cast<uint4 *>(pool + to[j0 + u]) = x[u];
+            }
+        }
+    }
+    if (!writes)
+        return;
+    int32_t *acc = a.accepted + (size_t)s * a.accepted_ld;
+    for (int j = tid; j < a.accepted_ld; j += AC_THREADS)
+        acc[j] = j < count ? (st.parent ? path[j] : j) : -1;
+    if (tid == 0)
+    {
+        a.n_accepted[s] = count;
+        a.next_token[s] = count ? a.picks[q.row0 + last] : -1;
+        a.new_length[s] = q.n + count; // of a request that is left out: as it was
+    }
+}
+
+cudaError_t paged_accept_launch(const PagedAcceptArgs &a, int num_sms, cudaStream_t s)
+{
+    if (a.st.n_seq <= 0)
+        return cudaSuccess;
+    // about eight CTAs an SM at most, each with at least one round of moves
+    const int64_t rounds = a.st.parent ? ((int64_t)2 * a.layers * a.c.hkv + AC_HALF - 1) / AC_HALF : 1;
+    const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(rounds, (int64_t)num_sms * 8 / a.st.n_seq));
+    paged_accept_kernel<<<dim3((unsigned)slices, (unsigned)a.st.n_seq), AC_THREADS, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+} // namespace ylm

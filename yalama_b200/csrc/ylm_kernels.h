@@ -294,6 +294,65 @@ struct Kv8EvictArgs
 cudaError_t kv8_evict_launch(const Kv8EvictArgs &a, cudaStream_t s);
 cudaError_t kv8_prepare();
 
+// ------------------------------------------------------------------ paged cache of several requests
+struct PagedCache
+{
+    __half *k, *v; // [n_pages][hkv][page][128]
+    int n_pages, page, page_shift, hkv;
+};
+// A step's rows and whom they belong to; the arrays are on the device (paged.cuh checks them there).
+struct PagedStep
+{
+    const int32_t *row_start; // [n_seq + 1]
+    const int32_t *length;    // [n_seq]
+    const int32_t *table;     // [n_seq][table_ld]
+    const int32_t *parent;    // [rows] or null: chains
+    int32_t *fault;           // or null
+    int n_seq, table_ld, rows, max_rows;
+};
+struct PagedAppendArgs
+{
+    PagedCache c;
+    PagedStep st;
+    const __half *q, *k, *v; // [rows], strides in halves
+    int64_t q_stride, k_stride, v_stride;
+    int hq;
+    const __half *q_norm, *k_norm; // [128] or null
+    float eps;
+    const __half *rope_cos, *rope_sin; // [max_pos][64] or null
+    int max_pos;
+    __half *q_out;
+    int64_t q_out_stride;
+};
+cudaError_t paged_append_launch(const PagedAppendArgs &a, cudaStream_t s);
+struct PagedAttnArgs
+{
+    PagedCache c;
+    PagedStep st;
+    const __half *q;
+    int64_t q_stride;
+    int hq;
+    __half *out;
+    int64_t out_stride;
+};
+size_t paged_attn_workspace(const PagedAttnArgs &a, int num_sms);
+cudaError_t paged_attn_launch(const PagedAttnArgs &a, void *ws, int num_sms, cudaStream_t s);
+struct PagedAcceptArgs
+{
+    PagedCache c;
+    PagedStep st;
+    const int64_t *tokens, *picks; // [rows]
+    int layers;
+    int64_t layer_stride; // halves
+    int32_t *accepted;    // [n_seq][accepted_ld]
+    int accepted_ld;
+    int32_t *n_accepted;
+    int64_t *next_token;
+    int32_t *new_length;
+};
+cudaError_t paged_accept_launch(const PagedAcceptArgs &a, int num_sms, cudaStream_t s);
+cudaError_t paged_prepare();
+
 // ------------------------------------------------------------------ log probabilities
 struct LogprobArgs
 {

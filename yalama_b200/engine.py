@@ -120,6 +120,38 @@ class KV8Cache(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+        ("hkv", ctypes.c_int32),
+    ]
+
+
+class PagedStep(ctypes.Structure):
+    _fields_ = [
+        ("row_start", ctypes.c_void_p),
+        ("length", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("parent", ctypes.c_void_p),
+        ("fault", ctypes.c_void_p),
+        ("n_seq", ctypes.c_int32),
+        ("table_ld", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32),
+    ]
+
+
+class StepFault(enum.IntFlag):
+    """Bits of a paged step's fault word: what was met and left out."""
+    BAD_REQUEST = 1
+    BAD_PAGE = 2
+    BAD_PARENT = 4
+    BAD_POSITION = 8
+
+
 class YlmError(RuntimeError):
     def __init__(self, status: int, where: str, message: str):
         self.status = Status(status) if status in Status._value2member_map_ else status
@@ -187,6 +219,16 @@ SIGNATURES = {
                                                      ctypes.POINTER(ctypes.c_size_t)]),
     "ylm_k_kv8_evict": (ctypes.c_int, [ctypes.POINTER(KV8Cache), ctypes.POINTER(KV8Cache), _P, _P, ctypes.c_int32,
                                        ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P, _P]),
+    "ylm_k_paged_append": (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedStep), _P, ctypes.c_int64,
+                                          _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int32, _P, _P,
+                                          ctypes.c_float, _P, _P, ctypes.c_int32, _P, ctypes.c_int64, _P]),
+    "ylm_k_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedStep), _P,
+                                             ctypes.c_int64, ctypes.c_int32, _P, ctypes.c_int64, _P, ctypes.c_size_t,
+                                             _P]),
+    "ylm_k_paged_attention_workspace": (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedStep),
+                                                       ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
+    "ylm_k_paged_accept": (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedStep), _P, _P,
+                                          ctypes.c_int32, ctypes.c_int64, _P, _P, _P, _P, _P]),
     "ylm_k_logprobs": (ctypes.c_int, [_P, ctypes.c_int64, ctypes.c_int32, ctypes.c_int64, _P, _P, ctypes.c_int32,
                                       _P, _P, _P, _P, _P]),
 }
@@ -244,6 +286,26 @@ def kv8_attention_workspace(cache: KV8Cache, hq: int, t: int, n: int, with_acc: 
     b = ctypes.c_size_t()
     check(lib().ylm_k_kv8_attention_workspace(ctypes.byref(cache), hq, t, n, int(with_acc), ctypes.byref(b)),
           "ylm_k_kv8_attention_workspace")
+    return b.value
+
+
+def paged_cache(k: int, v: int, n_pages: int, page: int, hkv: int) -> PagedCache:
+    """Descriptor of a paged K/V pool from device pointers; the buffers stay the caller's and must outlive the calls
+    that use it."""
+    return PagedCache(k, v, n_pages, page, hkv)
+
+
+def paged_step(row_start: int, length: int, page_table: int, parent: Optional[int], n_seq: int, table_ld: int,
+               rows: int, max_rows: int, fault: Optional[int] = None) -> PagedStep:
+    """Descriptor of a step on a paged cache from device pointers (``parent`` None: chains)."""
+    return PagedStep(row_start, length, page_table, parent, fault, n_seq, table_ld, rows, max_rows)
+
+
+def paged_attention_workspace(cache: PagedCache, step: PagedStep, hq: int) -> int:
+    """Bytes of device workspace for ``ylm_k_paged_attention`` with these heads and ``max_rows``."""
+    b = ctypes.c_size_t()
+    check(lib().ylm_k_paged_attention_workspace(ctypes.byref(cache), ctypes.byref(step), hq, ctypes.byref(b)),
+          "ylm_k_paged_attention_workspace")
     return b.value
 
 
