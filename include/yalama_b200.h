@@ -381,7 +381,8 @@ typedef enum ylm_step_fault {
     YLM_STEP_BAD_REQUEST = 1,
     YLM_STEP_BAD_PAGE = 2,
     YLM_STEP_BAD_PARENT = 4,
-    YLM_STEP_BAD_POSITION = 8
+    YLM_STEP_BAD_POSITION = 8,
+    YLM_STEP_TIMEOUT = 16 /* a bounded wait inside the attention (2 s) ran out: its output is not complete */
 } ylm_step_fault;
 /* Append the step's keys and values, and turn its queries. q, k, v: [rows], token strides in halves (columns of a
  * fused projection will do; multiples of 8, pointers 16-byte aligned); row r's head h at q + r * q_stride + h * 128.

@@ -8,7 +8,7 @@
 using namespace ylm;
 
 static_assert(YLM_STEP_BAD_REQUEST == 1 && YLM_STEP_BAD_PAGE == 2 && YLM_STEP_BAD_PARENT == 4 &&
-                  YLM_STEP_BAD_POSITION == 8,
+                  YLM_STEP_BAD_POSITION == 8 && YLM_STEP_TIMEOUT == 16,
               "the bits of paged.cuh");
 
 namespace {

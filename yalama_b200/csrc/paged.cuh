@@ -10,7 +10,7 @@
 
 namespace ylm {
 
-constexpr int PAGED_BAD_REQUEST = 1, PAGED_BAD_PAGE = 2, PAGED_BAD_PARENT = 4, PAGED_BAD_POSITION = 8;
+constexpr int PAGED_BAD_REQUEST = 1, PAGED_BAD_PAGE = 2, PAGED_BAD_PARENT = 4, PAGED_BAD_POSITION = 8, PAGED_TIMEOUT = 16;
 constexpr int PAGED_TREE = 128; // most rows of a request in a tree
 
 __device__ __forceinline__ void paged_fault(const PagedStep &st, int bit)

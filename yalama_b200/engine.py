@@ -150,6 +150,7 @@ class StepFault(enum.IntFlag):
     BAD_PAGE = 2
     BAD_PARENT = 4
     BAD_POSITION = 8
+    TIMEOUT = 16
 
 
 class YlmError(RuntimeError):
