@@ -33,6 +33,7 @@ constexpr int PX_THREADS = 384;
 constexpr int PX_KST = 3;
 constexpr int PX_CONTROL = 3072; // barriers, the streams' (M, l)
 constexpr int PX_SMEM = 7 * PX_TILE + PX_CONTROL;
+constexpr int PX_CUT = 128; // bytes of a PagedCut
 constexpr float PX_SCALE = (float)(1.4426950408889634 / 11.313708498984760); // log2(e) / sqrt(128)
 // FP16 weights end at 2^16; a higher lead keeps more of the small ones and moves the reference more often
 constexpr float PX_LEAD = 11.f, PX_MOST = 15.9f;
@@ -42,6 +43,7 @@ struct PagedPlan
 {
     int G, tpt, tpi; // query heads per KV head, tokens per 128-row tile and per item
     int pair;        // 1: items of two tiles (some request may have more than tpt rows)
+    int box;         // tokens of a tile that are loaded: tpt, or fewer where no request has so many
     int cap;         // most rows of an item
     int ctas;
     size_t ml_off, o_off, bytes;
@@ -54,9 +56,10 @@ static PagedPlan paged_plan(const PagedAttnArgs &a, int num_sms)
     p.tpt = 128 / p.G;
     p.pair = a.st.max_rows > p.tpt;
     p.tpi = p.pair ? 2 * p.tpt : p.tpt;
+    p.box = std::max(1, std::min(p.tpt, a.st.max_rows));
     p.cap = std::max(1, std::min(p.tpi, a.st.max_rows)) * p.G;
     p.ctas = num_sms;
-    p.ml_off = ((size_t)p.ctas * 64 + 255) / 256 * 256;
+    p.ml_off = (size_t)p.ctas * PX_CUT;
     p.o_off = p.ml_off + ((size_t)p.ctas * 2 * p.cap * sizeof(float2) + 255) / 256 * 256;
     p.bytes = p.o_off + (size_t)p.ctas * 2 * p.cap * YLM_HEAD_DIM * sizeof(float);
     return p;
@@ -64,14 +67,24 @@ static PagedPlan paged_plan(const PagedAttnArgs &a, int num_sms)
 
 size_t paged_attn_workspace(const PagedAttnArgs &a, int num_sms) { return paged_plan(a, num_sms).bytes; }
 
-// Where a CTA's share starts; left in the workspace for the join.
+// A part of an item, as a share has it.
+struct PagedItem
+{
+    int s, row0, t, n;  // the request
+    int first, kvh;     // the item's first token, its KV head
+    int tile0, tiles;   // units [tile0, tile0 + tiles) are the share's; tiles = 0: the share's end
+    int units;          // units of the item
+};
+
+// A CTA's share of the units, and its first item; left in the workspace for the join.
 struct PagedCut
 {
     long long u0, u1;
-    int s, qp, kvh, tile0, kt;
-    int cut; // the share starts inside an item
+    long long each, more; // every share has `each` units, the first `more` of them one more
+    PagedItem it;
+    int cut;              // the share starts inside an item
 };
-static_assert(sizeof(PagedCut) <= 64, "64 bytes a CTA");
+static_assert(sizeof(PagedCut) <= PX_CUT, "the workspace's layout");
 
 struct PagedPass
 {
@@ -102,62 +115,104 @@ __device__ __forceinline__ long long px_before(int n, int k, int tpi)
 
 __device__ __forceinline__ long long px_request_units(const PagedRequest &r, int tpi, int hkv)
 {
-    const int items = (r.t + tpi - 1) / tpi;
-    return hkv * (px_before(r.n, items - 1, tpi) + px_units(r.n, r.t, items - 1, tpi));
+    const int last = r.t <= tpi ? 0 : (r.t - 1) / tpi;
+    return hkv * (px_before(r.n, last, tpi) + px_units(r.n, r.t, last, tpi));
 }
 
-// A CTA's way through its share: one item, or a part of one, after another. Every warp role walks it alike.
-struct PagedItem
+// slots below are seen by every row of the item
+__device__ __forceinline__ int px_open(const PagedPass &w, const PagedItem &it)
 {
-    int s, qp, kvh, tile0, tiles, seq; // seq: its number among the CTA's items
-    PagedRequest r;
-    long long left; // units of the share from here on
+    return it.n + (w.a.st.parent ? (it.t == 1 ? 1 : 0) : it.first + 1);
+}
+__device__ __forceinline__ bool px_two(const PagedPass &w, const PagedItem &it) { return it.t - it.first > w.p.tpt; }
 
-    __device__ __forceinline__ bool start(const PagedPass &w, const PagedCut &c)
+// a / b for b > 0; nearly every step's numbers have 32 bits
+__device__ __forceinline__ long long px_div(long long a, int b)
+{
+    return a >> 31 == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
+// Warp 0's way through the share, an item after another. The next requests, a lane each, are loaded ahead of their turn.
+struct PagedWalk
+{
+    PagedItem it;
+    long long left; // units of the share from here on
+    int base;       // ahead: requests base + lane
+    PagedRequest ahead;
+    bool there;
+
+    __device__ __forceinline__ void look(const PagedPass &w, int from, int lane)
     {
-        s = c.s, qp = c.qp, kvh = c.kvh, tile0 = c.tile0;
-        left = c.u1 - c.u0;
-        seq = 0;
-        if (left <= 0)
-            return false;
+        base = from;
         bool bad;
-        paged_request(w.a.st, w.a.c.page, s, r, bad);
-        tiles = (int)min((long long)(c.kt - tile0), left);
-        return true;
+        there = from + lane < w.a.st.n_seq && paged_request(w.a.st, w.a.c.page, from + lane, ahead, bad);
     }
-    __device__ __forceinline__ bool next(const PagedPass &w)
+    __device__ __forceinline__ void start(const PagedPass &w, const PagedCut &c, int lane)
     {
-        left -= tiles;
+        left = c.u1 - c.u0;
+        it = c.it;
+        if (it.tiles)
+            look(w, it.s + 1, lane);
+    }
+    __device__ __forceinline__ void next(const PagedPass &w, int lane)
+    {
+        left -= it.tiles;
+        it.tiles = 0;
         if (left <= 0)
-            return false;
-        seq++;
-        tile0 = 0;
-        if (++kvh == w.a.c.hkv)
+            return;
+        it.tile0 = 0;
+        if (++it.kvh == w.a.c.hkv)
         {
-            kvh = 0;
-            if (++qp * w.p.tpi >= r.t)
+            it.kvh = 0;
+            it.first += w.p.tpi;
+            if (it.first >= it.t)
             {
-                qp = 0;
-                bool bad;
-                do
+                it.first = 0;
+                unsigned hit;
+                while (!(hit = __ballot_sync(0xffffffffu, there && base + lane > it.s)))
                 {
-                    if (++s >= w.a.st.n_seq)
-                        return false;
-                } while (!paged_request(w.a.st, w.a.c.page, s, r, bad));
+                    if (base + 32 >= w.a.st.n_seq)
+                        return;
+                    look(w, base + 32, lane);
+                }
+                const int k = __ffs(hit) - 1;
+                it.s = base + k;
+                it.row0 = __shfl_sync(0xffffffffu, ahead.row0, k);
+                it.t = __shfl_sync(0xffffffffu, ahead.t, k);
+                it.n = __shfl_sync(0xffffffffu, ahead.n, k);
             }
         }
-        tiles = (int)min((long long)units(w), left);
-        return true;
+        it.units = (it.n + min(it.t, it.first + w.p.tpi) + 127) >> 7;
+        it.tiles = (int)min((long long)it.units, left);
     }
-    __device__ __forceinline__ int units(const PagedPass &w) const { return px_units(r.n, r.t, qp, w.p.tpi); }
-    __device__ __forceinline__ int first(const PagedPass &w) const { return qp * w.p.tpi; } // its first token
-    // slots below are seen by every row of the item
-    __device__ __forceinline__ int open(const PagedPass &w) const
-    {
-        return r.n + (w.a.st.parent ? (r.t == 1 ? 1 : 0) : first(w) + 1);
-    }
-    __device__ __forceinline__ bool two(const PagedPass &w) const { return r.t - first(w) > w.p.tpt; }
 };
+
+// ------------------------------------------------------------------ arithmetic of two values an instruction
+__device__ __forceinline__ float2 px_add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\t"
+        "mov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 px_fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, u;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 u, x, y, z;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+// the largest of three (of those that are not NaN, as fmaxf)
+__device__ __forceinline__ float px_max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 // ------------------------------------------------------------------ waits
 // Bounded: after 2 s, or once another warp gave up, *abort is set and the caller unwinds.
@@ -184,6 +239,16 @@ __device__ __forceinline__ bool px_wait_warp(uint64_t *bar, uint32_t parity, vol
     return __all_sync(0xffffffffu, px_wait(bar, parity, abort));
 }
 
+// One lane of a converged warp, the same every time.
+__device__ __forceinline__ bool px_elect()
+{
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+
+__device__ __forceinline__ bool px_stopped(volatile int *abort) { return __any_sync(0xffffffffu, *abort != 0); }
+
 // For copies and products that are on their way and need nobody else: whatever happened, they end first.
 __device__ __forceinline__ void px_drain(uint64_t *bar, uint32_t parity)
 {
@@ -201,21 +266,28 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, i
                  : "memory");
 }
 
-// One unit's K or V into a stage: a warp, a page's half of the dimensions a lane. Pages behind the request's
-// last slot, and pages that are not in the pool, arrive as zeros (coordinate -1).
-__device__ __forceinline__ void px_load(uint8_t *dst, const CUtensorMap *map, const PagedPass &w, const PagedItem &it,
-                                        int tile, uint64_t *bar, int lane)
+// Lane 2 p + h's page of a unit's slots (half h of its dimensions): page p of them; -1 behind the request's last slot,
+// and where it is not in the pool (bad).
+__device__ __forceinline__ int px_page(const PagedPass &w, const PagedItem &it, int tile, int lane, bool &bad)
 {
-    const int pages = 128 >> w.a.c.page_shift, k = lane >> 1, half = lane & 1;
+    const int k = lane >> 1, slot = tile * 128 + k * w.a.c.page;
+    bad = false;
+    if (k >= 128 >> w.a.c.page_shift || slot >= it.n + it.t)
+        return -1;
+    const int page = paged_page(w.a.st, w.a.c, it.s, slot);
+    bad = page < 0;
+    return page;
+}
+
+// A unit's K or V into a stage, from the pages that px_page gave (-1: zeros). Warp-wide.
+__device__ __forceinline__ void px_load(uint8_t *dst, const CUtensorMap *map, const PagedPass &w, int kvh, int page,
+                                        uint64_t *bar, int lane)
+{
     if (lane == 0)
         mbar_arrive_expect_tx(bar, PX_TILE);
     __syncwarp();
-    if (k < pages)
-    {
-        const int slot = tile * 128 + k * w.a.c.page;
-        const int page = slot < it.r.n + it.r.t ? paged_page(w.a.st, w.a.c, it.s, slot) : -1;
-        tma_load_4d(dst + half * (PX_TILE / 2) + k * w.a.c.page * 128, map, half * 64, 0, it.kvh, page, bar);
-    }
+    if (lane >> 1 < 128 >> w.a.c.page_shift)
+        tma_load_4d(dst + (lane & 1) * (PX_TILE / 2) + (lane >> 1) * w.a.c.page * 128, map, (lane & 1) * 64, 0, kvh, page, bar);
 }
 
 template <bool PAIR>
@@ -229,14 +301,19 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     uint8_t *control = smem + 7 * PX_TILE;
     uint64_t *bars = reinterpret_cast<uint64_t *>(control);
     uint64_t *k_full = bars, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST,
-             *v_clean = v_empty + VST, *q_full = v_clean + VST, *q_empty = q_full + 1, *s_full = q_empty + 1,
-             *p_full = s_full + 2, *o_done = p_full + 2, *joined = o_done + 2, *parted = joined + 1, *done = parted + 1;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(control + 256);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(control + 260);
-    volatile int *special = reinterpret_cast<volatile int *>(control + 264); // [8]: 1 + the item that had one, by its number mod 8
-    PagedCut *mine = reinterpret_cast<PagedCut *>(control + 320);
-    long long *sums = reinterpret_cast<long long *>(control + 384); // [12]
-    float2 *state = reinterpret_cast<float2 *>(control + 1024);     // [2][128]
+             *v_clean = v_empty + VST, *q_full = v_clean + VST, *q_empty = q_full + 2, *s_full = q_empty + 2,
+             *p_full = s_full + 2, *o_done = p_full + 2, *joined = o_done + 2, *parted = joined + 1, *done = parted + 1,
+             *item_full = done + 1; // [8]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(control + 320);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(control + 324);
+    volatile int *special = reinterpret_cast<volatile int *>(control + 328); // [8]: 1 + the item that had one, by its number mod 8
+    PagedCut *mine = reinterpret_cast<PagedCut *>(control + 384);
+    long long *sums = reinterpret_cast<long long *>(control + 512);          // [12]
+    // Rings of 8: warp 0 is never more than six items or units ahead of any other warp, since a K stage comes free by
+    // products that waited for everybody else's work on the items before.
+    PagedItem *items = reinterpret_cast<PagedItem *>(control + 640);
+    volatile uint32_t *lost = reinterpret_cast<volatile uint32_t *>(control + 960); // a unit's sixteens of slots that are not in the pool
+    float2 *state = reinterpret_cast<float2 *>(control + 1024);                     // [2][128]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedAttnArgs &a = w.a;
     const PagedStep &st = a.st;
@@ -255,10 +332,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             mbar_init(&v_empty[i], 1);
             mbar_init(&v_clean[i], 1);
         }
-        mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
         for (int i = 0; i < 2; i++)
         {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
@@ -268,9 +345,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         mbar_init(done, 1);
         *abort_flag = 0;
         for (int i = 0; i < 8; i++)
+        {
+            mbar_init(&item_full[i], 1);
             special[i] = 0;
+        }
         mine->u0 = mine->u1 = 0;
-        mine->cut = 0;
+        mine->it.tiles = 0;
         fence_mbar_init();
         prefetch_tensormap(&qmap);
         prefetch_tensormap(&kmap);
@@ -284,14 +364,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     }
 
     // ---- this CTA's share: requests in runs of `run` a thread, their units summed over the threads
-    const int run = (st.n_seq + PX_THREADS - 1) / PX_THREADS;
+    const int run = st.n_seq <= PX_THREADS ? 1 : (st.n_seq + PX_THREADS - 1) / PX_THREADS;
+    const int s_end = min(st.n_seq, (tid + 1) * run);
     long long own = 0;
-    for (int s = tid * run; s < min(st.n_seq, (tid + 1) * run); s++)
+    PagedRequest req; // the run's last (of a run of one: the request)
+    for (int s = tid * run; s < s_end; s++)
     {
-        PagedRequest r;
         bool bad;
-        if (paged_request(st, a.c.page, s, r, bad))
-            own += px_request_units(r, w.p.tpi, a.c.hkv);
+        if (paged_request(st, a.c.page, s, req, bad))
+            own += px_request_units(req, w.p.tpi, a.c.hkv);
         else if (bad && blockIdx.x == 0)
             paged_fault(st, PAGED_BAD_REQUEST);
     }
@@ -312,79 +393,121 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         total += sums[i];
         before += i < warp ? sums[i] : 0;
     }
-    const long long ctas = min((long long)gridDim.x, total);
-    if (blockIdx.x < ctas)
+    // share b: units [b * each + min(b, more), + each + (b < more))
+    const int b = blockIdx.x;
+    const long long each = px_div(total, (int)gridDim.x), over = total - each * gridDim.x;
+    const long long u0 = b * each + min((long long)b, over), u1 = u0 + each + (b < over);
+    if (u0 >= before && u0 < before + own && u1 > u0)
     {
-        const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-        if (u0 >= before && u0 < before + own)
-        {
-            long long rest = u0 - before;
-            int s = tid * run;
-            PagedRequest r;
-            bool bad;
+        long long rest = u0 - before;
+        int s = tid * run;
+        if (run > 1)
             for (;; s++)
             {
-                if (!paged_request(st, a.c.page, s, r, bad))
+                bool bad;
+                if (!paged_request(st, a.c.page, s, req, bad))
                     continue;
-                const long long u = px_request_units(r, w.p.tpi, a.c.hkv);
+                const long long u = px_request_units(req, w.p.tpi, a.c.hkv);
                 if (rest < u)
                     break;
                 rest -= u;
             }
-            // the last item row whose units before it do not pass `rest`
-            int lo = 0, hi = (r.t + w.p.tpi - 1) / w.p.tpi;
-            while (hi - lo > 1)
-            {
-                const int mid = (lo + hi) / 2;
-                if (a.c.hkv * px_before(r.n, mid, w.p.tpi) <= rest)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            rest -= a.c.hkv * px_before(r.n, lo, w.p.tpi);
-            PagedCut c;
-            c.u0 = u0;
-            c.u1 = u1;
-            c.s = s;
-            c.qp = lo;
-            c.kt = px_units(r.n, r.t, lo, w.p.tpi);
-            c.kvh = (int)(rest / c.kt);
-            c.tile0 = (int)(rest % c.kt);
-            c.cut = c.tile0 > 0;
-            *mine = c;
-            w.cuts[blockIdx.x] = c;
+        // the last of the request's token groups whose units before it do not pass `rest`
+        int lo = 0, hi = req.t <= w.p.tpi ? 1 : (req.t + w.p.tpi - 1) / w.p.tpi;
+        while (hi - lo > 1)
+        {
+            const int mid = (lo + hi) / 2;
+            if (a.c.hkv * px_before(req.n, mid, w.p.tpi) <= rest)
+                lo = mid;
+            else
+                hi = mid;
         }
+        rest -= a.c.hkv * px_before(req.n, lo, w.p.tpi);
+        PagedCut c;
+        c.u0 = u0;
+        c.u1 = u1;
+        c.each = each;
+        c.more = over;
+        c.it.s = s;
+        c.it.row0 = req.row0;
+        c.it.t = req.t;
+        c.it.n = req.n;
+        c.it.first = lo * w.p.tpi;
+        c.it.units = px_units(req.n, req.t, lo, w.p.tpi);
+        c.it.kvh = (int)px_div(rest, c.it.units);
+        c.it.tile0 = (int)(rest - (long long)c.it.kvh * c.it.units);
+        c.it.tiles = (int)min((long long)(c.it.units - c.it.tile0), u1 - u0);
+        c.cut = c.it.tile0 > 0;
+        *mine = c;
+        w.cuts[b] = c;
     }
-    else if (tid == 0)
+    else if (u0 == u1 && tid == 0)
     {
         PagedCut c = {};
-        c.u0 = c.u1 = total;
-        w.cuts[blockIdx.x] = c;
+        c.u0 = c.u1 = u0;
+        w.cuts[b] = c;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const PagedCut cut = *mine;
     const int G = w.p.G, tpt = w.p.tpt;
-    PagedItem it;
-    bool more = it.start(w, cut);
+    // item number j, once warp 0 has left it; tiles = 0 after the last, or where a wait ran out
+    const auto fetch = [&](int j) {
+        PagedItem it;
+        if (px_wait(&item_full[j & 7], (j >> 3) & 1, abort_flag))
+            it = items[j & 7];
+        else
+            it.tiles = 0;
+        return it;
+    };
+
+    // Two places for Q, so that the next item's is there in time: an item of one tile takes the other one than the last
+    // item's, an item of two tiles both. With one tile in shared memory the places are its halves of 64 rows,
+    // where no item has more (the products read 128 rows from there on, and nobody reads what comes of the others), or one.
+    const int q_places = PAIR || w.p.cap <= 64 ? 2 : 1;
+    const uint32_t q_step = PAIR ? PX_TILE : PX_TILE / 4;
 
     if (warp == 0)
     {
-        // ---- K tiles
+        // ---- the share's items, and K tiles
+        PagedWalk walk;
+        walk.start(w, *mine, lane);
         int kc = 0;
-        for (bool ok = true; more && ok; more = it.next(w))
+        for (int j = 0;; j++)
+        {
+            if (lane == 0)
+            {
+                items[j & 7] = walk.it;
+                mbar_arrive(&item_full[j & 7]);
+            }
+            const PagedItem it = walk.it;
+            bool bad, ok = true;
+            int page = it.tiles ? px_page(w, it, it.tile0, lane, bad) : -1;
             for (int t = 0; t < it.tiles; t++, kc++)
             {
                 const int s = kc % KST;
-                if (*abort_flag || (kc >= KST && !px_wait_warp(&k_empty[s], (kc / KST - 1) & 1, abort_flag)))
+                if (px_stopped(abort_flag) || (kc >= KST && !px_wait_warp(&k_empty[s], (kc / KST - 1) & 1, abort_flag)))
                 {
                     ok = false;
                     break;
                 }
-                px_load(sk + s * PX_TILE, &kmap, w, it, it.tile0 + t, &k_full[s], lane);
+                // a page covers page / 16 sixteens
+                const uint32_t bits = bad ? (0xFFu >> (8 - (a.c.page >> 4))) << ((lane >> 1) * (a.c.page >> 4)) : 0u;
+                const uint32_t all = __reduce_or_sync(0xffffffffu, bits);
+                if (lane == 0)
+                {
+                    lost[kc & 7] = all;
+                    if (all)
+                        paged_fault(st, PAGED_BAD_PAGE);
+                }
+                px_load(sk + s * PX_TILE, &kmap, w, it.kvh, page, &k_full[s], lane);
+                page = px_page(w, it, it.tile0 + t + 1, lane, bad); // on its way while the next stage comes free
             }
+            if (!ok || it.tiles == 0)
+                break;
+            walk.next(w, lane);
+        }
         // every copy has landed before the CTA can end
         for (int j = max(0, kc - KST); j < kc; j++)
             px_drain(&k_full[j % KST], (j / KST) & 1);
@@ -392,56 +515,80 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     else if (warp == 2)
     {
         // ---- the items' Q, and V tiles
-        int vc = 0, items = 0;
-        for (bool ok = true; more && ok; more = it.next(w), items++)
+        int vc = 0, place = 0, used[2] = {0, 0}; // the next item's place for Q; items that had each
+        bool ok = true;
+        for (int j = 0; ok; j++)
         {
-            if (*abort_flag || (items && !px_wait_warp(q_empty, (items - 1) & 1, abort_flag)))
+            const PagedItem it = fetch(j);
+            if (!__all_sync(0xffffffffu, it.tiles != 0) || px_stopped(abort_flag))
                 break;
-            if (lane == 0)
-            {
-                const int tiles = PAIR && it.two(w) ? 2 : 1, row = it.r.row0 + it.first(w);
-                mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * tpt * G * 256));
-                for (int i = 0; i < tiles; i++)
+            const bool two = PAIR && px_two(w, it);
+            if (two)
+                place = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if ((two || i == place) && ok)
                 {
-                    tma_load_3d(sq + i * PX_TILE, &qmap, 0, it.kvh * G, row + i * tpt, q_full);
-                    tma_load_3d(sq + i * PX_TILE + PX_TILE / 2, &qmap, 64, it.kvh * G, row + i * tpt, q_full);
+                    if (used[i] && !px_wait_warp(&q_empty[i], (used[i] - 1) & 1, abort_flag))
+                        ok = false;
+                    else
+                    {
+                        if (lane == 0)
+                        {
+                            const int row = it.row0 + it.first + (two ? i * tpt : 0);
+                            uint8_t *dst = sq + i * q_step;
+                            mbar_arrive_expect_tx(&q_full[i], (uint32_t)(w.p.box * G * 256));
+                            tma_load_3d(dst, &qmap, 0, it.kvh * G, row, &q_full[i]);
+                            tma_load_3d(dst + PX_TILE / 2, &qmap, 64, it.kvh * G, row, &q_full[i]);
+                        }
+                        used[i]++;
+                    }
                 }
-            }
+            if (!ok)
+                break;
+            place = two ? 0 : q_places == 2 ? place ^ 1 : 0;
             __syncwarp();
+            bool bad;
+            int page = px_page(w, it, it.tile0, lane, bad);
             for (int t = 0; t < it.tiles; t++, vc++)
             {
                 const int s = vc % VST;
-                if (*abort_flag || (vc >= VST && !px_wait_warp(&v_empty[s], (vc / VST - 1) & 1, abort_flag)))
+                if (px_stopped(abort_flag) || (vc >= VST && !px_wait_warp(&v_empty[s], (vc / VST - 1) & 1, abort_flag)))
                 {
-                    items++; // its Q is on the way
                     ok = false;
                     break;
                 }
-                px_load(sv + s * PX_TILE, &vmap, w, it, it.tile0 + t, &v_full[s], lane);
+                px_load(sv + s * PX_TILE, &vmap, w, it.kvh, page, &v_full[s], lane);
+                page = px_page(w, it, it.tile0 + t + 1, lane, bad);
             }
-            if (!ok)
-                break;
         }
-        if (items)
-            px_drain(q_full, (items - 1) & 1);
-        for (int j = max(0, vc - VST); j < vc; j++)
-            px_drain(&v_full[j % VST], (j / VST) & 1);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (used[i])
+                px_drain(&q_full[i], (used[i] - 1) & 1);
+        for (int i = max(0, vc - VST); i < vc; i++)
+            px_drain(&v_full[i % VST], (i / VST) & 1);
     }
     else if (warp == 3)
     {
         // ---- V without what is not finite in slots that some row does not see
         int vc = 0;
-        for (bool ok = true; more && ok; more = it.next(w))
+        bool ok = true;
+        for (int j = 0; ok; j++)
+        {
+            const PagedItem it = fetch(j);
+            if (!__all_sync(0xffffffffu, it.tiles != 0))
+                break;
             for (int t = 0; t < it.tiles; t++, vc++)
             {
-                const int s = vc % VST, k0 = (it.tile0 + t) * 128, n = it.r.n + it.r.t;
+                const int s = vc % VST, k0 = (it.tile0 + t) * 128, n = it.n + it.t;
                 if (!px_wait_warp(&v_full[s], (vc / VST) & 1, abort_flag))
                 {
                     ok = false;
                     break;
                 }
                 // (pages behind the last slot's are zeros)
-                const int lo = max(0, it.open(w) - k0), hi = min(128, ((n + a.c.page - 1) & -a.c.page) - k0);
+                const int lo = max(0, px_open(w, it) - k0), hi = min(128, ((n + a.c.page - 1) & -a.c.page) - k0);
                 if (lo < hi)
                 {
                     bool found = false;
@@ -466,79 +613,110 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                         }
                     }
                     if (found)
-                        special[it.seq & 7] = it.seq + 1;
+                        special[j & 7] = j + 1;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
                 if (lane == 0)
                     mbar_arrive(&v_clean[s]);
             }
+        }
     }
     else if (warp == 1)
     {
-        // ---- the products
-        if (lane == 0)
+        // ---- the products: every lane walks along, one issues
+        const uint32_t idesc_s = tc_idesc(128, 128);
+        const uint32_t idesc_o = tc_idesc(128, 128) | (1u << 16); // B (V) MN-major
+        const uint64_t dq = smem_desc_k128(smem_u32(sq)), dk = smem_desc_k128(smem_u32(sk)),
+                       dv = smem_desc_mn128(smem_u32(sv), PX_TILE / 2, 1024);
+        const bool issuer = px_elect();
+        int ks = 0, kp = 0, vs = 0, vp = 0, place = 0; // stages and their phases, the item's place for Q
+        int np[2] = {0, 0}, used[2] = {0, 0};
+        bool ok = true;
+        for (int j = 0; ok; j++)
         {
-            const uint32_t idesc_s = tc_idesc(128, 128);
-            const uint32_t idesc_o = tc_idesc(128, 128) | (1u << 16); // B (V) MN-major
-            int kc = 0, items = 0, np[2] = {0, 0};
-            bool ok = true;
-            for (; more && ok; more = it.next(w), items++)
-            {
-                const bool two = PAIR && it.two(w);
-                const int tasks = two ? 2 * it.tiles : it.tiles;
-                ok = px_wait(q_full, items & 1, abort_flag);
-                // task i: stream i & 1 on unit i (two streams of one tile), or on unit i / 2 (a tile each)
-                const auto scores = [&](int i) {
-                    const int unit = two ? i >> 1 : i, st_ = (kc + unit) % KST, s = i & 1;
-                    if (!px_wait(&k_full[st_], ((kc + unit) / KST) & 1, abort_flag))
-                        return false;
-                    tc_fence_after();
-                    const uint32_t q0 = smem_u32(sq + (two ? s * PX_TILE : 0)), k0 = smem_u32(sk + st_ * PX_TILE);
+            const PagedItem it = fetch(j);
+            if (!__all_sync(0xffffffffu, it.tiles != 0))
+                break;
+            const bool two = PAIR && px_two(w, it);
+            const int tasks = two ? 2 * it.tiles : it.tiles;
+            if (two)
+                place = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (two || i == place)
+                {
+                    ok = ok && px_wait_warp(&q_full[i], used[i] & 1, abort_flag);
+                    used[i]++;
+                }
+            // task i: stream i & 1 on unit i (two streams of one tile), or on unit i / 2 (a tile each)
+            const auto scores = [&](int i) {
+                const int s = i & 1;
+                if (!px_wait_warp(&k_full[ks], kp, abort_flag))
+                    return false;
+                tc_fence_after();
+                const bool last = !two || s; // of the unit
+                if (issuer)
+                {
+                    const uint64_t q0 = dq + (uint32_t)(two ? s : place) * (q_step >> 4), k0 = dk + (uint32_t)ks * (PX_TILE >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 8; kk++)
                     {
-                        const uint32_t off = (uint32_t)((kk >> 2) * (PX_TILE / 2) + (kk & 3) * 32);
-                        tc_mma(tmem + 128u * s, smem_desc_k128(q0 + off), smem_desc_k128(k0 + off), idesc_s, kk ? 1u : 0u);
+                        const uint32_t off = (uint32_t)((kk >> 2) * (PX_TILE / 2) + (kk & 3) * 32) >> 4;
+                        tc_mma(tmem + 128u * s, q0 + off, k0 + off, idesc_s, kk ? 1u : 0u);
                     }
                     tc_commit(&s_full[s]);
-                    if (!two || s)
-                        tc_commit(&k_empty[st_]);
-                    if (i == tasks - 1)
-                        tc_commit(q_empty);
-                    return true;
-                };
-                ok = ok && scores(0) && (tasks < 2 || scores(1));
-                for (int i = 0; ok && i < tasks; i++)
+                    if (last)
+                        tc_commit(&k_empty[ks]);
+                    if (two ? i >= tasks - 2 : i == tasks - 1)
+                        tc_commit(&q_empty[two ? s : place]);
+                }
+                if (last && ++ks == KST)
                 {
-                    const int unit = two ? i >> 1 : i, st_ = (kc + unit) % VST, s = i & 1;
-                    if (!px_wait(&p_full[s], np[s] & 1, abort_flag) ||
-                        !px_wait(&v_clean[st_], ((kc + unit) / VST) & 1, abort_flag))
-                    {
-                        ok = false;
-                        break;
-                    }
-                    np[s]++;
-                    tc_fence_after();
-                    const uint32_t v0 = smem_u32(sv + st_ * PX_TILE);
+                    ks = 0;
+                    kp ^= 1;
+                }
+                return true;
+            };
+            ok = ok && scores(0) && (tasks < 2 || scores(1));
+            for (int i = 0; ok && i < tasks; i++)
+            {
+                const int s = i & 1;
+                if (!px_wait_warp(&p_full[s], np[s] & 1, abort_flag) || !px_wait_warp(&v_clean[vs], vp, abort_flag))
+                {
+                    ok = false;
+                    break;
+                }
+                np[s]++;
+                tc_fence_after();
+                const bool last = !two || s;
+                if (issuer)
+                {
+                    const uint64_t v0 = dv + (uint32_t)vs * (PX_TILE >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 8; kk++)
-                        tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk,
-                                  smem_desc_mn128(v0 + kk * 2048, PX_TILE / 2, 1024), idesc_o, (i > 1 || kk) ? 1u : 0u);
+                        tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, v0 + kk * (2048 >> 4), idesc_o,
+                                  (i > 1 || kk) ? 1u : 0u);
                     tc_commit(&o_done[s]);
-                    if (!two || s)
-                        tc_commit(&v_empty[st_]);
-                    if (i + 2 < tasks)
-                        ok = scores(i + 2);
+                    if (last)
+                        tc_commit(&v_empty[vs]);
                 }
-                kc += it.tiles;
+                if (last && ++vs == VST)
+                {
+                    vs = 0;
+                    vp ^= 1;
+                }
+                if (i + 2 < tasks)
+                    ok = scores(i + 2);
             }
-            if (!ok)
-                *abort_flag = 1;
-            // all products are complete before TMEM is given back
-            tc_commit(done);
-            px_drain(done, 0);
+            place = two ? 0 : q_places == 2 ? place ^ 1 : 0;
         }
+        if (!ok)
+            *abort_flag = 1;
+        // all products are complete before TMEM is given back
+        if (issuer)
+            tc_commit(done);
+        px_drain(done, 0);
         __syncwarp();
     }
     else
@@ -547,23 +725,26 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         const int ws = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16), tS = trow + 128u * ws, tO = trow + 256u;
         int nt[2] = {0, 0}; // tasks of the streams so far
-        int meets = 0;
+        int meets = 0, kc = 0;
         bool ok = true;
-        for (; more && ok; more = it.next(w))
+        for (int j = 0; ok; j++)
         {
-            const bool two = PAIR && it.two(w);
-            const int n = it.r.n, t = it.r.t;
-            const int tok0 = it.first(w) + (two ? ws * tpt : 0);  // first token of this stream's tile
-            const int rows = min(tpt, t - tok0) * G;              // rows of the tile
+            const PagedItem it = fetch(j);
+            if (!__all_sync(0xffffffffu, it.tiles != 0))
+                break;
+            const bool two = PAIR && px_two(w, it);
+            const int n = it.n, t = it.t;
+            const int tok0 = it.first + (two ? ws * tpt : 0); // first token of this stream's tile
+            const int rows = min(tpt, t - tok0) * G;          // rows of the tile
             const int mine_t = two ? it.tiles : (it.tiles + 1 - ws) >> 1;
             const int i = tok0 + row / G; // this row's token (one of the request's where row < rows)
             const bool works = quad * 32 < rows;
-            const int clear = it.open(w);
+            const int clear = px_open(w, it);
             uint32_t anc[4] = {0, 0, 0, 0};
             if (st.parent && works)
             {
                 PagedTree tree;
-                if (tree.load(st, it.r, lane))
+                if (tree.load(st, PagedRequest{it.row0, t, n}, lane))
                     paged_fault(st, PAGED_BAD_PARENT);
                 int cur = i < t && row < rows ? i : -1;
                 while (__any_sync(0xffffffffu, cur >= 0))
@@ -602,16 +783,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             float mr = -INFINITY, l = 0.f;
             for (int u = 0; u < mine_t; u++)
             {
-                const int k0 = (it.tile0 + (two ? u : 2 * u + ws)) * 128;
-                uint32_t bad = 0; // sixteens of slots that are not in the pool
-                if (works)
-                {
-                    const int slot = k0 + lane * 16;
-                    const bool out = lane < 8 && slot < n + t && paged_page(st, a.c, it.s, slot) < 0;
-                    bad = __ballot_sync(0xffffffffu, out);
-                    if (out)
-                        paged_fault(st, PAGED_BAD_PAGE);
-                }
+                const int unit = two ? u : 2 * u + ws, k0 = (it.tile0 + unit) * 128;
                 // (the product before this one is complete, too, long since: nobody falls two phases of o_done behind,
                 // where a parity would say nothing)
                 if (!px_wait_warp(&s_full[ws], nt[ws] & 1, abort_flag) ||
@@ -623,10 +795,18 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 tc_fence_after();
                 if (works)
                 {
-                    const bool edge = bad || k0 + 128 > clear;
-                    const auto load = [&](int c, float(&v)[32]) {
-                        tmem_ld32(tS + 32u * c, v);
-                        if (edge)
+                    float v[128];
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        tmem_ld32_async(tS + 32u * c, v + 32 * c);
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        tmem_wait_ld32(v + 32 * c);
+                    const uint32_t bad = lost[(kc + unit) & 7];
+                    if (bad || k0 + 128 > clear)
+                    {
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
                         {
                             uint32_t bits = seen(k0 + 32 * c);
                             if (bad >> (2 * c) & 1u)
@@ -634,20 +814,22 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                             if (bad >> (2 * c) & 2u)
                                 bits &= 0x0000FFFFu;
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                v[j] = bits >> j & 1u ? v[j] : -INFINITY;
+                            for (int e = 0; e < 32; e++)
+                                v[32 * c + e] = bits >> e & 1u ? v[32 * c + e] : -INFINITY;
                         }
-                    };
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                    {
-                        float v[32];
-                        load(c, v);
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            mx = fmaxf(mx, v[j]);
                     }
+                    float most[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        most[e] = v[e];
+#pragma unroll
+                    for (int e = 8; e < 120; e += 2)
+                        most[(e >> 1) & 7] = px_max3(most[(e >> 1) & 7], v[e], v[e + 1]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        most[e] = fmaxf(most[e], v[120 + e]);
+                    const float mx = px_max3(px_max3(most[0], most[1], most[2]), px_max3(most[3], most[4], most[5]),
+                                             fmaxf(most[6], most[7]));
                     if (u == 0)
                         mr = mx;
                     else if (__any_sync(0xffffffffu, mx > mr + PX_RISE))
@@ -660,42 +842,38 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                             mr = mx;
                         }
                         l *= f;
-#pragma unroll
-                        for (int c = 0; c < 4; c++)
+#pragma unroll 1
+                        for (int c = 0; c < 8; c++)
                         {
-                            float v[32];
-                            tmem_ld32(tO + 128u * ws + 32u * c, v);
+                            float y[16];
+                            tmem_ld16(tO + 128u * ws + 16u * c, y);
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                v[j] *= f;
-                            tmem_st32(tO + 128u * ws + 32u * c, v);
+                            for (int e = 0; e < 16; e++)
+                                y[e] *= f;
+                            tmem_st16(tO + 128u * ws + 16u * c, y);
                         }
                     }
                     const float ref = mr == -INFINITY ? 0.f : mr; // nothing seen: every weight 0
-                    float sum[2] = {0.f, 0.f};
+                    const float2 less = make_float2(-ref, -ref), scale = make_float2(PX_SCALE, PX_SCALE),
+                                 lead = make_float2(PX_LEAD, PX_LEAD);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int c = 0; c < 4; c += 2)
+                    for (int c = 0; c < 4; c++)
                     {
-                        uint32_t pk[32];
+                        uint32_t pk[16];
 #pragma unroll
-                        for (int h = 0; h < 2; h++)
+                        for (int e = 0; e < 32; e += 2)
                         {
-                            float v[32];
-                            load(c + h, v);
-#pragma unroll
-                            for (int j = 0; j < 32; j += 2)
-                            {
-                                const float x = ex2_ftz(fmaf(v[j] - ref, PX_SCALE, PX_LEAD));
-                                const float y = ex2_ftz(fmaf(v[j + 1] - ref, PX_SCALE, PX_LEAD));
-                                sum[0] += x;
-                                sum[1] += y;
-                                const __half2 p = __floats2half2_rn(x, y);
-                                pk[16 * h + (j >> 1)] = *reinterpret_cast<const uint32_t *>(&p);
-                            }
+                            float2 x = make_float2(v[32 * c + e], v[32 * c + e + 1]);
+                            x = px_fma2(px_add2(x, less), scale, lead);
+                            x = make_float2(ex2_ftz(x.x), ex2_ftz(x.y));
+                            sum[e >> 1 & 1] = px_add2(sum[e >> 1 & 1], x);
+                            const __half2 p = __floats2half2_rn(x.x, x.y);
+                            pk[e >> 1] = *reinterpret_cast<const uint32_t *>(&p);
                         }
-                        tmem_st32(tS + 16u * c, reinterpret_cast<const float *>(pk));
+                        tmem_st16(tS + 16u * c, reinterpret_cast<const float *>(pk));
                     }
-                    l += sum[0] + sum[1];
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                 }
@@ -705,10 +883,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 nt[ws]++;
             }
             nt[ws ^ 1] += two ? it.tiles : (it.tiles + ws) >> 1;
+            kc += it.tiles;
             if (!ok)
                 break;
             // ---- the item's rows: whole, or this share's part
-            const bool whole = it.tile0 == 0 && it.tiles == it.units(w);
+            const bool whole = it.tiles == it.units;
             const int slot = it.tile0 ? 0 : 1;
             const int rho = (two ? ws * tpt * G : 0) + row; // the row's number in the item
             float M = mr, L = l, f0 = ws ? 0.f : 1.f, f1 = ws ? 1.f : 0.f;
@@ -748,9 +927,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             if (works)
             {
                 const bool both = !two && it.tiles > 1; // stream 1 of a single unit has no sums
-                const bool odd = special[it.seq & 7] == it.seq + 1;
+                const bool odd = special[j & 7] == j + 1;
                 const float inv = M == -INFINITY ? 0.f : 1.f / L;
-                const int64_t r = it.r.row0 + i;
+                const int64_t r = it.row0 + i;
                 for (int c = c0; c < c1; c++)
                 {
                     __syncwarp();
@@ -761,15 +940,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                     {
                         tmem_ld32(tO + 32u * c, v);
 #pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            v[j] *= f0;
+                        for (int e = 0; e < 32; e++)
+                            v[e] *= f0;
                         if (both)
                         {
                             float y[32];
                             tmem_ld32(tO + 128u + 32u * c, y);
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                v[j] = f1 == 0.f ? v[j] : fmaf(y[j], f1, v[j]);
+                            for (int e = 0; e < 32; e++)
+                                v[e] = f1 == 0.f ? v[e] : fmaf(y[e], f1, v[e]);
                         }
                     }
                     if (odd && row < rows)
@@ -784,10 +963,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                             const __half *src = a.c.v + paged_offset(a.c, page, k) +
                                                 (size_t)it.kvh * a.c.page * YLM_HEAD_DIM + 32 * c;
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
+                            for (int e = 0; e < 32; e++)
                             {
-                                const float x = h2f(src[j]);
-                                v[j] += x - x != 0.f ? x : 0.f; // (x - x is NaN)
+                                const float x = h2f(src[e]);
+                                v[e] += x - x != 0.f ? x : 0.f; // (x - x is NaN)
                             }
                         }
                     }
@@ -798,13 +977,13 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                             uint4 *dst = reinterpret_cast<uint4 *>(a.out + r * a.out_stride +
                                                                    (it.kvh * G + row % G) * YLM_HEAD_DIM + 32 * c);
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
+                            for (int e = 0; e < 4; e++)
                             {
                                 __half2 h[4];
 #pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                    h[e] = __floats2half2_rn(v[8 * j + 2 * e] * inv, v[8 * j + 2 * e + 1] * inv);
-                                dst[j] = *reinterpret_cast<const uint4 *>(h);
+                                for (int k = 0; k < 4; k++)
+                                    h[k] = __floats2half2_rn(v[8 * e + 2 * k] * inv, v[8 * e + 2 * k + 1] * inv);
+                                dst[e] = *reinterpret_cast<const uint4 *>(h);
                             }
                         }
                         else
@@ -812,8 +991,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                             float4 *dst = reinterpret_cast<float4 *>(
                                 w.o + (((size_t)blockIdx.x * 2 + slot) * w.p.cap + rho) * YLM_HEAD_DIM + 32 * c);
 #pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                            for (int e = 0; e < 8; e++)
+                                dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                         }
                     }
                 }
@@ -855,28 +1034,26 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(const __grid_
 {
     const int lane = threadIdx.x & 31, b = blockIdx.x + 1;
     pdl_wait();
-    const PagedCut c = w.cuts[b];
-    if (!c.cut || c.tile0 > c.u0 - w.cuts[b - 1].u0)
+    const PagedCut &c = w.cuts[b];
+    const long long u0 = c.u0;
+    // share b - 1 has the units below
+    if (!c.cut || c.it.tile0 > c.each + (b - 1 < c.more))
         return;
     const PagedAttnArgs &a = w.a;
-    PagedRequest r;
-    bool bad;
-    paged_request(a.st, a.c.page, c.s, r, bad);
-    const int tok0 = c.qp * w.p.tpi, rows = min(w.p.tpi, r.t - tok0) * w.p.G;
+    const int tok0 = c.it.first, rows = min(w.p.tpi, c.it.t - tok0) * w.p.G;
     const int rho = blockIdx.y * PJ_WARPS + (threadIdx.x >> 5);
     if (rho >= rows)
         return;
-    // part 0 is share b - 1's end, part k the start of share b - 1 + k
-    const long long end = c.u0 - c.tile0 + c.kt;
-    int parts = 2;
-    while (b + parts - 1 < (int)gridDim.x + 1 && w.cuts[b + parts - 1].u0 < end)
-        parts++;
+    // part 0 is share b - 1's end, part k the start of share b - 1 + k; the last one has the item's last unit
+    const long long last = u0 - c.it.tile0 + c.it.units - 1, big = c.more * (c.each + 1);
+    const int parts = (int)(last < big ? px_div(last, (int)(c.each + 1)) : c.more + px_div(last - big, (int)c.each)) - b + 2;
     const auto at = [&](int k) { return (size_t)((b - 1 + k) * 2 + (k == 0)) * w.p.cap + rho; };
     float M = -INFINITY, L = 0.f;
     for (int k = lane; k < parts; k += 32)
         M = fmaxf(M, w.ml[at(k)].x);
     M = warp_max(M);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int k = 0; k < parts; k++)
     {
         const float2 ml = w.ml[at(k)];
@@ -890,8 +1067,8 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(const __grid_
     }
     const float inv = M == -INFINITY ? 0.f : 1.f / L;
     __half2 h[2] = {__floats2half2_rn(o.x * inv, o.y * inv), __floats2half2_rn(o.z * inv, o.w * inv)};
-    *reinterpret_cast<uint2 *>(a.out + (int64_t)(r.row0 + tok0 + rho / w.p.G) * a.out_stride +
-                               (c.kvh * w.p.G + rho % w.p.G) * YLM_HEAD_DIM + lane * 4) = *reinterpret_cast<const uint2 *>(h);
+    *reinterpret_cast<uint2 *>(a.out + (int64_t)(c.it.row0 + tok0 + rho / w.p.G) * a.out_stride +
+                               (c.it.kvh * w.p.G + rho % w.p.G) * YLM_HEAD_DIM + lane * 4) = *reinterpret_cast<const uint2 *>(h);
 }
 
 // ------------------------------------------------------------------ host side
@@ -909,7 +1086,7 @@ static bool px_pool_map(CUtensorMap *map, const __half *p, const PagedCache &c)
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Q as [rows][hq][128], the G heads of tpt tokens and half of their dimensions a box: rows i * G + h of a tile.
+// Q as [rows][hq][128], the G heads of a tile's tokens and half of their dimensions a box: rows i * G + h of a tile.
 static bool px_q_map(CUtensorMap *map, const PagedAttnArgs &a, const PagedPlan &p)
 {
     auto enc = encoder();
@@ -917,7 +1094,7 @@ static bool px_q_map(CUtensorMap *map, const PagedAttnArgs &a, const PagedPlan &
         return false;
     cuuint64_t dims[3] = {128, (cuuint64_t)a.hq, (cuuint64_t)a.st.rows};
     cuuint64_t strides[2] = {256, (cuuint64_t)a.q_stride * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.tpt}, estr[3] = {1, 1, 1};
+    cuuint32_t box[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.box}, estr[3] = {1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half *>(a.q), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
