@@ -206,20 +206,13 @@ __device__ __forceinline__ float2 px_fma2(float2 a, float2 b, float2 c)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
 }
-// the largest of three (of those that are not NaN, as fmaxf)
-__device__ __forceinline__ float px_max3(float a, float b, float c)
-{
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
 // ------------------------------------------------------------------ waits
 // Bounded: after 2 s, or once another warp gave up, *abort is set and the caller unwinds.
 __device__ __forceinline__ bool px_wait(uint64_t *bar, uint32_t parity, volatile int *abort)
 {
-    if (mbar_try_wait(bar, parity))
-        return true;
+    for (int i = 0; i < 16; i++)
+        if (mbar_try_wait(bar, parity))
+            return true;
     const uint64_t t0 = globaltimer_ns();
     for (;;)
     {
@@ -629,9 +622,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         const uint32_t idesc_o = tc_idesc(128, 128) | (1u << 16); // B (V) MN-major
         const uint64_t dq = smem_desc_k128(smem_u32(sq)), dk = smem_desc_k128(smem_u32(sk)),
                        dv = smem_desc_mn128(smem_u32(sv), PX_TILE / 2, 1024);
-        const bool issuer = px_elect();
         int ks = 0, kp = 0, vs = 0, vp = 0, place = 0; // stages and their phases, the item's place for Q
-        int np[2] = {0, 0}, used[2] = {0, 0};
+        uint32_t pp = 0, qp = 0; // bit s: the phase of p_full[s] and of q_full[s]
         bool ok = true;
         for (int j = 0; ok; j++)
         {
@@ -646,8 +638,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             for (int i = 0; i < 2; i++)
                 if (two || i == place)
                 {
-                    ok = ok && px_wait_warp(&q_full[i], used[i] & 1, abort_flag);
-                    used[i]++;
+                    ok = ok && px_wait_warp(&q_full[i], qp >> i & 1, abort_flag);
+                    qp ^= 1u << i;
                 }
             // task i: stream i & 1 on unit i (two streams of one tile), or on unit i / 2 (a tile each)
             const auto scores = [&](int i) {
@@ -656,7 +648,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                     return false;
                 tc_fence_after();
                 const bool last = !two || s; // of the unit
-                if (issuer)
+                if (px_elect())
                 {
                     const uint64_t q0 = dq + (uint32_t)(two ? s : place) * (q_step >> 4), k0 = dk + (uint32_t)ks * (PX_TILE >> 4);
 #pragma unroll
@@ -682,15 +674,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             for (int i = 0; ok && i < tasks; i++)
             {
                 const int s = i & 1;
-                if (!px_wait_warp(&p_full[s], np[s] & 1, abort_flag) || !px_wait_warp(&v_clean[vs], vp, abort_flag))
+                if (!px_wait_warp(&p_full[s], pp >> s & 1, abort_flag) || !px_wait_warp(&v_clean[vs], vp, abort_flag))
                 {
                     ok = false;
                     break;
                 }
-                np[s]++;
+                pp ^= 1u << s;
                 tc_fence_after();
                 const bool last = !two || s;
-                if (issuer)
+                if (px_elect())
                 {
                     const uint64_t v0 = dv + (uint32_t)vs * (PX_TILE >> 4);
 #pragma unroll
@@ -714,7 +706,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         if (!ok)
             *abort_flag = 1;
         // all products are complete before TMEM is given back
-        if (issuer)
+        if (px_elect())
             tc_commit(done);
         px_drain(done, 0);
         __syncwarp();
@@ -724,7 +716,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         // ---- softmax: stream ws, row `row` of its tile
         const int ws = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16), tS = trow + 128u * ws, tO = trow + 256u;
-        int nt[2] = {0, 0}; // tasks of the streams so far
+        uint32_t nt = 0; // bit s: whether stream s has had an odd number of tasks
         int meets = 0, kc = 0;
         bool ok = true;
         for (int j = 0; ok; j++)
@@ -786,8 +778,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 const int unit = two ? u : 2 * u + ws, k0 = (it.tile0 + unit) * 128;
                 // (the product before this one is complete, too, long since: nobody falls two phases of o_done behind,
                 // where a parity would say nothing)
-                if (!px_wait_warp(&s_full[ws], nt[ws] & 1, abort_flag) ||
-                    (u && !px_wait_warp(&o_done[ws], (nt[ws] - 1) & 1, abort_flag)))
+                if (!px_wait_warp(&s_full[ws], nt >> ws & 1, abort_flag) ||
+                    (u && !px_wait_warp(&o_done[ws], ~nt >> ws & 1, abort_flag)))
                 {
                     ok = false;
                     break;
@@ -795,17 +787,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 tc_fence_after();
                 if (works)
                 {
-                    float v[128];
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        tmem_ld32_async(tS + 32u * c, v + 32 * c);
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        tmem_wait_ld32(v + 32 * c);
                     const uint32_t bad = lost[(kc + unit) & 7];
-                    if (bad || k0 + 128 > clear)
+                    if (__builtin_expect(bad || k0 + 128 > clear, 0))
                     {
-#pragma unroll
+                        // scores of hidden slots become -inf
+#pragma unroll 1
                         for (int c = 0; c < 4; c++)
                         {
                             uint32_t bits = seen(k0 + 32 * c);
@@ -813,26 +799,33 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                                 bits &= 0xFFFF0000u;
                             if (bad >> (2 * c) & 2u)
                                 bits &= 0x0000FFFFu;
+                            float v[32];
+                            tmem_ld32(tS + 32u * c, v);
 #pragma unroll
                             for (int e = 0; e < 32; e++)
-                                v[32 * c + e] = bits >> e & 1u ? v[32 * c + e] : -INFINITY;
+                                v[e] = bits >> e & 1u ? v[e] : -INFINITY;
+                            tmem_st32(tS + 32u * c, v);
                         }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
-                    float most[8];
+                    float mx;
+                    {
+                        float v[128];
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        most[e] = v[e];
+                        for (int c = 0; c < 4; c++)
+                            tmem_ld32_async(tS + 32u * c, v + 32 * c);
 #pragma unroll
-                    for (int e = 8; e < 120; e += 2)
-                        most[(e >> 1) & 7] = px_max3(most[(e >> 1) & 7], v[e], v[e + 1]);
+                        for (int c = 0; c < 4; c++)
+                            tmem_wait_ld32(v + 32 * c);
+                        float most[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        most[e] = fmaxf(most[e], v[120 + e]);
-                    const float mx = px_max3(px_max3(most[0], most[1], most[2]), px_max3(most[3], most[4], most[5]),
-                                             fmaxf(most[6], most[7]));
+                        for (int e = 4; e < 128; e++)
+                            most[e & 3] = fmaxf(most[e & 3], v[e]);
+                        mx = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                    }
                     if (u == 0)
                         mr = mx;
-                    else if (__any_sync(0xffffffffu, mx > mr + PX_RISE))
+                    else if (__builtin_expect(__any_sync(0xffffffffu, mx > mr + PX_RISE), 0))
                     {
                         // the sums so far in units of the new reference
                         float f = 1.f;
@@ -853,26 +846,39 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                             tmem_st16(tO + 128u * ws + 16u * c, y);
                         }
                     }
+                    // The weights. A loop whose code stays in the instruction cache: unrolled over all 128
+                    // scores it took half as long again.
                     const float ref = mr == -INFINITY ? 0.f : mr; // nothing seen: every weight 0
                     const float2 less = make_float2(-ref, -ref), scale = make_float2(PX_SCALE, PX_SCALE),
                                  lead = make_float2(PX_LEAD, PX_LEAD);
                     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                    {
+                    const auto weights = [&](const float(&v)[32], uint32_t at) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2)
                         {
-                            float2 x = make_float2(v[32 * c + e], v[32 * c + e + 1]);
-                            x = px_fma2(px_add2(x, less), scale, lead);
+                            float2 x = px_fma2(px_add2(make_float2(v[e], v[e + 1]), less), scale, lead);
                             x = make_float2(ex2_ftz(x.x), ex2_ftz(x.y));
                             sum[e >> 1 & 1] = px_add2(sum[e >> 1 & 1], x);
                             const __half2 p = __floats2half2_rn(x.x, x.y);
                             pk[e >> 1] = *reinterpret_cast<const uint32_t *>(&p);
                         }
-                        tmem_st16(tS + 16u * c, reinterpret_cast<const float *>(pk));
+                        tmem_st16(at, reinterpret_cast<const float *>(pk));
+                    };
+                    // (32 weights take the place of 16 scores: those are always read by then)
+                    float v0[32], v1[32];
+                    tmem_ld32_async(tS, v0);
+#pragma unroll 1
+                    for (int c = 0; c < 4; c += 2)
+                    {
+                        tmem_wait_ld32(v0);
+                        tmem_ld32_async(tS + 32u * (c + 1), v1);
+                        weights(v0, tS + 16u * c);
+                        tmem_wait_ld32(v1);
+                        tmem_ld32_async(tS + 32u * ((c + 2) & 3), v0); // (the last time for nothing)
+                        weights(v1, tS + 16u * (c + 1));
                     }
+                    tmem_wait_ld32(v0);
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
@@ -880,9 +886,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive(&p_full[ws]);
-                nt[ws]++;
+                nt ^= 1u << ws;
             }
-            nt[ws ^ 1] += two ? it.tiles : (it.tiles + ws) >> 1;
+            nt ^= (uint32_t)((two ? it.tiles : (it.tiles + ws) >> 1) & 1) << (ws ^ 1);
             kc += it.tiles;
             if (!ok)
                 break;
@@ -917,7 +923,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
 #pragma unroll
             for (int s = 0; s < 2; s++)
                 if (!two || s == ws)
-                    in = in && (nt[s] == 0 || px_wait_warp(&o_done[s], (nt[s] - 1) & 1, abort_flag));
+                    in = in && px_wait_warp(&o_done[s], ~nt >> s & 1, abort_flag); // (before its first task: at once)
             if (!in)
             {
                 ok = false;
