@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     uint64_t *bars = reinterpret_cast<uint64_t *>(control);
     uint64_t *k_full = bars, *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST,
              *v_clean = v_empty + VST, *q_full = v_clean + VST, *q_empty = q_full + 2, *s_full = q_empty + 2,
-             *p_full = s_full + 2, *o_done = p_full + 2, *joined = o_done + 2, *parted = joined + 1, *done = parted + 1,
+             *p_most = s_full + 2, *p_full = p_most + 2, *o_done = p_full + 2, *joined = o_done + 2, *parted = joined + 1, *done = parted + 1,
              *item_full = done + 1; // [8]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(control + 320);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(control + 324);
@@ -330,6 +330,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             mbar_init(&q_full[i], 1);
             mbar_init(&q_empty[i], 1);
             mbar_init(&s_full[i], 1);
+            mbar_init(&p_most[i], 4);
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
         }
@@ -674,25 +675,40 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             for (int i = 0; ok && i < tasks; i++)
             {
                 const int s = i & 1;
-                if (!px_wait_warp(&p_full[s], pp >> s & 1, abort_flag) || !px_wait_warp(&v_clean[vs], vp, abort_flag))
+                // the first three quarters of the slots while the softmax has the last one in work
+                if (!px_wait_warp(&v_clean[vs], vp, abort_flag) || !px_wait_warp(&p_most[s], pp >> s & 1, abort_flag))
+                {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const bool last = !two || s;
+                const uint64_t v0 = dv + (uint32_t)vs * (PX_TILE >> 4);
+                if (px_elect())
+                {
+#pragma unroll
+                    for (int kk = 0; kk < 6; kk++)
+                        tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, v0 + kk * (2048 >> 4), idesc_o,
+                                  (i > 1 || kk) ? 1u : 0u);
+                }
+                __syncwarp();
+                if (!px_wait_warp(&p_full[s], pp >> s & 1, abort_flag))
                 {
                     ok = false;
                     break;
                 }
                 pp ^= 1u << s;
                 tc_fence_after();
-                const bool last = !two || s;
                 if (px_elect())
                 {
-                    const uint64_t v0 = dv + (uint32_t)vs * (PX_TILE >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < 8; kk++)
-                        tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, v0 + kk * (2048 >> 4), idesc_o,
-                                  (i > 1 || kk) ? 1u : 0u);
+                    for (int kk = 6; kk < 8; kk++)
+                        tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, v0 + kk * (2048 >> 4), idesc_o, 1u);
                     tc_commit(&o_done[s]);
                     if (last)
                         tc_commit(&v_empty[vs]);
                 }
+                __syncwarp();
                 if (last && ++vs == VST)
                 {
                     vs = 0;
@@ -874,18 +890,31 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                         tmem_wait_ld32(v0);
                         tmem_ld32_async(tS + 32u * (c + 1), v1);
                         weights(v0, tS + 16u * c);
+                        if (c == 2)
+                        {
+                            // all but the last 32 are there
+                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0)
+                                mbar_arrive(&p_most[ws]);
+                        }
                         tmem_wait_ld32(v1);
-                        tmem_ld32_async(tS + 32u * ((c + 2) & 3), v0); // (the last time for nothing)
+                        if (c == 0)
+                            tmem_ld32_async(tS + 64u, v0);
                         weights(v1, tS + 16u * (c + 1));
                     }
-                    tmem_wait_ld32(v0);
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                 }
                 __syncwarp();
                 if (lane == 0)
+                {
+                    if (!works)
+                        mbar_arrive(&p_most[ws]);
                     mbar_arrive(&p_full[ws]);
+                }
                 nt ^= 1u << ws;
             }
             nt ^= (uint32_t)((two ? it.tiles : (it.tiles + ws) >> 1) & 1) << (ws ^ 1);
