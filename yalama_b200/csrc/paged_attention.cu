@@ -5,7 +5,8 @@
 //   o_r  = sum_j softmax(x_r)_j v_j,  0 where the row sees no slot
 //
 // An item is a request's KV head and up to tpi of its tokens: their G query heads each are the rows of one or two
-// tiles of 128 (row i * G + h). It has a unit for each 128 slots its tokens see. The units of all items, in order, are
+// tiles of 128 (row i * G + h). It has a unit for each 128 slots its tokens see, and PX_ITEM in front that stand for what it
+// costs beside them. The units of all items, in order, are
 // dealt evenly to one CTA per SM, so that requests of any lengths keep all SMs busy to the end; an item that
 // a CTA border cuts leaves sums (M, l, O) per CTA, which paged_join_kernel joins.
 //
@@ -30,6 +31,10 @@ namespace ylm {
 
 constexpr int PX_TILE = 128 * 128 * 2; // a tile of 128 rows or slots: two halves of 64 dimensions
 constexpr int PX_THREADS = 384;
+// What an item costs beside its units (its first loads, its sums' way out), in units, for the dealing.
+#ifndef PX_ITEM
+#define PX_ITEM 3
+#endif
 constexpr int PX_KST = 3;
 constexpr int PX_CONTROL = 3072; // barriers, the streams' (M, l)
 constexpr int PX_SMEM = 7 * PX_TILE + PX_CONTROL;
@@ -42,6 +47,7 @@ constexpr float PX_RISE = (PX_MOST - PX_LEAD) / PX_SCALE; // in scores
 struct PagedPlan
 {
     int G, tpt, tpi; // query heads per KV head, tokens per 128-row tile and per item
+    int over_g;      // r / G = r * over_g >> 16 for the rows of a tile (r G < 2^16)
     int pair;        // 1: items of two tiles (some request may have more than tpt rows)
     int box;         // tokens of a tile that are loaded: tpt, or fewer where no request has so many
     int cap;         // most rows of an item
@@ -54,6 +60,7 @@ static PagedPlan paged_plan(const PagedAttnArgs &a, int num_sms)
     PagedPlan p;
     p.G = a.hq / a.c.hkv;
     p.tpt = 128 / p.G;
+    p.over_g = 65536 / p.G + 1;
     p.pair = a.st.max_rows > p.tpt;
     p.tpi = p.pair ? 2 * p.tpt : p.tpt;
     p.box = std::max(1, std::min(p.tpt, a.st.max_rows));
@@ -81,6 +88,7 @@ struct PagedCut
 {
     long long u0, u1;
     long long each, more; // every share has `each` units, the first `more` of them one more
+    long long left;       // units behind its part of the first item
     PagedItem it;
     int cut;              // the share starts inside an item
 };
@@ -92,7 +100,7 @@ struct PagedPass
     PagedPlan p;
     PagedCut *cuts;
     float2 *ml; // [cta][2][cap]: (M, l) of the item that the share starts inside of, and of the one it ends inside of
-    float *o;   // [cta][2][cap][128]
+    float4 *o;  // [cta][2][32][cap]: four dimensions of every row after one another
 };
 
 // ------------------------------------------------------------------ units
@@ -101,7 +109,7 @@ __device__ __forceinline__ int px_units(int n, int t, int qp, int tpi) { return 
 
 // sum of ceil((n + i * tpi) / 128) over i = 1..k: each is (x + r) / 128 with r = -x mod 128, whose
 // values repeat after 128 / g and then are those that are congruent to -n mod g, for g the power of two in tpi
-__device__ __forceinline__ long long px_before(int n, int k, int tpi)
+__device__ __noinline__ long long px_before(int n, int k, int tpi)
 {
     if (k <= 0)
         return 0;
@@ -116,7 +124,7 @@ __device__ __forceinline__ long long px_before(int n, int k, int tpi)
 __device__ __forceinline__ long long px_request_units(const PagedRequest &r, int tpi, int hkv)
 {
     const int last = r.t <= tpi ? 0 : (r.t - 1) / tpi;
-    return hkv * (px_before(r.n, last, tpi) + px_units(r.n, r.t, last, tpi));
+    return hkv * (px_before(r.n, last, tpi) + px_units(r.n, r.t, last, tpi) + (long long)PX_ITEM * (last + 1));
 }
 
 // slots below are seen by every row of the item
@@ -136,7 +144,7 @@ __device__ __forceinline__ long long px_div(long long a, int b)
 struct PagedWalk
 {
     PagedItem it;
-    long long left; // units of the share from here on
+    long long left; // units of the share behind this item
     int base;       // ahead: requests base + lane
     PagedRequest ahead;
     bool there;
@@ -149,15 +157,14 @@ struct PagedWalk
     }
     __device__ __forceinline__ void start(const PagedPass &w, const PagedCut &c, int lane)
     {
-        left = c.u1 - c.u0;
+        left = c.left;
         it = c.it;
-        if (it.tiles)
-            look(w, it.s + 1, lane);
+        base = -1; // not yet looked ahead
     }
     __device__ __forceinline__ void next(const PagedPass &w, int lane)
     {
-        left -= it.tiles;
         it.tiles = 0;
+        left -= PX_ITEM;
         if (left <= 0)
             return;
         it.tile0 = 0;
@@ -169,6 +176,8 @@ struct PagedWalk
             {
                 it.first = 0;
                 unsigned hit;
+                if (base < 0)
+                    look(w, it.s + 1, lane);
                 while (!(hit = __ballot_sync(0xffffffffu, there && base + lane > it.s)))
                 {
                     if (base + 32 >= w.a.st.n_seq)
@@ -184,6 +193,7 @@ struct PagedWalk
         }
         it.units = (it.n + min(it.t, it.first + w.p.tpi) + 127) >> 7;
         it.tiles = (int)min((long long)it.units, left);
+        left -= it.tiles;
     }
 };
 
@@ -206,6 +216,21 @@ __device__ __forceinline__ float2 px_fma2(float2 a, float2 b, float2 c)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
 }
+// Between lanes 2 i and 2 i + 1: the lower one gets (x, the other's x), the upper one (the other's y, y).
+__device__ __forceinline__ void px_trade(uint4 &x, uint4 &y, int lane)
+{
+    const bool up = lane & 1;
+    uint4 give = up ? x : y;
+    give.x = __shfl_xor_sync(0xffffffffu, give.x, 1);
+    give.y = __shfl_xor_sync(0xffffffffu, give.y, 1);
+    give.z = __shfl_xor_sync(0xffffffffu, give.z, 1);
+    give.w = __shfl_xor_sync(0xffffffffu, give.w, 1);
+    if (up)
+        x = give;
+    else
+        y = give;
+}
+
 // ------------------------------------------------------------------ waits
 // Bounded: after 2 s, or once another warp gave up, *abort is set and the caller unwinds.
 __device__ __forceinline__ bool px_wait(uint64_t *bar, uint32_t parity, volatile int *abort)
@@ -311,7 +336,6 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     const PagedAttnArgs &a = w.a;
     const PagedStep &st = a.st;
 
-    pdl_launch_dependents(); // the joining CTAs may start; they wait for this grid's end
     if (tid == 0)
     {
         for (int i = 0; i < KST; i++)
@@ -357,6 +381,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
 
+    // (launched as a programmatic dependent: what comes before this grid in the stream may have run until here)
+    pdl_wait();
+    pdl_launch_dependents(); // the joining CTAs may start; they wait for this grid's end
     // ---- this CTA's share: requests in runs of `run` a thread, their units summed over the threads
     const int run = st.n_seq <= PX_THREADS ? 1 : (st.n_seq + PX_THREADS - 1) / PX_THREADS;
     const int s_end = min(st.n_seq, (tid + 1) * run);
@@ -411,12 +438,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         while (hi - lo > 1)
         {
             const int mid = (lo + hi) / 2;
-            if (a.c.hkv * px_before(req.n, mid, w.p.tpi) <= rest)
+            if (a.c.hkv * (px_before(req.n, mid, w.p.tpi) + (long long)PX_ITEM * mid) <= rest)
                 lo = mid;
             else
                 hi = mid;
         }
-        rest -= a.c.hkv * px_before(req.n, lo, w.p.tpi);
+        rest -= a.c.hkv * (px_before(req.n, lo, w.p.tpi) + (long long)PX_ITEM * lo);
         PagedCut c;
         c.u0 = u0;
         c.u1 = u1;
@@ -428,9 +455,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         c.it.n = req.n;
         c.it.first = lo * w.p.tpi;
         c.it.units = px_units(req.n, req.t, lo, w.p.tpi);
-        c.it.kvh = (int)px_div(rest, c.it.units);
-        c.it.tile0 = (int)(rest - (long long)c.it.kvh * c.it.units);
-        c.it.tiles = (int)min((long long)(c.it.units - c.it.tile0), u1 - u0);
+        c.it.kvh = (int)px_div(rest, c.it.units + PX_ITEM);
+        const int from = (int)(rest - (long long)c.it.kvh * (c.it.units + PX_ITEM)) - PX_ITEM; // below 0: in front of the item's units
+        c.it.tile0 = max(0, from);
+        c.it.tiles = (int)max(0ll, min((long long)c.it.units, u1 - u0 + from) - c.it.tile0);
+        c.left = u1 - u0 + from - c.it.tile0 - c.it.tiles;
         c.cut = c.it.tile0 > 0;
         *mine = c;
         w.cuts[b] = c;
@@ -497,6 +526,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 }
                 px_load(sk + s * PX_TILE, &kmap, w, it.kvh, page, &k_full[s], lane);
                 page = px_page(w, it, it.tile0 + t + 1, lane, bad); // on its way while the next stage comes free
+                if (walk.base < 0)
+                    walk.look(w, it.s + 1, lane);
             }
             if (!ok || it.tiles == 0)
                 break;
@@ -642,11 +673,60 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                     ok = ok && px_wait_warp(&q_full[i], qp >> i & 1, abort_flag);
                     qp ^= 1u << i;
                 }
-            // task i: stream i & 1 on unit i (two streams of one tile), or on unit i / 2 (a tile each)
-            const auto scores = [&](int i) {
+            // Task i: stream i & 1 on unit i (two streams of one tile), or on unit i / 2 (a tile each). S of a stream's next
+            // task follows O += P V of this one, which reads P where that S goes.
+            for (int i = -2; i < tasks; i++)
+            {
                 const int s = i & 1;
+                if (i >= 0)
+                {
+                    // the first three quarters of the slots while the softmax has the last one in work
+                    if (!px_wait_warp(&v_clean[vs], vp, abort_flag) || !px_wait_warp(&p_most[s], pp >> s & 1, abort_flag))
+                    {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const bool last = !two || s;
+                    const uint64_t v0 = dv + (uint32_t)vs * (PX_TILE >> 4);
+                    if (px_elect())
+                    {
+#pragma unroll
+                        for (int kk = 0; kk < 6; kk++)
+                            tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, v0 + kk * (2048 >> 4), idesc_o,
+                                      (i > 1 || kk) ? 1u : 0u);
+                    }
+                    __syncwarp();
+                    if (!px_wait_warp(&p_full[s], pp >> s & 1, abort_flag))
+                    {
+                        ok = false;
+                        break;
+                    }
+                    pp ^= 1u << s;
+                    tc_fence_after();
+                    if (px_elect())
+                    {
+#pragma unroll
+                        for (int kk = 6; kk < 8; kk++)
+                            tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, v0 + kk * (2048 >> 4), idesc_o, 1u);
+                        tc_commit(&o_done[s]);
+                        if (last)
+                            tc_commit(&v_empty[vs]);
+                    }
+                    __syncwarp();
+                    if (last && ++vs == VST)
+                    {
+                        vs = 0;
+                        vp ^= 1;
+                    }
+                }
+                if (i + 2 >= tasks)
+                    continue;
                 if (!px_wait_warp(&k_full[ks], kp, abort_flag))
-                    return false;
+                {
+                    ok = false;
+                    break;
+                }
                 tc_fence_after();
                 const bool last = !two || s; // of the unit
                 if (px_elect())
@@ -661,7 +741,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                     tc_commit(&s_full[s]);
                     if (last)
                         tc_commit(&k_empty[ks]);
-                    if (two ? i >= tasks - 2 : i == tasks - 1)
+                    if (two ? i >= tasks - 4 : i == tasks - 3)
                         tc_commit(&q_empty[two ? s : place]);
                 }
                 if (last && ++ks == KST)
@@ -669,53 +749,6 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                     ks = 0;
                     kp ^= 1;
                 }
-                return true;
-            };
-            ok = ok && scores(0) && (tasks < 2 || scores(1));
-            for (int i = 0; ok && i < tasks; i++)
-            {
-                const int s = i & 1;
-                // the first three quarters of the slots while the softmax has the last one in work
-                if (!px_wait_warp(&v_clean[vs], vp, abort_flag) || !px_wait_warp(&p_most[s], pp >> s & 1, abort_flag))
-                {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const bool last = !two || s;
-                const uint64_t v0 = dv + (uint32_t)vs * (PX_TILE >> 4);
-                if (px_elect())
-                {
-#pragma unroll
-                    for (int kk = 0; kk < 6; kk++)
-                        tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, v0 + kk * (2048 >> 4), idesc_o,
-                                  (i > 1 || kk) ? 1u : 0u);
-                }
-                __syncwarp();
-                if (!px_wait_warp(&p_full[s], pp >> s & 1, abort_flag))
-                {
-                    ok = false;
-                    break;
-                }
-                pp ^= 1u << s;
-                tc_fence_after();
-                if (px_elect())
-                {
-#pragma unroll
-                    for (int kk = 6; kk < 8; kk++)
-                        tc_mma_ts(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, v0 + kk * (2048 >> 4), idesc_o, 1u);
-                    tc_commit(&o_done[s]);
-                    if (last)
-                        tc_commit(&v_empty[vs]);
-                }
-                __syncwarp();
-                if (last && ++vs == VST)
-                {
-                    vs = 0;
-                    vp ^= 1;
-                }
-                if (i + 2 < tasks)
-                    ok = scores(i + 2);
             }
             place = two ? 0 : q_places == 2 ? place ^ 1 : 0;
         }
@@ -745,7 +778,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             const int tok0 = it.first + (two ? ws * tpt : 0); // first token of this stream's tile
             const int rows = min(tpt, t - tok0) * G;          // rows of the tile
             const int mine_t = two ? it.tiles : (it.tiles + 1 - ws) >> 1;
-            const int i = tok0 + row / G; // this row's token (one of the request's where row < rows)
+            const int i = tok0 + (row * w.p.over_g >> 16); // this row's token (one of the request's where row < rows)
             const bool works = quad * 32 < rows;
             const int clear = px_open(w, it);
             uint32_t anc[4] = {0, 0, 0, 0};
@@ -926,7 +959,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             const int slot = it.tile0 ? 0 : 1;
             const int rho = (two ? ws * tpt * G : 0) + row; // the row's number in the item
             float M = mr, L = l, f0 = ws ? 0.f : 1.f, f1 = ws ? 1.f : 0.f;
-            int c0 = 0, c1 = 4; // this thread's share of the dimensions, 32 each
+            int c0 = 0, c1 = 8; // this thread's share of the dimensions, 16 each
             if (!two)
             {
                 // the streams' sums are of the same rows: half of the dimensions each
@@ -944,8 +977,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 f0 = x.x == -INFINITY ? 0.f : ex2_ftz((x.x - M) * PX_SCALE);
                 f1 = y.x == -INFINITY ? 0.f : ex2_ftz((y.x - M) * PX_SCALE);
                 L = x.y * f0 + y.y * f1;
-                c0 = 2 * ws;
-                c1 = c0 + 2;
+                c0 = 4 * ws;
+                c1 = c0 + 4;
             }
             // every product of the item is in the sums
             bool in = true;
@@ -964,71 +997,81 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 const bool both = !two && it.tiles > 1; // stream 1 of a single unit has no sums
                 const bool odd = special[j & 7] == j + 1;
                 const float inv = M == -INFINITY ? 0.f : 1.f / L;
-                const int64_t r = it.row0 + i;
-                for (int c = c0; c < c1; c++)
+                int64_t to[2]; // where the two rows start whose pieces this lane stores
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                {
+                    const int r = quad * 32 + (lane & ~1) + e, token = r * w.p.over_g >> 16;
+                    to[e] = r < rows ? (int64_t)(it.row0 + tok0 + token) * a.out_stride + (it.kvh * G + r - token * G) * YLM_HEAD_DIM : -1;
+                }
+#pragma unroll 1
+                for (int c = c0; c < c1; c++) // 16 dimensions
                 {
                     __syncwarp();
-                    float v[32];
-                    if (two)
-                        tmem_ld32(tO + 128u * ws + 32u * c, v);
-                    else
+                    float v[16], y[16];
+                    tmem_ld16_async(tO + (two ? 128u * ws : 0u) + 16u * c, v);
+                    if (both)
+                        tmem_ld16_async(tO + 128u + 16u * c, y);
+                    tmem_wait_ld16(v);
+                    if (!two)
                     {
-                        tmem_ld32(tO + 32u * c, v);
 #pragma unroll
-                        for (int e = 0; e < 32; e++)
+                        for (int e = 0; e < 16; e++)
                             v[e] *= f0;
                         if (both)
                         {
-                            float y[32];
-                            tmem_ld32(tO + 128u + 32u * c, y);
+                            tmem_wait_ld16(y);
 #pragma unroll
-                            for (int e = 0; e < 32; e++)
+                            for (int e = 0; e < 16; e++)
                                 v[e] = f1 == 0.f ? v[e] : fmaf(y[e], f1, v[e]);
                         }
                     }
-                    if (odd && row < rows)
+                    if (__builtin_expect(odd && row < rows, 0))
                     {
                         // what was taken out of the values that this row sees
                         const int lo = max(clear, it.tile0 * 128), hi = min(n + t, (it.tile0 + it.tiles) * 128);
+#pragma unroll 1
                         for (int k = lo; k < hi; k++)
                         {
                             const int page = seen(k) & 1u ? paged_page(st, a.c, it.s, k) : -1;
                             if (page < 0)
                                 continue;
                             const __half *src = a.c.v + paged_offset(a.c, page, k) +
-                                                (size_t)it.kvh * a.c.page * YLM_HEAD_DIM + 32 * c;
+                                                (size_t)it.kvh * a.c.page * YLM_HEAD_DIM + 16 * c;
 #pragma unroll
-                            for (int e = 0; e < 32; e++)
+                            for (int e = 0; e < 16; e++)
                             {
                                 const float x = h2f(src[e]);
                                 v[e] += x - x != 0.f ? x : 0.f; // (x - x is NaN)
                             }
                         }
                     }
-                    if (row < rows)
+                    if (whole)
                     {
-                        if (whole)
+                        // a row's 16 values are two 16-byte pieces; two lanes trade theirs, so that each stores its piece of
+                        // two rows and a store covers whole sectors
+                        uint4 x[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
                         {
-                            uint4 *dst = reinterpret_cast<uint4 *>(a.out + r * a.out_stride +
-                                                                   (it.kvh * G + row % G) * YLM_HEAD_DIM + 32 * c);
+                            __half2 h[4];
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                            {
-                                __half2 h[4];
-#pragma unroll
-                                for (int k = 0; k < 4; k++)
-                                    h[k] = __floats2half2_rn(v[8 * e + 2 * k] * inv, v[8 * e + 2 * k + 1] * inv);
-                                dst[e] = *reinterpret_cast<const uint4 *>(h);
-                            }
+                            for (int k = 0; k < 4; k++)
+                                h[k] = __floats2half2_rn(v[8 * e + 2 * k] * inv, v[8 * e + 2 * k + 1] * inv);
+                            x[e] = *reinterpret_cast<const uint4 *>(h);
                         }
-                        else
-                        {
-                            float4 *dst = reinterpret_cast<float4 *>(
-                                w.o + (((size_t)blockIdx.x * 2 + slot) * w.p.cap + rho) * YLM_HEAD_DIM + 32 * c);
+                        px_trade(x[0], x[1], lane);
 #pragma unroll
-                            for (int e = 0; e < 8; e++)
-                                dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                        }
+                        for (int e = 0; e < 2; e++)
+                            if (to[e] >= 0)
+                                *reinterpret_cast<uint4 *>(a.out + to[e] + 16 * c + 8 * (lane & 1)) = x[e];
+                    }
+                    else if (row < rows)
+                    {
+                        float4 *dst = w.o + (((size_t)blockIdx.x * 2 + slot) * 32 + 4 * c) * w.p.cap + rho;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            dst[(size_t)e * w.p.cap] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                     }
                 }
                 if (!whole && row < rows && c0 == 0)
@@ -1061,49 +1104,89 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
 }
 
 // ------------------------------------------------------------------ join
-// CTA b, for the item that share b starts inside of, where share b - 1 holds its start: rows blockIdx.y * 8 + warp, four
-// dimensions a lane. Launched as a programmatic dependent.
-constexpr int PJ_WARPS = 8;
+// CTA b, for the item that share b starts inside of, where share b - 1 holds its start: 32 rows of it (fewer where items
+// have fewer: then the lanes' upper bits count parts), a row a lane, and four dimensions a warp at a time.
+// Launched as a programmatic dependent.
+constexpr int PJ_WARPS = 8, PJ_ROWS = 32;
 
-__global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(const __grid_constant__ PagedPass w)
+__global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(const __grid_constant__ PagedPass w, const int rows_log)
 {
-    const int lane = threadIdx.x & 31, b = blockIdx.x + 1;
+    __shared__ __align__(16) __half tile[PJ_ROWS][YLM_HEAD_DIM + 8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x + 1;
+    const int row = lane & ((1 << rows_log) - 1), group = lane >> rows_log, groups = 32 >> rows_log;
     pdl_wait();
+    pdl_launch_dependents(); // a next call's CTAs may set themselves up beside these
     const PagedCut &c = w.cuts[b];
-    const long long u0 = c.u0;
+    const long long u0 = c.u0, each = c.each, more = c.more;
+    const PagedItem it = c.it;
     // share b - 1 has the units below
-    if (!c.cut || c.it.tile0 > c.each + (b - 1 < c.more))
+    if (!c.cut || it.tile0 > each + (b - 1 < more))
         return;
     const PagedAttnArgs &a = w.a;
-    const int tok0 = c.it.first, rows = min(w.p.tpi, c.it.t - tok0) * w.p.G;
-    const int rho = blockIdx.y * PJ_WARPS + (threadIdx.x >> 5);
-    if (rho >= rows)
+    const int G = w.p.G, rows = min(w.p.tpi, it.t - it.first) * G, row0 = blockIdx.y * PJ_ROWS, rho = row0 + row;
+    if (row0 >= rows)
         return;
     // part 0 is share b - 1's end, part k the start of share b - 1 + k; the last one has the item's last unit
-    const long long last = u0 - c.it.tile0 + c.it.units - 1, big = c.more * (c.each + 1);
-    const int parts = (int)(last < big ? px_div(last, (int)(c.each + 1)) : c.more + px_div(last - big, (int)c.each)) - b + 2;
-    const auto at = [&](int k) { return (size_t)((b - 1 + k) * 2 + (k == 0)) * w.p.cap + rho; };
+    const long long last = u0 - it.tile0 + it.units - 1, big = more * (each + 1);
+    const int parts = (int)(last < big ? px_div(last, (int)(each + 1)) : more + px_div(last - big, (int)each)) - b + 2;
+    const auto at = [&](int k) { return (size_t)(b - 1 + k) * 2 + (k == 0); };
+    const int in = min(rho, rows - 1); // (lanes without a row read another one's)
     float M = -INFINITY, L = 0.f;
-    for (int k = lane; k < parts; k += 32)
-        M = fmaxf(M, w.ml[at(k)].x);
-    M = warp_max(M);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int k = 0; k < parts; k++)
+    for (int k = group; k < parts; k += groups)
+        M = fmaxf(M, w.ml[at(k) * w.p.cap + in].x);
+    for (int o = 1 << rows_log; o < 32; o <<= 1)
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    constexpr int PER = 32 / PJ_WARPS;
+    float4 o[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = group; k < parts; k += groups)
     {
-        const float2 ml = w.ml[at(k)];
+        const float2 ml = w.ml[at(k) * w.p.cap + in];
         const float f = ml.x == -INFINITY ? 0.f : ex2_ftz((ml.x - M) * PX_SCALE);
-        const float4 x = *reinterpret_cast<const float4 *>(w.o + at(k) * YLM_HEAD_DIM + lane * 4);
         L += ml.y * f;
-        o.x += x.x * f;
-        o.y += x.y * f;
-        o.z += x.z * f;
-        o.w += x.w * f;
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+        {
+            const float4 x = w.o[(at(k) * 32 + warp + PJ_WARPS * i) * w.p.cap + in];
+            o[i].x += x.x * f;
+            o[i].y += x.y * f;
+            o[i].z += x.z * f;
+            o[i].w += x.w * f;
+        }
+    }
+    for (int s = 1 << rows_log; s < 32; s <<= 1)
+    {
+        L += __shfl_xor_sync(0xffffffffu, L, s);
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+        {
+            o[i].x += __shfl_xor_sync(0xffffffffu, o[i].x, s);
+            o[i].y += __shfl_xor_sync(0xffffffffu, o[i].y, s);
+            o[i].z += __shfl_xor_sync(0xffffffffu, o[i].z, s);
+            o[i].w += __shfl_xor_sync(0xffffffffu, o[i].w, s);
+        }
     }
     const float inv = M == -INFINITY ? 0.f : 1.f / L;
-    __half2 h[2] = {__floats2half2_rn(o.x * inv, o.y * inv), __floats2half2_rn(o.z * inv, o.w * inv)};
-    *reinterpret_cast<uint2 *>(a.out + (int64_t)(c.it.row0 + tok0 + rho / w.p.G) * a.out_stride +
-                               (c.it.kvh * w.p.G + rho % w.p.G) * YLM_HEAD_DIM + lane * 4) = *reinterpret_cast<const uint2 *>(h);
+    if (group == 0)
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+        {
+            const __half2 h[2] = {__floats2half2_rn(o[i].x * inv, o[i].y * inv), __floats2half2_rn(o[i].z * inv, o[i].w * inv)};
+            *reinterpret_cast<uint2 *>(&tile[row][4 * (warp + PJ_WARPS * i)]) = *reinterpret_cast<const uint2 *>(h);
+        }
+    __syncthreads();
+    // 16 lanes a row
+    for (int r = threadIdx.x >> 4; r < min(1 << rows_log, rows - row0); r += 2 * PJ_WARPS)
+    {
+        const int x = row0 + r;
+        *reinterpret_cast<uint4 *>(a.out + (int64_t)(it.row0 + it.first + x / G) * a.out_stride +
+                                   (it.kvh * G + x % G) * YLM_HEAD_DIM + (lane & 15) * 8) =
+            *reinterpret_cast<const uint4 *>(&tile[r][(lane & 15) * 8]);
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -1145,27 +1228,31 @@ cudaError_t paged_attn_launch(const PagedAttnArgs &a, void *ws, int num_sms, cud
     char *base = static_cast<char *>(ws);
     w.cuts = reinterpret_cast<PagedCut *>(base);
     w.ml = reinterpret_cast<float2 *>(base + w.p.ml_off);
-    w.o = reinterpret_cast<float *>(base + w.p.o_off);
+    w.o = reinterpret_cast<float4 *>(base + w.p.o_off);
     CUtensorMap qm, km, vm;
     if (!px_q_map(&qm, a, w.p) || !px_pool_map(&km, a.c.k, a.c) || !px_pool_map(&vm, a.c.v, a.c))
         return cudaErrorNotSupported;
-    if (w.p.pair)
-        paged_attn_kernel<true><<<w.p.ctas, PX_THREADS, PX_SMEM, s>>>(qm, km, vm, w);
-    else
-        paged_attn_kernel<false><<<w.p.ctas, PX_THREADS, PX_SMEM, s>>>(qm, km, vm, w);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || w.p.ctas < 2)
-        return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)w.p.ctas - 1, (unsigned)((w.p.cap + PJ_WARPS - 1) / PJ_WARPS));
-    cfg.blockDim = dim3(32 * PJ_WARPS);
-    cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)w.p.ctas);
+    cfg.blockDim = dim3(PX_THREADS);
+    cfg.dynamicSmemBytes = PX_SMEM;
+    cfg.stream = s;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_join_kernel, w);
+    const cudaError_t e = w.p.pair ? cudaLaunchKernelEx(&cfg, paged_attn_kernel<true>, qm, km, vm, w)
+                                   : cudaLaunchKernelEx(&cfg, paged_attn_kernel<false>, qm, km, vm, w);
+    if (e != cudaSuccess || w.p.ctas < 2)
+        return e;
+    int rows_log = 0;
+    while (1 << rows_log < std::min(w.p.cap, PJ_ROWS))
+        rows_log++;
+    cfg.gridDim = dim3((unsigned)w.p.ctas - 1, (unsigned)((w.p.cap + PJ_ROWS - 1) / PJ_ROWS));
+    cfg.blockDim = dim3(32 * PJ_WARPS);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, paged_join_kernel, w, rows_log);
 }
 
 cudaError_t paged_prepare()
