@@ -1104,89 +1104,133 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
 }
 
 // ------------------------------------------------------------------ join
-// CTA b, for the item that share b starts inside of, where share b - 1 holds its start: 32 rows of it (fewer where items
-// have fewer: then the lanes' upper bits count parts), a row a lane, and four dimensions a warp at a time.
-// Launched as a programmatic dependent.
+// A task is 32 rows (fewer where items have fewer: then the lanes' upper bits count parts), a row a lane, by PER times 32
+// dimensions, four a warp at a time. An item of few parts has tasks of 128 dimensions, one of many parts of 32, so that
+// about as many loads are under way. CTA x is at the border between shares x and x + 1; the CTAs at the borders inside
+// an item share its tasks. Launched as a programmatic dependent.
 constexpr int PJ_WARPS = 8, PJ_ROWS = 32;
+constexpr int PJ_FEW = 4; // parts
 
-__global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(const __grid_constant__ PagedPass w, const int rows_log)
+template <int PER, int BATCH>
+__device__ __forceinline__ void px_join(const PagedPass &w, const PagedItem &it, int first, int parts, int rows, int task,
+                                        int rows_log, __half (*tile)[YLM_HEAD_DIM + 8])
 {
-    __shared__ __align__(16) __half tile[PJ_ROWS][YLM_HEAD_DIM + 8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x + 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = lane & ((1 << rows_log) - 1), group = lane >> rows_log, groups = 32 >> rows_log;
-    pdl_wait();
-    pdl_launch_dependents(); // a next call's CTAs may set themselves up beside these
-    const PagedCut &c = w.cuts[b];
-    const long long u0 = c.u0, each = c.each, more = c.more;
-    const PagedItem it = c.it;
-    // share b - 1 has the units below
-    if (!c.cut || it.tile0 > each + (b - 1 < more))
-        return;
-    const PagedAttnArgs &a = w.a;
-    const int G = w.p.G, rows = min(w.p.tpi, it.t - it.first) * G, row0 = blockIdx.y * PJ_ROWS, rho = row0 + row;
-    if (row0 >= rows)
-        return;
-    // part 0 is share b - 1's end, part k the start of share b - 1 + k; the last one has the item's last unit
-    const long long last = u0 - it.tile0 + it.units - 1, big = more * (each + 1);
-    const int parts = (int)(last < big ? px_div(last, (int)(each + 1)) : more + px_div(last - big, (int)each)) - b + 2;
-    const auto at = [&](int k) { return (size_t)(b - 1 + k) * 2 + (k == 0); };
-    const int in = min(rho, rows - 1); // (lanes without a row read another one's)
+    const int row0 = task / (4 / PER) * PJ_ROWS, d0 = task % (4 / PER) * 32;
+    const int in = min(row0 + row, rows - 1); // (lanes without a row read another one's)
+    // part 0 is share `first`'s end, part k the start of share first + k
+    const auto at = [&](int k) { return (size_t)(first + k) * 2 + (k == 0); };
     float M = -INFINITY, L = 0.f;
-#pragma unroll 4
-    for (int k = group; k < parts; k += groups)
-        M = fmaxf(M, w.ml[at(k) * w.p.cap + in].x);
-    for (int o = 1 << rows_log; o < 32; o <<= 1)
-        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    constexpr int PER = 32 / PJ_WARPS;
     float4 o[PER];
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = group; k < parts; k += groups)
+    for (int d = 0; d < PER; d++)
+        o[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = group; k0 < parts; k0 += groups * BATCH)
     {
-        const float2 ml = w.ml[at(k) * w.p.cap + in];
-        const float f = ml.x == -INFINITY ? 0.f : ex2_ftz((ml.x - M) * PX_SCALE);
-        L += ml.y * f;
+        float2 ml[BATCH];
+        float4 x[BATCH][PER];
 #pragma unroll
-        for (int i = 0; i < PER; i++)
+        for (int i = 0; i < BATCH; i++)
         {
-            const float4 x = w.o[(at(k) * 32 + warp + PJ_WARPS * i) * w.p.cap + in];
-            o[i].x += x.x * f;
-            o[i].y += x.y * f;
-            o[i].z += x.z * f;
-            o[i].w += x.w * f;
+            ml[i] = make_float2(-INFINITY, 0.f);
+            const int k = k0 + i * groups;
+            if (k < parts)
+            {
+                ml[i] = w.ml[at(k) * w.p.cap + in];
+#pragma unroll
+                for (int d = 0; d < PER; d++)
+                    x[i][d] = w.o[(at(k) * 32 + d0 / 4 + warp + PJ_WARPS * d) * w.p.cap + in];
+            }
         }
+        float m = M;
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            m = fmaxf(m, ml[i].x);
+        float f = M == -INFINITY ? 0.f : ex2_ftz((M - m) * PX_SCALE);
+        M = m;
+        L *= f;
+#pragma unroll
+        for (int d = 0; d < PER; d++)
+            o[d] = make_float4(o[d].x * f, o[d].y * f, o[d].z * f, o[d].w * f);
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            if (ml[i].x != -INFINITY)
+            {
+                f = ex2_ftz((ml[i].x - M) * PX_SCALE);
+                L += ml[i].y * f;
+#pragma unroll
+                for (int d = 0; d < PER; d++)
+                {
+                    o[d].x += x[i][d].x * f;
+                    o[d].y += x[i][d].y * f;
+                    o[d].z += x[i][d].z * f;
+                    o[d].w += x[i][d].w * f;
+                }
+            }
     }
     for (int s = 1 << rows_log; s < 32; s <<= 1)
     {
-        L += __shfl_xor_sync(0xffffffffu, L, s);
+        const float m = __shfl_xor_sync(0xffffffffu, M, s), top = fmaxf(M, m);
+        const float f = M == -INFINITY ? 0.f : ex2_ftz((M - top) * PX_SCALE);
+        const float g = m == -INFINITY ? 0.f : ex2_ftz((m - top) * PX_SCALE);
+        M = top;
+        L = L * f + __shfl_xor_sync(0xffffffffu, L, s) * g;
 #pragma unroll
-        for (int i = 0; i < PER; i++)
+        for (int d = 0; d < PER; d++)
         {
-            o[i].x += __shfl_xor_sync(0xffffffffu, o[i].x, s);
-            o[i].y += __shfl_xor_sync(0xffffffffu, o[i].y, s);
-            o[i].z += __shfl_xor_sync(0xffffffffu, o[i].z, s);
-            o[i].w += __shfl_xor_sync(0xffffffffu, o[i].w, s);
+            o[d].x = o[d].x * f + __shfl_xor_sync(0xffffffffu, o[d].x, s) * g;
+            o[d].y = o[d].y * f + __shfl_xor_sync(0xffffffffu, o[d].y, s) * g;
+            o[d].z = o[d].z * f + __shfl_xor_sync(0xffffffffu, o[d].z, s) * g;
+            o[d].w = o[d].w * f + __shfl_xor_sync(0xffffffffu, o[d].w, s) * g;
         }
     }
     const float inv = M == -INFINITY ? 0.f : 1.f / L;
     if (group == 0)
 #pragma unroll
-        for (int i = 0; i < PER; i++)
+        for (int d = 0; d < PER; d++)
         {
-            const __half2 h[2] = {__floats2half2_rn(o[i].x * inv, o[i].y * inv), __floats2half2_rn(o[i].z * inv, o[i].w * inv)};
-            *reinterpret_cast<uint2 *>(&tile[row][4 * (warp + PJ_WARPS * i)]) = *reinterpret_cast<const uint2 *>(h);
+            const __half2 h[2] = {__floats2half2_rn(o[d].x * inv, o[d].y * inv), __floats2half2_rn(o[d].z * inv, o[d].w * inv)};
+            *reinterpret_cast<uint2 *>(&tile[row][4 * (warp + PJ_WARPS * d)]) = *reinterpret_cast<const uint2 *>(h);
         }
     __syncthreads();
-    // 16 lanes a row
-    for (int r = threadIdx.x >> 4; r < min(1 << rows_log, rows - row0); r += 2 * PJ_WARPS)
+    // 4 PER lanes a row
+    const int G = w.p.G;
+    for (int i = threadIdx.x; i < min(1 << rows_log, rows - row0) * 4 * PER; i += 32 * PJ_WARPS)
     {
-        const int x = row0 + r;
-        *reinterpret_cast<uint4 *>(a.out + (int64_t)(it.row0 + it.first + x / G) * a.out_stride +
-                                   (it.kvh * G + x % G) * YLM_HEAD_DIM + (lane & 15) * 8) =
-            *reinterpret_cast<const uint4 *>(&tile[r][(lane & 15) * 8]);
+        const int r = i / (4 * PER), p = i % (4 * PER), y = row0 + r;
+        *reinterpret_cast<uint4 *>(w.a.out + (int64_t)(it.row0 + it.first + y / G) * w.a.out_stride +
+                                   (it.kvh * G + y % G) * YLM_HEAD_DIM + d0 + p * 8) =
+            *reinterpret_cast<const uint4 *>(&tile[r][p * 8]);
     }
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(const __grid_constant__ PagedPass w, const int rows_log)
+{
+    __shared__ __align__(16) __half tile[PJ_ROWS][YLM_HEAD_DIM + 8];
+    const int b = blockIdx.x + 1;
+    pdl_wait();
+    pdl_launch_dependents(); // a next call's CTAs may set themselves up beside these
+    const PagedCut &c = w.cuts[b];
+    const long long each = c.each, more = c.more, start = c.u0 - c.it.tile0; // the item's first unit
+    const PagedItem it = c.it;
+    if (!c.cut)
+        return;
+    // the shares with the item's first and last units
+    const auto share = [&](long long u) {
+        const long long big = more * (each + 1);
+        return (int)(u < big ? px_div(u, (int)(each + 1)) : more + px_div(u - big, (int)each));
+    };
+    const int first = share(start), parts = share(start + it.units - 1) - first + 1;
+    const int rows = min(w.p.tpi, it.t - it.first) * w.p.G, blocks = (rows + PJ_ROWS - 1) / PJ_ROWS;
+    const int mine = b - first - 1 + (parts - 1) * blockIdx.y, step = (parts - 1) * gridDim.y;
+    if (parts <= PJ_FEW)
+        for (int task = mine; task < blocks; task += step)
+            px_join<4, 2>(w, it, first, parts, rows, task, rows_log, tile);
+    else
+        for (int task = mine; task < 4 * blocks; task += step)
+            px_join<1, 8>(w, it, first, parts, rows, task, rows_log, tile);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1249,6 +1293,7 @@ cudaError_t paged_attn_launch(const PagedAttnArgs &a, void *ws, int num_sms, cud
     int rows_log = 0;
     while (1 << rows_log < std::min(w.p.cap, PJ_ROWS))
         rows_log++;
+    // (a task of an item of few parts a CTA; 8 a border at most)
     cfg.gridDim = dim3((unsigned)w.p.ctas - 1, (unsigned)((w.p.cap + PJ_ROWS - 1) / PJ_ROWS));
     cfg.blockDim = dim3(32 * PJ_WARPS);
     cfg.dynamicSmemBytes = 0;
