@@ -105,7 +105,8 @@ int ylm_k_paged_append(const ylm_paged_cache *cache, const ylm_paged_step *step,
         (hq && (bad_rows(q, q_stride, hq) || bad_rows(q_out, q_out_stride, hq))))
         return refuse(YLM_INVALID_ARG,
                       "rows must be 16-byte aligned, their strides multiples of 8 halves that hold the heads");
-    if (prepare_device() != cudaSuccess)
+    const int sms = device_sms();
+    if (!sms || prepare_device() != cudaSuccess)
         return no_device();
     PagedAppendArgs a;
     a.c = to_kernel(*cache);
@@ -125,7 +126,7 @@ int ylm_k_paged_append(const ylm_paged_cache *cache, const ylm_paged_step *step,
     a.max_pos = max_pos;
     a.q_out = static_cast<__half *>(q_out);
     a.q_out_stride = q_out_stride;
-    return done(paged_append_launch(a, static_cast<cudaStream_t>(stream)));
+    return done(paged_append_launch(a, sms, static_cast<cudaStream_t>(stream)));
 }
 
 int ylm_k_paged_attention_workspace(const ylm_paged_cache *cache, const ylm_paged_step *step, int32_t hq, size_t *bytes)
@@ -238,10 +239,8 @@ int ylm_k_paged_accept(const ylm_paged_cache *cache, const ylm_paged_step *step,
         for (size_t j = i + 1; j < 4; j++)
             if (overlap(out[i].p, out[i].n, out[j].p, out[j].n))
                 return refuse(YLM_INVALID_ARG, "the results must not overlap one another");
-    if (prepare_device() != cudaSuccess)
-        return no_device();
     const int sms = device_sms();
-    if (!sms)
+    if (!sms || prepare_device() != cudaSuccess)
         return no_device();
     PagedAcceptArgs a;
     a.c = to_kernel(*cache);

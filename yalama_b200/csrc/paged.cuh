@@ -57,6 +57,26 @@ __device__ __forceinline__ int paged_find(const PagedStep &st, int r, int lane)
     }
 }
 
+// Warp-wide: the request that row r belongs to, and what it has; -1: none, or one that is left out. Up to 32
+// requests are looked at in one round of loads.
+__device__ __forceinline__ int paged_row(const PagedStep &st, int page, int r, int lane, PagedRequest &q)
+{
+    bool bad;
+    if (st.n_seq <= 32)
+    {
+        q.row0 = q.t = q.n = 0;
+        const bool mine = lane < st.n_seq && paged_request(st, page, lane, q, bad) && r >= q.row0 && r < q.row0 + q.t;
+        // (requests that share rows, as none should: the last one)
+        const int s = 31 - __clz(__ballot_sync(0xffffffffu, mine));
+        q.row0 = __shfl_sync(0xffffffffu, q.row0, max(s, 0));
+        q.t = __shfl_sync(0xffffffffu, q.t, max(s, 0));
+        q.n = __shfl_sync(0xffffffffu, q.n, max(s, 0));
+        return s;
+    }
+    const int s = paged_find(st, r, lane);
+    return s >= 0 && paged_request(st, page, s, q, bad) && r >= q.row0 && r < q.row0 + q.t ? s : -1;
+}
+
 // The page of slot j, or -1 where the table names none of the pool.
 __device__ __forceinline__ int paged_page(const PagedStep &st, const PagedCache &c, int s, int j)
 {

@@ -5,18 +5,51 @@
 
 namespace ylm {
 
+// Launched as programmatic dependents: they wait for what comes before them in the stream first thing.
+template <typename A>
+static cudaError_t paged_launch(void (*kernel)(const A), dim3 grid, int threads, cudaStream_t s, const A &a)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 // ------------------------------------------------------------------ append
 //   x' = x * rsqrt(mean(x^2) + eps) * w   (where there is a norm)
 //   y_d = x'_d cos_d - x'_{d+64} sin_d,  y_{d+64} = x'_{d+64} cos_d + x'_d sin_d   for d < 64
 // in FP32, rounded to FP16 once.
 constexpr int PA_THREADS = 256;
-constexpr int PA_HEADS = PA_THREADS / 16; // 16 lanes a head, 8 dimensions each
+constexpr int PA_HEADS = PA_THREADS / 16; // a pass: 16 lanes a head, 8 dimensions each
+constexpr int PA_BATCH = 4;               // passes whose loads are under way together
 
-__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedAppendArgs a)
+// A CTA takes every gridDim.y-th pass of one row. The rows' values are on their way while the request is looked up.
+__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ PagedAppendArgs a)
 {
-    const int lane = threadIdx.x & 31, l = threadIdx.x & 15;
-    const int r = blockIdx.x;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, l = threadIdx.x & 15, hw = threadIdx.x >> 4;
+    const int r = blockIdx.x, heads = a.hq + 2 * a.c.hkv;
     const PagedStep &st = a.st;
+    // head h of the row: query heads, then keys, then values
+    const auto load = [&](int h) {
+        const int is = h < a.hq ? 0 : h < a.hq + a.c.hkv ? 1 : 2;
+        const __half *src = is == 0 ? a.q + (int64_t)r * a.q_stride + h * YLM_HEAD_DIM
+                          : is == 1 ? a.k + (int64_t)r * a.k_stride + (h - a.hq) * YLM_HEAD_DIM
+                                    : a.v + (int64_t)r * a.v_stride + (h - a.hq - a.c.hkv) * YLM_HEAD_DIM;
+        return h < heads ? *reinterpret_cast<const uint4 *>(src + l * 8) : make_uint4(0, 0, 0, 0);
+    };
+    uint4 w[PA_BATCH];
+#pragma unroll
+    for (int k = 0; k < PA_BATCH; k++)
+        w[k] = load((blockIdx.y + k * gridDim.y) * PA_HEADS + hw);
+
     if (st.fault && blockIdx.y == 0)
         for (int64_t s = (int64_t)r * PA_THREADS + threadIdx.x; s < st.n_seq; s += (int64_t)gridDim.x * PA_THREADS)
         {
@@ -26,10 +59,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
             if (bad)
                 paged_fault(st, PAGED_BAD_REQUEST);
         }
-    const int s = paged_find(st, r, lane);
     PagedRequest q;
-    bool bad = false;
-    if (s < 0 || !paged_request(st, a.c.page, s, q, bad) || r < q.row0 || r >= q.row0 + q.t)
+    const int s = paged_row(st, a.c.page, r, lane, q);
+    if (s < 0)
         return;
     const int i = r - q.row0, slot = q.n + i;
     int pos = slot;
@@ -50,75 +82,91 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
     const int page = paged_page(st, a.c, s, slot);
     if (page < 0)
         paged_fault(st, PAGED_BAD_PAGE);
-    const int h = blockIdx.y * PA_HEADS + (threadIdx.x >> 4); // query heads, then keys, then values
-    const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.c.hkv, is = h < a.hq + 2 * a.c.hkv;
-    const int g = is_q ? h : is_k ? h - a.hq : h - a.hq - a.c.hkv;
-    const __half *src = is_q ? a.q + (int64_t)r * a.q_stride : is_k ? a.k + (int64_t)r * a.k_stride
-                                                                     : a.v + (int64_t)r * a.v_stride;
-    __half *dst = nullptr;
-    if (is_q)
-        dst = a.q_out + (int64_t)r * a.q_out_stride + g * YLM_HEAD_DIM;
-    else if (is && page >= 0)
-        dst = (is_k ? a.c.k : a.c.v) + paged_offset(a.c, page, slot) + (size_t)g * a.c.page * YLM_HEAD_DIM;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (is)
-        w = *reinterpret_cast<const uint4 *>(src + g * YLM_HEAD_DIM + l * 8);
-    // (every lane takes part in the shuffles, whatever its head is)
-    const __half *norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
-    const bool turn = a.rope_cos && (is_q || is_k);
-    if (__any_sync(0xffffffffu, norm != nullptr || turn))
+    const size_t at = page < 0 ? 0 : paged_offset(a.c, page, slot);
+    uint4 cw = make_uint4(0, 0, 0, 0), sw = cw;
+    if (a.rope_cos)
     {
-        float x[8];
-        unpack8(w, x);
-        float ss = 0.f;
+        const int64_t t = (int64_t)pos * 64 + (l & 7) * 8;
+        cw = *reinterpret_cast<const uint4 *>(a.rope_cos + t);
+        sw = *reinterpret_cast<const uint4 *>(a.rope_sin + t);
+    }
+    for (int p0 = blockIdx.y; p0 * PA_HEADS < heads; p0 += PA_BATCH * gridDim.y)
+    {
+        if (p0 != blockIdx.y)
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            ss += x[e] * x[e];
+            for (int k = 0; k < PA_BATCH; k++)
+                w[k] = load((p0 + k * gridDim.y) * PA_HEADS + hw);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1)
-            ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (norm)
+        for (int k = 0; k < PA_BATCH; k++)
         {
-            float nw[8];
-            unpack8(*reinterpret_cast<const uint4 *>(norm + l * 8), nw);
-            const float d = rsqrtf(ss * (1.0f / YLM_HEAD_DIM) + a.eps);
+            const int h = (p0 + k * gridDim.y) * PA_HEADS + hw;
+            const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.c.hkv;
+            // (every lane takes part in the shuffles, whatever its head is)
+            const __half *norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+            const bool turn = a.rope_cos && (is_q || is_k);
+            if (__any_sync(0xffffffffu, norm != nullptr || turn))
+            {
+                float x[8];
+                unpack8(w[k], x);
+                if (__any_sync(0xffffffffu, norm != nullptr))
+                {
+                    float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                x[e] = x[e] * d * nw[e];
-        }
-        float y[8];
+                    for (int e = 0; e < 8; e++)
+                        ss += x[e] * x[e];
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            y[e] = __shfl_xor_sync(0xffffffffu, x[e], 8);
-        if (turn)
-        {
-            float c[8], sn[8];
-            const int64_t at = (int64_t)pos * 64 + (l & 7) * 8;
-            unpack8(*reinterpret_cast<const uint4 *>(a.rope_cos + at), c);
-            unpack8(*reinterpret_cast<const uint4 *>(a.rope_sin + at), sn);
+                    for (int o = 8; o > 0; o >>= 1)
+                        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    if (norm)
+                    {
+                        float nw[8];
+                        unpack8(*reinterpret_cast<const uint4 *>(norm + l * 8), nw);
+                        const float d = rsqrtf(ss * (1.0f / YLM_HEAD_DIM) + a.eps);
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                x[e] = fmaf(x[e], c[e], l < 8 ? -y[e] * sn[e] : y[e] * sn[e]);
-        }
-        if (norm || turn)
-        {
-            __half2 *o = reinterpret_cast<__half2 *>(&w);
+                        for (int e = 0; e < 8; e++)
+                            x[e] = x[e] * d * nw[e];
+                    }
+                }
+                float y[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                o[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+                for (int e = 0; e < 8; e++)
+                    y[e] = __shfl_xor_sync(0xffffffffu, x[e], 8);
+                if (turn)
+                {
+                    float c[8], sn[8];
+                    unpack8(cw, c);
+                    unpack8(sw, sn);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        x[e] = fmaf(x[e], c[e], l < 8 ? -y[e] * sn[e] : y[e] * sn[e]);
+                }
+                if (norm || turn)
+                {
+                    __half2 *o = reinterpret_cast<__half2 *>(&w[k]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+                }
+            }
+            __half *dst = nullptr;
+            if (is_q)
+                dst = a.q_out + (int64_t)r * a.q_out_stride + h * YLM_HEAD_DIM;
+            else if (h < heads && page >= 0)
+                dst = (is_k ? a.c.k : a.c.v) + at + (size_t)(is_k ? h - a.hq : h - a.hq - a.c.hkv) * a.c.page * YLM_HEAD_DIM;
+            if (dst)
+                *reinterpret_cast<uint4 *>(dst + l * 8) = w[k];
         }
     }
-    if (dst)
-        *reinterpret_cast<uint4 *>(dst + l * 8) = w;
 }
 
-cudaError_t paged_append_launch(const PagedAppendArgs &a, cudaStream_t s)
+cudaError_t paged_append_launch(const PagedAppendArgs &a, int num_sms, cudaStream_t s)
 {
     if (a.st.rows <= 0 || a.st.n_seq <= 0)
         return cudaSuccess;
-    const int heads = a.hq + 2 * a.c.hkv;
-    paged_append_kernel<<<dim3((unsigned)a.st.rows, (unsigned)((heads + PA_HEADS - 1) / PA_HEADS)), PA_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    const int passes = (a.hq + 2 * a.c.hkv + PA_HEADS - 1) / PA_HEADS;
+    // few rows: a CTA a pass, so that more SMs take part
+    const int y = a.st.rows < num_sms ? std::min(passes, 65535) : 1;
+    return paged_launch(paged_append_kernel, dim3((unsigned)a.st.rows, (unsigned)y), PA_THREADS, s, a);
 }
 
 // ------------------------------------------------------------------ accept
@@ -130,11 +178,13 @@ constexpr int AC_THREADS = 128;
 constexpr int AC_HALF = AC_THREADS / 16;
 constexpr int AC_BATCH = 8; // rows in flight per 16 lanes
 
-__global__ void __launch_bounds__(AC_THREADS) paged_accept_kernel(const PagedAcceptArgs a)
+__global__ void __launch_bounds__(AC_THREADS) paged_accept_kernel(const __grid_constant__ PagedAcceptArgs a)
 {
     __shared__ int path[PAGED_TREE];
-    __shared__ int64_t from[PAGED_TREE], to[PAGED_TREE];
+    __shared__ int64_t from[PAGED_TREE], to[PAGED_TREE], picks[PAGED_TREE];
     __shared__ int count_s;
+    pdl_wait();
+    pdl_launch_dependents();
     const PagedStep &st = a.st;
     const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const bool writes = blockIdx.x == 0;
@@ -174,14 +224,20 @@ __global__ void __launch_bounds__(AC_THREADS) paged_accept_kernel(const PagedAcc
             int64_t token[PAGED_TREE / 32];
 #pragma unroll
             for (int k = 0; k < PAGED_TREE / 32; k++)
-                token[k] = lane + 32 * k < q.t ? a.tokens[q.row0 + lane + 32 * k] : 0;
+            {
+                const int i = lane + 32 * k;
+                token[k] = i < q.t ? a.tokens[q.row0 + i] : 0;
+                if (i < q.t)
+                    picks[i] = a.picks[q.row0 + i];
+            }
+            __syncwarp();
             int cur = 0, m = 0;
             for (;;)
             {
                 if (lane == 0)
                     path[m] = cur;
                 m++;
-                const int64_t pick = a.picks[q.row0 + cur];
+                const int64_t pick = picks[cur];
                 int next = -1;
 #pragma unroll
                 for (int k = PAGED_TREE / 32 - 1; k >= 0; k--)
@@ -252,8 +308,7 @@ cudaError_t paged_accept_launch(const PagedAcceptArgs &a, int num_sms, cudaStrea
     // about eight CTAs an SM at most, each with at least one round of moves
     const int64_t rounds = a.st.parent ? ((int64_t)2 * a.layers * a.c.hkv + AC_HALF - 1) / AC_HALF : 1;
     const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(rounds, (int64_t)num_sms * 8 / a.st.n_seq));
-    paged_accept_kernel<<<dim3((unsigned)slices, (unsigned)a.st.n_seq), AC_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    return paged_launch(paged_accept_kernel, dim3((unsigned)slices, (unsigned)a.st.n_seq), AC_THREADS, s, a);
 }
 
 } // namespace ylm

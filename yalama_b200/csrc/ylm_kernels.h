@@ -324,7 +324,7 @@ struct PagedAppendArgs
     __half *q_out;
     int64_t q_out_stride;
 };
-cudaError_t paged_append_launch(const PagedAppendArgs &a, cudaStream_t s);
+cudaError_t paged_append_launch(const PagedAppendArgs &a, int num_sms, cudaStream_t s);
 struct PagedAttnArgs
 {
     PagedCache c;
