@@ -27,9 +27,11 @@ static cudaError_t paged_launch(void (*kernel)(const A), dim3 grid, int threads,
 // in FP32, rounded to FP16 once.
 constexpr int PA_THREADS = 256;
 constexpr int PA_HEADS = PA_THREADS / 16; // a pass: 16 lanes a head, 8 dimensions each
-constexpr int PA_BATCH = 4;               // passes whose loads are under way together
 
-// A CTA takes every gridDim.y-th pass of one row. The rows' values are on their way while the request is looked up.
+// A CTA takes every gridDim.y-th pass of one row; the loads of BATCH passes are under way while the request is looked up.
+// BATCH covers the row where it can: 4522 rows of 80 heads 41 us with 5, 46 with 4 and one more behind them (4.5 TB/s; bound
+// by the lookup's chain of loads with four CTAs an SM).
+template <int BATCH>
 __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ PagedAppendArgs a)
 {
     pdl_wait();
@@ -45,9 +47,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
                                     : a.v + (int64_t)r * a.v_stride + (h - a.hq - a.c.hkv) * YLM_HEAD_DIM;
         return h < heads ? *reinterpret_cast<const uint4 *>(src + l * 8) : make_uint4(0, 0, 0, 0);
     };
-    uint4 w[PA_BATCH];
+    uint4 w[BATCH];
 #pragma unroll
-    for (int k = 0; k < PA_BATCH; k++)
+    for (int k = 0; k < BATCH; k++)
         w[k] = load((blockIdx.y + k * gridDim.y) * PA_HEADS + hw);
 
     if (st.fault && blockIdx.y == 0)
@@ -90,14 +92,14 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
         cw = *reinterpret_cast<const uint4 *>(a.rope_cos + t);
         sw = *reinterpret_cast<const uint4 *>(a.rope_sin + t);
     }
-    for (int p0 = blockIdx.y; p0 * PA_HEADS < heads; p0 += PA_BATCH * gridDim.y)
+    for (int p0 = blockIdx.y; p0 * PA_HEADS < heads; p0 += BATCH * gridDim.y)
     {
         if (p0 != blockIdx.y)
 #pragma unroll
-            for (int k = 0; k < PA_BATCH; k++)
+            for (int k = 0; k < BATCH; k++)
                 w[k] = load((p0 + k * gridDim.y) * PA_HEADS + hw);
 #pragma unroll
-        for (int k = 0; k < PA_BATCH; k++)
+        for (int k = 0; k < BATCH; k++)
         {
             const int h = (p0 + k * gridDim.y) * PA_HEADS + hw;
             const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.c.hkv;
@@ -166,7 +168,13 @@ cudaError_t paged_append_launch(const PagedAppendArgs &a, int num_sms, cudaStrea
     const int passes = (a.hq + 2 * a.c.hkv + PA_HEADS - 1) / PA_HEADS;
     // few rows: a CTA a pass, so that more SMs take part
     const int y = a.st.rows < num_sms ? std::min(passes, 65535) : 1;
-    return paged_launch(paged_append_kernel, dim3((unsigned)a.st.rows, (unsigned)y), PA_THREADS, s, a);
+    const dim3 grid((unsigned)a.st.rows, (unsigned)y);
+    const int batch = (passes + y - 1) / y;
+    return batch <= 1   ? paged_launch(paged_append_kernel<1>, grid, PA_THREADS, s, a)
+           : batch == 2 ? paged_launch(paged_append_kernel<2>, grid, PA_THREADS, s, a)
+           : batch == 3 ? paged_launch(paged_append_kernel<3>, grid, PA_THREADS, s, a)
+           : batch == 4 ? paged_launch(paged_append_kernel<4>, grid, PA_THREADS, s, a)
+                        : paged_launch(paged_append_kernel<5>, grid, PA_THREADS, s, a);
 }
 
 // ------------------------------------------------------------------ accept
