@@ -5,9 +5,8 @@
 //   o_r  = sum_j softmax(x_r)_j v_j,  0 where the row sees no slot
 //
 // An item is a request's KV head and up to tpi of its tokens: their G query heads each are the rows of one or two
-// tiles of 128 (row i * G + h). It has a unit for each 128 slots its tokens see, and PX_ITEM in front that stand for what it
-// costs beside them. The units of all items, in order, are
-// dealt evenly to one CTA per SM, so that requests of any lengths keep all SMs busy to the end; an item that
+// tiles of 128 (row i * G + h). It has a unit for each 128 slots its tokens see. The units of all items, in order, are
+// dealt evenly, by what they cost, to one CTA per SM, so that requests of any lengths keep all SMs busy to the end; an item that
 // a CTA border cuts leaves sums (M, l, O) per CTA, which paged_join_kernel joins.
 //
 // Both products run on the 5th-generation tensor cores, from two streams that take turns, so that one stream's softmax
@@ -31,10 +30,10 @@ namespace ylm {
 
 constexpr int PX_TILE = 128 * 128 * 2; // a tile of 128 rows or slots: two halves of 64 dimensions
 constexpr int PX_THREADS = 384;
-// What an item costs beside its units (its first loads, its sums' way out), in units, for the dealing.
-#ifndef PX_ITEM
-#define PX_ITEM 3
-#endif
+// What an item costs beside its units (its first loads, its sums' way out), for the dealing, where a unit of one tile
+// costs 1 and a unit of two tiles 2 (2050 and 3870 cycles). With 0, 1, 2, 3, 4: 48 requests of 20 to 9000 slots 57, 47, 41,
+// 39.5, 40 us.
+constexpr int PX_ITEM = 3;
 constexpr int PX_KST = 3;
 constexpr int PX_CONTROL = 3072; // barriers, the streams' (M, l)
 constexpr int PX_SMEM = 7 * PX_TILE + PX_CONTROL;
@@ -83,12 +82,14 @@ struct PagedItem
     int units;          // units of the item
 };
 
-// A CTA's share of the units, and its first item; left in the workspace for the join.
+// A CTA's share, as what the items and units in front of its borders cost together, and its first item; left in the
+// workspace for the join. Unit k of an item lies at zero + k * px_cost: it is the share's in which that is.
 struct PagedCut
 {
     long long u0, u1;
-    long long each, more; // every share has `each` units, the first `more` of them one more
-    long long left;       // units behind its part of the first item
+    long long each, more; // every share is `each` long, the first `more` of them one more; the rest are empty
+    long long left;       // what is behind its part of the first item
+    long long zero;       // where the first item's unit 0 lies
     PagedItem it;
     int cut;              // the share starts inside an item
 };
@@ -121,10 +122,17 @@ __device__ __noinline__ long long px_before(int n, int k, int tpi)
     return sum >> 7;
 }
 
-__device__ __forceinline__ long long px_request_units(const PagedRequest &r, int tpi, int hkv)
+// what a request's items and their units cost in front of token group k, for one KV head: all of its groups are full
+__device__ __forceinline__ long long px_front(int n, int k, const PagedPlan &p)
 {
-    const int last = r.t <= tpi ? 0 : (r.t - 1) / tpi;
-    return hkv * (px_before(r.n, last, tpi) + px_units(r.n, r.t, last, tpi) + (long long)PX_ITEM * (last + 1));
+    return (p.pair ? 2 : 1) * px_before(n, k, p.tpi) + (long long)PX_ITEM * k;
+}
+
+__device__ __forceinline__ long long px_request_cost(const PagedRequest &r, const PagedPlan &p, int hkv)
+{
+    const int last = r.t <= p.tpi ? 0 : (r.t - 1) / p.tpi;
+    return hkv * (px_front(r.n, last, p) + PX_ITEM +
+                  (r.t - last * p.tpi > p.tpt ? 2 : 1) * px_units(r.n, r.t, last, p.tpi));
 }
 
 // slots below are seen by every row of the item
@@ -133,6 +141,8 @@ __device__ __forceinline__ int px_open(const PagedPass &w, const PagedItem &it)
     return it.n + (w.a.st.parent ? (it.t == 1 ? 1 : 0) : it.first + 1);
 }
 __device__ __forceinline__ bool px_two(const PagedPass &w, const PagedItem &it) { return it.t - it.first > w.p.tpt; }
+
+__device__ __forceinline__ int px_cost(const PagedPass &w, const PagedItem &it) { return w.p.pair && px_two(w, it) ? 2 : 1; }
 
 // a / b for b > 0; nearly every step's numbers have 32 bits
 __device__ __forceinline__ long long px_div(long long a, int b)
@@ -144,7 +154,7 @@ __device__ __forceinline__ long long px_div(long long a, int b)
 struct PagedWalk
 {
     PagedItem it;
-    long long left; // units of the share behind this item
+    long long left; // what of the share is behind this item
     int base;       // ahead: requests base + lane
     PagedRequest ahead;
     bool there;
@@ -160,11 +170,13 @@ struct PagedWalk
         left = c.left;
         it = c.it;
         base = -1; // not yet looked ahead
+        if (it.tiles == 0)
+            next(w, lane);
     }
     __device__ __forceinline__ void next(const PagedPass &w, int lane)
     {
         it.tiles = 0;
-        left -= PX_ITEM;
+        left -= PX_ITEM; // (where the item goes on in the next share, left is below 0)
         if (left <= 0)
             return;
         it.tile0 = 0;
@@ -192,8 +204,9 @@ struct PagedWalk
             }
         }
         it.units = (it.n + min(it.t, it.first + w.p.tpi) + 127) >> 7;
-        it.tiles = (int)min((long long)it.units, left);
-        left -= it.tiles;
+        const int cost = px_cost(w, it);
+        it.tiles = (int)min((long long)it.units, (left + cost - 1) / cost);
+        left -= (long long)cost * it.units;
     }
 };
 
@@ -367,7 +380,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
             mbar_init(&item_full[i], 1);
             special[i] = 0;
         }
-        mine->u0 = mine->u1 = 0;
+        mine->left = 0; // an empty share
         mine->it.tiles = 0;
         fence_mbar_init();
         prefetch_tensormap(&qmap);
@@ -393,7 +406,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     {
         bool bad;
         if (paged_request(st, a.c.page, s, req, bad))
-            own += px_request_units(req, w.p.tpi, a.c.hkv);
+            own += px_request_cost(req, w.p, a.c.hkv);
         else if (bad && blockIdx.x == 0)
             paged_fault(st, PAGED_BAD_REQUEST);
     }
@@ -414,10 +427,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         total += sums[i];
         before += i < warp ? sums[i] : 0;
     }
-    // share b: units [b * each + min(b, more), + each + (b < more))
+    // share b: [b * each + min(b, more), + each + (b < more)); none so short that a unit of two tiles is longer
     const int b = blockIdx.x;
-    const long long each = px_div(total, (int)gridDim.x), over = total - each * gridDim.x;
-    const long long u0 = b * each + min((long long)b, over), u1 = u0 + each + (b < over);
+    const int shares = PAIR ? (int)max(1ll, min((long long)gridDim.x, total / 2)) : (int)gridDim.x;
+    const long long each = px_div(total, shares), over = total - each * shares;
+    const long long u0 = b < shares ? b * each + min((long long)b, over) : total;
+    const long long u1 = b < shares ? u0 + each + (b < over) : total;
     if (u0 >= before && u0 < before + own && u1 > u0)
     {
         long long rest = u0 - before;
@@ -428,7 +443,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                 bool bad;
                 if (!paged_request(st, a.c.page, s, req, bad))
                     continue;
-                const long long u = px_request_units(req, w.p.tpi, a.c.hkv);
+                const long long u = px_request_cost(req, w.p, a.c.hkv);
                 if (rest < u)
                     break;
                 rest -= u;
@@ -438,12 +453,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         while (hi - lo > 1)
         {
             const int mid = (lo + hi) / 2;
-            if (a.c.hkv * (px_before(req.n, mid, w.p.tpi) + (long long)PX_ITEM * mid) <= rest)
+            if (a.c.hkv * px_front(req.n, mid, w.p) <= rest)
                 lo = mid;
             else
                 hi = mid;
         }
-        rest -= a.c.hkv * (px_before(req.n, lo, w.p.tpi) + (long long)PX_ITEM * lo);
+        rest -= a.c.hkv * px_front(req.n, lo, w.p);
         PagedCut c;
         c.u0 = u0;
         c.u1 = u1;
@@ -455,12 +470,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         c.it.n = req.n;
         c.it.first = lo * w.p.tpi;
         c.it.units = px_units(req.n, req.t, lo, w.p.tpi);
-        c.it.kvh = (int)px_div(rest, c.it.units + PX_ITEM);
-        const int from = (int)(rest - (long long)c.it.kvh * (c.it.units + PX_ITEM)) - PX_ITEM; // below 0: in front of the item's units
-        c.it.tile0 = max(0, from);
-        c.it.tiles = (int)max(0ll, min((long long)c.it.units, u1 - u0 + from) - c.it.tile0);
-        c.left = u1 - u0 + from - c.it.tile0 - c.it.tiles;
-        c.cut = c.it.tile0 > 0;
+        const int cost = px_cost(w, c.it), all = PX_ITEM + cost * c.it.units;
+        c.it.kvh = (int)px_div(rest, all);
+        const int from = (int)(rest - (long long)c.it.kvh * all) - PX_ITEM; // from unit 0 to the share's start
+        const long long to = u1 - u0 + from;
+        c.zero = u0 - from;
+        c.it.tile0 = from <= 0 ? 0 : (from + cost - 1) / cost;
+        c.it.tiles = to <= 0 ? 0 : (int)min((long long)c.it.units, (to + cost - 1) / cost) - c.it.tile0;
+        c.left = to - (long long)cost * c.it.units;
+        c.cut = c.it.tile0 > 0 && c.it.tiles > 0;
         *mine = c;
         w.cuts[b] = c;
     }
@@ -1213,7 +1231,7 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(const __grid_
     pdl_wait();
     pdl_launch_dependents(); // a next call's CTAs may set themselves up beside these
     const PagedCut &c = w.cuts[b];
-    const long long each = c.each, more = c.more, start = c.u0 - c.it.tile0; // the item's first unit
+    const long long each = c.each, more = c.more;
     const PagedItem it = c.it;
     if (!c.cut)
         return;
@@ -1222,7 +1240,7 @@ __global__ void __launch_bounds__(32 * PJ_WARPS) paged_join_kernel(const __grid_
         const long long big = more * (each + 1);
         return (int)(u < big ? px_div(u, (int)(each + 1)) : more + px_div(u - big, (int)each));
     };
-    const int first = share(start), parts = share(start + it.units - 1) - first + 1;
+    const int first = share(c.zero), parts = share(c.zero + (long long)px_cost(w, it) * (it.units - 1)) - first + 1;
     const int rows = min(w.p.tpi, it.t - it.first) * w.p.G, blocks = (rows + PJ_ROWS - 1) / PJ_ROWS;
     const int mine = b - first - 1 + (parts - 1) * blockIdx.y, step = (parts - 1) * gridDim.y;
     if (parts <= PJ_FEW)
