@@ -30,10 +30,6 @@ namespace ylm {
 
 constexpr int PX_TILE = 128 * 128 * 2; // a tile of 128 rows or slots: two halves of 64 dimensions
 constexpr int PX_THREADS = 384;
-// What an item costs beside its units (its first loads, its sums' way out), for the dealing, where a unit of one tile
-// costs 1 and a unit of two tiles 2 (2050 and 3870 cycles). With 0, 1, 2, 3, 4: 48 requests of 20 to 9000 slots 57, 47, 41,
-// 39.5, 40 us.
-constexpr int PX_ITEM = 3;
 constexpr int PX_KST = 3;
 constexpr int PX_CONTROL = 3072; // barriers, the streams' (M, l)
 constexpr int PX_SMEM = 7 * PX_TILE + PX_CONTROL;
@@ -50,6 +46,7 @@ struct PagedPlan
     int pair;        // 1: items of two tiles (some request may have more than tpt rows)
     int box;         // tokens of a tile that are loaded: tpt, or fewer where no request has so many
     int cap;         // most rows of an item
+    int item;        // what an item costs beside its units, for the dealing
     int ctas;
     size_t ml_off, o_off, bytes;
 };
@@ -64,6 +61,10 @@ static PagedPlan paged_plan(const PagedAttnArgs &a, int num_sms)
     p.tpi = p.pair ? 2 * p.tpt : p.tpt;
     p.box = std::max(1, std::min(p.tpt, a.st.max_rows));
     p.cap = std::max(1, std::min(p.tpi, a.st.max_rows)) * p.G;
+    // An item's first loads and its sums' way out, where a unit of one tile costs 1 and a unit of two tiles 2 (2050 and
+    // 3870 cycles). Few rows, with 0, 1, 2, 3, 4: 48 requests of 20 to 9000 slots 57, 47, 41, 39.5, 40 us. More rows, with 3,
+    // 4, 5, 6: 32 trees 71, 67, 66, 64 us.
+    p.item = p.cap <= 32 ? 3 : 6;
     p.ctas = num_sms;
     p.ml_off = (size_t)p.ctas * PX_CUT;
     p.o_off = p.ml_off + ((size_t)p.ctas * 2 * p.cap * sizeof(float2) + 255) / 256 * 256;
@@ -125,14 +126,15 @@ __device__ __noinline__ long long px_before(int n, int k, int tpi)
 // what a request's items and their units cost in front of token group k, for one KV head: all of its groups are full
 __device__ __forceinline__ long long px_front(int n, int k, const PagedPlan &p)
 {
-    return (p.pair ? 2 : 1) * px_before(n, k, p.tpi) + (long long)PX_ITEM * k;
+    const int cost = p.pair ? 2 : 1;
+    return cost * px_before(n, k, p.tpi) + (long long)p.item * k;
 }
 
 __device__ __forceinline__ long long px_request_cost(const PagedRequest &r, const PagedPlan &p, int hkv)
 {
     const int last = r.t <= p.tpi ? 0 : (r.t - 1) / p.tpi;
-    return hkv * (px_front(r.n, last, p) + PX_ITEM +
-                  (r.t - last * p.tpi > p.tpt ? 2 : 1) * px_units(r.n, r.t, last, p.tpi));
+    const int cost = r.t - last * p.tpi > p.tpt ? 2 : 1;
+    return hkv * (px_front(r.n, last, p) + p.item + cost * px_units(r.n, r.t, last, p.tpi));
 }
 
 // slots below are seen by every row of the item
@@ -176,8 +178,7 @@ struct PagedWalk
     __device__ __forceinline__ void next(const PagedPass &w, int lane)
     {
         it.tiles = 0;
-        left -= PX_ITEM; // (where the item goes on in the next share, left is below 0)
-        if (left <= 0)
+        if (left <= 0) // (where the item goes on in the next share, left is below 0)
             return;
         it.tile0 = 0;
         if (++it.kvh == w.a.c.hkv)
@@ -205,7 +206,8 @@ struct PagedWalk
         }
         it.units = (it.n + min(it.t, it.first + w.p.tpi) + 127) >> 7;
         const int cost = px_cost(w, it);
-        it.tiles = (int)min((long long)it.units, (left + cost - 1) / cost);
+        left -= w.p.item;
+        it.tiles = left <= 0 ? 0 : (int)min((long long)it.units, (left + cost - 1) / cost);
         left -= (long long)cost * it.units;
     }
 };
@@ -470,9 +472,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         c.it.n = req.n;
         c.it.first = lo * w.p.tpi;
         c.it.units = px_units(req.n, req.t, lo, w.p.tpi);
-        const int cost = px_cost(w, c.it), all = PX_ITEM + cost * c.it.units;
+        const int cost = px_cost(w, c.it), all = w.p.item + cost * c.it.units;
         c.it.kvh = (int)px_div(rest, all);
-        const int from = (int)(rest - (long long)c.it.kvh * all) - PX_ITEM; // from unit 0 to the share's start
+        const int from = (int)(rest - (long long)c.it.kvh * all) - w.p.item; // from unit 0 to the share's start
         const long long to = u1 - u0 + from;
         c.zero = u0 - from;
         c.it.tile0 = from <= 0 ? 0 : (from + cost - 1) / cost;
