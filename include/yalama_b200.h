@@ -348,7 +348,8 @@ int ylm_k_kv8_evict(const ylm_kv8_cache *src, const ylm_kv8_cache *dst, const fl
  * model's picks are known (ylm_k_logprobs with n_top = 1: top_ids) accept.
  *
  * The cache of a layer is a pool of pages; a request's tokens [i * page, (i + 1) * page) lie on the
- * page that its row of the page table names. FP16, head dimension 128. Calls on one pool are
+ * page that its row of the page table names. Requests may share pages (a common prefix) that no step writes: all but
+ * those that hold slots from length[s] on. FP16, head dimension 128. Calls on one pool are
  * ordered by the caller (one stream, or events). */
 typedef struct ylm_paged_cache {
     void *k, *v;     /* [n_pages][hkv][page][128], 16-byte aligned */
@@ -397,7 +398,9 @@ int ylm_k_paged_append(const ylm_paged_cache *cache, const ylm_paged_step *step,
  * cached tokens, its ancestors and itself, scores scaled by 1 / sqrt(128). q, out: [rows][hq * 128] (strides as
  * above), RoPE applied; at most 128 query heads per KV head. Scores, softmax statistics and sums are FP32. A row that
  * sees no slot (its pages are not in the pool), or only scores of -inf, gets zeros; what hidden slots hold
- * does not matter, NaN and infinities either.
+ * does not matter, NaN and infinities either (an infinite value that a row sees makes its element infinite, or NaN where the
+ * slot's weight is below 2^-36 of the row's largest). Each weight is rounded to FP16 for the product with the values (by
+ * 2^-11 of itself; of weights below 2^-25 of the row's largest, by 2^-36 of that one), the result once more.
  * workspace: device memory of at least ylm_k_paged_attention_workspace bytes, 16-byte aligned, for this call alone
  * until it has run: calls that may overlap on the GPU, and graphs that may, need one each. null: allocated and
  * freed in stream order. */
@@ -405,7 +408,7 @@ int ylm_k_paged_attention(const ylm_paged_cache *cache, const ylm_paged_step *st
                           int32_t hq, void *out, int64_t out_stride, void *workspace, size_t workspace_bytes,
                           void *stream);
 /* Bytes of workspace that ylm_k_paged_attention needs on the current device for any step of this hq, hkv and
- * max_rows (or fewer). */
+ * max_rows (or fewer), whatever its requests, rows and lengths. */
 int ylm_k_paged_attention_workspace(const ylm_paged_cache *cache, const ylm_paged_step *step, int32_t hq,
                                     size_t *bytes);
 /* Accept drafted tokens. tokens[r] is row r's token, picks[r] the token that the model chose to follow it

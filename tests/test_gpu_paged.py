@@ -352,6 +352,13 @@ ATTENDS = [  # page, lengths, rows, trees, hq, hkv, pad
     (16, [1500, 3, 40, 800, 0, 9], [1, 64, 0, 1, 30, 2], None, 8, 2, 4),
     (64, [4000, 100], [1, 300], None, 8, 2, 0),
     (16, [i % 50 for i in range(1000)], [i % 2 for i in range(1000)], None, 2, 1, 0),
+    # many units and items for every CTA: short and long requests side by side
+    (16, [(i * 977) % 4001 for i in range(60)], [1] * 60, None, 14, 7, 2),
+    (64, [(i * 613) % 2500 for i in range(24)], [(i * 7) % 60 + 1 for i in range(24)], "random", 16, 4, 0),
+    (32, [(i * 613) % 2500 for i in range(24)], [(i * 5) % 27 + 1 for i in range(24)], "forest", 16, 4, 1),
+    (128, [40000, 3], [1, 2], None, 6, 2, 0),
+    (32, [700, 0, 2500], [400, 150, 333], None, 8, 2, 0),
+    (16, [30 * i for i in range(130)], [1 + i % 2 for i in range(130)], None, 4, 2, 0),
 ]
 
 
@@ -747,6 +754,52 @@ def test_one_graph_serves_steps_of_other_lengths_and_trees():
             np.testing.assert_array_equal(vals[s][1][n:], new[st.start[s]:st.start[s + 1], hq + hkv:])
         check(d, vals, q.cpu().numpy(), out)
         assert d.faults() == 0
+
+
+def test_graphs_with_a_workspace_each_and_an_eager_call_between():
+    rng = np.random.default_rng(21)
+    made = []
+    for i in range(2):
+        st = make(rng, 16, [900, 33, 200], [20, 60, 7], "random")
+        d = Device(st, 2)
+        vals = fill(rng, d)
+        q = rng.standard_normal((d.rows, 8, D)).astype(np.float16)
+        tokens, picks = ints(rng.integers(0, 3, d.rows), np.int64), ints(rng.integers(0, 3, d.rows), np.int64)
+        m = dict(d=d, vals=vals, q=q, dq=half(q), ws=workspace(d, 8), out=torch.full((d.rows, 8, D), 7.0, dtype=torch.float16, device="cuda"),
+                 tokens=tokens, picks=picks, graph=torch.cuda.CUDAGraph())
+        attend(d, m["dq"], 8, out=m["out"], ws=m["ws"])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(m["graph"]):
+            attend(d, m["dq"], 8, out=m["out"], ws=m["ws"])
+            m["res"] = accept(d, tokens, picks, 0)
+        made.append(m)
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for m, side in zip(made, sides):
+            m["out"].record_stream(side)
+            with torch.cuda.stream(side):
+                m["graph"].replay()
+        x = attend(made[0]["d"], made[0]["dq"], 8)  # meanwhile, on the current stream
+    torch.cuda.synchronize()
+    for m in made:
+        check(m["d"], m["vals"], m["q"], m["out"])
+        st = m["d"].step
+        for s in range(3):
+            a, b = int(st.start[s]), int(st.start[s + 1])
+            path = R.accept(st.parents(s), m["tokens"][a:b].cpu().numpy(), m["picks"][a:b].cpu().numpy())
+            assert m["res"]["accepted"][s, :len(path)].cpu().tolist() == path
+    check(made[0]["d"], made[0]["vals"], made[0]["q"], x)
+
+
+def test_a_workspace_for_max_rows_serves_steps_of_more_rows():
+    rng = np.random.default_rng(22)
+    d = Device(make(rng, 16, [300] * 12, [40] * 12, None), 2)
+    fill(rng, d)
+    big = E.paged_attention_workspace(d.cache, d.st, 8)
+    d.rows = 40
+    d.handle()
+    assert E.paged_attention_workspace(d.cache, d.st, 8) == big
 
 
 def test_two_streams_with_a_workspace_each():

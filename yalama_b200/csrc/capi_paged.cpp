@@ -143,6 +143,7 @@ int ylm_k_paged_attention_workspace(const ylm_paged_cache *cache, const ylm_page
     PagedAttnArgs a = {};
     a.c = to_kernel(*cache);
     a.st = to_kernel(*step);
+    a.st.max_rows = step->max_rows; // whatever `rows` a step of it will have
     a.hq = hq;
     *bytes = paged_attn_workspace(a, sms);
     return done(cudaSuccess);

@@ -1284,7 +1284,7 @@ static bool px_q_map(CUtensorMap *map, const PagedAttnArgs &a, const PagedPlan &
 
 cudaError_t paged_attn_launch(const PagedAttnArgs &a, void *ws, int num_sms, cudaStream_t s)
 {
-    if (a.st.rows <= 0 || a.st.n_seq <= 0 || a.st.max_rows <= 0)
+    if (a.st.rows <= 0 || a.st.n_seq <= 0)
         return cudaSuccess;
     PagedPass w;
     w.a = a;
