@@ -290,12 +290,12 @@ __device__ __forceinline__ void px_drain(uint64_t *bar, uint32_t parity)
         ;
 }
 
-__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z,
-                                            int32_t u, uint64_t *bar)
+__device__ __forceinline__ void tma_load_4d_hint(void *dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z,
+                                                 int32_t u, uint64_t *bar, uint64_t policy)
 {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(
                      smem_u32(dst)),
-                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_u32(bar))
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_u32(bar)), "l"(policy)
                  : "memory");
 }
 
@@ -314,13 +314,14 @@ __device__ __forceinline__ int px_page(const PagedPass &w, const PagedItem &it, 
 
 // A unit's K or V into a stage, from the pages that px_page gave (-1: zeros). Warp-wide.
 __device__ __forceinline__ void px_load(uint8_t *dst, const CUtensorMap *map, const PagedPass &w, int kvh, int page,
-                                        uint64_t *bar, int lane)
+                                        uint64_t *bar, uint64_t policy, int lane)
 {
     if (lane == 0)
         mbar_arrive_expect_tx(bar, PX_TILE);
     __syncwarp();
     if (lane >> 1 < 128 >> w.a.c.page_shift)
-        tma_load_4d(dst + (lane & 1) * (PX_TILE / 2) + (lane >> 1) * w.a.c.page * 128, map, (lane & 1) * 64, 0, kvh, page, bar);
+        tma_load_4d_hint(dst + (lane & 1) * (PX_TILE / 2) + (lane >> 1) * w.a.c.page * 128, map, (lane & 1) * 64, 0, kvh, page,
+                         bar, policy);
 }
 
 template <bool PAIR>
@@ -510,6 +511,13 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     // where no item has more (the products read 128 rows from there on, and nobody reads what comes of the others), or one.
     const int q_places = PAIR || w.p.cap <= 64 ? 2 : 1;
     const uint32_t q_step = PAIR ? PX_TILE : PX_TILE / 4;
+    // Where every request is one item a KV head, its K and V are read once, and the sums should stay in L2: 48 requests of 20
+    // to 9000 slots 36.8 us against 39.6 with the normal policy, 131071 slots 95 against 96.
+    uint64_t policy;
+    if (st.max_rows <= w.p.tpi)
+        policy = l2_policy_evict_first();
+    else
+        asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
 
     if (warp == 0)
     {
@@ -544,7 +552,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                     if (all)
                         paged_fault(st, PAGED_BAD_PAGE);
                 }
-                px_load(sk + s * PX_TILE, &kmap, w, it.kvh, page, &k_full[s], lane);
+                px_load(sk + s * PX_TILE, &kmap, w, it.kvh, page, &k_full[s], policy, lane);
                 page = px_page(w, it, it.tile0 + t + 1, lane, bad); // on its way while the next stage comes free
                 if (walk.base < 0)
                     walk.look(w, it.s + 1, lane);
@@ -603,7 +611,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                     ok = false;
                     break;
                 }
-                px_load(sv + s * PX_TILE, &vmap, w, it.kvh, page, &v_full[s], lane);
+                px_load(sv + s * PX_TILE, &vmap, w, it.kvh, page, &v_full[s], policy, lane);
                 page = px_page(w, it, it.tile0 + t + 1, lane, bad);
             }
         }
