@@ -25,32 +25,38 @@ static cudaError_t paged_launch(void (*kernel)(const A), dim3 grid, int threads,
 //   x' = x * rsqrt(mean(x^2) + eps) * w   (where there is a norm)
 //   y_d = x'_d cos_d - x'_{d+64} sin_d,  y_{d+64} = x'_{d+64} cos_d + x'_d sin_d   for d < 64
 // in FP32, rounded to FP16 once.
-constexpr int PA_THREADS = 256;
-constexpr int PA_HEADS = PA_THREADS / 16; // a pass: 16 lanes a head, 8 dimensions each
+constexpr int PA_THREADS = 128;
+constexpr int PA_HEADS = PA_THREADS / 8; // a pass: 8 lanes a head, 8 dimensions d and their partners d + 64 each
 
 // A CTA takes every gridDim.y-th pass of one row; the loads of BATCH passes are under way while the request is looked up.
-// BATCH covers the row where it can: 4522 rows of 80 heads 41 us with 5, 46 with 4 and one more behind them (4.5 TB/s; bound
-// by the lookup's chain of loads with four CTAs an SM).
+// With a dimension and its partner in one lane the rotation needs no exchange. Bound by HBM behind the lookup's chain of
+// loads, which eight CTAs an SM cover: 4522 rows of 80 heads 33.9 us = 5.5 TB/s (256 threads, four CTAs an SM 37.6 us; five
+// passes at a time, and fewer CTAs, 36 to 41 us; 16 lanes a head, with shuffles for the partners, 41 us). One row of 48
+// heads 2.3 us: the chain's latency.
 template <int BATCH>
-__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ PagedAppendArgs a)
+__global__ void __launch_bounds__(PA_THREADS, 8) paged_append_kernel(const __grid_constant__ PagedAppendArgs a)
 {
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, l = threadIdx.x & 15, hw = threadIdx.x >> 4;
+    const int lane = threadIdx.x & 31, l = threadIdx.x & 7, at_head = threadIdx.x >> 3;
     const int r = blockIdx.x, heads = a.hq + 2 * a.c.hkv;
     const PagedStep &st = a.st;
+    uint4 w[BATCH][2];
     // head h of the row: query heads, then keys, then values
-    const auto load = [&](int h) {
-        const int is = h < a.hq ? 0 : h < a.hq + a.c.hkv ? 1 : 2;
-        const __half *src = is == 0 ? a.q + (int64_t)r * a.q_stride + h * YLM_HEAD_DIM
-                          : is == 1 ? a.k + (int64_t)r * a.k_stride + (h - a.hq) * YLM_HEAD_DIM
-                                    : a.v + (int64_t)r * a.v_stride + (h - a.hq - a.c.hkv) * YLM_HEAD_DIM;
-        return h < heads ? *reinterpret_cast<const uint4 *>(src + l * 8) : make_uint4(0, 0, 0, 0);
+    const auto load = [&](int h, uint4(&x)[2]) {
+        const __half *src = h < a.hq             ? a.q + (int64_t)r * a.q_stride + h * YLM_HEAD_DIM
+                            : h < a.hq + a.c.hkv ? a.k + (int64_t)r * a.k_stride + (h - a.hq) * YLM_HEAD_DIM
+                                                 : a.v + (int64_t)r * a.v_stride + (h - a.hq - a.c.hkv) * YLM_HEAD_DIM;
+        x[0] = x[1] = make_uint4(0, 0, 0, 0);
+        if (h < heads)
+        {
+            x[0] = *reinterpret_cast<const uint4 *>(src + l * 8);
+            x[1] = *reinterpret_cast<const uint4 *>(src + 64 + l * 8);
+        }
     };
-    uint4 w[BATCH];
 #pragma unroll
     for (int k = 0; k < BATCH; k++)
-        w[k] = load((blockIdx.y + k * gridDim.y) * PA_HEADS + hw);
+        load((blockIdx.y + k * gridDim.y) * PA_HEADS + at_head, w[k]);
 
     if (st.fault && blockIdx.y == 0)
         for (int64_t s = (int64_t)r * PA_THREADS + threadIdx.x; s < st.n_seq; s += (int64_t)gridDim.x * PA_THREADS)
@@ -88,7 +94,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
     uint4 cw = make_uint4(0, 0, 0, 0), sw = cw;
     if (a.rope_cos)
     {
-        const int64_t t = (int64_t)pos * 64 + (l & 7) * 8;
+        const int64_t t = (int64_t)pos * 64 + l * 8;
         cw = *reinterpret_cast<const uint4 *>(a.rope_cos + t);
         sw = *reinterpret_cast<const uint4 *>(a.rope_sin + t);
     }
@@ -97,42 +103,44 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
         if (p0 != blockIdx.y)
 #pragma unroll
             for (int k = 0; k < BATCH; k++)
-                w[k] = load((p0 + k * gridDim.y) * PA_HEADS + hw);
+                load((p0 + k * gridDim.y) * PA_HEADS + at_head, w[k]);
 #pragma unroll
         for (int k = 0; k < BATCH; k++)
         {
-            const int h = (p0 + k * gridDim.y) * PA_HEADS + hw;
+            const int h = (p0 + k * gridDim.y) * PA_HEADS + at_head;
             const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.c.hkv;
-            // (every lane takes part in the shuffles, whatever its head is)
             const __half *norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
             const bool turn = a.rope_cos && (is_q || is_k);
-            if (__any_sync(0xffffffffu, norm != nullptr || turn))
+            // (every lane takes part in the shuffles, whatever its head is)
+            const bool any_norm = __any_sync(0xffffffffu, norm != nullptr);
+            if (any_norm || turn)
             {
-                float x[8];
-                unpack8(w[k], x);
-                if (__any_sync(0xffffffffu, norm != nullptr))
+                float x[8], y[8];
+                unpack8(w[k][0], x);
+                unpack8(w[k][1], y);
+                if (any_norm)
                 {
                     float ss = 0.f;
 #pragma unroll
                     for (int e = 0; e < 8; e++)
-                        ss += x[e] * x[e];
+                        ss += x[e] * x[e] + y[e] * y[e];
 #pragma unroll
-                    for (int o = 8; o > 0; o >>= 1)
+                    for (int o = 4; o > 0; o >>= 1)
                         ss += __shfl_xor_sync(0xffffffffu, ss, o);
                     if (norm)
                     {
-                        float nw[8];
-                        unpack8(*reinterpret_cast<const uint4 *>(norm + l * 8), nw);
+                        float nx[8], ny[8];
+                        unpack8(*reinterpret_cast<const uint4 *>(norm + l * 8), nx);
+                        unpack8(*reinterpret_cast<const uint4 *>(norm + 64 + l * 8), ny);
                         const float d = rsqrtf(ss * (1.0f / YLM_HEAD_DIM) + a.eps);
 #pragma unroll
                         for (int e = 0; e < 8; e++)
-                            x[e] = x[e] * d * nw[e];
+                        {
+                            x[e] = x[e] * d * nx[e];
+                            y[e] = y[e] * d * ny[e];
+                        }
                     }
                 }
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    y[e] = __shfl_xor_sync(0xffffffffu, x[e], 8);
                 if (turn)
                 {
                     float c[8], sn[8];
@@ -140,14 +148,21 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
                     unpack8(sw, sn);
 #pragma unroll
                     for (int e = 0; e < 8; e++)
-                        x[e] = fmaf(x[e], c[e], l < 8 ? -y[e] * sn[e] : y[e] * sn[e]);
+                    {
+                        const float u = x[e];
+                        x[e] = fmaf(u, c[e], -y[e] * sn[e]);
+                        y[e] = fmaf(y[e], c[e], u * sn[e]);
+                    }
                 }
                 if (norm || turn)
                 {
-                    __half2 *o = reinterpret_cast<__half2 *>(&w[k]);
+                    __half2 *ox = reinterpret_cast<__half2 *>(&w[k][0]), *oy = reinterpret_cast<__half2 *>(&w[k][1]);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        o[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+                    {
+                        ox[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+                        oy[e] = __floats2half2_rn(y[2 * e], y[2 * e + 1]);
+                    }
                 }
             }
             __half *dst = nullptr;
@@ -156,7 +171,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
             else if (h < heads && page >= 0)
                 dst = (is_k ? a.c.k : a.c.v) + at + (size_t)(is_k ? h - a.hq : h - a.hq - a.c.hkv) * a.c.page * YLM_HEAD_DIM;
             if (dst)
-                *reinterpret_cast<uint4 *>(dst + l * 8) = w[k];
+            {
+                *reinterpret_cast<uint4 *>(dst + l * 8) = w[k][0];
+                *reinterpret_cast<uint4 *>(dst + 64 + l * 8) = w[k][1];
+            }
         }
     }
 }
@@ -172,9 +190,7 @@ cudaError_t paged_append_launch(const PagedAppendArgs &a, int num_sms, cudaStrea
     const int batch = (passes + y - 1) / y;
     return batch <= 1   ? paged_launch(paged_append_kernel<1>, grid, PA_THREADS, s, a)
            : batch == 2 ? paged_launch(paged_append_kernel<2>, grid, PA_THREADS, s, a)
-           : batch == 3 ? paged_launch(paged_append_kernel<3>, grid, PA_THREADS, s, a)
-           : batch == 4 ? paged_launch(paged_append_kernel<4>, grid, PA_THREADS, s, a)
-                        : paged_launch(paged_append_kernel<5>, grid, PA_THREADS, s, a);
+                        : paged_launch(paged_append_kernel<3>, grid, PA_THREADS, s, a);
 }
 
 // ------------------------------------------------------------------ accept
