@@ -22,6 +22,20 @@
 // A hidden slot's weight is 0, but 0 x NaN is not: where some row of an item does not see some slot (the last
 // units), warp 3 sets what is not finite in those rows of V to 0 before the product, and says so where the slot is one of the
 // step's; the rows that do see it then get it added at the end. Scores of hidden slots are replaced, whatever they are.
+//
+// Measured (B200, 32 / 8 heads but where noted, device time in a captured graph, join included):
+//   one token over 131071 slots: 96 us = 5.6 TB/s. The CTAs end after 74 to 89 us, as HBM serves them.
+//   48 requests of 20 to 9000 slots (28 / 4 heads) 37 us, 32 trees of 9 to 45 tokens over 300 to 5000 slots 62 us: a unit of one
+//   tile takes 2050 cycles, one of two 3870, and an item some 5500 beside its units.
+//   a tree of 64 tokens over 8200 slots: 30 us, the attention's CTAs ending after 14 to 20; partial sums of 19 MB are joined.
+//   2049 rows behind 6145 slots: 251 us = 960 TFLOP/s. A stream's unit is 2000 cycles of softmax (a quarter of it maxima) and
+//   1900 of hand-over and products, with the other stream's in between: tensor pipe 48 %, exponential unit 47 % of the time.
+//   611 slots: 12.4 us, one unit a CTA: in a CTA's 15800 cycles the share takes 4100, the item and its first
+//   loads 3500, S 900, the weights 2800, the product 1200, the way out 3200. The rest is the join.
+// Tried and slower, the 2049 rows: all 128 scores of a row unrolled (380 us, registers spilled), the reference taken from the
+// tile before (342, code beyond the instruction cache), two threads a row (271 against 259: an SM quarter's two warps
+// share its exponential unit), a quarter or half of the exponentials by polynomial (263 and 281 against 261), units of 64 slots with two S a
+// stream (358: twice the commits and waits of the issuing warp).
 #include "paged.cuh"
 #include "ylm_tc.cuh"
 #include <algorithm>
@@ -31,7 +45,7 @@ namespace ylm {
 constexpr int PX_TILE = 128 * 128 * 2; // a tile of 128 rows or slots: two halves of 64 dimensions
 constexpr int PX_THREADS = 384;
 constexpr int PX_KST = 3;
-constexpr int PX_CONTROL = 3072; // barriers, the streams' (M, l)
+constexpr int PX_CONTROL = 3 * 1024; // barriers, the streams' (M, l)
 constexpr int PX_SMEM = 7 * PX_TILE + PX_CONTROL;
 constexpr int PX_CUT = 128; // bytes of a PagedCut
 constexpr float PX_SCALE = (float)(1.4426950408889634 / 11.313708498984760); // log2(e) / sqrt(128)

@@ -198,6 +198,10 @@ cudaError_t paged_append_launch(const PagedAppendArgs &a, int num_sms, cudaStrea
 // path only rise, so path[j] >= j: moved in order, no slot is overwritten before it has been read.
 // Each CTA of a request walks for itself (a warp, a shuffle and four ballots a step) and then moves its share of the
 // 2 * layers * hkv rows of 256 bytes that an accepted token has, 16 lanes each.
+// 60 trees of 50 to 64 tokens, 32 layers of 8 heads: 11.8 us = 3.4 TB/s: 2.6 when no draft is accepted, 3.9 with the moves
+// of one layer, so most of it is the moves, rows of 256 bytes apart from one another. 28 layers of 4 heads, one tree of 8: 3.5 us, of
+// which 2.3 are there without an accepted draft. CTAs an SM by threads, 60 trees: 8 x 128 11.9 us, 4 x 128 15.2, 16 x 128 12.6,
+// 4 x 256 12.1, 8 x 256 12.7, 16 x 64 12.4.
 constexpr int AC_THREADS = 128;
 constexpr int AC_HALF = AC_THREADS / 16;
 constexpr int AC_BATCH = 8; // rows in flight per 16 lanes
