@@ -116,6 +116,13 @@ def test_accept_refuses_results_over_the_parents():
     assert accept(st=step(parent=6 * A), new=6 * A + 76) == INV
 
 
+@pytest.mark.parametrize("parent", [None, 6 * A])
+def test_accept_without_rows_needs_its_results_all_the_same(parent):
+    """max_rows entries a request are written, whatever the rows."""
+    assert accept(st=step(rows=0, parent=parent), tokens=None, picks=None, acc=None) == INV
+    assert b"output" in E.lib().ylm_last_error()
+
+
 def test_nothing_to_do_is_fine():
     for st in (step(n_seq=0, row_start=None, length=None, page_table=None), step(n_seq=0, rows=0, table_ld=0)):
         assert append(st=st, q=None, k=None, v=None, out=None) == OK

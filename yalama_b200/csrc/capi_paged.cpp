@@ -215,7 +215,7 @@ int ylm_k_paged_accept(const ylm_paged_cache *cache, const ylm_paged_step *step,
         return done(cudaSuccess);
     if ((step->rows && (!tokens || !picks)) || !aligned(tokens, 8) || !aligned(picks, 8))
         return refuse(YLM_INVALID_ARG, "tokens and picks must be 8-byte aligned");
-    if ((step->rows && step->max_rows && !accepted) || !n_accepted || !next_token || !new_length || !aligned(accepted, 4) ||
+    if ((step->max_rows && !accepted) || !n_accepted || !next_token || !new_length || !aligned(accepted, 4) ||
         !aligned(n_accepted, 4) || !aligned(next_token, 8) || !aligned(new_length, 4))
         return refuse(YLM_INVALID_ARG, "null or misaligned output");
     const PagedStep st = to_kernel(*step);
