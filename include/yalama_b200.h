@@ -352,7 +352,7 @@ int ylm_k_kv8_evict(const ylm_kv8_cache *src, const ylm_kv8_cache *dst, const fl
  * those that hold slots from length[s] on. FP16, head dimension 128. Calls on one pool are
  * ordered by the caller (one stream, or events). */
 typedef struct ylm_paged_cache {
-    void *k, *v;     /* [n_pages][hkv][page][128], 16-byte aligned */
+    void *k, *v;     /* [n_pages][hkv][page][128], 16-byte aligned, not overlapping */
     int32_t n_pages;
     int32_t page;    /* tokens a page: 16, 32, 64 or 128 */
     int32_t hkv;     /* KV heads */
@@ -389,14 +389,15 @@ typedef enum ylm_step_fault {
  * fused projection will do; multiples of 8, pointers 16-byte aligned); row r's head h at q + r * q_stride + h * 128.
  * q_norm, k_norm [128] or null: per-head RMSNorm with eps; rope_cos, rope_sin [max_pos][64] FP16, or both null: no
  * rotation. Both in FP32 and rounded once (the engine's own step rounds after every operation, as the reference does:
- * values differ by FP16 steps). q_out [rows][hq * 128], which may be q; hq = 0: keys and values alone. */
+ * values differ by FP16 steps). q_out [rows][hq * 128] is q, with its stride, or does not overlap q, k
+ * and v; hq = 0: keys and values alone. */
 int ylm_k_paged_append(const ylm_paged_cache *cache, const ylm_paged_step *step, const void *q, int64_t q_stride,
                        const void *k, int64_t k_stride, const void *v, int64_t v_stride, int32_t hq,
                        const void *q_norm, const void *k_norm, float eps, const void *rope_cos, const void *rope_sin,
                        int32_t max_pos, void *q_out, int64_t q_out_stride, void *stream);
 /* Attention of the step's rows, whose keys and values have been appended: row i of a request sees the request's
  * cached tokens, its ancestors and itself, scores scaled by 1 / sqrt(128). q, out: [rows][hq * 128] (strides as
- * above), RoPE applied; at most 128 query heads per KV head. Scores, softmax statistics and sums are FP32. A row that
+ * above; out does not overlap q), RoPE applied; at most 128 query heads per KV head. Scores, softmax statistics and sums are FP32. A row that
  * sees no slot (its pages are not in the pool), or only scores of -inf, gets zeros; what hidden slots hold
  * does not matter, NaN and infinities either (an infinite value that a row sees makes its element infinite, or NaN where the
  * slot's weight is below 2^-36 of the row's largest). Each weight is rounded to FP16 for the product with the values (by
@@ -416,7 +417,7 @@ int ylm_k_paged_attention_workspace(const ylm_paged_cache *cache, const ylm_page
  * row 0 is accepted, then the lowest child of the last accepted row whose token is that row's pick, and so on;
  * accepted [n_seq][max_rows]: these rows, -1 behind; n_accepted; next_token: the last one's pick;
  * new_length = length + n_accepted. The keys and values of accepted row number j move to slot length + j, in `layers`
- * layers whose pools lie layer_stride halves apart from cache's on (0 layers: none); the slots behind new_length hold
+ * layers whose pools lie layer_stride halves apart from cache's on, none over another (0 layers: none); the slots behind new_length hold
  * anything then. A request without rows, or left out: 0 accepted, next_token -1, its length. The results
  * must not overlap the step, the tokens or the picks. */
 int ylm_k_paged_accept(const ylm_paged_cache *cache, const ylm_paged_step *step, const int64_t *tokens,

@@ -3,6 +3,7 @@ no GPU. The pointers are placeholders that nothing reads."""
 import ctypes
 
 import pytest
+import torch
 
 from yalama_b200 import engine as E
 
@@ -46,8 +47,10 @@ def accept(c=None, st=None, tokens=14 * A, picks=15 * A, layers=2, stride=16 * A
                                       stride, acc, n, nxt, new, None)
 
 
+LAYER_BYTES = 50 * 2 * 16 * 128 * 2  # of the placeholder cache
 BAD_CACHES = [dict(k=None), dict(v=None), dict(k=A + 8), dict(v=A + 2), dict(page=0), dict(page=8), dict(page=48),
               dict(page=256), dict(page=-16), dict(n_pages=0), dict(n_pages=-1), dict(hkv=0), dict(hkv=65536)]
+BAD_CACHES += [dict(v=A), dict(v=A + LAYER_BYTES - 16), dict(k=2 * A + 16)]
 BAD_STEPS = [dict(row_start=None), dict(length=None), dict(page_table=None), dict(row_start=A + 2), dict(length=A + 1),
              dict(page_table=A + 3), dict(parent=A + 2), dict(fault=A + 1), dict(n_seq=-1), dict(n_seq=65536),
              dict(table_ld=0), dict(table_ld=-3), dict(table_ld=(1 << 26) + 1), dict(table_ld=2 ** 31 - 1), dict(rows=-1),
@@ -99,6 +102,43 @@ def test_attention_workspace_refuses(hq):
     assert size(hq=hq) == INV
 
 
+Q = 8 * A  # where the queries of append() and attend() lie: 20 rows of 512 halves
+
+
+# (addresses are bytes: a row of 512 halves is 1024 of them)
+@pytest.mark.parametrize("bad", [dict(out=Q, os=520), dict(out=Q + 16), dict(out=Q + 1024), dict(out=Q - 1024),
+                                 dict(out=Q + 19 * 1024 + 1008), dict(out=9 * A + 512), dict(out=10 * A + 19 * 512),
+                                 # a fused projection of 4 + 2 + 2 heads: the keys' and the values' columns
+                                 dict(qs=1024, k=Q + 1024, ks=1024, v=Q + 1536, vs=1024, out=Q + 1024, os=1024),
+                                 dict(qs=1024, k=Q + 1024, ks=1024, v=Q + 1536, vs=1024, out=Q + 512, os=1024),
+                                 dict(qs=1024, k=Q + 1024, ks=1024, v=Q + 1536, vs=1024, out=Q, os=512),
+                                 dict(qs=1024, k=Q + 1024, ks=1024, v=Q + 1536, vs=1024, out=Q + 2048, os=1024)], ids=str)
+def test_append_refuses_queries_out_over_other_rows(bad):
+    assert append(**bad) == INV
+    assert b"overlap" in E.lib().ylm_last_error()
+
+
+# (what is not refused stops at the device, which is not looked for before every check has passed)
+@pytest.mark.parametrize("good", [dict(out=Q), dict(out=Q + 20 * 1024), dict(out=Q - 20 * 1024),
+                                  dict(qs=1024, k=Q + 1024, ks=1024, v=Q + 1536, vs=1024, out=Q, os=1024)], ids=str)
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are placeholders")
+def test_append_takes_queries_out_in_place_or_elsewhere(good):
+    assert append(**good) not in (INV, OK)
+
+
+@pytest.mark.parametrize("bad", [dict(out=Q), dict(out=Q + 1024), dict(out=Q, os=520), dict(out=Q - 19 * 1024 - 16),
+                                 dict(qs=1024, out=Q + 512, os=1024)], ids=str)
+def test_attention_refuses_out_over_the_queries(bad):
+    assert attend(**bad) == INV
+    assert b"overlap" in E.lib().ylm_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are placeholders")
+@pytest.mark.parametrize("good", [dict(out=Q + 20 * 1024), dict(qs=1024, out=Q + 1024, os=1024)], ids=str)
+def test_attention_takes_columns_beside_the_queries(good):
+    assert attend(**good) not in (INV, OK)
+
+
 LAYER = 50 * 2 * 16 * 128  # halves of the placeholder cache's layer
 
 
@@ -110,6 +150,11 @@ LAYER = 50 * 2 * 16 * 128  # halves of the placeholder cache's layer
                                  dict(nxt=16 * A + 88)], ids=str)
 def test_accept_refuses(bad):
     assert accept(**bad) == INV
+
+
+def test_accept_refuses_a_layers_keys_over_another_layers_values():
+    assert accept(stride=A // 2) == INV  # layer 1's keys lie where layer 0's values do
+    assert b"overlap" in E.lib().ylm_last_error()
 
 
 def test_accept_refuses_results_over_the_parents():

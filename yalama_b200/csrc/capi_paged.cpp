@@ -13,6 +13,21 @@ static_assert(YLM_STEP_BAD_REQUEST == 1 && YLM_STEP_BAD_PAGE == 2 && YLM_STEP_BA
 
 namespace {
 
+// Whether some of n rows of wa halves at a, sa halves apart, share memory with some of n rows of wb at b.
+bool rows_overlap(const void *a, int64_t sa, int64_t wa, const void *b, int64_t sb, int64_t wb, int64_t n)
+{
+    if (n <= 0 || wa <= 0 || wb <= 0)
+        return false;
+    using Wide = __int128; // a stride can be anything
+    const Wide x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    if (x >= y + 2 * ((Wide)(n - 1) * sb + wb) || y >= x + 2 * ((Wide)(n - 1) * sa + wa))
+        return false;
+    if (sa != sb || n == 1)
+        return true; // (rows of other strides inside one another: none that can be told apart simply)
+    const Wide pitch = 2 * (Wide)sa, d = ((y - x) % pitch + pitch) % pitch; // columns of the same rows
+    return d < 2 * wa || d + 2 * wb > pitch;
+}
+
 // Null when the cache and the step can be used, else what is wrong with them.
 const char *step_fault(const ylm_paged_cache *c, const ylm_paged_step *st)
 {
@@ -24,6 +39,9 @@ const char *step_fault(const ylm_paged_cache *c, const ylm_paged_step *st)
         return "a page must be 16, 32, 64 or 128 tokens";
     if (c->n_pages <= 0 || c->hkv <= 0 || c->hkv > 65535)
         return "cache needs 1 page at least and 1..65535 KV heads";
+    const int64_t layer = (int64_t)c->n_pages * c->hkv * c->page * YLM_HEAD_DIM;
+    if (rows_overlap(c->k, layer, layer, c->v, layer, layer, 1))
+        return "keys and values must not overlap";
     if (!st)
         return "null step";
     if (st->n_seq < 0 || st->n_seq > 65535 || st->rows < 0 || st->max_rows < 0)
@@ -105,6 +123,12 @@ int ylm_k_paged_append(const ylm_paged_cache *cache, const ylm_paged_step *step,
         (hq && (bad_rows(q, q_stride, hq) || bad_rows(q_out, q_out_stride, hq))))
         return refuse(YLM_INVALID_ARG,
                       "rows must be 16-byte aligned, their strides multiples of 8 halves that hold the heads");
+    // a row's blocks read and write their own heads, at any time before or after another row's
+    const int64_t wq = (int64_t)hq * YLM_HEAD_DIM, wk = (int64_t)cache->hkv * YLM_HEAD_DIM;
+    if (((q_out != q || q_out_stride != q_stride) && rows_overlap(q_out, q_out_stride, wq, q, q_stride, wq, step->rows)) ||
+        rows_overlap(q_out, q_out_stride, wq, k, k_stride, wk, step->rows) ||
+        rows_overlap(q_out, q_out_stride, wq, v, v_stride, wk, step->rows))
+        return refuse(YLM_INVALID_ARG, "q_out must be q with its stride, or not overlap q, k and v");
     const int sms = device_sms();
     if (!sms || prepare_device() != cudaSuccess)
         return no_device();
@@ -162,6 +186,9 @@ int ylm_k_paged_attention(const ylm_paged_cache *cache, const ylm_paged_step *st
     if (bad_rows(q, q_stride, hq) || bad_rows(out, out_stride, hq))
         return refuse(YLM_INVALID_ARG,
                       "rows must be 16-byte aligned, their strides multiples of 8 halves that hold the heads");
+    const int64_t wq = (int64_t)hq * YLM_HEAD_DIM;
+    if (rows_overlap(out, out_stride, wq, q, q_stride, wq, step->rows))
+        return refuse(YLM_INVALID_ARG, "out must not overlap q");
     if (workspace && !aligned(workspace, 16))
         return refuse(YLM_INVALID_ARG, "workspace must be 16-byte aligned");
     const int sms = device_sms();
@@ -209,7 +236,8 @@ int ylm_k_paged_accept(const ylm_paged_cache *cache, const ylm_paged_step *step,
     if (const char *f = step_fault(cache, step))
         return refuse(YLM_INVALID_ARG, f);
     const int64_t layer = (int64_t)cache->n_pages * cache->hkv * cache->page * YLM_HEAD_DIM;
-    if (layers < 0 || (layers > 1 && (layer_stride < layer || layer_stride % 8)))
+    if (layers < 0 || (layers > 1 && (layer_stride < layer || layer_stride % 8)) ||
+        rows_overlap(cache->k, layer_stride, layer, cache->v, layer_stride, layer, layers > 1 ? layers : 1))
         return refuse(YLM_INVALID_ARG, "layers must not overlap, and their stride be a multiple of 8 halves");
     if (step->n_seq == 0)
         return done(cudaSuccess);
