@@ -856,3 +856,50 @@ def test_offsets_beyond_32_bits():
         for k, y in zip("kv", vals[s]):
             got = pool[k][torch.from_numpy(p).cuda(), :, torch.from_numpy(c).cuda()].cpu().numpy()
             np.testing.assert_array_equal(got, y[n + np.array(path)])
+
+
+def dominated(rng, seqs, units, hq, low=0.0):
+    """Requests of one row over `units` units of 128 slots, keys of one channel, values of many sizes; enough of them that
+    a CTA has several units of an item, and borders lie inside of others."""
+    d = Device(make(rng, 16, [128 * units - 1] * seqs, [1] * seqs, None), 1)
+    k = np.full((seqs, 128 * units, D), 0.0)
+    k[:, :, 0] = low
+    v = rng.standard_normal((seqs, 128 * units, D)).astype(np.float16)
+    q = np.zeros((seqs, hq, D), np.float16)
+    return d, k, v, q
+
+
+def put_all(d, k, v):
+    vals = []
+    for s in range(len(d.step.rows)):
+        x = [a[s][:, None].astype(np.float16) for a in (k, v)]
+        for kind, y in zip("kv", x):
+            d.put(kind, s, np.arange(y.shape[0]), y)
+        vals.append(x)
+    d.upload()
+    return vals
+
+
+def test_infinities_and_nan_under_a_dominating_score():
+    # wherever the slot lies, a value that is not finite is not lost when another slot's score is 141 above its own
+    rng = np.random.default_rng(23)
+    cases = [(a, b, x) for a in range(4) for b in range(4) for x in (np.inf, -np.inf, np.nan)] * 6
+    d, k, v, q = dominated(rng, len(cases), 4, 2)
+    q[:, 0, 0] = 16
+    for s, (a, b, x) in enumerate(cases):
+        k[s, a * 128 + 5, 0] = 100
+        v[s, b * 128 + 77, 3] = x
+    vals = put_all(d, k, v)
+    out = attend(d, half(q), 2)
+    got = out.float().cpu().numpy()
+    special = np.array([x for _, _, x in cases], np.float32)
+    np.testing.assert_array_equal(got[:, 1, 3], special)  # every slot weighs the same
+    assert not np.any(np.isfinite(got[:, 0, 3]))
+    assert np.all(np.isnan(got[np.isnan(special), 0, 3]))
+    # the other elements as if it were not there
+    for x in vals:
+        x[1][~np.isfinite(x[1])] = 0
+    out[:, :, 3] = 0
+    for s, x in enumerate(vals):
+        x[1][:, :, 3] = 0
+    check(d, vals, q, out)

@@ -1065,7 +1065,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                             tmem_wait_ld16(y);
 #pragma unroll
                             for (int e = 0; e < 16; e++)
-                                v[e] = f1 == 0.f ? v[e] : fmaf(y[e], f1, v[e]);
+                                v[e] = fmaf(y[e], f1, v[e]); // (a sum that is not finite stays in, whatever its factor)
                         }
                     }
                     if (__builtin_expect(odd && row < rows, 0))
