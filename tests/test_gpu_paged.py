@@ -903,3 +903,47 @@ def test_infinities_and_nan_under_a_dominating_score():
     for s, x in enumerate(vals):
         x[1][:, :, 3] = 0
     check(d, vals, q, out)
+
+
+@pytest.mark.parametrize("seqs", [1, 300])
+def test_scores_that_are_nan_in_one_part_of_an_item(seqs):
+    # rows that see one slot of the last unit, its score NaN, or -inf with a value that is NaN: the request in one CTA's
+    # share, or every unit in another one's
+    rng = np.random.default_rng(24)
+    t = 20
+    d = Device(R.Step(rng, 16, [256] * seqs, [t] * seqs, [[-1] * t] * seqs), 1)
+    vals = fill(rng, d)
+    q = rng.standard_normal((d.rows, 2, D)).astype(np.float16)
+    q[:, :, 8] = 1
+    for s in range(seqs):
+        k, v = vals[s]
+        k[256 + 3, 0, 20] = np.nan
+        k[256 + 5, 0, 8] = -np.inf
+        v[256 + 5, 0, 7] = np.nan
+        d.put("k", s, np.arange(256 + t), k)
+        d.put("v", s, np.arange(256 + t), v)
+    d.upload()
+    out = attend(d, half(q), 2)
+    got = out.float().cpu().numpy().reshape(seqs, t, 2, D)
+    assert np.all(np.isnan(got[:, 3])) and np.all(np.isnan(got[:, 5, :, 7]))
+    # the rest as if those slots were hidden
+    hidden = []
+    for s in range(seqs):
+        k, v = vals[s]
+        k[~np.isfinite(k)], v[~np.isfinite(v)] = 0, 0
+        h = np.zeros(256 + t, bool)
+        h[[256 + 3, 256 + 5]] = True
+        hidden.append(h)
+    clean = out.clone().view(seqs, t, 2, D)
+    clean[:, 3] = 0
+    clean[:, 5, :, 7] = 0
+    for s in range(seqs):
+        for g, h in ((i, j) for i in range(t) for j in range(2)):
+            see = d.step.sees(s)[g:g + 1] & ~hidden[s]
+            kk, vv = vals[s][0][:, 0].astype(np.float64), vals[s][1][:, 0].astype(np.float64)
+            want, pv, mag = R.attention(q[s * t + g:s * t + g + 1, h:h + 1].astype(np.float64), kk, vv, see)
+            ok = np.ones(D, bool)
+            ok[7] = g != 5
+            if g != 3:
+                err = abs(got[s, g, h] - want[0, 0])[ok]
+                assert np.all(err <= bounds(want, pv, mag, vv, see)[0, 0][ok])

@@ -1197,9 +1197,10 @@ __device__ __forceinline__ void px_join(const PagedPass &w, const PagedItem &it,
             o[d] = make_float4(o[d].x * f, o[d].y * f, o[d].z * f, o[d].w * f);
 #pragma unroll
         for (int i = 0; i < BATCH; i++)
-            if (ml[i].x != -INFINITY)
+            if (k0 + i * groups < parts)
             {
-                f = ex2_ftz((ml[i].x - M) * PX_SCALE);
+                // (a part without a score above -inf counts nothing, but one that is NaN, or has such values, stays)
+                f = ml[i].x == -INFINITY ? 0.f : ex2_ftz((ml[i].x - M) * PX_SCALE);
                 L += ml[i].y * f;
 #pragma unroll
                 for (int d = 0; d < PER; d++)
