@@ -947,3 +947,19 @@ def test_scores_that_are_nan_in_one_part_of_an_item(seqs):
             if g != 3:
                 err = abs(got[s, g, h] - want[0, 0])[ok]
                 assert np.all(err <= bounds(want, pv, mag, vv, see)[0, 0][ok])
+
+
+def test_scores_whose_steps_are_as_far_apart_as_weights_reach():
+    # scores of 2^29 + 64 j (before the scale): neighbours in FP32, with weights 2^8 apart
+    rng = np.random.default_rng(26)
+    d, k, v, q = dominated(rng, 200, 6, 2)
+    q[:, :, 0], q[:, :, 1] = 2.0 ** 14, [8, -8]
+    k[:, :, 0], k[:, :, 1] = 2.0 ** 15, 8 * (np.arange(768) // 256)
+    vals = put_all(d, k, v)
+    out = attend(d, half(q), 2)
+    # the large product is the same for every slot and both are powers of two: no score is rounded, and without
+    # it the weights are the same
+    small = [(x[0].copy(), x[1]) for x in vals]
+    for x in small:
+        x[0][:, :, 0] = 0
+    check(d, small, q, out)

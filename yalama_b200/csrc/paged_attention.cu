@@ -916,11 +916,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                     }
                     if (u == 0)
                         mr = mx;
-                    else if (__builtin_expect(__any_sync(0xffffffffu, mx > mr + PX_RISE), 0))
+                    // (by the difference, which is exact for scores so near: mr + PX_RISE could round past the next score)
+                    else if (__builtin_expect(__any_sync(0xffffffffu, mx - mr > PX_RISE), 0))
                     {
                         // the sums so far in units of the new reference
                         float f = 1.f;
-                        if (mx > mr + PX_RISE)
+                        if (mx - mr > PX_RISE)
                         {
                             f = ex2_ftz((mr - mx) * PX_SCALE);
                             mr = mx;
