@@ -963,3 +963,17 @@ def test_scores_whose_steps_are_as_far_apart_as_weights_reach():
     for x in small:
         x[0][:, :, 0] = 0
     check(d, small, q, out)
+
+
+def test_values_at_the_ends_of_fp16():
+    # one slot a unit counts, each stream's next one up to 2^4.8 times as much as its last: the reference stays behind,
+    # weights are rounded, and what they weigh is the largest there is
+    rng = np.random.default_rng(25)
+    d, k, v, q = dominated(rng, 200, 6, 8, low=-200)
+    k[:, 9::128, 0] = np.arange(6) // 2
+    q[:, :, 0] = rng.uniform(0.5, 4.8, (200, 8)) * np.log(2) * np.sqrt(D)
+    v[:, :, ::2], v[:, :, 1::2] = 65504, -65504
+    vals = put_all(d, k, v)
+    out = attend(d, half(q), 8)
+    assert bool(torch.isfinite(out).all())
+    check(d, vals, q, out)

@@ -245,6 +245,19 @@ __device__ __forceinline__ float2 px_fma2(float2 a, float2 b, float2 c)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
 }
+// Two results to FP16. A row's weights sum to one before they are rounded for the product, after it to 1 + 2^-11 at most:
+// a finite result that rounds to infinity is FP16's largest value, where the values that it is made of end; rounded towards
+// zero it stops there, and an infinite one stays. (48 requests of 20 to 9000 slots: 0.1 us; clamped in FP32 0.7 us.)
+__device__ __forceinline__ __half2 px_result(float x, float y)
+{
+    const __half2 h = __floats2half2_rn(x, y);
+    const uint32_t inf = __heq2_mask(__habs2(h), __half2half2(__ushort_as_half(0x7C00)));
+    uint32_t down;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(down) : "f"(y), "f"(x));
+    const uint32_t r = (*reinterpret_cast<const uint32_t *>(&h) & ~inf) | (down & inf);
+    return *reinterpret_cast<const __half2 *>(&r);
+}
+
 // Between lanes 2 i and 2 i + 1: the lower one gets (x, the other's x), the upper one (the other's y, y).
 __device__ __forceinline__ void px_trade(uint4 &x, uint4 &y, int lane)
 {
@@ -1100,7 +1113,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
                             __half2 h[4];
 #pragma unroll
                             for (int k = 0; k < 4; k++)
-                                h[k] = __floats2half2_rn(v[8 * e + 2 * k] * inv, v[8 * e + 2 * k + 1] * inv);
+                                h[k] = px_result(v[8 * e + 2 * k] * inv, v[8 * e + 2 * k + 1] * inv);
                             x[e] = *reinterpret_cast<const uint4 *>(h);
                         }
                         px_trade(x[0], x[1], lane);
@@ -1234,7 +1247,7 @@ __device__ __forceinline__ void px_join(const PagedPass &w, const PagedItem &it,
 #pragma unroll
         for (int d = 0; d < PER; d++)
         {
-            const __half2 h[2] = {__floats2half2_rn(o[d].x * inv, o[d].y * inv), __floats2half2_rn(o[d].z * inv, o[d].w * inv)};
+            const __half2 h[2] = {px_result(o[d].x * inv, o[d].y * inv), px_result(o[d].z * inv, o[d].w * inv)};
             *reinterpret_cast<uint2 *>(&tile[row][4 * (warp + PJ_WARPS * d)]) = *reinterpret_cast<const uint2 *>(h);
         }
     __syncthreads();
