@@ -361,6 +361,8 @@ typedef struct ylm_paged_cache {
  * length[s] tokens in the cache before the step; its row i goes to slot length[s] + i and to position
  * length[s] + depth(i). With parent, the rows are trees: parent[row_start[s] + i] is the row of request s that row i
  * follows (an earlier one), -1 for one that follows the cached tokens; without, chains (depth i).
+ * Single tokens, pieces of prompts (chains) and trees may share a step; with parent no request has more
+ * than YLM_TREE_ROWS rows, so longer pieces of prompts go without trees.
  * The arrays are on the device: a captured graph serves other lengths, tables and trees, and any rows within
  * `rows` and max_rows. Rows that belong to no request are left as they were. */
 typedef struct ylm_paged_step {
@@ -418,7 +420,10 @@ int ylm_k_paged_attention_workspace(const ylm_paged_cache *cache, const ylm_page
  * accepted [n_seq][max_rows]: these rows, -1 behind; n_accepted; next_token: the last one's pick;
  * new_length = length + n_accepted. The keys and values of accepted row number j move to slot length + j, in `layers`
  * layers whose pools lie layer_stride halves apart from cache's on, none over another (0 layers: none); the slots behind new_length hold
- * anything then. A request without rows, or left out: 0 accepted, next_token -1, its length. The results
+ * anything then. Rows that are given and not drafted (a prompt's piece): before the call, set the pick of each but the
+ * last to the next row's token; all of them are accepted then, and next_token is the last one's pick (which
+ * means nothing while the prompt goes on). Left as the model's picks, they end the piece at the first
+ * token that it would not have chosen. A request without rows, or left out: 0 accepted, next_token -1, its length. The results
  * must not overlap the step, the tokens or the picks. */
 int ylm_k_paged_accept(const ylm_paged_cache *cache, const ylm_paged_step *step, const int64_t *tokens,
                        const int64_t *picks, int32_t layers, int64_t layer_stride, int32_t *accepted,

@@ -977,3 +977,95 @@ def test_values_at_the_ends_of_fp16():
     out = attend(d, half(q), 8)
     assert bool(torch.isfinite(out).all())
     check(d, vals, q, out)
+
+
+@pytest.mark.parametrize("trees", [False, True])
+def test_prompt_pieces_beside_single_tokens_and_trees(trees):
+    """One step holds pieces of prompts, single tokens and drafted ones. The picks of given rows are set to the next given
+    token, so that all of them are accepted; the cache then holds each request's tokens in order."""
+    rng = np.random.default_rng(27)
+    hq, hkv, page, layers, vocab, most = 4, 2, 16, 2, 40, 128 if trees else 300
+    prompts = [rng.integers(0, vocab, n) for n in ((250, 1, 90, 128) if trees else (700, 1, 90, 300))]
+    seqs, ld = 4, 60
+    tab = [half(a) for a in rope_tables(rng, 900)]
+    embed = rng.standard_normal((vocab, hq + 2 * hkv, D)).astype(np.float16)  # a token's q, k, v before rotation
+    table = rng.permutation(seqs * ld).reshape(seqs, ld)
+    dtab = ints(table)
+    pools = [[torch.zeros(layers, seqs * ld, hkv, page, D, dtype=torch.float16, device="cuda") for _ in "kv"] for _ in range(2)]
+
+    def run(pool, lengths, tokens, parents, max_rows):
+        starts = np.concatenate([[0], np.cumsum([len(t) for t in tokens])])
+        rows = int(starts[-1])
+        keep = [ints(starts), ints(lengths), None if parents is None else ints(np.concatenate(parents))]
+        st = E.paged_step(ptr(keep[0]), ptr(keep[1]), ptr(dtab), ptr(keep[2]), seqs, ld, rows, max_rows)
+        x = half(embed[np.concatenate(tokens)])
+        out = torch.zeros(rows, hq, D, dtype=torch.float16, device="cuda")
+        q = torch.empty_like(out)
+        for i in range(layers):
+            c = E.paged_cache(ptr(pool[0][i]), ptr(pool[1][i]), seqs * ld, page, hkv)
+            E.check(E.lib().ylm_k_paged_append(c, st, ptr(x), x.stride(0), ptr(x[:, hq:]), x.stride(0),
+                                               ptr(x[:, hq + hkv:]), x.stride(0), hq, None, None, 0.0, ptr(tab[0]),
+                                               ptr(tab[1]), 900, ptr(q), q.stride(0), stream()), "append")
+            E.check(E.lib().ylm_k_paged_attention(c, st, ptr(q), q.stride(0), hq, ptr(out), out.stride(0), None, 0,
+                                                  stream()), "attention")
+        return st, keep, out, starts
+
+    lengths, last, at = [0] * seqs, [0] * seqs, [0] * seqs
+    history, given_outs = [[] for _ in range(seqs)], {}
+    for step in range(12):
+        tokens, parents, given = [], [], []
+        for s, p in enumerate(prompts):
+            left = p[at[s]:]
+            if len(left):  # a piece of the prompt, as long as the step allows
+                tokens.append(left[:int(rng.integers(1, most + 1))])
+                parents.append(list(range(-1, len(tokens[-1]) - 1)))
+            else:
+                t = 1 if s == 1 else int(rng.integers(2, 30))
+                tokens.append(np.concatenate([[last[s]], rng.integers(0, vocab, t - 1)]))
+                parents.append(R.tree(rng, "random", t) if trees else list(range(-1, t - 1)))
+            given.append(len(left) > 0)
+        st, keep, out, starts = run(pools[0], lengths, tokens, parents if trees else None, most)
+        rows = int(starts[-1])
+        logits = torch.randn(rows, vocab, device="cuda").half()
+        for s in range(seqs):
+            for i, p in enumerate(parents[s]):
+                if p >= 0 and rng.random() < 0.6:
+                    logits[int(starts[s]) + p, int(tokens[s][i])] = 30
+        picks = torch.empty(rows, dtype=torch.int64, device="cuda")
+        lp = torch.empty(rows, device="cuda")
+        E.check(E.lib().ylm_k_logprobs(ptr(logits), vocab, rows, vocab, None, None, 1, None, None, ptr(picks), ptr(lp),
+                                       stream()), "logprobs")
+        model = picks.cpu().numpy()
+        flat = ints(np.concatenate(tokens), np.int64)
+        for s in range(seqs):
+            if given[s]:
+                a, b = int(starts[s]), int(starts[s + 1])
+                picks[a:b - 1] = flat[a + 1:b]
+        res = [torch.empty(seqs, most, dtype=torch.int32, device="cuda"), torch.empty(seqs, dtype=torch.int32, device="cuda"),
+               torch.empty(seqs, dtype=torch.int64, device="cuda"), torch.empty(seqs, dtype=torch.int32, device="cuda")]
+        first = E.paged_cache(ptr(pools[0][0]), ptr(pools[0][1]), seqs * ld, page, hkv)
+        E.check(E.lib().ylm_k_paged_accept(first, st, ptr(flat), ptr(picks), layers, pools[0][0].stride(0),
+                                           *[ptr(x) for x in res], stream()), "accept")
+        accepted, count, following, new = (x.cpu().numpy() for x in res)
+        for s in range(seqs):
+            a, t = int(starts[s]), len(tokens[s])
+            path = list(range(t)) if given[s] else R.accept(parents[s], tokens[s], model[a:a + t])
+            assert accepted[s].tolist() == path + [-1] * (most - len(path)) and count[s] == len(path)
+            assert new[s] == lengths[s] + len(path) and following[s] == model[a + path[-1]]
+            for i in path:
+                given_outs[s, len(history[s])] = out[a + i].float()
+                history[s].append(int(tokens[s][i]))
+            if given[s]:
+                at[s] += t
+            last[s] = int(following[s])
+        lengths = new.tolist()
+    assert all(at[s] == len(prompts[s]) for s in range(seqs)) and min(lengths) > 1
+    # every request's tokens as one chain
+    _, _, out, starts = run(pools[1], [0] * seqs, [np.array(h) for h in history], None, max(lengths))
+    for s in range(seqs):
+        p, c = dtab[s][torch.arange(lengths[s], device="cuda") // page].long(), torch.arange(lengths[s], device="cuda") % page
+        for x, y in zip(*pools):
+            assert torch.equal(x[:, p, :, c], y[:, p, :, c])
+        for j in range(lengths[s]):
+            # each is within 2^-11 |o| + 2^-11 sum p |v| of the same value: |v| stays below 6, plus dp
+            assert float((given_outs[s, j] - out[int(starts[s]) + j].float()).abs().max()) <= 4 * EPS16 * 6
