@@ -1069,3 +1069,40 @@ def test_prompt_pieces_beside_single_tokens_and_trees(trees):
         for j in range(lengths[s]):
             # each is within 2^-11 |o| + 2^-11 sum p |v| of the same value: |v| stays below 6, plus dp
             assert float((given_outs[s, j] - out[int(starts[s]) + j].float()).abs().max()) <= 4 * EPS16 * 6
+
+
+@pytest.mark.parametrize("trees", [None, "random"])
+def test_requests_that_share_the_pages_of_a_prefix(trees):
+    # pages below the new rows' are of two requests and more, in a step that could have more rows: attention sees them
+    # for each, and append and accept leave them as they are
+    rng = np.random.default_rng(28)
+    page, prefix, hkv, hq = 32, 256, 2, 8
+    own, rows = [0, 40, 300, 7, 1000, 31], [1] * 6 if trees is None else [1, 20, 64, 9, 2, 33]
+    st = make(rng, page, [prefix + n for n in own], rows, trees, 3)
+    st.table[1:4, :prefix // page] = st.table[0, :prefix // page]
+    st.table[5, :prefix // page] = st.table[4, :prefix // page]
+    d = Device(st, hkv, max_rows=128)
+    vals = []
+    for s, n in enumerate(st.lengths):
+        k, v = (rng.standard_normal((n + rows[s], hkv, D)).astype(np.float16) for _ in "kv")
+        if s in (1, 2, 3, 5):
+            k[:prefix], v[:prefix] = (x[:prefix] for x in vals[0 if s < 4 else 4])
+        d.put("k", s, np.arange(n), k[:n])
+        d.put("v", s, np.arange(n), v[:n])
+        vals.append((k, v))
+    d.upload()
+    before = {x: d.pool[x].clone() for x in "kv"}
+    new = [half(np.concatenate([x[i][n:] for x, n in zip(vals, st.lengths)] + [np.zeros((3, hkv, D))])) for i in range(2)]
+    append(d, None, new[0], new[1], 0)
+    q = rng.standard_normal((d.rows, hq, D)).astype(np.float16)
+    check(d, vals, q, attend(d, half(q), hq))
+    tokens = ints(np.zeros(d.rows), np.int64)
+    accept(d, tokens, tokens, 1)  # every row's lowest child
+    for s, n in enumerate(st.lengths):
+        path = R.accept(st.parents(s), [0] * rows[s], [0] * rows[s])
+        p, c = st.place(s, n + np.arange(len(path)))
+        for x, y in zip("kv", vals[s]):
+            np.testing.assert_array_equal(d.pool[x].cpu().numpy()[p, :, c], y[n + np.array(path)])
+            common = st.table[s, :prefix // page]
+            assert torch.equal(d.pool[x][common].view(torch.int16), before[x][common].view(torch.int16))
+    assert d.faults() == 0

@@ -538,8 +538,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     // where no item has more (the products read 128 rows from there on, and nobody reads what comes of the others), or one.
     const int q_places = PAIR || w.p.cap <= 64 ? 2 : 1;
     const uint32_t q_step = PAIR ? PX_TILE : PX_TILE / 4;
-    // Where every request is one item a KV head, its K and V are read once, and the sums should stay in L2: 48 requests of 20
-    // to 9000 slots 36.8 us against 39.6 with the normal policy, 131071 slots 95 against 96.
+    // Where every request is one item a KV head, K and V on pages of its own are read once, and the sums should stay in L2
+    // instead: 48 requests of 20 to 9000 slots 57.3 us against 63.5 with the normal policy (L2 full of other data before),
+    // 32 trees 90 against 94, 131071 slots 115 against 121. Pages that requests share are read by
+    // each of them, and leave L2 early for it: 48 requests behind a common prefix of 4096 or 8192 slots 77.5 and 137.2 against
+    // 75.8 and 137.0, 64 with 4000 slots of their own behind one of 8192 (1.1 GB) 414 against 391, the most that was met.
     uint64_t policy;
     if (st.max_rows <= w.p.tpi)
         policy = l2_policy_evict_first();
