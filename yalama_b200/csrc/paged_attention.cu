@@ -97,11 +97,10 @@ struct PagedItem
     int units;          // units of the item
 };
 
-// A CTA's share, as what the items and units in front of its borders cost together, and its first item; left in the
-// workspace for the join. Unit k of an item lies at zero + k * px_cost: it is the share's in which that is.
+// A CTA's share and its first item; left in the workspace for the join. Places are what the items and units in front of
+// them cost together: unit k of an item lies at zero + k * px_cost, and is the share's in which that is.
 struct PagedCut
 {
-    long long u0, u1;
     long long each, more; // every share is `each` long, the first `more` of them one more; the rest are empty
     long long left;       // what is behind its part of the first item
     long long zero;       // where the first item's unit 0 lies
@@ -490,8 +489,6 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         }
         rest -= a.c.hkv * px_front(req.n, lo, w.p);
         PagedCut c;
-        c.u0 = u0;
-        c.u1 = u1;
         c.each = each;
         c.more = over;
         c.it.s = s;
@@ -513,11 +510,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         w.cuts[b] = c;
     }
     else if (u0 == u1 && tid == 0)
-    {
-        PagedCut c = {};
-        c.u0 = c.u1 = u0;
-        w.cuts[b] = c;
-    }
+        w.cuts[b] = PagedCut{};
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

@@ -166,8 +166,8 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, i
                  : "memory");
 }
 
-// 2^x with the PTX ex2.approx instruction, subnormal results flushed to zero:
-// the softmax's arguments are <= 0, and values below 2^-126 vanish in FP16 P.
+// 2^x with the PTX ex2.approx instruction, subnormal results flushed to zero: of a softmax's weights and factors
+// (arguments of 16 at most), values below 2^-126 vanish in FP16 P and beside the sums.
 __device__ __forceinline__ float ex2_ftz(float x)
 {
     float y;
