@@ -1186,6 +1186,9 @@ __device__ __forceinline__ void px_join(const PagedPass &w, const PagedItem &it,
         for (int i = 0; i < BATCH; i++)
         {
             ml[i] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int d = 0; d < PER; d++)
+                x[i][d] = make_float4(0.f, 0.f, 0.f, 0.f);
             const int k = k0 + i * groups;
             if (k < parts)
             {
@@ -1207,20 +1210,19 @@ __device__ __forceinline__ void px_join(const PagedPass &w, const PagedItem &it,
             o[d] = make_float4(o[d].x * f, o[d].y * f, o[d].z * f, o[d].w * f);
 #pragma unroll
         for (int i = 0; i < BATCH; i++)
-            if (k0 + i * groups < parts)
-            {
-                // (a part without a score above -inf counts nothing, but one that is NaN, or has such values, stays)
-                f = ml[i].x == -INFINITY ? 0.f : ex2_ftz((ml[i].x - M) * PX_SCALE);
-                L += ml[i].y * f;
+        {
+            // (a part without a score above -inf counts nothing, but one that is NaN, or has such values, stays)
+            f = ml[i].x == -INFINITY ? 0.f : ex2_ftz((ml[i].x - M) * PX_SCALE);
+            L += ml[i].y * f;
 #pragma unroll
-                for (int d = 0; d < PER; d++)
-                {
-                    o[d].x += x[i][d].x * f;
-                    o[d].y += x[i][d].y * f;
-                    o[d].z += x[i][d].z * f;
-                    o[d].w += x[i][d].w * f;
-                }
+            for (int d = 0; d < PER; d++)
+            {
+                o[d].x += x[i][d].x * f;
+                o[d].y += x[i][d].y * f;
+                o[d].z += x[i][d].z * f;
+                o[d].w += x[i][d].w * f;
             }
+        }
     }
     for (int s = 1 << rows_log; s < 32; s <<= 1)
     {
