@@ -402,7 +402,8 @@ int ylm_k_paged_append(const ylm_paged_cache *cache, const ylm_paged_step *step,
  * above; out does not overlap q), RoPE applied; at most 128 query heads per KV head. Scores, softmax statistics and sums are FP32. A row that
  * sees no slot (its pages are not in the pool), or only scores of -inf, gets zeros; what hidden slots hold
  * does not matter, NaN and infinities either (an infinite value that a row sees makes its element infinite, or NaN where the
- * slot's weight is below 2^-36 of the row's largest). Each weight is rounded to FP16 for the product with the values (by
+ * slot's weight is below 2^-36 of the row's largest; a NaN makes it NaN, and a score of NaN or +inf the whole
+ * row's head). Finite queries, keys and values give finite results. Each weight is rounded to FP16 for the product with the values (by
  * 2^-11 of itself; of weights below 2^-25 of the row's largest, by 2^-36 of that one), the result once more.
  * workspace: device memory of at least ylm_k_paged_attention_workspace bytes, 16-byte aligned, for this call alone
  * until it has run: calls that may overlap on the GPU, and graphs that may, need one each. null: allocated and

@@ -23,16 +23,20 @@
 // units), warp 3 sets what is not finite in those rows of V to 0 before the product, and says so where the slot is one of the
 // step's; the rows that do see it then get it added at the end. Scores of hidden slots are replaced, whatever they are.
 //
-// Measured (B200, 32 / 8 heads but where noted, device time in a captured graph, join included):
-//   one token over 131071 slots: 96 us = 5.6 TB/s. The CTAs end after 74 to 89 us, as HBM serves them.
-//   48 requests of 20 to 9000 slots (28 / 4 heads) 37 us, 32 trees of 9 to 45 tokens over 300 to 5000 slots 62 us: a unit of one
-//   tile takes 2050 cycles, one of two 3870, and an item some 5500 beside its units.
+// Measured (B200, 32 / 8 heads but where noted, device time in a captured graph that is repeated without pause, join
+// included; the card's power limit lowers the clock of the long cases, which is given with them):
+//   one token over 131071 slots: 98 us = 5.4 TB/s at 1540 MHz (95 after a pause). The CTAs end after 74 to 89 us, as HBM
+//   serves them.
+//   48 requests of 20 to 9000 slots (28 / 4 heads) 37 us, 32 trees of 9 to 45 tokens over 300 to 5000 slots 65 us at 1850 MHz: a
+//   unit of one tile takes 2050 cycles, one of two 3870, and an item some 5500 beside its units.
 //   a tree of 64 tokens over 8200 slots: 30 us, the attention's CTAs ending after 14 to 20; partial sums of 19 MB are joined.
-//   2049 rows behind 6145 slots: 251 us = 960 TFLOP/s. A stream's unit is 2000 cycles of softmax (a quarter of it maxima) and
-//   1900 of hand-over and products, with the other stream's in between: tensor pipe 48 %, exponential unit 47 % of the time.
-//   611 slots: 12.4 us, one unit a CTA: in a CTA's 15800 cycles the share takes 4100, the item and its first
-//   loads 3500, S 900, the weights 2800, the product 1200, the way out 3200. The rest is the join.
-// Tried and slower, the 2049 rows: all 128 scores of a row unrolled (380 us, registers spilled), the reference taken from the
+//   2049 rows behind 6145 slots: 281 us = 857 TFLOP/s at 1740 MHz (263 = 915 after a pause). A stream's unit is 2000 cycles of
+//   softmax (a quarter of it maxima) and 1900 of hand-over and products, with the other stream's in between: tensor pipe
+//   48 %, exponential unit 47 % of the time.
+//   611 slots: 12.2 us, one unit a CTA: in a CTA's 15800 cycles the share takes 4100, the item and its first
+//   loads 3500, S 900, the weights 2800, the product 1200, the way out 3200. The rest is the join. That is this kernel's
+//   set-up, not the case: the 8-bit cache's attention, a kernel for few rows, takes 5 us for as many slots.
+// Tried and slower, the 2049 rows (after a pause): all 128 scores of a row unrolled (380 us, registers spilled), the reference taken from the
 // tile before (342, code beyond the instruction cache), two threads a row (271 against 259: an SM quarter's two warps
 // share its exponential unit), a quarter or half of the exponentials by polynomial (263 and 281 against 261), units of 64 slots with two S a
 // stream (358: twice the commits and waits of the issuing warp).
@@ -77,7 +81,9 @@ static PagedPlan paged_plan(const PagedAttnArgs &a, int num_sms)
     p.cap = std::max(1, std::min(p.tpi, a.st.max_rows)) * p.G;
     // An item's first loads and its sums' way out, where a unit of one tile costs 1 and a unit of two tiles 2 (2050 and
     // 3870 cycles). Few rows, with 0, 1, 2, 3, 4: 48 requests of 20 to 9000 slots 57, 47, 41, 39.5, 40 us. More rows, with 3,
-    // 4, 5, 6: 32 trees 71, 67, 66, 64 us.
+    // 4, 5, 6: 32 trees 71, 67, 66, 64 us. All requests alike in rows, with 3, 4, 6: 4 rows an item 64, 61, 66 us (48 requests of 20
+    // to 9000 slots) and 64, 66, 70 (100 of 50 to 2000); 64 rows 74, 70, 71 and 73, 72, 75; 180 rows 130, 121, 117 and 125,
+    // 118, 116. So the turn belongs between 64 and 180 rows, and 4 would be 1 to 5 % faster from 16 to 64.
     p.item = p.cap <= 32 ? 3 : 6;
     p.ctas = num_sms;
     p.ml_off = (size_t)p.ctas * PX_CUT;

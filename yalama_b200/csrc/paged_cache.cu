@@ -31,8 +31,9 @@ constexpr int PA_HEADS = PA_THREADS / 8; // a pass: 8 lanes a head, 8 dimensions
 // A CTA takes every gridDim.y-th pass of one row; the loads of BATCH passes are under way while the request is looked up.
 // With a dimension and its partner in one lane the rotation needs no exchange. Bound by HBM behind the lookup's chain of
 // loads, which eight CTAs an SM cover: 4522 rows of 80 heads 33.9 us = 5.5 TB/s (256 threads, four CTAs an SM 37.6 us; five
-// passes at a time, and fewer CTAs, 36 to 41 us; 16 lanes a head, with shuffles for the partners, 41 us). One row of 48
-// heads 2.3 us: the chain's latency.
+// passes at a time, and fewer CTAs, 36 to 41 us; 16 lanes a head, with shuffles for the partners, 41 us). The price of
+// eight CTAs is 64 registers a thread: of the three passes' state 84 bytes are spilled and 160 loaded back (of two 24 and
+// 24). One row of 48 heads 2.1 us: the chain's latency.
 template <int BATCH>
 __global__ void __launch_bounds__(PA_THREADS, 8) paged_append_kernel(const __grid_constant__ PagedAppendArgs a)
 {
